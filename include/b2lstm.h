@@ -20,6 +20,8 @@
  *   b2_lstm_*     one (b)lstm layer on caller's buffers <-> layers::LstmLayer<Gpu>
  *   b2_net_*      layer stack + minibatch step          <-> NeuralNetwork + Optimizer::_processDataSet
  *   b2_dp_*       gradient all-reduce across GPUs (no counterpart: the reference is single-GPU)
+ * and, beside the layers, the operators of models over tokens (no counterpart: the reference has real-valued inputs and targets):
+ *   b2_embedding_*, b2_block_norm_*, b2_logprob_*, b2_gradient_*
  */
 #ifndef B2LSTM_H
 #define B2LSTM_H
@@ -145,6 +147,100 @@ const char *b2_lstm_recurrence_kernel(const b2_lstm *layer, int backward);
 int b2_lstm_synchronize(b2_lstm *layer, b2_stream stream);
 /* Bytes of private device memory the layer holds. */
 size_t b2_lstm_state_bytes(const b2_lstm *layer);
+
+/* ------------------------------------------------------------------------------------------
+ * Operators of a token model around the recurrent layers.  No counterpart in the reference toolkit.
+ *
+ * All of them work on the caller's device buffers, on the caller's stream, without allocating, synchronising or keeping anything between
+ * calls; scratch, where one is needed, comes from the caller (the matching _workspace function tells its size; its contents need no
+ * set-up and may be overwritten between calls).  Calls that share a workspace have to be ordered, by one stream for instance.  Arithmetic
+ * is fp32 whatever the tensors' type, results are rounded once, sums are added in a fixed order (the same bits every time).
+ * Rows are the frames of a fraction, row t*P + p for frame t of sequence p; row r of a tensor starts ld elements behind row r - 1.  Any
+ * address that is a multiple of the element size is accepted; 16-byte aligned rows are the fastest.
+ * Padding frames have the token -1 (any negative one) or the pattern type 0: their results and gradients are zero.
+ * ------------------------------------------------------------------------------------------ */
+enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };   /* element types */
+
+/* Embedding lookup: out[r][:] = scale * table[tokens[r]][:], n rows of dim channels; zeros for a negative token, NaN for one that is not
+ * below vocab.  Output and table may differ in type. */
+int b2_embedding_forward(void *out, int out_type, long long ld_out, const void *table, int table_type, long long ld_table, int vocab,
+                         int dim, const int *tokens_dev, long long n, float scale, b2_stream stream);
+/* Its gradient: dtable[v][:] = scale * sum of dout[r][:] over the rows r with tokens[r] = v, in the order of the rows, for all v (zeros
+ * where no row has v); with accumulate non-zero it is added to dtable, and rows of tokens that do not occur are left alone.  Tokens outside
+ * the table contribute nothing.  workspace: aligned to 256 bytes. */
+size_t b2_embedding_backward_workspace(long long n, int vocab, int dim);
+int b2_embedding_backward(void *dtable, int dtable_type, long long ld_dtable, int vocab, int dim, const void *dout, int dout_type,
+                          long long ld_dout, const int *tokens_dev, long long n, float scale, int accumulate, void *workspace,
+                          size_t workspace_bytes, b2_stream stream);
+
+/* Norms before and after a residual block, fused with the block's gate and residual scale:
+ *   y = x + residual_scale * gate * (w_post * norm(f) + b_post)        f: the block's output
+ *   h = w_pre * norm(y) + b_pre                                          the next block's input
+ * norm: (v - mean) / sqrt(var + eps) if layer_norm is non-zero, else v / sqrt(mean(v^2) + eps), over the dim channels (at most 8192) of a
+ * frame.  y is rounded to the tensors' type before its own norm.  The gate (may be NULL: 1) has gate_rows rows, frame r takes row
+ * r % gate_rows: 1 row for all frames, P rows for one per sequence, `rows` rows for one per frame.  Weights and biases (fp32) may be
+ * NULL: 1 and 0.  pat_types (may be NULL): pattern types, frames of type 0 come out as zeros.
+ * stats: 4 floats a frame (mean and 1/deviation of f, then of y; the means are 0 without layer_norm), written by the forward pass unless
+ * NULL, read by the backward pass. */
+typedef struct {
+    int type;                /* of x, f, y, h, gate and their gradients */
+    int dim;
+    long long rows;
+    int layer_norm;
+    float eps;
+    float residual_scale;
+    const char *pat_types;
+    const float *w_pre, *b_pre, *w_post, *b_post;
+    const void *gate;
+    long long gate_rows, ld_gate;
+    float *stats;
+} b2_block_norm;
+/* f NULL: no block yet, y = x (y may then be NULL: not copied) and h = norm of x.  h NULL: the last block, no norm behind it.  y may take
+ * the place of x. */
+int b2_block_norm_forward(const b2_block_norm *desc, const void *x, long long ld_x, const void *f, long long ld_f, void *y, long long ld_y,
+                          void *h, long long ld_h, b2_stream stream);
+/* Gradients from dy (of y, may be NULL: 0) and dh (of h, NULL where the forward pass had no h) with y (x where there was no f) and f of the
+ * forward pass.  Outputs may be NULL, and are OVERWRITTEN: dx, df, dgate (gate_rows rows) in the tensors' type, the sums over frames dw_pre,
+ * db_pre, dw_post, db_post (dim floats each).  dx and df may take the place of an input that has the same leading dimension.
+ * workspace: aligned to 16 bytes; gate_rows 0 without a gate. */
+size_t b2_block_norm_backward_workspace(long long rows, int dim, long long gate_rows);
+int b2_block_norm_backward(const b2_block_norm *desc, void *dx, long long ld_dx, void *df, long long ld_df, void *dgate, long long ld_dgate,
+                           float *dw_pre, float *db_pre, float *dw_post, float *db_post, const void *dy, long long ld_dy, const void *dh,
+                           long long ld_dh, const void *y, long long ld_y, const void *f, long long ld_f, void *workspace,
+                           size_t workspace_bytes, b2_stream stream);
+
+/* Log probabilities of given tokens under rows of vocab logits x: with z = scale * x where the token is allowed and -inf elsewhere,
+ *   lse = log sum exp z,   logprob = z[token] - lse,   entropy = -sum p log p,   and the `top` (at most 32) most likely tokens, best
+ * first, equal ones by their index: top_tokens / top_logprobs [rows][top], -1 / -inf where a row has fewer with a probability above 0.
+ * mask (may be NULL): a byte per token, 0 = not allowed; row r's starts at mask + r * ld_mask (ld_mask 0: the same for all rows).
+ * A negative token gives logprob 0 (lse, entropy and alternatives are computed all the same), one that is not below vocab NaN.  A row
+ * with nothing allowed (or nothing above -inf): lse -inf, entropy 0, no alternatives, logprob -inf.  NaN or +inf among a row's allowed
+ * logits: lse, logprob and entropy NaN (NaN ranks first among the alternatives).
+ * lse is always written, logprob, entropy (NULL) and alternatives (top 0) where asked for. */
+int b2_logprob_forward(const void *logits, int type, long long rows, int vocab, long long ld, const unsigned char *mask, long long ld_mask,
+                       float scale, const int *tokens_dev, float *logprob, float *lse, float *entropy, int top, int *top_tokens,
+                       float *top_logprobs, b2_stream stream);
+/* The gradient of sum(dlogprob * logprob + dentropy * entropy) with respect to the logits, in their type; lse and entropy as the forward
+ * pass left them.  dlogprob or dentropy may be NULL (0).  Rows with a negative token and rows with nothing allowed get zeros, entries that
+ * are not allowed too; a token that is not below vocab gives NaN.  dlogits may take the place of the logits. */
+int b2_logprob_backward(void *dlogits, long long ld_dlogits, const void *logits, int type, long long rows, int vocab, long long ld,
+                        const unsigned char *mask, long long ld_mask, float scale, const int *tokens_dev, const float *lse,
+                        const float *dlogprob, const float *entropy, const float *dentropy, b2_stream stream);
+
+/* The L2 norm over all elements of n tensors, in one float on the device (squares are summed in fp64: no overflow short of the float's
+ * own range).  The list is read during the call only.  workspace: aligned to 8 bytes. */
+typedef struct {
+    void *data;
+    size_t count;     /* elements, contiguous */
+    int type;
+} b2_tensor;
+size_t b2_gradient_norm_workspace(void);
+int b2_gradient_norm(const b2_tensor *tensors, int n, float *norm_dev, void *workspace, size_t workspace_bytes, b2_stream stream);
+/* The same, and out = tensors * min(1, max_norm / norm), element by element; out[i] has tensors[i]'s count and may have another type.
+ * out NULL: in place.  A norm that is NaN or infinite leaves the values as they are (the update of b2_net then zeroes the entries that are
+ * no numbers).  Tensors must not overlap, save that out[i] may be tensors[i]. */
+int b2_gradient_clip(const b2_tensor *tensors, const b2_tensor *out, int n, float max_norm, float *norm_dev, void *workspace,
+                     size_t workspace_bytes, b2_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * NeuralNetwork + Optimizer::_processDataSet + SteepestDescentOptimizer

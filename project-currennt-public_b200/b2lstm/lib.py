@@ -33,6 +33,22 @@ SIGNATURES = {
                                      C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "b2_matrix_multiply_noalloc": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int,
                                              C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "b2_embedding_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_void_p,
+                                       C.c_longlong, C.c_float, C.c_void_p]),
+    "b2_embedding_backward_workspace": (C.c_size_t, [C.c_longlong, C.c_int, C.c_int]),
+    "b2_embedding_backward": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p,
+                                        C.c_longlong, C.c_float, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b2_block_norm_forward": (C.c_int, [C.c_void_p] + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
+    "b2_block_norm_backward_workspace": (C.c_size_t, [C.c_longlong, C.c_int, C.c_longlong]),
+    "b2_block_norm_backward": (C.c_int, [C.c_void_p] + [C.c_void_p, C.c_longlong] * 3 + [C.c_void_p] * 4 + [C.c_void_p, C.c_longlong] * 4 +
+                               [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b2_logprob_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_float, C.c_void_p,
+                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b2_logprob_backward": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p,
+                                      C.c_longlong, C.c_float] + [C.c_void_p] * 6),
+    "b2_gradient_norm_workspace": (C.c_size_t, []),
+    "b2_gradient_norm": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b2_gradient_clip": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "b2_lstm_num_weights": (C.c_size_t, [C.c_void_p]),
     "b2_lstm_create": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "b2_lstm_destroy": (None, [C.c_void_p]),

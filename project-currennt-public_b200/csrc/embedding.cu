@@ -1,0 +1,587 @@
+// Embedding lookup with scaling, and its gradient.
+//
+//   out[r] = s * table[tok[r]]                      dtable[v] (+)= s * sum over r with tok[r] = v of dout[r]
+//
+// Lookup: a group of threads per row, every thread a few vectors of the row; memory latency and bandwidth are all there is.
+//
+// Gradient: the rows are sorted by token (stable radix sort, so rows of one token keep their order), then summed in that order in
+// fp32: no atomics on values, the same bits every time.
+//   1. sort: digits of up to 9 bits; up to SMALL_SORT tokens one block does all passes in shared memory, otherwise two launches a pass
+//      (digit counts of every tile; ranks and scatter).  Tokens outside the table get the key `vocab` and end up last.
+//   2. sum: the sorted rows are cut into pieces of `piece` rows; a group of threads sums a piece column by column.  A token whose
+//      rows lie inside one piece is written at once; one that crosses a border leaves a partial sum per piece ("head": it began in
+//      an earlier piece; "tail": it begins here and goes on).
+//   3. join: the pieces with a tail (a list, filled by atomics: its order changes no result) add the heads that follow.
+// A frequent token is thus spread over as many groups as it has pieces.  Without accumulation the rows of tokens that do not occur are
+// zeroed by extra blocks of the same launches: the table is written once, and the sort's launches, which occupy few
+// multiprocessors, hide behind that.
+#include <math.h>
+
+#include "typed.cuh"
+
+namespace b2 {
+namespace {
+
+// ---- lookup -------------------------------------------------------------------------------------------------------------------
+// tpr threads a row (a power of two up to 256), W elements an access
+template <typename T, typename U, int W>
+__global__ void __launch_bounds__(256) embedding_forward_kernel(U *__restrict__ out, long long ld_out, const T *__restrict__ table, long long ld_table, int vocab,
+                                                                int dim, const int *__restrict__ tokens, long long rows, float scale, int tpr) {
+    const int lane = threadIdx.x & (tpr - 1);
+    const int per_block = 256 / tpr;
+    for (long long r = (long long)blockIdx.x * per_block + threadIdx.x / tpr; r < rows; r += (long long)gridDim.x * per_block) {
+        const int tok = __ldg(tokens + r);
+        U *to = out + r * ld_out;
+        if (tok >= 0 && tok < vocab) {
+            const T *from = table + (long long)tok * ld_table;
+            int c = lane * W;
+            for (; c + 3 * tpr * W < dim; c += 4 * tpr * W) {
+                float v[4][W];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load_vec<T, W>(v[i], from + c + i * tpr * W);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) v[i][j] *= scale;
+                    store_vec<U, W>(to + c + i * tpr * W, v[i]);
+                }
+            }
+            for (; c < dim; c += tpr * W) {
+                float v[W];
+                load_vec<T, W>(v, from + c);
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[j] *= scale;
+                store_vec<U, W>(to + c, v);
+            }
+        } else {
+            // a padding frame is zero; a token beyond the table shows as NaN
+            const float fill = tok < 0 ? 0.0f : nanf("");
+            float v[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] = fill;
+            for (int c = lane * W; c < dim; c += tpr * W) store_vec<U, W>(to + c, v);
+        }
+    }
+}
+
+// ---- sort ---------------------------------------------------------------------------------------------------------------------
+constexpr int MAX_DIGIT_BITS = 9;
+constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32;
+constexpr int SMALL_SORT = 4096;             // tokens one block sorts in shared memory
+
+__device__ __forceinline__ unsigned key_of(int tok, int vocab) { return (tok >= 0 && tok < vocab) ? (unsigned)tok : (unsigned)vocab; }
+
+// How many of the warp's earlier lanes hold the same digit, and whether this lane is the last of them.
+__device__ __forceinline__ unsigned same_digit(unsigned active, unsigned digit) { return __match_any_sync(active, digit); }
+
+// Exclusive prefix sum over n values in shared memory (n <= 16 * SORT_THREADS); all threads of the block call it.
+__device__ __forceinline__ void block_exclusive_scan(unsigned *x, int n, unsigned *warp_tot) {
+    const int per = (n + SORT_THREADS - 1) / SORT_THREADS, a = min(n, (int)threadIdx.x * per), b = min(n, a + per);
+    unsigned s = 0;
+    for (int i = a; i < b; ++i) s += x[i];
+    unsigned inc = s;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    if (lane == 31) warp_tot[w] = inc;
+    __syncthreads();
+    unsigned before = inc - s;
+    for (int i = 0; i < w; ++i) before += warp_tot[i];
+    for (int i = a; i < b; ++i) { const unsigned y = x[i]; x[i] = before; before += y; }
+    __syncthreads();
+}
+
+// All passes for up to SMALL_SORT tokens.  Warp w ranks the keys [w * seg, (w + 1) * seg) in rounds of 32, counts kept per (digit, warp),
+// so equal digits stay in order.
+__global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__restrict__ tokens, int n, int vocab, int passes, int bits, unsigned *__restrict__ keys_out,
+                                                                  int *__restrict__ rows_out, unsigned *__restrict__ present, unsigned *__restrict__ list_count) {
+    extern __shared__ unsigned sm[];
+    unsigned *key[2] = {sm, sm + SMALL_SORT};
+    unsigned short *row[2] = {(unsigned short *)(sm + 2 * SMALL_SORT), (unsigned short *)(sm + 2 * SMALL_SORT) + SMALL_SORT};
+    unsigned *count = sm + 3 * SMALL_SORT;                 // [digits][SORT_WARPS]
+    __shared__ unsigned warp_tot[SORT_WARPS];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, digits = 1 << bits;
+    grid_wait();
+    if (threadIdx.x == 0) *list_count = 0;
+    for (int i = threadIdx.x; i < (vocab + 31) / 32; i += SORT_THREADS) present[i] = 0;
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { key[0][i] = key_of(tokens[i], vocab); row[0][i] = (unsigned short)i; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS)
+        if (key[0][i] < (unsigned)vocab) atomicOr(present + (key[0][i] >> 5), 1u << (key[0][i] & 31));
+    const int seg = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) & ~31;
+    for (int p = 0; p < passes; ++p) {
+        const unsigned *kin = key[p & 1];
+        const unsigned short *rin = row[p & 1];
+        unsigned *kout = key[(p & 1) ^ 1];
+        unsigned short *rout = row[(p & 1) ^ 1];
+        for (int i = threadIdx.x; i < digits * SORT_WARPS; i += SORT_THREADS) count[i] = 0;
+        __syncthreads();
+        unsigned short rank[SMALL_SORT / SORT_THREADS];
+#pragma unroll
+        for (int k = 0; k < SMALL_SORT / SORT_THREADS; ++k) {
+            const int i = w * seg + k * 32 + lane;
+            const bool on = k * 32 < seg && i < n;
+            const unsigned active = __ballot_sync(0xffffffffu, on);
+            if (on) {
+                const unsigned d = (kin[i] >> (p * bits)) & (digits - 1);
+                const unsigned same = same_digit(active, d), c = count[d * SORT_WARPS + w];
+                __syncwarp(active);
+                if (lane == 31 - __clz(same)) count[d * SORT_WARPS + w] = c + __popc(same);
+                rank[k] = (unsigned short)(c + __popc(same & ((1u << lane) - 1)));
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+        block_exclusive_scan(count, digits * SORT_WARPS, warp_tot);
+#pragma unroll
+        for (int k = 0; k < SMALL_SORT / SORT_THREADS; ++k) {
+            const int i = w * seg + k * 32 + lane;
+            if (k * 32 < seg && i < n) {
+                const unsigned d = (kin[i] >> (p * bits)) & (digits - 1), at = count[d * SORT_WARPS + w] + rank[k];
+                kout[at] = kin[i];
+                rout[at] = rin[i];
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { keys_out[i] = key[passes & 1][i]; rows_out[i] = row[passes & 1][i]; }
+    grid_release();
+}
+
+struct SortArgs {
+    const int *tokens;                     // first pass: the keys come from here, the rows are 0, 1, 2, ...
+    const unsigned *kin; const int *rin;   // later passes
+    unsigned *kout; int *rout;
+    unsigned *hist;                        // [tiles][digits]
+    unsigned *present, *list_count;
+    int n, vocab, shift, bits, tiles, tile;
+};
+// rows of the gradient that extra blocks of a launch zero: tokens in [v0, v1) that do not occur
+struct ZeroArgs {
+    void *dtable;
+    long long row_bytes, ld_bytes;
+    const unsigned *present;
+    int v0, v1;
+    int unit;                              // bytes of a store that every row starts and ends on: 16, 4 or 2
+};
+
+__device__ __forceinline__ unsigned sort_key(const SortArgs &a, int i) { return a.tokens ? key_of(a.tokens[i], a.vocab) : a.kin[i]; }
+
+// one warp a row; block `blk` of `blks`
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int blk, int blks) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    for (long long v = (long long)z.v0 + (long long)blk * warps + (threadIdx.x >> 5); v < z.v1; v += (long long)blks * warps) {
+        if (z.present[v >> 5] >> (v & 31) & 1) continue;
+        char *p = (char *)z.dtable + v * z.ld_bytes;
+        if (z.unit == 16)
+            for (long long b = lane * 16; b < z.row_bytes; b += 512) *reinterpret_cast<uint4 *>(p + b) = make_uint4(0, 0, 0, 0);
+        else if (z.unit == 4)
+            for (long long b = lane * 4; b < z.row_bytes; b += 128) *reinterpret_cast<unsigned *>(p + b) = 0;
+        else
+            for (long long b = lane * 2; b < z.row_bytes; b += 64) *reinterpret_cast<unsigned short *>(p + b) = 0;
+    }
+}
+
+// digit counts of every tile; the first pass also notes which tokens occur (their bits were cleared before)
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortArgs a, const ZeroArgs z) {
+    grid_wait();
+    if ((int)blockIdx.x >= a.tiles) { zero_rows(z, blockIdx.x - a.tiles, gridDim.x - a.tiles); return; }
+    extern __shared__ unsigned sm[];
+    const int digits = 1 << a.bits;
+    for (int i = threadIdx.x; i < digits; i += SORT_THREADS) sm[i] = 0;
+    __syncthreads();
+    const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile);
+    for (int i = i0 + threadIdx.x; i < i1; i += SORT_THREADS) {
+        const unsigned k = sort_key(a, i);
+        atomicAdd(sm + ((k >> a.shift) & (digits - 1)), 1u);
+        if (a.tokens && k < (unsigned)a.vocab) atomicOr(a.present + (k >> 5), 1u << (k & 31));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < digits; i += SORT_THREADS) a.hist[(size_t)blockIdx.x * digits + i] = sm[i];
+}
+
+// ranks of a tile's keys and scatter; every block adds up the counts before its own by itself
+__global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const SortArgs a, const ZeroArgs z) {
+    grid_wait();
+    if ((int)blockIdx.x >= a.tiles) { zero_rows(z, blockIdx.x - a.tiles, gridDim.x - a.tiles); return; }
+    extern __shared__ unsigned sm[];
+    __shared__ unsigned warp_tot[SORT_WARPS];
+    const int digits = 1 << a.bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    unsigned *base = sm, *count = sm + digits;             // [digits], [digits][SORT_WARPS]
+    unsigned before = 0;
+    if ((int)threadIdx.x < digits) {
+        unsigned total = 0;
+#pragma unroll 4
+        for (int t = 0; t < a.tiles; ++t) {
+            const unsigned h = a.hist[(size_t)t * digits + threadIdx.x];
+            if (t < (int)blockIdx.x) before += h;
+            total += h;
+        }
+        base[threadIdx.x] = total;
+    }
+    for (int i = threadIdx.x; i < digits * SORT_WARPS; i += SORT_THREADS) count[i] = 0;
+    __syncthreads();
+    block_exclusive_scan(base, digits, warp_tot);
+    if ((int)threadIdx.x < digits) base[threadIdx.x] += before;
+    // counts of every warp's segment of the tile
+    const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile), seg = a.tile / SORT_WARPS;
+    const int s0 = i0 + w * seg, s1 = min(i1, s0 + seg);
+    for (int i = s0 + lane; i < s1; i += 32) atomicAdd(count + ((sort_key(a, i) >> a.shift) & (digits - 1)) * SORT_WARPS + w, 1u);
+    __syncthreads();
+    if ((int)threadIdx.x < digits) {
+        unsigned at = base[threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < SORT_WARPS; ++i) { const unsigned c = count[threadIdx.x * SORT_WARPS + i]; count[threadIdx.x * SORT_WARPS + i] = at; at += c; }
+    }
+    __syncthreads();
+    for (int j = s0; j < s1; j += 32) {
+        const int i = j + lane;
+        const bool on = i < s1;
+        const unsigned active = __ballot_sync(0xffffffffu, on);
+        if (on) {
+            const unsigned k = sort_key(a, i), d = (k >> a.shift) & (digits - 1);
+            const unsigned same = same_digit(active, d), c = count[d * SORT_WARPS + w];
+            __syncwarp(active);
+            if (lane == 31 - __clz(same)) count[d * SORT_WARPS + w] = c + __popc(same);
+            const unsigned at = c + __popc(same & ((1u << lane) - 1));
+            a.kout[at] = k;
+            a.rout[at] = a.tokens ? i : a.rin[i];
+        }
+        __syncwarp();
+    }
+}
+
+// ---- sums ---------------------------------------------------------------------------------------------------------------------
+struct SumArgs {
+    const unsigned *keys; const int *rows;
+    float *partial;                 // [pieces][2][dim_pad]
+    int *list; unsigned *list_count;
+    long long ld_dout, ld_dtable;
+    int n, vocab, dim, dim_pad, piece, pieces, tpr, accumulate;
+    float scale;
+};
+
+template <typename U, int W> __device__ __forceinline__ void put_row(U *to, const float (&s)[W], float scale, int accumulate) {
+    float v[W];
+    if (accumulate) {
+        load_vec<U, W>(v, to);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = fmaf(scale, s[j], v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = scale * s[j];
+    }
+    store_vec<U, W>(to, v);
+}
+
+constexpr int SUM_THREADS = 128;
+
+// A group of tpr threads (a power of two up to SUM_THREADS) takes W * tpr columns of a piece: blockIdx.y counts the column tiles.
+// Blocks beyond the pieces zero absent rows.
+template <typename T, typename U, int W>
+__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks) {
+    grid_wait();
+    if ((int)blockIdx.x >= sum_blocks) { zero_rows(z, blockIdx.x - sum_blocks, gridDim.x - sum_blocks); return; }
+    const int tiles = (a.dim + a.tpr * W - 1) / (a.tpr * W);
+    const int per_block = SUM_THREADS / a.tpr;
+    const long long unit = (long long)blockIdx.x * per_block + threadIdx.x / a.tpr;
+    const int p = (int)(unit / tiles), col = ((int)(unit - (long long)p * tiles) * a.tpr + (threadIdx.x & (a.tpr - 1))) * W;
+    if (p >= a.pieces) return;
+    const int i0 = p * a.piece, i1 = min(a.n, i0 + a.piece);
+    unsigned cur = __ldg(a.keys + i0);
+    if (cur >= (unsigned)a.vocab) return;                  // nothing but padding from here on
+    bool from_before = i0 > 0 && __ldg(a.keys + i0 - 1) == cur;
+    if (col >= a.dim) return;
+    float acc[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+    constexpr int U8 = 8;
+    for (int i = i0; i < i1; i += U8) {
+        float v[U8][W];
+        unsigned k[U8];
+#pragma unroll
+        for (int u = 0; u < U8; ++u) {
+            k[u] = i + u < i1 ? __ldg(a.keys + i + u) : 0xffffffffu;
+            if (k[u] < (unsigned)a.vocab) load_vec<T, W>(v[u], dout + (long long)__ldg(a.rows + i + u) * a.ld_dout + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U8; ++u) {
+            if (k[u] != cur && cur < (unsigned)a.vocab) {
+                // the token is complete here (the end of the piece is handled below)
+                if (i + u < i1) {
+                    if (from_before) store_vec<float, W>(a.partial + (size_t)p * 2 * a.dim_pad + col, acc);
+                    else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+                    from_before = false;
+                    cur = k[u];
+#pragma unroll
+                    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+                }
+            }
+            if (k[u] < (unsigned)a.vocab) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) acc[j] += v[u][j];
+            }
+        }
+    }
+    if (cur >= (unsigned)a.vocab) return;
+    const bool goes_on = i1 < a.n && __ldg(a.keys + i1) == cur;
+    if (from_before) store_vec<float, W>(a.partial + (size_t)p * 2 * a.dim_pad + col, acc);
+    else if (goes_on) {
+        store_vec<float, W>(a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col, acc);
+        if (col == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
+    } else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+}
+
+// Tokens that cross pieces: tail of the first piece plus the heads of those that follow.  A block is 32 column vectors x 8 phases:
+// phase y adds every eighth head, the eight sums are added in fixed order.
+template <typename U, int W>
+__global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dtable, const SumArgs a) {
+    __shared__ float part[8][32][W];
+    grid_wait();
+    const int tiles = (a.dim + 32 * W - 1) / (32 * W);
+    const unsigned n_list = *a.list_count;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    for (long long unit = blockIdx.x; unit < (long long)n_list * tiles; unit += gridDim.x) {
+        const int li = (int)(unit / tiles), p = a.list[li], col = ((int)(unit - (long long)li * tiles) * 32 + x) * W;
+        const unsigned key = __ldg(a.keys + (size_t)(p + 1) * a.piece);
+        float s[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) s[j] = 0.0f;
+        if (col < a.dim) {
+            if (y == 0) load_vec<float, W>(s, a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col);
+            for (int q = p + 1 + y; q < a.pieces && __ldg(a.keys + (size_t)q * a.piece) == key; q += 32) {
+                float v[4][W];
+                bool on[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    on[u] = q + 8 * u < a.pieces && __ldg(a.keys + (size_t)(q + 8 * u) * a.piece) == key;
+                    if (on[u]) load_vec<float, W>(v[u], a.partial + (size_t)(q + 8 * u) * 2 * a.dim_pad + col);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (on[u]) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) s[j] += v[u][j];
+                    }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) part[y][x][j] = s[j];
+        __syncthreads();
+        if (y == 0 && col < a.dim) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) s[j] += part[i][x][j];
+            put_row<U, W>(dtable + (long long)key * a.ld_dtable + col, s, a.scale, a.accumulate);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- plan of a gradient call --------------------------------------------------------------------------------------------------
+struct Plan {
+    int bits, passes, tiles, tile, piece, pieces, dim_pad;
+    size_t present, count, keys[2], rows[2], hist, list, partial, total;   // byte offsets in the workspace
+};
+size_t pad256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+Plan make_plan(long long n, int vocab, int dim) {
+    Plan p;
+    int bits = 1;
+    while (((unsigned)vocab >> bits) != 0) ++bits;                          // keys 0 .. vocab
+    p.passes = (bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    // tiles: as few keys as fill the device, so that a tile's rounds are short; at least 2048
+    long long tile = (n + 147) / 148;
+    tile = tile < 2048 ? 2048 : (tile + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
+    p.tile = (int)tile;
+    p.tiles = (int)((n + tile - 1) / tile);
+    // pieces: few rows give parallel groups, many rows few partial sums
+    p.piece = n <= 4096 ? 8 : n <= 16384 ? 16 : n <= 262144 ? 32 : 64;
+    p.pieces = (int)((n + p.piece - 1) / p.piece);
+    p.dim_pad = (dim + 15) / 16 * 16;
+    size_t at = 0;
+    const auto take = [&at](size_t bytes) { const size_t o = at; at += pad256(bytes); return o; };
+    p.count = take(4);
+    p.present = take(((size_t)vocab + 31) / 32 * 4);
+    p.keys[0] = take((size_t)n * 4); p.keys[1] = take((size_t)n * 4);
+    p.rows[0] = take((size_t)n * 4); p.rows[1] = take((size_t)n * 4);
+    p.hist = take((size_t)p.tiles * (1 << p.bits) * 4);
+    p.list = take((size_t)p.pieces * 4);
+    p.partial = take((size_t)p.pieces * 2 * p.dim_pad * 4);
+    p.total = at;
+    return p;
+}
+
+bool bad_sizes(const char *who, long long n, int vocab, int dim) {
+    if (n < 0 || n > (1ll << 30) || vocab < 1 || vocab > (1 << 27) || dim < 1 || dim > (1 << 20)) {
+        set_error("%s: %lld tokens, %d table rows of %d (at most 2^30, 2^27 and 2^20)", who, n, vocab, dim);
+        return true;
+    }
+    return false;
+}
+
+// the widest access that dim, both leading dimensions and both addresses allow
+int common_width(int most, int dim, const void *a, long long lda, int ea, const void *b, long long ldb, int eb) {
+    for (int w = most; w > 1; w >>= 1) {
+        const size_t ba = (size_t)w * ea < 16 ? (size_t)w * ea : 16, bb = (size_t)w * eb < 16 ? (size_t)w * eb : 16;
+        if (dim % w == 0 && lda % w == 0 && ldb % w == 0 && aligned_to(a, ba) && aligned_to(b, bb)) return w;
+    }
+    return 1;
+}
+
+template <typename T, typename U, int W>
+int forward(U *out, long long ld_out, const T *table, long long ld_table, int vocab, int dim, const int *tokens, long long n, float scale, cudaStream_t st) {
+    // few rows: a thread per vector, so that all loads go out at once; many rows: four vectors a thread
+    const unsigned vecs = (unsigned)((dim + W - 1) / W);
+    const bool few = (double)n * vecs < 148.0 * 2048;
+    unsigned tpr = pow2_at_least(few ? vecs : (vecs + 3) / 4);
+    if (tpr > 256) tpr = 256;
+    const long long per = 256 / tpr, want = (n + per - 1) / per, most = 0x7fffffff;
+    embedding_forward_kernel<T, U, W><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(out, ld_out, table, ld_table, vocab, dim, tokens, n, scale, (int)tpr);
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
+
+template <typename T, typename U, int W>
+int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int zero_blocks, cudaStream_t st) {
+    SumArgs a = base;
+    unsigned tpr = pow2_at_least((unsigned)((a.dim + W - 1) / W));
+    if (tpr > SUM_THREADS) tpr = SUM_THREADS;
+    a.tpr = (int)tpr;
+    const long long tiles = (a.dim + (long long)tpr * W - 1) / ((long long)tpr * W), per = SUM_THREADS / tpr;
+    const long long blocks = (a.pieces * tiles + per - 1) / per;
+    if (blocks + zero_blocks > 0x7fffffffll) { set_error("b2_embedding_backward: %lld blocks", blocks); return B2_ERR_BAD_SHAPE; }
+    B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks));
+    const long long join = (long long)a.pieces * ((a.dim + 32 * W - 1) / (32 * W)), most = sm_count() * 8;
+    return launch_chained(embedding_join_kernel<U, W>, dim3((unsigned)(join < most ? join : most)), dim3(256), 0, st, dtable, a);
+}
+
+template <typename T, typename U>
+int backward(U *dtable, long long ld_dtable, int vocab, int dim, const T *dout, long long ld_dout, const int *tokens, long long n, float scale, bool accumulate,
+             char *ws, cudaStream_t st) {
+    const Plan p = make_plan(n, vocab, dim);
+    unsigned *present = (unsigned *)(ws + p.present), *count = (unsigned *)(ws + p.count), *keys[2] = {(unsigned *)(ws + p.keys[0]), (unsigned *)(ws + p.keys[1])};
+    int *rows[2] = {(int *)(ws + p.rows[0]), (int *)(ws + p.rows[1])};
+    ZeroArgs z = {dtable, (long long)dim * (long long)sizeof(U), ld_dtable * (long long)sizeof(U), present, 0, accumulate ? 0 : vocab, 16};
+    while (z.unit > 2 && (z.row_bytes % z.unit || z.ld_bytes % z.unit || !aligned_to(dtable, z.unit))) z.unit = z.unit == 16 ? 4 : 2;
+    int last = 0;
+    if (n <= SMALL_SORT) {
+        const int smem = (3 * SMALL_SORT + (1 << p.bits) * SORT_WARPS) * 4;
+        B2_TRY(set_max_dynamic_smem((const void *)sort_small_kernel, (3 * SMALL_SORT + (1 << MAX_DIGIT_BITS) * SORT_WARPS) * 4));
+        B2_TRY(launch_chained(sort_small_kernel, dim3(1), dim3(SORT_THREADS), smem, st, tokens, (int)n, vocab, p.passes, p.bits, keys[0], rows[0], present, count));
+    } else {
+        B2_CUDA(cudaMemsetAsync(ws, 0, p.keys[0], st));                   // the list's length and the bits of the tokens that occur
+        // rows that a launch of the sort zeroes besides: about as much as fits under its latency
+        const long long share = (16ll << 20) / (z.row_bytes > 0 ? z.row_bytes : 1);
+        SortArgs a = {tokens, nullptr, nullptr, nullptr, nullptr, (unsigned *)(ws + p.hist), present, count, (int)n, vocab, 0, p.bits, p.tiles, p.tile};
+        const int digits = 1 << p.bits;
+        B2_TRY(set_max_dynamic_smem((const void *)sort_scatter_kernel, (1 + SORT_WARPS) * (1 << MAX_DIGIT_BITS) * 4));
+        const int rest = z.v1;
+        for (int i = 0; i < p.passes; ++i) {
+            a.shift = i * p.bits;
+            a.kout = keys[i & 1]; a.rout = rows[i & 1];
+            for (int half = 0; half < 2; ++half) {
+                ZeroArgs zz = z;
+                zz.v1 = z.v0;
+                if (i || half) zz.v1 = (int)(z.v0 + share < rest ? z.v0 + share : rest);   // the first launch finds out which tokens occur
+                const int zb = zz.v1 > zz.v0 ? 2 * sm_count() : 0;
+                z.v0 = zz.v1;
+                if (half == 0) B2_TRY(launch_chained(sort_count_kernel, dim3(p.tiles + zb), dim3(SORT_THREADS), digits * 4, st, a, zz));
+                else B2_TRY(launch_chained(sort_scatter_kernel, dim3(p.tiles + zb), dim3(SORT_THREADS), digits * (1 + SORT_WARPS) * 4, st, a, zz));
+            }
+            last = i & 1;
+            a.tokens = nullptr;
+            a.kin = a.kout; a.rin = a.rout;
+        }
+    }
+    SumArgs a = {keys[last], rows[last], (float *)(ws + p.partial), (int *)(ws + p.list), count, ld_dout, ld_dtable, (int)n, vocab, dim, p.dim_pad, p.piece, p.pieces,
+                 0, accumulate ? 1 : 0, scale};
+    const long long left = z.v1 - z.v0, zero_blocks = left > 0 ? (left + 3) / 4 < sm_count() * 16ll ? (left + 3) / 4 : sm_count() * 16ll : 0;
+    const int w = common_width(16 / (int)sizeof(T), dim, dout, ld_dout, sizeof(T), dtable, ld_dtable, sizeof(U));
+    if (w == 8) return sums<T, U, (16 / sizeof(T))>(dtable, dout, a, z, (int)zero_blocks, st);
+    if (w >= 4) return sums<T, U, 4>(dtable, dout, a, z, (int)zero_blocks, st);
+    if (w >= 2) return sums<T, U, 2>(dtable, dout, a, z, (int)zero_blocks, st);
+    return sums<T, U, 1>(dtable, dout, a, z, (int)zero_blocks, st);
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_embedding_forward(void *out, int out_type, long long ld_out, const void *table, int table_type, long long ld_table, int vocab, int dim, const int *tokens_dev,
+                         long long n, float scale, b2_stream stream) {
+    if (bad_sizes("b2_embedding_forward", n, vocab, dim)) return B2_ERR_BAD_SHAPE;
+    const int eo = type_size(out_type), et = type_size(table_type);
+    if (!eo || !et) { set_error("b2_embedding_forward: unknown element type (output %d, table %d)", out_type, table_type); return B2_ERR_BAD_ARG; }
+    if (ld_out < dim || ld_table < dim) {
+        set_error("b2_embedding_forward: leading dimension too small (output %lld, table %lld for %d columns)", ld_out, ld_table, dim);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!n) return B2_OK;
+    if (!out || !table || !tokens_dev) { set_error("b2_embedding_forward: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(out, eo) || !aligned_to(table, et) || !aligned_to(tokens_dev, 4)) {
+        set_error("b2_embedding_forward: an address is not aligned to its elements");
+        return B2_ERR_BAD_ARG;
+    }
+    return with_type(table_type, [&](auto *t) {
+        return with_type(out_type, [&](auto *o) {
+            typedef B2_ELEM(t) T;
+            typedef B2_ELEM(o) U;
+            const int w = common_width(16 / (int)sizeof(T), dim, table, ld_table, et, out, ld_out, eo);
+            const auto go = [&](auto width) {
+                return forward<T, U, decltype(width)::value>((U *)out, ld_out, (const T *)table, ld_table, vocab, dim, tokens_dev, n, scale, (cudaStream_t)stream);
+            };
+            if (w == 8) return go(std::integral_constant<int, 16 / (int)sizeof(T)>());
+            if (w >= 4) return go(std::integral_constant<int, 4>());
+            if (w >= 2) return go(std::integral_constant<int, 2>());
+            return go(std::integral_constant<int, 1>());
+        });
+    });
+}
+
+size_t b2_embedding_backward_workspace(long long n, int vocab, int dim) {
+    if (n < 1 || bad_sizes("b2_embedding_backward_workspace", n, vocab, dim)) return 0;
+    return make_plan(n, vocab, dim).total;
+}
+
+int b2_embedding_backward(void *dtable, int dtable_type, long long ld_dtable, int vocab, int dim, const void *dout, int dout_type, long long ld_dout,
+                          const int *tokens_dev, long long n, float scale, int accumulate, void *workspace, size_t workspace_bytes, b2_stream stream) {
+    if (bad_sizes("b2_embedding_backward", n, vocab, dim)) return B2_ERR_BAD_SHAPE;
+    const int et = type_size(dtable_type), ed = type_size(dout_type);
+    if (!et || !ed) { set_error("b2_embedding_backward: unknown element type (table %d, output errors %d)", dtable_type, dout_type); return B2_ERR_BAD_ARG; }
+    if (ld_dtable < dim || ld_dout < dim) {
+        set_error("b2_embedding_backward: leading dimension too small (table %lld, output errors %lld for %d columns)", ld_dtable, ld_dout, dim);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!dtable || !aligned_to(dtable, et)) { set_error("b2_embedding_backward: the table's gradient is missing or not aligned to its elements"); return B2_ERR_BAD_ARG; }
+    if (!n) {
+        if (!accumulate) B2_CUDA(cudaMemset2DAsync(dtable, (size_t)ld_dtable * et, 0, (size_t)dim * et, vocab, (cudaStream_t)stream));
+        return B2_OK;
+    }
+    if (!dout || !tokens_dev || !workspace) { set_error("b2_embedding_backward: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(dout, ed) || !aligned_to(tokens_dev, 4) || !aligned_to(workspace, 256)) {
+        set_error("b2_embedding_backward: an address is not aligned to its elements, or the workspace not to 256 bytes");
+        return B2_ERR_BAD_ARG;
+    }
+    const size_t need = b2_embedding_backward_workspace(n, vocab, dim);
+    if (workspace_bytes < need) { set_error("b2_embedding_backward: %zu bytes of workspace, %zu are needed", workspace_bytes, need); return B2_ERR_BAD_SHAPE; }
+    return with_type(dout_type, [&](auto *d) {
+        return with_type(dtable_type, [&](auto *t) {
+            typedef B2_ELEM(d) T;
+            typedef B2_ELEM(t) U;
+            return backward<T, U>((U *)dtable, ld_dtable, vocab, dim, (const T *)dout, ld_dout, tokens_dev, n, scale, accumulate != 0, (char *)workspace,
+                                  (cudaStream_t)stream);
+        });
+    });
+}
+
+}  // extern "C"

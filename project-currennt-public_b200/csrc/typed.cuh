@@ -1,0 +1,82 @@
+// Element types of the token operators (fp32, bf16, fp16): conversions, 16-byte vectors of them, and what their launches share.
+// Arithmetic is fp32 everywhere; a value is rounded to its type once, when it is stored.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace b2 {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// N elements that are loaded and stored as one naturally aligned access (N * sizeof(T) <= 16), or as several of 16 bytes
+template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec { T v[N]; };
+template <typename T, int N> __device__ __forceinline__ void load_vec(float (&out)[N], const T *p) {
+    const Vec<T, N> x = *reinterpret_cast<const Vec<T, N> *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_float(x.v[i]);
+}
+template <typename T, int N> __device__ __forceinline__ void store_vec(T *p, const float (&in)[N]) {
+    Vec<T, N> x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = from_float<T>(in[i]);
+    *reinterpret_cast<Vec<T, N> *>(p) = x;
+}
+
+inline int type_size(int type) { return type == B2_F32 ? 4 : (type == B2_BF16 || type == B2_F16) ? 2 : 0; }
+inline bool aligned_to(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+inline unsigned pow2_at_least(unsigned x) { unsigned p = 1; while (p < x) p <<= 1; return p; }
+
+// calls f with a null pointer of the element type
+template <typename F> int with_type(int type, F &&f) {
+    switch (type) {
+        case B2_F32: return f((float *)nullptr);
+        case B2_BF16: return f((__nv_bfloat16 *)nullptr);
+        case B2_F16: return f((__half *)nullptr);
+    }
+    set_error("unknown element type %d", type);
+    return B2_ERR_BAD_ARG;
+}
+#define B2_ELEM(p) std::remove_pointer_t<decltype(p)>
+
+// A launch that may start while the kernel before it on the stream drains; the kernel calls grid_wait() before it touches
+// what that one wrote (and before it writes what that one reads).
+template <typename... KArgs, typename... Args>
+int launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    count_launch();
+    B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+    return B2_OK;
+}
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// sums over a warp; every lane gets the result
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+}  // namespace b2

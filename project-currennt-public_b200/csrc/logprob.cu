@@ -75,58 +75,173 @@ template <int N> __device__ __forceinline__ void add_values(Sums &a, const float
     a.e += e;
 }
 
+// ---- vectors of 16 bytes as they were loaded ------------------------------------------------------------------------------------------
+typedef unsigned long long Pair;   // two fp32 values for the packed instructions
+__device__ __forceinline__ Pair pair(float x, float y) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y)); return p; }
+__device__ __forceinline__ float2 halves(Pair p) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    static constexpr unsigned NONE = 0xff800000u;      // -inf in every place of a word
+    static __device__ __forceinline__ void values(float (&z)[4], const uint4 &q) {
+        z[0] = __uint_as_float(q.x); z[1] = __uint_as_float(q.y); z[2] = __uint_as_float(q.z); z[3] = __uint_as_float(q.w);
+    }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ float largest(unsigned a) { return __uint_as_float(a); }
+};
+template <> struct Raw<__nv_bfloat16> {
+    static constexpr unsigned NONE = 0xff80ff80u;
+    static __device__ __forceinline__ float2 two(unsigned a) { return make_float2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)); }
+    static __device__ __forceinline__ void values(float (&z)[8], const uint4 &q) {
+        const float2 a = two(q.x), b = two(q.y), c = two(q.z), d = two(q.w);
+        z[0] = a.x; z[1] = a.y; z[2] = b.x; z[3] = b.y; z[4] = c.x; z[5] = c.y; z[6] = d.x; z[7] = d.y;
+    }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { unsigned y; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b)); return y; }
+    static __device__ __forceinline__ float largest(unsigned a) { const float2 v = two(a); return max_nan(v.x, v.y); }
+};
+template <> struct Raw<__half> {
+    static constexpr unsigned NONE = 0xfc00fc00u;
+    static __device__ __forceinline__ float2 two(unsigned a) { return __half22float2(*reinterpret_cast<const __half2 *>(&a)); }
+    static __device__ __forceinline__ void values(float (&z)[8], const uint4 &q) {
+        const float2 a = two(q.x), b = two(q.y), c = two(q.z), d = two(q.w);
+        z[0] = a.x; z[1] = a.y; z[2] = b.x; z[3] = b.y; z[4] = c.x; z[5] = c.y; z[6] = d.x; z[7] = d.y;
+    }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { unsigned y; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b)); return y; }
+    static __device__ __forceinline__ float largest(unsigned a) { const float2 v = two(a); return max_nan(v.x, v.y); }
+};
+template <typename T> __device__ __forceinline__ unsigned larger_of(const uint4 &q) {
+    typedef Raw<T> R;
+    return R::larger(R::larger(q.x, q.y), R::larger(q.z, q.w));
+}
+// The sums over U vectors of logits x; top: their largest x (NaN if one is NaN).  A pair of entries costs two conversions, one packed maximum
+// (by the caller), two packed FMAs, a packed product and sum, and two exponentials.  Where an entry is -inf the sum of w * d turns NaN and is taken
+// again with the differences held above -inf; SAFE does so at once.
+template <typename T, int U, bool SAFE> __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&q)[U], float top, float scale) {
+    constexpr int W = 16 / sizeof(T);
+    const float m = __fmul_rn(top, scale);
+    if (!(m <= a.m)) {
+        if (a.m != neg_inf()) rescale(a, m); else a = {m, 0.0f, 0.0f};
+    }
+    if (a.m == neg_inf()) return;
+    if (!SAFE) {
+        const Pair sc = pair(scale, scale), mm = pair(-a.m, -a.m), l2 = pair(LOG2E, LOG2E);
+        Pair s = 0, e = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[W];
+            Raw<T>::values(x, q[u]);
+#pragma unroll
+            for (int j = 0; j < W; j += 2) {
+                const Pair d = fma2(pair(x[j], x[j + 1]), sc, mm);
+                const float2 t = halves(mul2(d, l2));
+                const Pair w = pair(ex2(t.x), ex2(t.y));
+                s = add2(s, w);
+                e = fma2(w, d, e);
+            }
+        }
+        const float2 sv = halves(s), ev = halves(e);
+        const float en = ev.x + ev.y;
+        if (en == en) {
+            a.s += sv.x + sv.y;
+            a.e += en;
+            return;
+        }
+    }
+    float s = 0.0f, e = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float x[W];
+        Raw<T>::values(x, q[u]);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const float d = max_nan(fmaf(x[j], scale, -a.m), -3.402823466e38f), w = ex2(d * LOG2E);
+            s += w;
+            e = fmaf(w, d, e);
+        }
+    }
+    a.s += s;
+    a.e += e;
+}
+
 // ---- the K largest ------------------------------------------------------------------------------------------------------------------
 // An entry is one 64-bit key: the value as an ordered integer above, the complement of its index below; larger is better.  0 is no entry.
 typedef unsigned long long Key;
-__device__ __forceinline__ Key make_key(float z, int index) {
+__device__ __forceinline__ unsigned ordered(float z) {
     const unsigned b = __float_as_uint(z + 0.0f);           // -0 counts as 0
-    const unsigned o = z != z ? FULL : (b ^ ((b >> 31) ? FULL : 0x80000000u));
-    return ((Key)o << 32) | (unsigned)~index;
+    return z != z ? FULL : (b ^ ((b >> 31) ? FULL : 0x80000000u));
 }
-__device__ __forceinline__ float key_value(Key k) {
-    const unsigned o = (unsigned)(k >> 32);
-    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : FULL));
-}
+__device__ __forceinline__ float ordered_value(unsigned o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : FULL)); }
+__device__ __forceinline__ Key make_key(float z, int index) { return ((Key)ordered(z) << 32) | (unsigned)~index; }
+__device__ __forceinline__ float key_value(Key k) { return ordered_value((unsigned)(k >> 32)); }
 __device__ __forceinline__ int key_index(Key k) { return (int)~(unsigned)k; }
 
 // Lane l holds the l-th best of the warp, descending.  A value is of interest if it is not below `limit` (the K-th best, or a bound known
-// from elsewhere) and above `floor`: the K-th best of what came before the current vectors, whose indices are all lower, so that an
-// equal value loses against it.
+// from elsewhere) and above `floor`: the K-th best of the batches before the current one, whose indices are all lower, so that an equal
+// value loses against it.
 struct TopList {
-    Key key;
+    Key key, last;     // last: the K-th entry, the same in all lanes
     float limit, floor;
-    __device__ __forceinline__ void clear() { key = 0; limit = floor = neg_inf(); }
+    __device__ __forceinline__ void clear() { key = last = 0; limit = floor = neg_inf(); }
     __device__ __forceinline__ bool wants(float z) const { return !(z < limit) && !(z <= floor); }
     __device__ __forceinline__ void insert(Key k, int K) {
         const int lane = threadIdx.x & 31;
         const int pos = __popc(__ballot_sync(FULL, key > k));
         const Key up = __shfl_up_sync(FULL, key, 1);
         if (lane >= pos) key = lane == pos ? k : up;
-        const Key last = __shfl_sync(FULL, key, K - 1);
-        if (last) limit = key_value(last);
+        last = __shfl_sync(FULL, key, K - 1);
+        if (last) limit = fmaxf(limit, key_value(last));
     }
-    __device__ __forceinline__ void settle(int K) {
-        const Key last = __shfl_sync(FULL, key, K - 1);
-        if (last) floor = key_value(last);
-    }
+    __device__ __forceinline__ void settle() { if (last) floor = key_value(last); }
 };
-// Offers every lane's N values of the indices at, at + step, ...
-template <int N> __device__ __forceinline__ void offer(TopList &t, const float (&z)[N], int at, int step, int K) {
+// Offers N values of every lane, those of value i at the indices at + i * 32 over the lanes.
+template <int N> __device__ __forceinline__ void offer(TopList &t, const float (&z)[N], int at, int K) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         unsigned who = __ballot_sync(FULL, t.wants(z[i]));
         while (who) {
             const int src = __ffs(who) - 1;
-            const Key k = make_key(__shfl_sync(FULL, z[i], src), __shfl_sync(FULL, at + i * step, src));
-            if (k > __shfl_sync(FULL, t.key, K - 1)) t.insert(k, K);
+            const Key k = make_key(__shfl_sync(FULL, z[i], src), at + i * 32 + src);
+            if (k > t.last) t.insert(k, K);
             who &= who - 1;
             who &= __ballot_sync(FULL, t.wants(z[i]));
         }
     }
-    t.settle(K);
 }
-// The K-th largest of the 32 lanes' values: a bound that at least K values of the warp reach.
-__device__ __forceinline__ float kth_of_lanes(float v, int K) {
+// Offers a batch of U vectors a lane, vector u of lane l at the indices at + (u * step + l) * W ...; top: the lane's largest logit.  A lane that
+// has a candidate lays its vectors down in `spread`, and every lane looks at one entry (U * W <= 32).
+template <typename T, int U>
+__device__ __forceinline__ void offer_vectors(TopList &t, const uint4 (&q)[U], float top, float scale, int at, int step, uint4 *spread, int K) {
+    constexpr int W = 16 / sizeof(T);
+    static_assert(U * W <= 32, "an entry a lane");
+    const int lane = threadIdx.x & 31;
+    const float ztop = __fmul_rn(top, scale);
+    unsigned who = __ballot_sync(FULL, t.wants(ztop));
+    while (who) {
+        const int src = __ffs(who) - 1;
+        if (lane == src)
+#pragma unroll
+            for (int u = 0; u < U; ++u) spread[u] = q[u];
+        __syncwarp();
+        const float z = lane < U * W ? __fmul_rn(to_float(reinterpret_cast<const T *>(spread)[lane]), scale) : neg_inf();
+        __syncwarp();
+        unsigned which = __ballot_sync(FULL, t.wants(z));
+        while (which) {
+            const int e = __ffs(which) - 1;
+            const Key k = make_key(__shfl_sync(FULL, z, e), at + (e / W * step + src) * W + e % W);
+            if (k > t.last) t.insert(k, K);
+            which &= which - 1;
+            which &= __ballot_sync(FULL, t.wants(z));
+        }
+        who &= who - 1;
+        who &= __ballot_sync(FULL, t.wants(ztop));
+    }
+    t.settle();
+}
+// The 32 lanes' values in descending order (NaN counts as +inf): at least k + 1 values of the warp reach that of lane k.
+__device__ __forceinline__ float sort_lanes(float v) {
     const int lane = threadIdx.x & 31;
     if (v != v) v = __int_as_float(0x7f800000);
 #pragma unroll
@@ -137,22 +252,24 @@ __device__ __forceinline__ float kth_of_lanes(float v, int K) {
             const bool desc = (lane & k) == 0, low = (lane & j) == 0;
             v = (desc == low) ? fmaxf(v, o) : fminf(v, o);
         }
-    return __shfl_sync(FULL, v, K - 1);
+    return v;
 }
-// Lane l, if `have`, holds a list of K keys (descending, 0 behind the last): the best K of all lists, lane k the k-th.
-__device__ __forceinline__ Key merge_lists(const Key *list, int K, bool have) {
-    const int lane = threadIdx.x & 31;
-    int at = 0;
-    Key head = have ? list[0] : 0, mine = 0;
-    for (int k = 0; k < K; ++k) {
-        const unsigned hi = __reduce_max_sync(FULL, (unsigned)(head >> 32));
-        if (!hi) break;
-        const unsigned lo = __reduce_max_sync(FULL, (unsigned)(head >> 32) == hi ? (unsigned)head : 0u);
-        const Key best = ((Key)hi << 32) | lo;
-        if (head == best) { ++at; head = at < K ? list[at] : 0; }
-        if (lane == k) mine = best;
-    }
-    return mine;
+// The best K of N lists, put in order into out.  Every list holds 32 keys, descending, 0 behind the last; thread (warp l, lane j) brings key j
+// of list l.  A key's place is the number of larger keys, found by bisection in every list.  out holds zeros before; the caller's
+// barriers stand before and behind.
+template <int N> __device__ __forceinline__ void join_lists(Key *out, const Key (*lists)[MAX_TOP], Key mine, int K) {
+    if (!mine) return;
+    int at[N];
+#pragma unroll
+    for (int l = 0; l < N; ++l) at[l] = 0;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+        for (int l = 0; l < N; ++l) at[l] += lists[l][at[l] + s - 1] > mine ? s : 0;
+    int place = 0;
+#pragma unroll
+    for (int l = 0; l < N; ++l) place += at[l] + (lists[l][31] > mine);
+    if (place < K) out[place] = mine;
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------
@@ -236,24 +353,65 @@ template <typename T, int NV> __global__ void __launch_bounds__(256) logprob_war
         ls = __shfl_sync(FULL, ls, 0);
         TopList best;
         best.clear();
-        best.limit = kth_of_lanes(top, a.top);
-        offer<NV>(best, z, lane, 32, a.top);
+        best.limit = __shfl_sync(FULL, sort_lanes(top), a.top - 1);
+        offer<NV>(best, z, 0, a.top);
         write_top(a, r, best.key, t, ls);
     }
 }
 
+// Several rows a warp, for rows of which no alternatives are asked: G lanes a row, NV entries a lane.  The reductions and the row's closing
+// arithmetic then serve 32 / G rows at once; they are as much work as 100 entries.
+template <typename T, int G, int NV> __global__ void __launch_bounds__(256) logprob_rows_kernel(const T *__restrict__ logits, const FwdArgs a) {
+    const int lane = threadIdx.x & (G - 1);
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+    const bool real = r < a.rows;
+    const T *x = logits + (real ? r : 0) * a.ld;
+    float z[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) z[i] = lane + G * i < a.vocab ? to_float(x[lane + G * i]) : neg_inf();
+    Given g = {-1, 0.0f};
+    if (real && lane == 0) g = load_given(a, r, x);
+    if (a.mask) {
+        const unsigned char *mk = a.mask + (real ? r : 0) * a.ld_mask;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + G * i < a.vocab && !mk[lane + G * i]) z[i] = neg_inf();
+    }
+    float top = neg_inf();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        z[i] = __fmul_rn(z[i], a.scale);
+        top = max_nan(top, z[i]);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(FULL, top, o));
+    Sums t = {neg_inf(), 0.0f, 0.0f};
+    add_values<NV>(t, z, top);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+        t.s += __shfl_xor_sync(FULL, t.s, o);
+        t.e += __shfl_xor_sync(FULL, t.e, o);
+    }
+    if (real && lane == 0) write_row(a, r, g, t);
+}
+
 // blocks_per_row blocks a row (a thread-block cluster where there are several).  Entries are taken in vectors of W = 16 bytes from the
-// 16-byte boundary at or below the row's start, U vectors a thread and batch.
+// 16-byte boundary at or below the row's start, U vectors a thread and batch; the next batch is on its way while one is worked on.
 template <typename T, int THREADS, bool TOP, bool MASK>
-__global__ void __launch_bounds__(THREADS) logprob_row_kernel(const T *__restrict__ logits, const FwdArgs a, int blocks_per_row) {
-    constexpr int W = 16 / sizeof(T), U = 4, WARPS = THREADS / 32, MOST = 16;
+__global__ void __launch_bounds__(THREADS, 640 / THREADS) logprob_row_kernel(const T *__restrict__ logits, const FwdArgs a, int blocks_per_row) {
+    constexpr int W = 16 / sizeof(T), U = 4, WARPS = THREADS / 32, MOST = 8;
     __shared__ Sums sums[WARPS], all_sums[MOST];
-    __shared__ Key lists[WARPS][MAX_TOP], all_lists[MOST][MAX_TOP];
+    __shared__ Key lists[WARPS][MAX_TOP], all_lists[MOST][MAX_TOP], joined[3][MAX_TOP];
+    __shared__ uint4 spread[WARPS][U];
+    __shared__ unsigned block_limit;                         // the highest limit of the block's warps, as an ordered integer
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const long long r = blockIdx.x / (unsigned)blocks_per_row;
     const int part = (int)(blockIdx.x % (unsigned)blocks_per_row);
     // the first block's shared memory may be written once that block runs: arrive here, wait before the write
-    if (blocks_per_row > 1) cg::this_cluster().barrier_arrive();
+    if (blocks_per_row > 1) {
+        if (TOP && w < MOST) all_lists[w][lane] = 0;         // a cluster has 8 warps a block
+        cg::this_cluster().barrier_arrive();
+    }
     const T *x = logits + r * a.ld;
     const unsigned char *mk = MASK ? a.mask + r * a.ld_mask : nullptr;
     const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
@@ -261,85 +419,125 @@ __global__ void __launch_bounds__(THREADS) logprob_row_kernel(const T *__restric
     const int end = mis + a.vocab, vecs = (end + W - 1) / W; // vector v holds the entries v * W - mis ...
     const int v0 = (int)((long long)vecs * part / blocks_per_row), v1 = (int)((long long)vecs * (part + 1) / blocks_per_row);
     const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
-    Given g = {-1, 0.0f};
-    if (part == 0 && threadIdx.x == 0) g = load_given(a, r, x);
-    Sums t = {neg_inf(), 0.0f, 0.0f};
-    TopList best;
-    best.clear();
-    for (int b = v0 + w * 32; b < v1; b += THREADS * U) {
-        float z[U * W];
+    typedef Vec<unsigned char, W> Allowed;
+    const auto load = [&](uint4 (&q)[U], Allowed (&on)[U], int b) {
         const int last = b + THREADS * (U - 1) + 32;         // one behind the batch's last vector
         if ((b > 0 || mis == 0) && last <= v1 && last * W <= end) {
-            float q[U][W];
 #pragma unroll
-            for (int u = 0; u < U; ++u) load_vec<T, W>(q[u], base + (size_t)(b + u * THREADS + lane) * W);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < W; ++j) z[u * W + j] = q[u][j];
+            for (int u = 0; u < U; ++u) q[u] = __ldg(reinterpret_cast<const uint4 *>(base + (size_t)(b + u * THREADS + lane) * W));
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int v = b + u * THREADS + lane;
-                float q[W];
+                q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+                if (v >= v1) continue;
+                if (v * W >= mis && (v + 1) * W <= end) q[u] = __ldg(reinterpret_cast<const uint4 *>(base + (size_t)v * W));
+                else {
+                    Vec<T, W> part_of = *reinterpret_cast<const Vec<T, W> *>(&q[u]);
 #pragma unroll
-                for (int j = 0; j < W; ++j) q[j] = neg_inf();
-                if (v < v1) {
-                    if (v * W >= mis && (v + 1) * W <= end) load_vec<T, W>(q, base + (size_t)v * W);
-                    else
-#pragma unroll
-                        for (int j = 0; j < W; ++j)
-                            if (v * W + j >= mis && v * W + j < end) q[j] = to_float(base[v * W + j]);
+                    for (int j = 0; j < W; ++j)
+                        if (v * W + j >= mis && v * W + j < end) part_of.v[j] = base[v * W + j];
+                    q[u] = *reinterpret_cast<const uint4 *>(&part_of);
                 }
-#pragma unroll
-                for (int j = 0; j < W; ++j) z[u * W + j] = q[j];
             }
         }
         if (MASK) {
+            if (mask_vec && (b > 0 || mis == 0) && last <= v1 && last * W <= end) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int v = b + u * THREADS + lane;
-                Vec<unsigned char, W> on;
-                if (v < v1 && mask_vec && v * W >= mis && (v + 1) * W <= end) on = *reinterpret_cast<const Vec<unsigned char, W> *>(mk - mis + v * W);
-                else
+                for (int u = 0; u < U; ++u) on[u] = *reinterpret_cast<const Allowed *>(mk - mis + (b + u * THREADS + lane) * W);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) on.v[j] = v < v1 && v * W + j >= mis && v * W + j < end ? mk[v * W + j - mis] : 0;
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < W; ++j)
-                    if (!on.v[j]) z[u * W + j] = neg_inf();
+                    for (int j = 0; j < W; ++j) {
+                        const int v = b + u * THREADS + lane, i = v * W + j;
+                        on[u].v[j] = v < v1 && i >= mis && i < end ? mk[i - mis] : 0;
+                    }
             }
         }
-        float top = neg_inf();
+    };
+    const auto rule_out = [&](uint4 (&q)[U], const Allowed (&on)[U]) {
 #pragma unroll
-        for (int i = 0; i < U * W; ++i) {
-            z[i] = __fmul_rn(z[i], a.scale);
-            top = max_nan(top, z[i]);
+        for (int u = 0; u < U; ++u) {
+            unsigned *word = reinterpret_cast<unsigned *>(&q[u]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const unsigned place = sizeof(T) == 4 ? FULL : 0xffffu << (16 * (j & 1));
+                if (!on[u].v[j]) word[j * (int)sizeof(T) / 4] = (word[j * (int)sizeof(T) / 4] & ~place) | (Raw<T>::NONE & place);
+            }
         }
-        add_values<U * W>(t, z, top);
+    };
+    Given g = {-1, 0.0f};
+    Sums t = {neg_inf(), 0.0f, 0.0f};
+    TopList best;
+    best.clear();
+    uint4 now[U], next[U];
+    Allowed on[U], on_next[U];
+    int b = v0 + w * 32;
+    if (b < v1) load(now, on, b);
+    if (part == 0 && threadIdx.x == 0) g = load_given(a, r, x);
+    const auto largest = [&](const uint4 (&q)[U]) {
+        unsigned most = larger_of<T>(q[0]);
+#pragma unroll
+        for (int u = 1; u < U; ++u) most = Raw<T>::larger(most, larger_of<T>(q[u]));
+        return Raw<T>::largest(most);
+    };
+    const auto post = [&](float limit) {
+        if (lane == 0 && limit > neg_inf()) atomicMax(&block_limit, ordered(limit));
+    };
+    if (TOP) {
+        // a bound from the first batches, so that the lists do not fill up with what will not stay: the K-th largest of all lanes' maxima
+        if (MASK && b < v1) rule_out(now, on);
+        const float most = sort_lanes(b < v1 ? __fmul_rn(largest(now), a.scale) : neg_inf());
+        if (WARPS == 1) best.limit = __shfl_sync(FULL, most, a.top - 1);
+        else {
+            const Key key = lane < a.top ? make_key(most, w * 32 + lane) : 0;
+            lists[w][lane] = key;
+            if (w < 3) joined[w][lane] = 0;
+            if (threadIdx.x == 0) block_limit = 0;
+            __syncthreads();
+            join_lists<WARPS>(joined[0], lists, key, a.top);
+            __syncthreads();
+            best.limit = key_value(joined[0][a.top - 1]);
+        }
+    }
+    for (; b < v1; b += THREADS * U) {
+        if (b + THREADS * U < v1) load(next, on_next, b + THREADS * U);
+        if (MASK) rule_out(now, on);
+        const float top = largest(now);
+        add_vectors<T, U, MASK>(t, now, top, a.scale);
         if (TOP) {
-            if (best.limit == neg_inf()) best.limit = kth_of_lanes(top, a.top);
-            if (__any_sync(FULL, best.wants(top))) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    float q[W];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) q[j] = z[u * W + j];
-                    offer<W>(best, q, (b + u * THREADS + lane) * W - mis, 1, a.top);
-                }
+            if (WARPS > 1) {
+                const unsigned known = *(volatile unsigned *)&block_limit;
+                if (known) best.limit = fmaxf(best.limit, ordered_value(known));
             }
+            if (__any_sync(FULL, best.wants(__fmul_rn(top, a.scale)))) {
+                offer_vectors<T, U>(best, now, top, a.scale, b * W - mis, THREADS, spread[w], a.top);
+                if (WARPS > 1) post(best.limit);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            now[u] = next[u];
+            if (MASK) on[u] = on_next[u];
         }
     }
     t = warp_merge(t);
-    if (lane == 0) sums[w] = t;
-    if (TOP) lists[w][lane] = best.key;
-    __syncthreads();
-    // the first warp joins the block's warps, then that of the first block the row's blocks
-    Key k = 0;
-    if (w == 0) {
-        t = warp_merge(lane < WARPS ? sums[lane] : Sums{neg_inf(), 0.0f, 0.0f});
-        if (TOP) k = merge_lists(lists[lane < WARPS ? lane : 0], a.top, lane < WARPS);
+    Key k = best.key;
+    if (WARPS > 1) {
+        if (lane == 0) sums[w] = t;
+        if (lane >= a.top) k = 0;
+        if (TOP) lists[w][lane] = k;
+        __syncthreads();
+        if (w == 0) t = warp_merge(lane < WARPS ? sums[lane] : Sums{neg_inf(), 0.0f, 0.0f});
+        if (TOP) {
+            join_lists<WARPS>(joined[1], lists, k, a.top);
+            __syncthreads();
+            k = joined[1][lane];
+        }
     }
     if (blocks_per_row > 1) {
+        // the row's blocks hand over to the first
         cg::cluster_group cluster = cg::this_cluster();
         cluster.barrier_wait();
         if (w == 0) {
@@ -348,9 +546,11 @@ __global__ void __launch_bounds__(THREADS) logprob_row_kernel(const T *__restric
         }
         cluster.sync();
         if (part != 0) return;
-        if (w == 0) {
-            t = warp_merge(lane < blocks_per_row ? all_sums[lane] : Sums{neg_inf(), 0.0f, 0.0f});
-            if (TOP) k = merge_lists(all_lists[lane < blocks_per_row ? lane : 0], a.top, lane < blocks_per_row);
+        if (w == 0) t = warp_merge(lane < blocks_per_row ? all_sums[lane] : Sums{neg_inf(), 0.0f, 0.0f});
+        if (TOP) {
+            if (w < blocks_per_row) join_lists<MOST>(joined[2], all_lists, all_lists[w][lane], a.top);
+            __syncthreads();
+            k = joined[2][lane];
         }
     }
     if (w == 0) {
@@ -360,15 +560,15 @@ __global__ void __launch_bounds__(THREADS) logprob_row_kernel(const T *__restric
     }
 }
 
-template <typename T, bool TOP, bool MASK> int launch_rows(const T *logits, const FwdArgs &a, cudaStream_t st) {
+template <typename T, int THREADS, bool TOP, bool MASK> int launch_rows(const T *logits, const FwdArgs &a, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
-    // few rows: several blocks a row, as long as each has at least a batch of 256 threads
+    // few rows: several blocks a row, as long as each has at least a batch
     int per_row = 1;
-    while (per_row < 8 && a.rows * per_row * 2 <= 2 * sm_count() && (a.vocab / (per_row * 2)) >= 256 * 4 * W) per_row *= 2;
+    while (THREADS == 256 && per_row < 8 && a.rows * per_row * 2 <= 2 * sm_count() && (a.vocab / (per_row * 2)) >= THREADS * 4 * W) per_row *= 2;
     if (a.rows * per_row > 0x7fffffffll) { set_error("b2_logprob_forward: %lld rows", a.rows); return B2_ERR_BAD_SHAPE; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * per_row));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -377,11 +577,26 @@ template <typename T, bool TOP, bool MASK> int launch_rows(const T *logits, cons
     cfg.attrs = at;
     cfg.numAttrs = per_row > 1 ? 1 : 0;
     count_launch();
-    B2_CUDA(cudaLaunchKernelEx(&cfg, logprob_row_kernel<T, 256, TOP, MASK>, logits, a, per_row));
+    B2_CUDA(cudaLaunchKernelEx(&cfg, logprob_row_kernel<T, THREADS, TOP, MASK>, logits, a, per_row));
     return B2_OK;
 }
 
 template <typename T> int forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    if (a.vocab <= 1024 && !a.top) {
+        const auto go = [&](auto kernel, int lanes) -> int {
+            const long long blocks = (a.rows * lanes + 255) / 256;
+            if (blocks > 0x7fffffffll) { set_error("b2_logprob_forward: %lld rows", a.rows); return B2_ERR_BAD_SHAPE; }
+            kernel<<<(unsigned)blocks, 256, 0, st>>>(logits, a);
+            count_launch();
+            B2_CUDA(cudaGetLastError());
+            return B2_OK;
+        };
+        if (a.vocab <= 4 * 20) return go(logprob_rows_kernel<T, 4, 20>, 4);
+        if (a.vocab <= 4 * 36) return go(logprob_rows_kernel<T, 4, 36>, 4);
+        if (a.vocab <= 8 * 36) return go(logprob_rows_kernel<T, 8, 36>, 8);
+        if (a.vocab <= 16 * 36) return go(logprob_rows_kernel<T, 16, 36>, 16);
+        return go(logprob_rows_kernel<T, 32, 32>, 32);
+    }
     if (a.vocab <= 1024) {
         const long long blocks = (a.rows + 7) / 8;
         if (blocks > 0x7fffffffll) { set_error("b2_logprob_forward: %lld rows", a.rows); return B2_ERR_BAD_SHAPE; }
@@ -394,8 +609,16 @@ template <typename T> int forward(const T *logits, const FwdArgs &a, cudaStream_
         B2_CUDA(cudaGetLastError());
         return B2_OK;
     }
-    if (a.top) return a.mask ? launch_rows<T, true, true>(logits, a, st) : launch_rows<T, true, false>(logits, a, st);
-    return a.mask ? launch_rows<T, false, true>(logits, a, st) : launch_rows<T, false, false>(logits, a, st);
+    // What a warp does once a row (its first list, the joins) is the less the fewer warps a row has: one where the rows alone fill the device
+    // (8192 rows of 50001: 175 us, with four warps 251 us), four for some rows (1200 rows of 200000: 119 us, with one warp 153 us)
+    const auto go = [&](auto threads) -> int {
+        constexpr int N = decltype(threads)::value;
+        if (a.top) return a.mask ? launch_rows<T, N, true, true>(logits, a, st) : launch_rows<T, N, true, false>(logits, a, st);
+        return a.mask ? launch_rows<T, N, false, true>(logits, a, st) : launch_rows<T, N, false, false>(logits, a, st);
+    };
+    if (a.rows >= 16 * sm_count()) return go(std::integral_constant<int, 32>());
+    if (a.rows >= 4 * sm_count()) return go(std::integral_constant<int, 128>());
+    return go(std::integral_constant<int, 256>());
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------

@@ -35,31 +35,40 @@ struct NormArgs {
     float eps, a, inv_dim;
 };
 
-// sums over the threads of a row: a warp, or all warps of the block (buffers alternate, so one barrier a sum is enough)
-template <int N> __device__ __forceinline__ void row_sums(float (&x)[N], int warps, float (*red)[N], int &phase) {
+// Sums over the threads of a row: a warp, or all warps of the block (buffers alternate, so one barrier a sum is enough).  red holds 2 * N * 32
+// floats; those of warps that are not there are zero.
+template <int N> __device__ __forceinline__ void row_sums(float (&x)[N], int warps, float4 (*red)[8], int &phase) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = warp_sum(x[i]);
     if (warps == 1) return;
-    float(*buf)[N] = red + (phase & 1) * 32;
+    float4(*buf)[8] = red + (phase & 1) * N;
     ++phase;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-        for (int i = 0; i < N; ++i) buf[threadIdx.x >> 5][i] = x[i];
+        for (int i = 0; i < N; ++i) reinterpret_cast<float *>(buf[i])[threadIdx.x >> 5] = x[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float y = (int)(threadIdx.x & 31) < warps ? buf[threadIdx.x & 31][i] : 0.0f;
-        x[i] = warp_sum(y);
+        float4 s = buf[i][0];
+        for (int k = 1; k < (warps + 3) >> 2; ++k) {
+            const float4 y = buf[i][k];
+            s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
+        }
+        x[i] = (s.x + s.y) + (s.z + s.w);
     }
+}
+__device__ __forceinline__ void clear_sums(float4 *red, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) red[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
 }
 
 // columns of a thread: vector i starts at column (i * tpr + lane) * W
-template <typename T, int W, int NV> struct Cols {
+template <typename T, int W, int NV, bool FULL = false> struct Cols {
     static __device__ __forceinline__ void load(float (&v)[NV][W], const T *row, int tpr, int lane, int dim, float other) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * tpr + lane) * W;
-            if (c < dim) load_vec<T, W>(v[i], row + c);
+            if (FULL || c < dim) load_vec<T, W>(v[i], row + c);
             else
 #pragma unroll
                 for (int j = 0; j < W; ++j) v[i][j] = other;
@@ -69,14 +78,14 @@ template <typename T, int W, int NV> struct Cols {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * tpr + lane) * W;
-            if (c < dim) store_vec<T, W>(row + c, v[i]);
+            if (FULL || c < dim) store_vec<T, W>(row + c, v[i]);
         }
     }
 };
 
 // v becomes its normalised self; columns beyond dim are zero before and stay so
 template <int W, int NV>
-__device__ __forceinline__ void normalise(float (&v)[NV][W], const NormArgs &a, int tpr, int lane, int warps, float (*red)[1], int &phase, float &mean, float &rstd) {
+__device__ __forceinline__ void normalise(float (&v)[NV][W], const NormArgs &a, int tpr, int lane, int warps, float4 (*red)[8], int &phase, float &mean, float &rstd) {
     float s[1] = {0.0f};
     mean = 0.0f;
     if (a.layer_norm) {
@@ -127,10 +136,11 @@ template <int W, int NV> __device__ __forceinline__ void affine(float (&v)[NV][W
 template <typename T, int W, int NV>
 __global__ void __launch_bounds__(NV == 8 ? 1024 : 512) block_norm_forward_kernel(const NormArgs a, const T *x, long long ld_x, const T *f, long long ld_f, T *y,
                                                                                   long long ld_y, T *h, long long ld_h, int tpr) {
-    __shared__ float red[64][1];
+    __shared__ float4 red[2][8];
     const int warps = tpr >> 5, lane = warps == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const long long r = warps == 1 ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     if (r >= a.rows) return;
+    if (warps > 1) clear_sums(red[0], 16);
     int phase = 0;
     typedef Cols<T, W, NV> C;
     float v[NV][W], n[NV][W];
@@ -170,140 +180,267 @@ __global__ void __launch_bounds__(NV == 8 ? 1024 : 512) block_norm_forward_kerne
 }
 
 struct BackArgs {
-    long long ld_dx, ld_df, ld_dy, ld_dh, ld_y, ld_f, ld_dgate;
+    unsigned ld_dx, ld_df, ld_dy, ld_dh, ld_y, ld_f, ld_dgate;
     void *dgate;
     float *partial;                   // [blocks][4][dim_pad]: dw1, db1, dw2, db2 of every block
     float *partial_gate;              // [workers][dim_pad], where several workers share a row of the gate
     int dim_pad, per_group, groups_at_once;
 };
 
+// Copies of 16 bytes (the first `bytes` of them, zeros behind) into shared memory that nobody waits for before cp_wait
+__device__ __forceinline__ void cp_async(unsigned to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async(unsigned to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most n (0 to 2) of the newest groups are under way
+__device__ __forceinline__ void cp_wait(int n) {
+    if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+
+// The rows a worker takes, one after another: rows member, member + per_group, ... of the R frames that share a row of the gate, for every
+// such group of the worker.
+struct RowWalk {
+    int g, m, G, R, member, per_group, groups;
+    __device__ __forceinline__ bool ended() const { return g >= G; }
+    __device__ __forceinline__ unsigned row() const { return (unsigned)m * (unsigned)G + (unsigned)g; }
+    __device__ __forceinline__ bool last_of_group() const { return (long long)m + per_group >= R; }
+    __device__ __forceinline__ void next() {
+        if (last_of_group()) { m = member; g = groups < G - g ? g + groups : G; } else m += per_group;
+    }
+};
+
+// Stores a thread's columns, held as pairs
+template <int W, int NV, bool FULL> struct Out {
+    int tpr, lane, dim;
+    template <typename T> __device__ __forceinline__ void operator()(T *to, const Pair (&v)[NV * W / 2]) const {
+        float q[NV][W];
+#pragma unroll
+        for (int n = 0; n < NV * W / 2; ++n) {
+            const float2 x = halves(v[n]);
+            q[2 * n / W][2 * n % W] = x.x;
+            q[(2 * n + 1) / W][(2 * n + 1) % W] = x.y;
+        }
+        Cols<T, W, NV, FULL>::store(to, q, tpr, lane, dim);
+    }
+};
+
 // A worker is a warp (tpr = 32) or a block.  per_group workers share a row of the gate (all workers, if there is one row or none), and
-// groups_at_once rows of the gate are worked on side by side.
-// BIAS: means are subtracted or the norms have a bias (without both, sums are saved).
-template <typename T, int W, int NV, int MAXT, bool BIAS>
-__global__ void __launch_bounds__(MAXT) block_norm_backward_kernel(const NormArgs a, const BackArgs k, T *dx, T *df, const T *dy, const T *dh, const T *y, const T *f, int tpr) {
-    constexpr int S = BIAS ? 2 : 1;
-    __shared__ float red[64][S];
-    extern __shared__ __align__(16) float join[];   // [warps][32 * W * NV], tpr = 32 only
-    typedef Cols<T, W, NV> C;
+// groups_at_once rows of the gate are worked on side by side.  BIAS: means are subtracted or the norms have a bias (without both, sums are saved).
+// FULL: dy, dh, f, dx and df are all there and the threads' columns are just the row's: a third of the instructions were tests of that.
+// The next `stages` - 1 rows are on their way into shared memory while one is worked on: what a row's two sums over the threads leave idle
+// would otherwise be the memory.  With whole vectors a thread copies the vectors that it will read; rows that start anywhere (W = 1) are
+// copied as the 16-byte pieces that hold them, by all their threads, and read element by element, so that loads and stores stay coalesced.
+template <typename T, int W, int NV, int MAXT, bool BIAS, bool FULL>
+__global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) block_norm_backward_kernel(const NormArgs a, const BackArgs k, T *dx, T *df, const T *dy, const T *dh, const T *y,
+                                                                                        const T *f, int tpr, int stages) {
+    constexpr int S = BIAS ? 2 : 1, N = NV * W, H = N / 2;   // a thread's columns, as pairs
+    constexpr bool KEEP = MAXT <= 256 && !BIAS;         // the weights stay in registers
+    __shared__ float4 red[2 * S][8];
+    extern __shared__ __align__(16) char ring[];
     const int warps = tpr >> 5, lane = warps == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const long long worker = warps == 1 ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    const long long G = a.gate_rows > 0 ? a.gate_rows : 1, R = a.rows / G;
+    const int worker = warps == 1 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const int G = a.gate_rows > 0 ? (int)a.gate_rows : 1;
+    clear_sums(red[0], 2 * S * 8);
     int phase = 0;
-    float w1[NV][W], w2[NV][W], b2[NV][W];
-    float s_w1[NV][W], s_b1[NV][W], s_w2[NV][W], s_b2[NV][W], s_g[NV][W];
+    const auto column = [&](int i) { return (i * tpr + lane) * W; };   // of vector i
+    const auto weights = [&](Pair (&v)[H], const float *w) {
+        float q[NV][W];
+        Cols<float, W, NV, FULL>::load(q, w, tpr, lane, a.dim, 0.0f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int n = 0; n < H; ++n) v[n] = pair(q[2 * n / W][2 * n % W], q[(2 * n + 1) / W][(2 * n + 1) % W]);
+    };
+    const auto fill = [](Pair (&v)[H], float x) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            w1[i][j] = w2[i][j] = 1.0f;
-            b2[i][j] = s_w1[i][j] = s_b1[i][j] = s_w2[i][j] = s_b2[i][j] = s_g[i][j] = 0.0f;
+        for (int n = 0; n < H; ++n) v[n] = pair(x, x);
+    };
+    Pair w1[H], w2[H], b2[H], s_w1[H], s_b1[H], s_w2[H], s_b2[H], s_g[H];
+    fill(w1, 1.0f); fill(w2, 1.0f); fill(b2, 0.0f);
+    fill(s_w1, 0.0f); fill(s_b1, 0.0f); fill(s_w2, 0.0f); fill(s_b2, 0.0f); fill(s_g, 0.0f);
+    if (KEEP && a.w1) weights(w1, a.w1);
+    if (KEEP && a.w2) weights(w2, a.w2);
+    const int group0 = worker / k.per_group, member = worker - group0 * k.per_group;
+    RowWalk now = {group0 < k.groups_at_once ? group0 : G, member, G, (int)(a.rows / G), member, k.per_group, k.groups_at_once}, ahead = now;
+    // shared memory, per stage: 5 tensors x NV vectors of 16 bytes a thread, or the rows of 5 tensors for every row group; then 16 bytes a warp for
+    // the statistics
+    const int pitch = W > 1 ? NV * (int)blockDim.x * 16 : (int)blockDim.x / tpr * (tpr * NV * (int)sizeof(T) + 32);   // of a tensor
+    const int stage_bytes = 5 * pitch + (int)(blockDim.x >> 5) * 16, stat_at = 5 * pitch + (int)(threadIdx.x >> 5) * 16;
+    const unsigned ring0 = (unsigned)__cvta_generic_to_shared(ring);
+    const int mine = W > 1 ? (int)threadIdx.x * 16 : (warps == 1 ? (int)(threadIdx.x >> 5) : 0) * (tpr * NV * (int)sizeof(T) + 32);
+    const auto copy = [&](int stage, int what, const T *p, unsigned row, unsigned ld) {
+        const T *from = p + (unsigned long long)row * ld;
+        if constexpr (W > 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (FULL || column(i) < a.dim) cp_async(ring0 + stage + mine + what * pitch + i * (int)blockDim.x * 16, from + column(i));
+        } else {
+            const int mis = (int)((uintptr_t)from & 15), bytes = mis + a.dim * (int)sizeof(T);
+            const unsigned to = ring0 + stage + mine + what * pitch;
+            for (int at = lane * 16; at < bytes; at += tpr * 16) cp_async(to + at, (const char *)from - mis + at, bytes - at < 16 ? bytes - at : 16);
         }
-    if (a.w1) Cols<float, W, NV>::load(w1, a.w1, tpr, lane, a.dim, 0.0f);
-    if (a.w2) Cols<float, W, NV>::load(w2, a.w2, tpr, lane, a.dim, 0.0f);
-    if (BIAS && a.b2) Cols<float, W, NV>::load(b2, a.b2, tpr, lane, a.dim, 0.0f);
-    const long long group0 = worker / k.per_group;
-    const int member = (int)(worker - group0 * k.per_group);
-    if (group0 < k.groups_at_once)
-        for (long long g = group0; g < G; g += k.groups_at_once) {
-            for (long long m = member; m < R; m += k.per_group) {
-                const long long r = m * G + g;
-                if (a.pat && a.pat[r] == PAT_NONE) {
-                    float z[NV][W];
+    };
+    // a row as it was copied; `other` beyond its end
+    const auto take = [&](Pair (&v)[H], int stage, int what, const T *p, unsigned row, unsigned ld, float other) {
+        float q[N];
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float x[W];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) z[i][j] = 0.0f;
-                    if (dx) C::store(dx + r * k.ld_dx, z, tpr, lane, a.dim);
-                    if (df) C::store(df + r * k.ld_df, z, tpr, lane, a.dim);
-                    continue;
+            for (int j = 0; j < W; ++j) x[j] = other;
+            if constexpr (W > 1) {
+                if (FULL || column(i) < a.dim) load_vec<T, W>(x, reinterpret_cast<const T *>(ring + stage + mine + what * pitch + i * (int)blockDim.x * 16));
+            } else {
+                const int mis = (int)((uintptr_t)(p + (unsigned long long)row * ld) & 15);
+                if (FULL || column(i) < a.dim) load_vec<T, W>(x, reinterpret_cast<const T *>(ring + stage + mine + what * pitch + mis) + column(i));
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) q[i * W + j] = x[j];
+        }
+#pragma unroll
+        for (int n = 0; n < H; ++n) v[n] = pair(q[2 * n], q[2 * n + 1]);
+    };
+    const Out<W, NV, FULL> put = {tpr, lane, a.dim};
+    const auto row_barrier = [&]() {
+        if (W == 1 && warps > 1) __syncthreads();
+        else __syncwarp();                              // the statistics come by the warp's first lane
+    };
+    const auto next_stage = [&](int stage) { return stage + stage_bytes < stages * stage_bytes ? stage + stage_bytes : 0; };
+    unsigned on_bits = 0, on_at = 0, on_to = 0;         // which of the rows under way are no padding: bits come in at on_to, go out at on_at
+    char pat_ahead = !ahead.ended() && a.pat ? __ldg(a.pat + ahead.row()) : 1;
+    const auto advance = [&](int stage) {
+        const bool on = !ahead.ended() && pat_ahead != PAT_NONE;
+        on_bits = (on_bits & ~(1u << on_to)) | ((unsigned)on << on_to);
+        on_to = (on_to + 1) & 31;
+        if (on) {
+            const unsigned r = ahead.row();
+            if ((threadIdx.x & 31) == 0) cp_async(ring0 + stage + stat_at, a.stats + r);
+            if (FULL || dh) { copy(stage, 0, dh, r, k.ld_dh); copy(stage, 1, y, r, k.ld_y); }
+            if (FULL || dy) copy(stage, 2, dy, r, k.ld_dy);
+            if (FULL || f) copy(stage, 3, f, r, k.ld_f);
+            if ((FULL || f) && a.gate) copy(stage, 4, (const T *)a.gate, ahead.g, (unsigned)a.ld_gate);
+        }
+        cp_commit();
+        if (ahead.ended()) return;
+        ahead.next();
+        if (a.pat && !ahead.ended()) pat_ahead = __ldg(a.pat + ahead.row());   // looked at when the next copies start
+    };
+    int at = 0, to = 0;                                 // the stage worked on, and the one that is filled next
+    for (int s = 0; s + 1 < stages; ++s) { advance(to); to = next_stage(to); }
+    for (; !now.ended(); at = next_stage(at), to = next_stage(to)) {
+        if (stages > 1) {
+            cp_wait(stages - 2);
+            row_barrier();                              // the row is there for all its threads, and all have left the one before
+            advance(to);
+        } else {
+            row_barrier();
+            advance(0);
+            cp_wait(0);
+            row_barrier();
+        }
+        const unsigned r = now.row(), g = now.g;
+        const bool on = on_bits >> on_at & 1, done = now.last_of_group();
+        on_at = (on_at + 1) & 31;
+        now.next();
+        Pair d[H], u[H], t[H];
+        if (!on) {
+            fill(d, 0.0f);
+            if (FULL || dx) put(dx + (unsigned long long)r * k.ld_dx, d);
+            if (FULL || df) put(df + (unsigned long long)r * k.ld_df, d);
+        } else {
+            const float4 st = *reinterpret_cast<const float4 *>(ring + at + stat_at);
+            // u = (v - mean) / deviation; sums of d and of d u
+            const auto centre = [&](float mean, float rstd) {
+                const Pair mm = pair(-mean, -mean), rr = pair(rstd, rstd);
+#pragma unroll
+                for (int n = 0; n < H; ++n) u[n] = mul2(BIAS ? add2(u[n], mm) : u[n], rr);
+            };
+            const auto joint = [&](float (&s)[S]) {
+                Pair p = 0, q = 0;
+#pragma unroll
+                for (int n = 0; n < H; ++n) {
+                    p = fma2(d[n], u[n], p);
+                    if (BIAS) q = add2(q, d[n]);
                 }
-                float t[NV][W], u[NV][W], d[NV][W], gt[NV][W];
-                const float4 st = a.stats[r];
-                if (dy) C::load(t, dy + r * k.ld_dy, tpr, lane, a.dim, 0.0f);
-                else
+                const float2 x = halves(p), z = halves(q);
+                s[0] = x.x + x.y;
+                if (BIAS) s[S - 1] = z.x + z.y;
+                row_sums<S>(s, warps, red, phase);
+                s[0] = -s[0] * a.inv_dim;
+                if (BIAS) s[S - 1] = a.layer_norm ? -s[S - 1] * a.inv_dim : 0.0f;
+            };
+            if (FULL || dh) {
+                float s[S];
+                take(d, at, 0, dh, r, k.ld_dh, 0.0f);
+                take(u, at, 1, y, r, k.ld_y, st.z);
+                if (!KEEP && a.w1) weights(w1, a.w1);
+                centre(st.z, st.w);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int j = 0; j < W; ++j) t[i][j] = 0.0f;
-                if (dh) {
-                    C::load(d, dh + r * k.ld_dh, tpr, lane, a.dim, 0.0f);
-                    C::load(u, y + r * k.ld_y, tpr, lane, a.dim, st.z);
+                for (int n = 0; n < H; ++n) {
+                    s_w1[n] = fma2(d[n], u[n], s_w1[n]);
+                    if (BIAS) s_b1[n] = add2(s_b1[n], d[n]);
+                    d[n] = mul2(d[n], w1[n]);
                 }
-                float fv[NV][W];
-                if (f) {
-                    C::load(fv, f + r * k.ld_f, tpr, lane, a.dim, st.x);
-                    if (a.gate) C::load(gt, (const T *)a.gate + g * a.ld_gate, tpr, lane, a.dim, 0.0f);
+                joint(s);
+                const Pair p = pair(s[0], s[0]), q = pair(s[S - 1], s[S - 1]), rr = pair(st.w, st.w);
+                if (FULL || dy) take(t, at, 2, dy, r, k.ld_dy, 0.0f);
+                else fill(t, 0.0f);
+#pragma unroll
+                for (int n = 0; n < H; ++n) d[n] = fma2(fma2(u[n], p, BIAS ? add2(d[n], q) : d[n]), rr, t[n]);
+            } else if (dy) take(d, at, 2, dy, r, k.ld_dy, 0.0f);
+            if (FULL || dx) put(dx + (unsigned long long)r * k.ld_dx, d);
+            if (FULL || f) {
+                float s[S];
+                take(u, at, 3, f, r, k.ld_f, st.x);
+                if (a.gate) take(t, at, 4, (const T *)a.gate, g, (unsigned)a.ld_gate, 0.0f);
+                else {
+#pragma unroll
+                    for (int n = 0; n < H; ++n) t[n] = pair(FULL || column(2 * n / W) < a.dim ? 1.0f : 0.0f, FULL || column((2 * n + 1) / W) < a.dim ? 1.0f : 0.0f);
                 }
-                if (dh) {
-                    float s[S] = {};
+                if (!KEEP && a.w2) weights(w2, a.w2);
+                if (BIAS && a.b2) weights(b2, a.b2);
+                centre(st.x, st.y);
+                const Pair aa = pair(a.a, a.a);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int j = 0; j < W; ++j) {
-                            u[i][j] = (u[i][j] - st.z) * st.w;
-                            s_w1[i][j] = fmaf(d[i][j], u[i][j], s_w1[i][j]);
-                            if (BIAS) s_b1[i][j] += d[i][j];
-                            d[i][j] *= w1[i][j];
-                            s[0] = fmaf(d[i][j], u[i][j], s[0]);
-                            if (BIAS) s[S - 1] += d[i][j];
-                        }
-                    row_sums<S>(s, warps, red, phase);
-                    const float p = s[0] * a.inv_dim, q = BIAS && a.layer_norm ? s[S - 1] * a.inv_dim : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int j = 0; j < W; ++j) t[i][j] = fmaf(st.w, fmaf(-u[i][j], p, d[i][j] - q), t[i][j]);
+                for (int n = 0; n < H; ++n) {
+                    d[n] = mul2(d[n], aa);
+                    s_g[n] = fma2(d[n], BIAS ? fma2(u[n], w2[n], b2[n]) : mul2(u[n], w2[n]), s_g[n]);
+                    d[n] = mul2(d[n], t[n]);
+                    s_w2[n] = fma2(d[n], u[n], s_w2[n]);
+                    if (BIAS) s_b2[n] = add2(s_b2[n], d[n]);
+                    d[n] = mul2(d[n], w2[n]);
                 }
-                if (dx) C::store(dx + r * k.ld_dx, t, tpr, lane, a.dim);
-                if (f) {
-                    float s[S] = {};
+                if (FULL || df) {
+                    joint(s);
+                    const Pair p = pair(s[0], s[0]), q = pair(s[S - 1], s[S - 1]), rr = pair(st.y, st.y);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int j = 0; j < W; ++j) {
-                            u[i][j] = (fv[i][j] - st.x) * st.y;
-                            const float at = a.a * t[i][j];
-                            s_g[i][j] = fmaf(at, fmaf(u[i][j], w2[i][j], b2[i][j]), s_g[i][j]);
-                            const float dn = (i * tpr + lane) * W < a.dim ? (a.gate ? at * gt[i][j] : at) : 0.0f;
-                            s_w2[i][j] = fmaf(dn, u[i][j], s_w2[i][j]);
-                            if (BIAS) s_b2[i][j] += dn;
-                            d[i][j] = dn * w2[i][j];
-                            s[0] = fmaf(d[i][j], u[i][j], s[0]);
-                            if (BIAS) s[S - 1] += d[i][j];
-                        }
-                    if (df) {
-                        row_sums<S>(s, warps, red, phase);
-                        const float p = s[0] * a.inv_dim, q = BIAS && a.layer_norm ? s[S - 1] * a.inv_dim : 0.0f;
-#pragma unroll
-                        for (int i = 0; i < NV; ++i)
-#pragma unroll
-                            for (int j = 0; j < W; ++j) d[i][j] = st.y * fmaf(-u[i][j], p, d[i][j] - q);
-                        C::store(df + r * k.ld_df, d, tpr, lane, a.dim);
-                    }
+                    for (int n = 0; n < H; ++n) d[n] = mul2(fma2(u[n], p, BIAS ? add2(d[n], q) : d[n]), rr);
+                    put(df + (unsigned long long)r * k.ld_df, d);
                 }
             }
-            if (k.dgate) {
-                if (k.per_group == 1) C::store((T *)k.dgate + g * k.ld_dgate, s_g, tpr, lane, a.dim);
-                else Cols<float, W, NV>::store(k.partial_gate + worker * k.dim_pad, s_g, tpr, lane, a.dim);
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < W; ++j) s_g[i][j] = 0.0f;
-            }
         }
+        if (done && k.dgate) {
+            if (k.per_group == 1) put((T *)k.dgate + (unsigned long long)g * k.ld_dgate, s_g);
+            else put(k.partial_gate + (size_t)worker * k.dim_pad, s_g);
+            fill(s_g, 0.0f);
+        }
+    }
+    cp_wait(0);
     if (!k.partial) return;
     float *out = k.partial + (size_t)blockIdx.x * 4 * k.dim_pad;
     if (warps > 1) {
-        Cols<float, W, NV>::store(out, s_w1, tpr, lane, a.dim);
-        Cols<float, W, NV>::store(out + k.dim_pad, s_b1, tpr, lane, a.dim);
-        Cols<float, W, NV>::store(out + 2 * k.dim_pad, s_w2, tpr, lane, a.dim);
-        Cols<float, W, NV>::store(out + 3 * k.dim_pad, s_b2, tpr, lane, a.dim);
+        put(out, s_w1);
+        put(out + k.dim_pad, s_b1);
+        put(out + 2 * k.dim_pad, s_w2);
+        put(out + 3 * k.dim_pad, s_b2);
     } else {
-        const int w = threadIdx.x >> 5, nw = blockDim.x >> 5, width = 32 * W * NV;
+        float *join = reinterpret_cast<float *>(ring);
+        const int w = threadIdx.x >> 5, nw = blockDim.x >> 5, width = 32 * N;
+        __syncthreads();                                // the copies of all warps have arrived
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            Cols<float, W, NV>::store(join + w * width, q == 0 ? s_w1 : q == 1 ? s_b1 : q == 2 ? s_w2 : s_b2, tpr, lane, width);
+            put(join + w * width, q == 0 ? s_w1 : q == 1 ? s_b1 : q == 2 ? s_w2 : s_b2);
             __syncthreads();
             for (int c = threadIdx.x; c < a.dim; c += blockDim.x) {
                 float s = 0.0f;
@@ -381,7 +518,10 @@ int check(const char *who, const b2_block_norm *d) {
             set_error("%s: a gate of %lld rows for %lld frames (the frames must be a multiple)", who, d->gate_rows, d->rows);
             return B2_ERR_BAD_SHAPE;
         }
-        if (d->ld_gate < d->dim) { set_error("%s: leading dimension of the gate too small (%lld for %d columns)", who, d->ld_gate, d->dim); return B2_ERR_BAD_ARG; }
+        if (d->ld_gate < d->dim || d->ld_gate > 0x7fffffffll) {
+            set_error("%s: leading dimension of the gate too small or beyond 2^31 (%lld for %d columns)", who, d->ld_gate, d->dim);
+            return B2_ERR_BAD_ARG;
+        }
         if (!aligned_to(d->gate, e)) { set_error("%s: the gate is not aligned to its elements", who); return B2_ERR_BAD_ARG; }
     }
     if (!aligned_to(d->w_pre, 4) || !aligned_to(d->b_pre, 4) || !aligned_to(d->w_post, 4) || !aligned_to(d->b_post, 4) || !aligned_to(d->stats, 16)) {
@@ -392,7 +532,10 @@ int check(const char *who, const b2_block_norm *d) {
 }
 int check_rows(const char *who, const char *name, const b2_block_norm *d, const void *p, long long ld) {
     if (!p) return B2_OK;
-    if (ld < d->dim) { set_error("%s: leading dimension of %s too small (%lld for %d columns)", who, name, ld, d->dim); return B2_ERR_BAD_ARG; }
+    if (ld < d->dim || ld > 0x7fffffffll) {
+        set_error("%s: leading dimension of %s too small or beyond 2^31 (%lld for %d columns)", who, name, ld, d->dim);
+        return B2_ERR_BAD_ARG;
+    }
     if (!aligned_to(p, type_size(d->type))) { set_error("%s: %s is not aligned to its elements", who, name); return B2_ERR_BAD_ARG; }
     return B2_OK;
 }
@@ -419,18 +562,16 @@ int forward(const b2_block_norm *d, const T *x, long long ld_x, const T *f, long
     return go(block_norm_forward_kernel<T, W, 8>, (int)pow2_at_least((unsigned)(vecs + 7) / 8));
 }
 
-// Workers of the backward pass.  tpr: threads a row; blocks: as many as 1024 threads per multiprocessor give
+// Workers of the backward pass.  tpr: threads a row, each with `per_thread` columns or two times as many; blocks: as many as 512 threads a
+// multiprocessor give (their registers, and the shared memory of a deep ring)
 struct BackPlan { int tpr, threads, blocks, workers, per_group, groups_at_once; };
-int back_tpr(int vecs) {
-    const int t = (int)pow2_at_least((unsigned)vecs);
-    return t < 32 ? 32 : t > 1024 ? 1024 : t;
-}
-BackPlan back_plan(long long rows, int vecs, long long gate_rows) {
+BackPlan back_plan(long long rows, int dim, int per_thread, long long gate_rows) {
     BackPlan p;
-    p.tpr = back_tpr(vecs);
+    const unsigned t = pow2_at_least((unsigned)((dim + per_thread - 1) / per_thread));
+    p.tpr = t < 32 ? 32 : t > 1024 ? 1024 : (int)t;
     p.threads = p.tpr == 32 ? 256 : p.tpr;
     const int each = p.threads / p.tpr;
-    long long blocks = (long long)sm_count() * 1024 / (p.threads < 256 ? 256 : p.threads);
+    long long blocks = (long long)sm_count() * (512 > p.threads ? 512 / p.threads : 1);
     if (blocks * each > rows) blocks = (rows + each - 1) / each;
     p.blocks = (int)blocks;
     p.workers = p.blocks * each;
@@ -446,27 +587,42 @@ template <typename T, int W>
 int backward(const b2_block_norm *d, T *dx, long long ld_dx, T *df, long long ld_df, T *dgate, long long ld_dgate, float *const (&dw)[4], const T *dy, long long ld_dy,
              const T *dh, long long ld_dh, const T *y, long long ld_y, const T *f, long long ld_f, float *ws, cudaStream_t st) {
     const NormArgs a = args_of(d);
-    const int vecs = (d->dim + W - 1) / W;
-    const BackPlan p = back_plan(d->rows, vecs, d->gate ? d->gate_rows : 0);
-    BackArgs k = {ld_dx, ld_df, ld_dy, ld_dh, ld_y, ld_f, ld_dgate, dgate, nullptr, nullptr, (d->dim + 15) / 16 * 16, p.per_group, p.groups_at_once};
+    const int per_thread = W > 1 ? W : 8;
+    const BackPlan p = back_plan(d->rows, d->dim, per_thread, d->gate ? d->gate_rows : 0);
+    BackArgs k = {(unsigned)ld_dx, (unsigned)ld_df, (unsigned)ld_dy, (unsigned)ld_dh, (unsigned)ld_y, (unsigned)ld_f, (unsigned)ld_dgate, dgate, nullptr, nullptr, (d->dim + 15) / 16 * 16, p.per_group, p.groups_at_once};
     const bool sums = dw[0] || dw[1] || dw[2] || dw[3], gate_sums = dgate && p.per_group > 1;
     if (sums) k.partial = ws;
     k.partial_gate = ws + (size_t)p.blocks * 4 * k.dim_pad;
-    const auto go = [&](auto kernel, int smem) -> int {
-        kernel<<<p.blocks, p.threads, smem, st>>>(a, k, dx, df, dy, dh, y, f, p.tpr);
+    // the ring: up to 4 rows in what the blocks of a multiprocessor share
+    const int nv = W == 1 ? 8 : d->dim > p.tpr * W ? 2 : 1, here = 512 > p.threads ? 512 / p.threads : 1;
+    const int pitch = W > 1 ? nv * p.threads * 16 : p.threads / p.tpr * (p.tpr * nv * (int)sizeof(T) + 32), stage_bytes = 5 * pitch + p.threads / 32 * 16;
+    const int most = 208 * 1024, join_bytes = p.tpr == 32 ? 8 * 32 * W * nv * 4 : 0;
+    int stages = most / here / stage_bytes;
+    stages = stages > 4 ? 4 : stages < 1 ? 1 : stages;
+    const int smem = stages * stage_bytes > join_bytes ? stages * stage_bytes : join_bytes;
+    const auto go = [&](auto kernel) -> int {
+        B2_TRY(set_max_dynamic_smem((const void *)kernel, most));
+        kernel<<<p.blocks, p.threads, smem, st>>>(a, k, dx, df, dy, dh, y, f, p.tpr, stages);
         count_launch();
         B2_CUDA(cudaGetLastError());
         return B2_OK;
     };
-    const int smem = p.tpr == 32 ? 8 * 32 * W * 4 : 0;
     const bool bias = d->layer_norm || dw[1] || dw[3] || d->b_post;
+    const bool full = W > 1 && d->dim == p.tpr * W && dx && df && dy && dh && f;
     const auto pick = [&](auto b) {
         constexpr bool B = decltype(b)::value;
-        if (vecs <= 256) return go(block_norm_backward_kernel<T, W, 1, 256, B>, smem);
-        if (vecs <= 512) return go(block_norm_backward_kernel<T, W, 1, 512, B>, 0);
-        if (vecs <= 1024) return go(block_norm_backward_kernel<T, W, 1, 1024, B>, 0);
-        if (vecs <= 2048) return go(block_norm_backward_kernel<T, W, 2, 1024, B>, 0);
-        return go(block_norm_backward_kernel<T, 1, 8, 1024, B>, 0);
+        constexpr int NV = W == 1 ? 8 : 1;
+        if constexpr (W > 1)
+            if (full) {
+                if (p.threads <= 256) return go(block_norm_backward_kernel<T, W, 1, 256, B, true>);
+                if (p.threads <= 512) return go(block_norm_backward_kernel<T, W, 1, 512, B, true>);
+                return go(block_norm_backward_kernel<T, W, 1, 1024, B, true>);
+            }
+        if (p.threads <= 256) return go(block_norm_backward_kernel<T, W, NV, 256, B, false>);
+        if (p.threads <= 512) return go(block_norm_backward_kernel<T, W, NV, 512, B, false>);
+        if constexpr (W == 4)
+            if (nv == 2) return go(block_norm_backward_kernel<T, W, 2, 1024, B, false>);
+        return go(block_norm_backward_kernel<T, W, NV, 1024, B, false>);
     };
     B2_TRY(bias ? pick(std::true_type()) : pick(std::false_type()));
     if (!sums && !gate_sums) return B2_OK;
@@ -506,10 +662,10 @@ int b2_block_norm_forward(const b2_block_norm *d, const void *x, long long ld_x,
 
 size_t b2_block_norm_backward_workspace(long long rows, int dim, long long gate_rows) {
     if (rows < 1 || rows > 0x7fffffffll || dim < 1 || dim > MAX_DIM || gate_rows < 0) return 0;
-    // enough for any type and alignment, that is for every width of the vectors
+    // enough for any type and alignment
     size_t most = 0;
-    for (int w = 1; w <= 8; w *= 2) {
-        const BackPlan p = back_plan(rows, (dim + w - 1) / w, gate_rows);
+    for (int per_thread = 4; per_thread <= 8; per_thread *= 2) {
+        const BackPlan p = back_plan(rows, dim, per_thread, gate_rows);
         const size_t n = (size_t)p.blocks * 4 + p.workers;
         if (n > most) most = n;
     }

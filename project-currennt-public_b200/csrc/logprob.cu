@@ -76,13 +76,6 @@ template <int N> __device__ __forceinline__ void add_values(Sums &a, const float
 }
 
 // ---- vectors of 16 bytes as they were loaded ------------------------------------------------------------------------------------------
-typedef unsigned long long Pair;   // two fp32 values for the packed instructions
-__device__ __forceinline__ Pair pair(float x, float y) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y)); return p; }
-__device__ __forceinline__ float2 halves(Pair p) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-__device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-
 template <typename T> struct Raw;
 template <> struct Raw<float> {
     static constexpr unsigned NONE = 0xff800000u;      // -inf in every place of a word

@@ -23,10 +23,13 @@ namespace b2 {
 namespace {
 
 // ---- lookup -------------------------------------------------------------------------------------------------------------------
+// Loads a thread has under way: the narrower, the more
+__host__ __device__ constexpr int in_flight(int w) { return w >= 4 ? 4 : w == 2 ? 8 : 16; }
 // tpr threads a row (a power of two up to 256), W elements an access
 template <typename T, typename U, int W>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(U *__restrict__ out, long long ld_out, const T *__restrict__ table, long long ld_table, int vocab,
                                                                 int dim, const int *__restrict__ tokens, long long rows, float scale, int tpr) {
+    constexpr int UN = in_flight(W);
     const int lane = threadIdx.x & (tpr - 1);
     const int per_block = 256 / tpr;
     for (long long r = (long long)blockIdx.x * per_block + threadIdx.x / tpr; r < rows; r += (long long)gridDim.x * per_block) {
@@ -35,12 +38,12 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(U *__restrict__ 
         if (tok >= 0 && tok < vocab) {
             const T *from = table + (long long)tok * ld_table;
             int c = lane * W;
-            for (; c + 3 * tpr * W < dim; c += 4 * tpr * W) {
-                float v[4][W];
+            for (; c + (UN - 1) * tpr * W < dim; c += UN * tpr * W) {
+                float v[UN][W];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) load_vec<T, W>(v[i], from + c + i * tpr * W);
+                for (int i = 0; i < UN; ++i) load_vec<T, W>(v[i], from + c + i * tpr * W);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < UN; ++i) {
 #pragma unroll
                     for (int j = 0; j < W; ++j) v[i][j] *= scale;
                     store_vec<U, W>(to + c + i * tpr * W, v[i]);
@@ -74,13 +77,10 @@ __device__ __forceinline__ unsigned key_of(int tok, int vocab) { return (tok >= 
 // How many of the warp's earlier lanes hold the same digit, and whether this lane is the last of them.
 __device__ __forceinline__ unsigned same_digit(unsigned active, unsigned digit) { return __match_any_sync(active, digit); }
 
-// Exclusive prefix sum over n values in shared memory (n <= 16 * SORT_THREADS); all threads of the block call it.
-__device__ __forceinline__ void block_exclusive_scan(unsigned *x, int n, unsigned *warp_tot) {
-    const int per = (n + SORT_THREADS - 1) / SORT_THREADS, a = min(n, (int)threadIdx.x * per), b = min(n, a + per);
-    unsigned s = 0;
-    for (int i = a; i < b; ++i) s += x[i];
-    unsigned inc = s;
+// Exclusive prefix sum over one value a thread; all threads of the block call it.
+__device__ __forceinline__ unsigned block_exclusive_scan(unsigned x, unsigned *warp_tot) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    unsigned inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -88,9 +88,20 @@ __device__ __forceinline__ void block_exclusive_scan(unsigned *x, int n, unsigne
     }
     if (lane == 31) warp_tot[w] = inc;
     __syncthreads();
-    unsigned before = inc - s;
-    for (int i = 0; i < w; ++i) before += warp_tot[i];
-    for (int i = a; i < b; ++i) { const unsigned y = x[i]; x[i] = before; before += y; }
+    unsigned before = inc - x;
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) before += i < w ? warp_tot[i] : 0;
+    __syncthreads();
+    return before;
+}
+// count[warp][digit] becomes the place of the first key of (digit, warp): digits in order, within a digit the warps in order, behind `base`
+// (thread d's own value, for digit d).
+__device__ __forceinline__ void places(unsigned *count, int digits, unsigned base) {
+    const int d = threadIdx.x;
+    if (d < digits) {
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; ++w) { const unsigned c = count[w * digits + d]; count[w * digits + d] = base; base += c; }
+    }
     __syncthreads();
 }
 
@@ -101,7 +112,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__r
     extern __shared__ unsigned sm[];
     unsigned *key[2] = {sm, sm + SMALL_SORT};
     unsigned short *row[2] = {(unsigned short *)(sm + 2 * SMALL_SORT), (unsigned short *)(sm + 2 * SMALL_SORT) + SMALL_SORT};
-    unsigned *count = sm + 3 * SMALL_SORT;                 // [digits][SORT_WARPS]
+    unsigned *count = sm + 3 * SMALL_SORT;                 // [SORT_WARPS][digits]
     __shared__ unsigned warp_tot[SORT_WARPS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, digits = 1 << bits;
     grid_wait();
@@ -127,20 +138,24 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__r
             const unsigned active = __ballot_sync(0xffffffffu, on);
             if (on) {
                 const unsigned d = (kin[i] >> (p * bits)) & (digits - 1);
-                const unsigned same = same_digit(active, d), c = count[d * SORT_WARPS + w];
+                const unsigned same = same_digit(active, d), c = count[w * digits + d];
                 __syncwarp(active);
-                if (lane == 31 - __clz(same)) count[d * SORT_WARPS + w] = c + __popc(same);
+                if (lane == 31 - __clz(same)) count[w * digits + d] = c + __popc(same);
                 rank[k] = (unsigned short)(c + __popc(same & ((1u << lane) - 1)));
             }
             __syncwarp();
         }
         __syncthreads();
-        block_exclusive_scan(count, digits * SORT_WARPS, warp_tot);
+        unsigned total = 0;
+        if ((int)threadIdx.x < digits)
+#pragma unroll
+            for (int i = 0; i < SORT_WARPS; ++i) total += count[i * digits + threadIdx.x];
+        places(count, digits, block_exclusive_scan(total, warp_tot));
 #pragma unroll
         for (int k = 0; k < SMALL_SORT / SORT_THREADS; ++k) {
             const int i = w * seg + k * 32 + lane;
             if (k * 32 < seg && i < n) {
-                const unsigned d = (kin[i] >> (p * bits)) & (digits - 1), at = count[d * SORT_WARPS + w] + rank[k];
+                const unsigned d = (kin[i] >> (p * bits)) & (digits - 1), at = count[w * digits + d] + rank[k];
                 kout[at] = kin[i];
                 rout[at] = rin[i];
             }
@@ -188,6 +203,7 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int blk, int blks) 
 // digit counts of every tile; the first pass also notes which tokens occur (their bits were cleared before)
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortArgs a, const ZeroArgs z) {
     grid_wait();
+    grid_release();
     if ((int)blockIdx.x >= a.tiles) { zero_rows(z, blockIdx.x - a.tiles, gridDim.x - a.tiles); return; }
     extern __shared__ unsigned sm[];
     const int digits = 1 << a.bits;
@@ -206,46 +222,38 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortArgs
 // ranks of a tile's keys and scatter; every block adds up the counts before its own by itself
 __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const SortArgs a, const ZeroArgs z) {
     grid_wait();
+    grid_release();
     if ((int)blockIdx.x >= a.tiles) { zero_rows(z, blockIdx.x - a.tiles, gridDim.x - a.tiles); return; }
     extern __shared__ unsigned sm[];
     __shared__ unsigned warp_tot[SORT_WARPS];
     const int digits = 1 << a.bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    unsigned *base = sm, *count = sm + digits;             // [digits], [digits][SORT_WARPS]
-    unsigned before = 0;
+    unsigned *count = sm;                                  // [SORT_WARPS][digits]
+    for (int i = threadIdx.x; i < digits * SORT_WARPS; i += SORT_THREADS) count[i] = 0;
+    unsigned before = 0, total = 0;
     if ((int)threadIdx.x < digits) {
-        unsigned total = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int t = 0; t < a.tiles; ++t) {
             const unsigned h = a.hist[(size_t)t * digits + threadIdx.x];
             if (t < (int)blockIdx.x) before += h;
             total += h;
         }
-        base[threadIdx.x] = total;
     }
-    for (int i = threadIdx.x; i < digits * SORT_WARPS; i += SORT_THREADS) count[i] = 0;
     __syncthreads();
-    block_exclusive_scan(base, digits, warp_tot);
-    if ((int)threadIdx.x < digits) base[threadIdx.x] += before;
     // counts of every warp's segment of the tile
     const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile), seg = a.tile / SORT_WARPS;
     const int s0 = i0 + w * seg, s1 = min(i1, s0 + seg);
-    for (int i = s0 + lane; i < s1; i += 32) atomicAdd(count + ((sort_key(a, i) >> a.shift) & (digits - 1)) * SORT_WARPS + w, 1u);
-    __syncthreads();
-    if ((int)threadIdx.x < digits) {
-        unsigned at = base[threadIdx.x];
-#pragma unroll
-        for (int i = 0; i < SORT_WARPS; ++i) { const unsigned c = count[threadIdx.x * SORT_WARPS + i]; count[threadIdx.x * SORT_WARPS + i] = at; at += c; }
-    }
-    __syncthreads();
+    for (int i = s0 + lane; i < s1; i += 32) atomicAdd(count + w * digits + ((sort_key(a, i) >> a.shift) & (digits - 1)), 1u);
+    const unsigned base = block_exclusive_scan(total, warp_tot);   // its barriers stand behind the counts
+    places(count, digits, base + before);
     for (int j = s0; j < s1; j += 32) {
         const int i = j + lane;
         const bool on = i < s1;
         const unsigned active = __ballot_sync(0xffffffffu, on);
         if (on) {
             const unsigned k = sort_key(a, i), d = (k >> a.shift) & (digits - 1);
-            const unsigned same = same_digit(active, d), c = count[d * SORT_WARPS + w];
+            const unsigned same = same_digit(active, d), c = count[w * digits + d];
             __syncwarp(active);
-            if (lane == 31 - __clz(same)) count[d * SORT_WARPS + w] = c + __popc(same);
+            if (lane == 31 - __clz(same)) count[w * digits + d] = c + __popc(same);
             const unsigned at = c + __popc(same & ((1u << lane) - 1));
             a.kout[at] = k;
             a.rout[at] = a.tokens ? i : a.rin[i];
@@ -277,60 +285,74 @@ template <typename U, int W> __device__ __forceinline__ void put_row(U *to, cons
     store_vec<U, W>(to, v);
 }
 
-constexpr int SUM_THREADS = 128;
+constexpr int SUM_THREADS = 128, MIN_GROUP = 8, MAX_PIECE = 64;
 
-// A group of tpr threads (a power of two up to SUM_THREADS) takes W * tpr columns of a piece: blockIdx.y counts the column tiles.
-// Blocks beyond the pieces zero absent rows.
+// A group of tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes W * tpr columns of a piece.  Every other block zeroes absent rows as long as
+// there are any: stores that nothing waits for, beside loads that the sums wait for.
 template <typename T, typename U, int W>
-__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks) {
+__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
+                                                                    int zero_blocks) {
+    __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
+    __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
     grid_wait();
-    if ((int)blockIdx.x >= sum_blocks) { zero_rows(z, blockIdx.x - sum_blocks, gridDim.x - sum_blocks); return; }
+    grid_release();
+    const int both = 2 * min(sum_blocks, zero_blocks);
+    int block = blockIdx.x;
+    if (block < both) {
+        if (block & 1) { zero_rows(z, block >> 1, zero_blocks); return; }
+        block >>= 1;
+    } else {
+        block -= both >> 1;
+        if (zero_blocks > sum_blocks) { zero_rows(z, block, zero_blocks); return; }
+    }
     const int tiles = (a.dim + a.tpr * W - 1) / (a.tpr * W);
-    const int per_block = SUM_THREADS / a.tpr;
-    const long long unit = (long long)blockIdx.x * per_block + threadIdx.x / a.tpr;
-    const int p = (int)(unit / tiles), col = ((int)(unit - (long long)p * tiles) * a.tpr + (threadIdx.x & (a.tpr - 1))) * W;
-    if (p >= a.pieces) return;
-    const int i0 = p * a.piece, i1 = min(a.n, i0 + a.piece);
-    unsigned cur = __ldg(a.keys + i0);
+    const int group = threadIdx.x / a.tpr, lane = threadIdx.x & (a.tpr - 1);
+    const long long unit = (long long)block * (SUM_THREADS / a.tpr) + group;
+    const int p = (int)(unit / tiles), col = ((int)(unit - (long long)p * tiles) * a.tpr + lane) * W;
+    // the piece's keys and rows first: then the rows themselves can all be asked for at once
+    const int i0 = p < a.pieces ? p * a.piece : a.n, n = min(a.n - i0, a.piece);
+    unsigned *key = s_key + group * a.piece;
+    int *row = s_row + group * a.piece;
+    for (int i = lane; i < n; i += a.tpr) { key[i] = __ldg(a.keys + i0 + i); row[i] = __ldg(a.rows + i0 + i); }
+    const unsigned before = n > 0 && i0 > 0 ? __ldg(a.keys + i0 - 1) : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? __ldg(a.keys + i0 + n) : 0xffffffffu;
+    __syncthreads();
+    if (n <= 0 || col >= a.dim) return;
+    unsigned cur = key[0];
     if (cur >= (unsigned)a.vocab) return;                  // nothing but padding from here on
-    bool from_before = i0 > 0 && __ldg(a.keys + i0 - 1) == cur;
-    if (col >= a.dim) return;
+    bool from_before = before == cur;
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-    constexpr int U8 = 8;
-    for (int i = i0; i < i1; i += U8) {
-        float v[U8][W];
-        unsigned k[U8];
+    float *head = a.partial + (size_t)p * 2 * a.dim_pad + col;
+    for (int i = 0; i < n; i += 8) {
+        Vec<T, W> v[8];
+        unsigned k[8];
 #pragma unroll
-        for (int u = 0; u < U8; ++u) {
-            k[u] = i + u < i1 ? __ldg(a.keys + i + u) : 0xffffffffu;
-            if (k[u] < (unsigned)a.vocab) load_vec<T, W>(v[u], dout + (long long)__ldg(a.rows + i + u) * a.ld_dout + col);
+        for (int u = 0; u < 8; ++u) {
+            k[u] = i + u < n ? key[i + u] : 0xffffffffu;
+            if (k[u] < (unsigned)a.vocab) v[u] = *reinterpret_cast<const Vec<T, W> *>(dout + (long long)row[i + u] * a.ld_dout + col);
         }
 #pragma unroll
-        for (int u = 0; u < U8; ++u) {
-            if (k[u] != cur && cur < (unsigned)a.vocab) {
-                // the token is complete here (the end of the piece is handled below)
-                if (i + u < i1) {
-                    if (from_before) store_vec<float, W>(a.partial + (size_t)p * 2 * a.dim_pad + col, acc);
-                    else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
-                    from_before = false;
-                    cur = k[u];
+        for (int u = 0; u < 8; ++u) {
+            // another token, or padding: the one before is complete (what ends with the piece is seen to below)
+            if (k[u] != cur && i + u < n && cur < (unsigned)a.vocab) {
+                if (from_before) store_vec<float, W>(head, acc);
+                else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+                from_before = false;
+                cur = k[u];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-                }
+                for (int j = 0; j < W; ++j) acc[j] = 0.0f;
             }
             if (k[u] < (unsigned)a.vocab) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) acc[j] += v[u][j];
+                for (int j = 0; j < W; ++j) acc[j] += to_float(v[u].v[j]);
             }
         }
     }
     if (cur >= (unsigned)a.vocab) return;
-    const bool goes_on = i1 < a.n && __ldg(a.keys + i1) == cur;
-    if (from_before) store_vec<float, W>(a.partial + (size_t)p * 2 * a.dim_pad + col, acc);
-    else if (goes_on) {
-        store_vec<float, W>(a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col, acc);
+    if (from_before) store_vec<float, W>(head, acc);
+    else if (behind == cur) {
+        store_vec<float, W>(head + a.dim_pad, acc);
         if (col == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
     } else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
 }
@@ -352,20 +374,23 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dta
         for (int j = 0; j < W; ++j) s[j] = 0.0f;
         if (col < a.dim) {
             if (y == 0) load_vec<float, W>(s, a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col);
-            for (int q = p + 1 + y; q < a.pieces && __ldg(a.keys + (size_t)q * a.piece) == key; q += 32) {
+            for (int q = p + 1 + y; q < a.pieces; q += 32) {
                 float v[4][W];
-                bool on[4];
+                unsigned k[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    on[u] = q + 8 * u < a.pieces && __ldg(a.keys + (size_t)(q + 8 * u) * a.piece) == key;
-                    if (on[u]) load_vec<float, W>(v[u], a.partial + (size_t)(q + 8 * u) * 2 * a.dim_pad + col);
+                    // the head is fetched beside the key that tells whether it is one
+                    const int at = min(q + 8 * u, a.pieces - 1);
+                    k[u] = q + 8 * u < a.pieces ? __ldg(a.keys + (size_t)at * a.piece) : 0xffffffffu;
+                    load_vec<float, W>(v[u], a.partial + (size_t)at * 2 * a.dim_pad + col);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (on[u]) {
+                    if (k[u] == key) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) s[j] += v[u][j];
                     }
+                if (k[3] != key) break;
             }
         }
 #pragma unroll
@@ -401,7 +426,7 @@ Plan make_plan(long long n, int vocab, int dim) {
     p.tile = (int)tile;
     p.tiles = (int)((n + tile - 1) / tile);
     // pieces: few rows give parallel groups, many rows few partial sums
-    p.piece = n <= 4096 ? 8 : n <= 16384 ? 16 : n <= 262144 ? 32 : 64;
+    p.piece = n <= 4096 ? 8 : n <= 16384 ? 16 : n <= 262144 ? 32 : MAX_PIECE;
     p.pieces = (int)((n + p.piece - 1) / p.piece);
     p.dim_pad = (dim + 15) / 16 * 16;
     size_t at = 0;
@@ -436,10 +461,10 @@ int common_width(int most, int dim, const void *a, long long lda, int ea, const 
 
 template <typename T, typename U, int W>
 int forward(U *out, long long ld_out, const T *table, long long ld_table, int vocab, int dim, const int *tokens, long long n, float scale, cudaStream_t st) {
-    // few rows: a thread per vector, so that all loads go out at once; many rows: four vectors a thread
+    // few rows: a thread per vector, so that all loads go out at once; many rows: as many as a thread has under way
     const unsigned vecs = (unsigned)((dim + W - 1) / W);
     const bool few = (double)n * vecs < 148.0 * 2048;
-    unsigned tpr = pow2_at_least(few ? vecs : (vecs + 3) / 4);
+    unsigned tpr = pow2_at_least(few ? vecs : (vecs + in_flight(W) - 1) / in_flight(W));
     if (tpr > 256) tpr = 256;
     const long long per = 256 / tpr, want = (n + per - 1) / per, most = 0x7fffffff;
     embedding_forward_kernel<T, U, W><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(out, ld_out, table, ld_table, vocab, dim, tokens, n, scale, (int)tpr);
@@ -452,12 +477,12 @@ template <typename T, typename U, int W>
 int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int zero_blocks, cudaStream_t st) {
     SumArgs a = base;
     unsigned tpr = pow2_at_least((unsigned)((a.dim + W - 1) / W));
-    if (tpr > SUM_THREADS) tpr = SUM_THREADS;
+    tpr = tpr > SUM_THREADS ? SUM_THREADS : tpr < MIN_GROUP ? MIN_GROUP : tpr;
     a.tpr = (int)tpr;
     const long long tiles = (a.dim + (long long)tpr * W - 1) / ((long long)tpr * W), per = SUM_THREADS / tpr;
     const long long blocks = (a.pieces * tiles + per - 1) / per;
     if (blocks + zero_blocks > 0x7fffffffll) { set_error("b2_embedding_backward: %lld blocks", blocks); return B2_ERR_BAD_SHAPE; }
-    B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks));
+    B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks, zero_blocks));
     const long long join = (long long)a.pieces * ((a.dim + 32 * W - 1) / (32 * W)), most = sm_count() * 8;
     return launch_chained(embedding_join_kernel<U, W>, dim3((unsigned)(join < most ? join : most)), dim3(256), 0, st, dtable, a);
 }
@@ -478,10 +503,9 @@ int backward(U *dtable, long long ld_dtable, int vocab, int dim, const T *dout, 
     } else {
         B2_CUDA(cudaMemsetAsync(ws, 0, p.keys[0], st));                   // the list's length and the bits of the tokens that occur
         // rows that a launch of the sort zeroes besides: about as much as fits under its latency
-        const long long share = (16ll << 20) / (z.row_bytes > 0 ? z.row_bytes : 1);
+        const long long share = (20ll << 20) / (z.row_bytes > 0 ? z.row_bytes : 1);
         SortArgs a = {tokens, nullptr, nullptr, nullptr, nullptr, (unsigned *)(ws + p.hist), present, count, (int)n, vocab, 0, p.bits, p.tiles, p.tile};
         const int digits = 1 << p.bits;
-        B2_TRY(set_max_dynamic_smem((const void *)sort_scatter_kernel, (1 + SORT_WARPS) * (1 << MAX_DIGIT_BITS) * 4));
         const int rest = z.v1;
         for (int i = 0; i < p.passes; ++i) {
             a.shift = i * p.bits;
@@ -493,7 +517,7 @@ int backward(U *dtable, long long ld_dtable, int vocab, int dim, const T *dout, 
                 const int zb = zz.v1 > zz.v0 ? 2 * sm_count() : 0;
                 z.v0 = zz.v1;
                 if (half == 0) B2_TRY(launch_chained(sort_count_kernel, dim3(p.tiles + zb), dim3(SORT_THREADS), digits * 4, st, a, zz));
-                else B2_TRY(launch_chained(sort_scatter_kernel, dim3(p.tiles + zb), dim3(SORT_THREADS), digits * (1 + SORT_WARPS) * 4, st, a, zz));
+                else B2_TRY(launch_chained(sort_scatter_kernel, dim3(p.tiles + zb), dim3(SORT_THREADS), digits * SORT_WARPS * 4, st, a, zz));
             }
             last = i & 1;
             a.tokens = nullptr;

@@ -352,40 +352,82 @@ template <typename T, int NV> __global__ void __launch_bounds__(256) logprob_war
     }
 }
 
-// Several rows a warp, for rows of which no alternatives are asked: G lanes a row, NV entries a lane.  The reductions and the row's closing
+// Several rows a warp, for rows of which no alternatives are asked: G lanes a row, NV vectors a lane.  The reductions and the row's closing
 // arithmetic then serve 32 / G rows at once; they are as much work as 100 entries.
 template <typename T, int G, int NV> __global__ void __launch_bounds__(256) logprob_rows_kernel(const T *__restrict__ logits, const FwdArgs a) {
+    constexpr int W = 16 / sizeof(T);
     const int lane = threadIdx.x & (G - 1);
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
-    const bool real = r < a.rows;
-    const T *x = logits + (real ? r : 0) * a.ld;
-    float z[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) z[i] = lane + G * i < a.vocab ? to_float(x[lane + G * i]) : neg_inf();
-    Given g = {-1, 0.0f};
-    if (real && lane == 0) g = load_given(a, r, x);
-    if (a.mask) {
-        const unsigned char *mk = a.mask + (real ? r : 0) * a.ld_mask;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + G * i < a.vocab && !mk[lane + G * i]) z[i] = neg_inf();
-    }
-    float top = neg_inf();
+    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / G, r = at < a.rows ? at : a.rows - 1;
+    const T *x = logits + r * a.ld;
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T)), end = mis + a.vocab;
+    const T *base = x - mis;
+    uint4 q[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        z[i] = __fmul_rn(z[i], a.scale);
-        top = max_nan(top, z[i]);
+        const int v = (lane + G * i) * W;
+        q[i] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+        if (v >= mis && v + W <= end) q[i] = __ldg(reinterpret_cast<const uint4 *>(base + v));
     }
+    // the row's first and last entries, where their vectors are shared with the neighbours
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = (lane + G * i) * W;
+        if (v >= end || (v >= mis && v + W <= end)) continue;
+        Vec<T, W> part_of = *reinterpret_cast<const Vec<T, W> *>(&q[i]);
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (v + j >= mis && v + j < end) part_of.v[j] = base[v + j];
+        q[i] = *reinterpret_cast<const uint4 *>(&part_of);
+    }
+    Given g = {-1, 0.0f};
+    if (at < a.rows && lane == 0) g = load_given(a, r, x);
+    if (a.mask) {
+        const unsigned char *mk = a.mask + r * a.ld_mask;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            Vec<T, W> part_of = *reinterpret_cast<const Vec<T, W> *>(&q[i]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int e = (lane + G * i) * W + j - mis;
+                if (e >= 0 && e < a.vocab && !mk[e]) part_of.v[j] = from_float<T>(neg_inf());
+            }
+            q[i] = *reinterpret_cast<const uint4 *>(&part_of);
+        }
+    }
+    unsigned most = larger_of<T>(q[0]);
+#pragma unroll
+    for (int i = 1; i < NV; ++i) most = Raw<T>::larger(most, larger_of<T>(q[i]));
+    float top = Raw<T>::largest(most);
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(FULL, top, o));
-    Sums t = {neg_inf(), 0.0f, 0.0f};
-    add_values<NV>(t, z, top);
+    Sums t = {__fmul_rn(top, a.scale), 0.0f, 0.0f};
+    if (t.m != neg_inf()) {
+        const Pair sc = pair(a.scale, a.scale), mm = pair(-t.m, -t.m), l2 = pair(LOG2E, LOG2E);
+        Pair s = 0, e = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float z[W];
+            Raw<T>::values(z, q[i]);
+#pragma unroll
+            for (int j = 0; j < W; j += 2) {
+                const float2 v = halves(fma2(pair(z[j], z[j + 1]), sc, mm));
+                const Pair d = pair(max_nan(v.x, -3.402823466e38f), max_nan(v.y, -3.402823466e38f));   // as in add_values
+                const float2 y = halves(mul2(d, l2));
+                const Pair w = pair(ex2(y.x), ex2(y.y));
+                s = add2(s, w);
+                e = fma2(w, d, e);
+            }
+        }
+        const float2 sv = halves(s), ev = halves(e);
+        t.s = sv.x + sv.y;
+        t.e = ev.x + ev.y;
+    }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) {
         t.s += __shfl_xor_sync(FULL, t.s, o);
         t.e += __shfl_xor_sync(FULL, t.e, o);
     }
-    if (real && lane == 0) write_row(a, r, g, t);
+    if (at < a.rows && lane == 0) write_row(a, r, g, t);
 }
 
 // blocks_per_row blocks a row (a thread-block cluster where there are several).  Entries are taken in vectors of W = 16 bytes from the
@@ -584,11 +626,12 @@ template <typename T> int forward(const T *logits, const FwdArgs &a, cudaStream_
             B2_CUDA(cudaGetLastError());
             return B2_OK;
         };
-        if (a.vocab <= 4 * 20) return go(logprob_rows_kernel<T, 4, 20>, 4);
-        if (a.vocab <= 4 * 36) return go(logprob_rows_kernel<T, 4, 36>, 4);
-        if (a.vocab <= 8 * 36) return go(logprob_rows_kernel<T, 8, 36>, 8);
-        if (a.vocab <= 16 * 36) return go(logprob_rows_kernel<T, 16, 36>, 16);
-        return go(logprob_rows_kernel<T, 32, 32>, 32);
+        constexpr int W = 16 / sizeof(T), NV = W == 4 ? 9 : 5;
+        const int vecs = (a.vocab + W - 1) / W + 1;           // one more: a row may start inside a vector
+        if (vecs <= 4 * NV) return go(logprob_rows_kernel<T, 4, NV>, 4);
+        if (vecs <= 8 * NV) return go(logprob_rows_kernel<T, 8, NV>, 8);
+        if (vecs <= 16 * NV) return go(logprob_rows_kernel<T, 16, NV>, 16);
+        return go(logprob_rows_kernel<T, 32, NV>, 32);
     }
     if (a.vocab <= 1024) {
         const long long blocks = (a.rows + 7) / 8;
@@ -624,24 +667,37 @@ struct BwdArgs {
     float scale;
 };
 // fp32 gradients with the exponential of the full accuracy, 16-bit ones with the hardware's: its error of 2^-22 is lost in their rounding
-template <typename T> __device__ __forceinline__ float exp_for(float x) { return sizeof(T) == 4 ? expf(x) : ex2(x * LOG2E); }
-
-struct RowGrad { float lse, g, h, H; int tok; };
-template <typename T, bool ENT> __device__ __forceinline__ float entry_grad(const RowGrad &q, float x, float scale, bool on, int i) {
-    if (!on) return 0.0f;
-    const float lp = __fmul_rn(x, scale) - q.lse;
-    const float p = exp_for<T>(lp);
-    float d = -q.g * p;
-    // p = 0 has no share in the entropy's gradient, whatever log p is; NaN stays
-    if (ENT) d = p == 0.0f ? d : fmaf(-q.h * p, lp + q.H, d);
-    if (i == q.tok) d += q.g;
-    return d * scale;
+template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
+    const float2 v = halves(sizeof(T) == 4 ? x : mul2(x, pair(LOG2E, LOG2E)));
+    return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
+}
+// What a row's entries share: dx = p (c0 + c1 log p) with c0 = -s (g + h H), c1 = -s h, and s g more at the token.
+struct RowGrad { float neg_lse, c0, c1, at_token; int tok; };
+// N entries from index i0 on
+template <typename T, int N, bool ENT> __device__ __forceinline__ void entry_grads(float (&o)[N], const float (&x)[N], const RowGrad &q, float scale, int i0) {
+    const Pair sc = pair(scale, scale), nl = pair(q.neg_lse, q.neg_lse), c0 = pair(q.c0, q.c0), c1 = pair(q.c1, q.c1);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        Pair lp = fma2(pair(x[j], x[j + 1]), sc, nl);
+        if (ENT) {
+            // below -1000 the probability is 0 whatever the logarithm is; -inf must not meet that 0
+            const float2 v = halves(lp);
+            lp = pair(max_nan(v.x, -1000.0f), max_nan(v.y, -1000.0f));
+        }
+        const float2 d = halves(mul2(exp_pair<T>(lp), ENT ? fma2(lp, c1, c0) : c0));
+        o[j] = d.x;
+        o[j + 1] = d.y;
+    }
+    if ((unsigned)(q.tok - i0) < (unsigned)N)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (i0 + j == q.tok) o[j] += q.at_token;
 }
 
-// Threads go over (row, vector) pairs: tpr threads a row, each up to U vectors apart by tpr.
-template <typename T, bool ENT, bool MASK>
+// tpr threads a row, each up to U vectors apart by tpr; a long row takes several blocks.  Bound by memory (5 to 6 issue slots an entry).
+template <typename T, bool ENT, bool MASK, int U>
 __global__ void __launch_bounds__(256) logprob_backward_kernel(T *__restrict__ dlogits, const T *logits, const BwdArgs a, int tpr, int segs) {
-    constexpr int W = 16 / sizeof(T), U = 2;
+    constexpr int W = 16 / sizeof(T);
     const int per_block = 256 / tpr;
     // a row of several segments takes whole blocks (tpr = 256)
     const long long r = segs > 1 ? (long long)(blockIdx.x / (unsigned)segs) : (long long)blockIdx.x * per_block + threadIdx.x / tpr;
@@ -651,68 +707,76 @@ __global__ void __launch_bounds__(256) logprob_backward_kernel(T *__restrict__ d
     T *d = dlogits + r * a.ld_out;
     const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
     const bool out_vec = (((uintptr_t)(d - mis)) & 15) == 0;
+    const int first = seg * tpr * U + (threadIdx.x & (tpr - 1));
+    const auto whole = [&](int v) { return v * W >= mis && (v + 1) * W <= mis + a.vocab; };
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (whole(first + u * tpr)) raw[u] = *reinterpret_cast<const uint4 *>(x - mis + (size_t)(first + u * tpr) * W);
     RowGrad q;
     q.tok = __ldg(a.tokens + r);
-    q.lse = __ldg(a.lse + r);
-    q.g = a.dlogprob ? __ldg(a.dlogprob + r) : 0.0f;
-    q.h = ENT ? __ldg(a.dentropy + r) : 0.0f;
-    q.H = ENT ? __ldg(a.entropy + r) : 0.0f;
+    const float lse = __ldg(a.lse + r), g = a.dlogprob ? __ldg(a.dlogprob + r) : 0.0f, h = ENT ? __ldg(a.dentropy + r) : 0.0f;
+    q.neg_lse = -lse;
+    q.c0 = -a.scale * (ENT ? fmaf(h, __ldg(a.entropy + r), g) : g);
+    q.c1 = -a.scale * h;
+    q.at_token = a.scale * g;
     // padding, and a row that allows nothing: no gradient.  A token beyond the vocabulary shows as NaN, as its log probability does.
-    const bool zero = q.tok < 0 || q.lse == neg_inf();
-    const float bad = q.tok >= a.vocab ? nanf("") : 0.0f;
+    const bool zero = q.tok < 0 || lse == neg_inf();
+    if (q.tok >= a.vocab) q.c0 = nanf("");
     const unsigned char *mk = MASK ? a.mask + r * a.ld_mask : nullptr;
     const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
-    const int first = seg * tpr * U + (threadIdx.x & (tpr - 1));
-    float z[U][W];
-    bool whole[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int v = first + u * tpr;
-        whole[u] = v * W >= mis && (v + 1) * W <= mis + a.vocab;
-        if (whole[u] && !zero) load_vec<T, W>(z[u], x - mis + (size_t)v * W);
-    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int v = first + u * tpr, i0 = v * W - mis;
-        if (whole[u]) {
-            unsigned char on[W];
-            if (MASK) {
-                if (mask_vec) *reinterpret_cast<Vec<unsigned char, W> *>(on) = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
-                else {
+        if (i0 >= a.vocab) break;
+        const bool inside = whole(v);
+        float z[W], o[W];
+        if (inside) Raw<T>::values(z, raw[u]);
+        else
 #pragma unroll
-                    for (int j = 0; j < W; ++j) on[j] = mk[i0 + j];
-                }
-            }
-            float o[W];
+            for (int j = 0; j < W; ++j) z[j] = i0 + j >= 0 && i0 + j < a.vocab ? to_float(x[i0 + j]) : 0.0f;
+        if (zero) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) o[j] = zero ? 0.0f : entry_grad<T, ENT>(q, z[u][j], a.scale, !MASK || on[j], i0 + j) + bad;
-            if (out_vec) store_vec<T, W>(d + i0, o);
-            else {
-#pragma unroll
-                for (int j = 0; j < W; ++j) d[i0 + j] = from_float<T>(o[j]);
-            }
+            for (int j = 0; j < W; ++j) o[j] = 0.0f;
         } else {
-            for (int j = 0; j < W; ++j) {
-                const int i = i0 + j;
-                if (i < 0 || i >= a.vocab) continue;
-                d[i] = from_float<T>(zero ? 0.0f : entry_grad<T, ENT>(q, to_float(x[i]), a.scale, !MASK || mk[i], i) + bad);
+            entry_grads<T, W, ENT>(o, z, q, a.scale, i0);
+            if (MASK) {
+                Vec<unsigned char, W> on;
+                if (inside && mask_vec) on = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
+                else
+#pragma unroll
+                    for (int j = 0; j < W; ++j) on.v[j] = i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
+#pragma unroll
+                for (int j = 0; j < W; ++j) o[j] = on.v[j] ? o[j] : 0.0f;
             }
         }
+        if (inside && out_vec) store_vec<T, W>(d + i0, o);
+        else
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (i0 + j >= 0 && i0 + j < a.vocab) d[i0 + j] = from_float<T>(o[j]);
     }
 }
 
 template <typename T, bool ENT, bool MASK> int backward(T *dlogits, const T *logits, const BwdArgs &a, cudaStream_t st) {
-    constexpr int W = 16 / sizeof(T), U = 2;
+    constexpr int W = 16 / sizeof(T);
     const int vecs = (a.vocab + W - 1) / W + 1;               // one more: a row may start inside a vector
-    unsigned tpr = pow2_at_least((unsigned)((vecs + U - 1) / U));
-    if (tpr > 256) tpr = 256;
-    const int segs = (vecs + (int)tpr * U - 1) / ((int)tpr * U);
-    const long long per = 256 / tpr, blocks = (a.rows * segs + per - 1) / per;
-    if (blocks > 0x7fffffffll) { set_error("b2_logprob_backward: %lld rows of %d", a.rows, a.vocab); return B2_ERR_BAD_SHAPE; }
-    logprob_backward_kernel<T, ENT, MASK><<<(unsigned)blocks, 256, 0, st>>>(dlogits, logits, a, (int)tpr, segs);
-    count_launch();
-    B2_CUDA(cudaGetLastError());
-    return B2_OK;
+    const auto go = [&](auto vectors) -> int {
+        constexpr int U = decltype(vectors)::value;
+        unsigned tpr = pow2_at_least((unsigned)((vecs + U - 1) / U));
+        if (tpr > 256) tpr = 256;
+        const int segs = (vecs + (int)tpr * U - 1) / ((int)tpr * U);
+        const long long per = 256 / tpr, blocks = (a.rows * segs + per - 1) / per;
+        if (blocks > 0x7fffffffll) { set_error("b2_logprob_backward: %lld rows of %d", a.rows, a.vocab); return B2_ERR_BAD_SHAPE; }
+        logprob_backward_kernel<T, ENT, MASK, U><<<(unsigned)blocks, 256, 0, st>>>(dlogits, logits, a, (int)tpr, segs);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+        return B2_OK;
+    };
+    // Vectors of a thread: 2 where the rows do not fill the device (16 rows of 32003: 2.7 us, with 8 4.0 us), else 8 (8192 rows: 167 us, with 4 172 us,
+    // with 2 211 us), with a mask 4 (300 us, with 8 337 us)
+    if ((double)a.rows * vecs < 4096.0 * sm_count()) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, MASK ? 4 : 8>());
 }
 
 int check(const char *who, const void *logits, int type, long long rows, int vocab, long long ld, const unsigned char *mask, long long ld_mask, float scale) {

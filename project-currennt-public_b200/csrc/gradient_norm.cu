@@ -3,7 +3,7 @@
 //   n = sqrt(sum_i sum_j x_ij^2),   out_ij = x_ij * (n > max ? max / n : 1)
 //
 // The list travels as a kernel argument: no table in device memory, no copy, nothing kept between calls.  Every tensor is cut
-// into chunks of CHUNK elements that start on 16-byte boundaries; a block takes a contiguous range of all chunks, so it looks up
+// into chunks of CHUNK bytes that start on 16-byte boundaries; a block takes a contiguous range of all chunks, so it looks up
 // its first tensor once.  Squares are summed in fp64: the square of any finite fp32 value is a normal fp64 number, so neither large
 // nor tiny gradients need a scale, and the order of the sums (thread, block, launch) is fixed.
 // Bound by memory: one read for the norm, one read and one write for the scaled tensors.  The second kernel walks each range
@@ -16,7 +16,7 @@ namespace b2 {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;
+constexpr int CHUNK = 16384;       // bytes
 constexpr int MAX_BLOCKS = 2048;   // partial sums in the workspace
 
 template <int CAP> struct List {
@@ -49,34 +49,65 @@ __device__ __forceinline__ double block_sum(double x, double *red) {
     return s;
 }
 
-// sum of squares of one chunk; positions are counted from the 16-byte boundary at or below the tensor's start
-template <typename T> __device__ __forceinline__ double chunk_squares(const T *p, unsigned long long count, unsigned chunk) {
-    constexpr int W = 16 / sizeof(T);
-    const int mis = (int)(((uintptr_t)p & 15) / sizeof(T));
-    const T *base = p - mis;
-    const unsigned long long lo = mis, hi = mis + count, at = (unsigned long long)chunk * CHUNK;
-    double s = 0.0;
-    if (at >= lo && at + CHUNK <= hi) {
-        constexpr int N = CHUNK / (THREADS * W);
-        float v[N][W];
+// One chunk of a tensor: bytes [at, at + CHUNK), counted from the 16-byte boundary at or below the tensor's start, `mis` bytes before it.
+struct Piece {
+    const char *src;
+    char *dst;
+    unsigned long long bytes, at;   // of the tensor; of the chunk
+    int mis, src_type, dst_type;
+    bool whole;                     // every byte of the chunk is the tensor's
+};
+template <int CAP> __device__ __forceinline__ Piece piece_of(const List<CAP> &l, int i, unsigned chunk) {
+    Piece p;
+    p.src_type = l.src_type[i];
+    p.dst_type = l.dst_type[i];
+    p.src = (const char *)l.src[i];
+    p.dst = (char *)l.dst[i];
+    p.bytes = l.count[i] << (p.src_type == B2_F32 ? 2 : 1);
+    p.at = (unsigned long long)(chunk - l.first[i]) * CHUNK;
+    p.mis = (int)((uintptr_t)p.src & 15);
+    p.whole = p.at >= (unsigned)p.mis && p.at + CHUNK <= p.mis + p.bytes;
+    return p;
+}
+constexpr int VECTORS = CHUNK / (16 * THREADS);   // of a thread, THREADS vectors apart
+__device__ __forceinline__ unsigned long long place(const Piece &p, int i) { return p.at + (unsigned)(i * THREADS + threadIdx.x) * 16u; }
+__device__ __forceinline__ bool inside(const Piece &p, unsigned long long at) { return p.whole || (at >= (unsigned)p.mis && at + 16 <= p.mis + p.bytes); }
+// A vector that the tensor has only a part of is gathered by 2 bytes, zeros elsewhere; all of them lie at a tensor's two ends.
+__device__ __forceinline__ void fetch(uint4 (&q)[VECTORS], const Piece &p) {
+    const char *base = p.src - p.mis;
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_vec<T, W>(v[i], base + at + (size_t)(i * THREADS + threadIdx.x) * W);
+    for (int i = 0; i < VECTORS; ++i) {
+        const unsigned long long at = place(p, i), end = p.mis + p.bytes;
+        if (inside(p, at)) q[i] = *reinterpret_cast<const uint4 *>(base + at);
+        else {
+            unsigned w[4] = {0, 0, 0, 0};
+            if (at < end && at + 16 > (unsigned)p.mis)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < W; ++j) { const double x = v[i][j]; s = fma(x, x, s); }
-    } else {
-        const unsigned long long end = at + CHUNK < hi ? at + CHUNK : hi;
-        for (unsigned long long e = (at > lo ? at : lo) + threadIdx.x; e < end; e += THREADS) {
-            const double x = to_float(base[e]);
-            s = fma(x, x, s);
+                for (int j = 0; j < 8; ++j)
+                    if (at + 2 * j >= (unsigned)p.mis && at + 2 * j < end) w[j / 2] |= (unsigned)*reinterpret_cast<const unsigned short *>(base + at + 2 * j) << (16 * (j & 1));
+            q[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
+    }
+}
+template <typename T, int W> __device__ __forceinline__ void values(float (&v)[W], const uint4 &q) {
+    const Vec<T, W> x = *reinterpret_cast<const Vec<T, W> *>(&q);
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = to_float(x.v[j]);
+}
+template <typename T> __device__ __forceinline__ double squares(const uint4 (&q)[VECTORS], double s) {
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < VECTORS; ++i) {
+        float v[W];
+        values<T, W>(v, q[i]);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { const double x = v[j]; s = fma(x, x, s); }
     }
     return s;
 }
 
-// partial[block] (+)= the squares of the block's chunks
-template <int CAP> __global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ List<CAP> l, double *__restrict__ partial, int add) {
+// partial[block] (+)= the squares of the block's chunks; the next chunk is on its way while one is added up
+template <int CAP> __global__ void __launch_bounds__(THREADS, 3) squares_kernel(const __grid_constant__ List<CAP> l, double *__restrict__ partial, int add) {
     __shared__ double red[THREADS / 32];
     grid_wait();
     grid_release();
@@ -85,12 +116,21 @@ template <int CAP> __global__ void __launch_bounds__(THREADS) squares_kernel(con
     double s = 0.0;
     if (c0 < c1) {
         int i = find_tensor(l, c0);
+        Piece now = piece_of(l, i, c0), next = now;
+        uint4 q[VECTORS], r[VECTORS];
+        fetch(q, now);
         for (unsigned c = c0; c < c1; ++c) {
-            while (c >= l.first[i + 1]) ++i;
-            const unsigned k = c - l.first[i];
-            if (l.src_type[i] == B2_F32) s += chunk_squares((const float *)l.src[i], l.count[i], k);
-            else if (l.src_type[i] == B2_BF16) s += chunk_squares((const __nv_bfloat16 *)l.src[i], l.count[i], k);
-            else s += chunk_squares((const __half *)l.src[i], l.count[i], k);
+            if (c + 1 < c1) {
+                while (c + 1 >= l.first[i + 1]) ++i;
+                next = piece_of(l, i, c + 1);
+                fetch(r, next);
+            }
+            if (now.src_type == B2_F32) s = squares<float>(q, s);
+            else if (now.src_type == B2_BF16) s = squares<__nv_bfloat16>(q, s);
+            else s = squares<__half>(q, s);
+            now = next;
+#pragma unroll
+            for (int j = 0; j < VECTORS; ++j) q[j] = r[j];
         }
     }
     s = block_sum(s, red);
@@ -100,62 +140,74 @@ template <int CAP> __global__ void __launch_bounds__(THREADS) squares_kernel(con
 // the norm from the partial sums; every block of a launch adds them in the same order
 __device__ __forceinline__ double norm_of(const double *partial, int n, double *red) {
     double s = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += THREADS) s += partial[i];
     return sqrt(block_sum(s, red));
 }
 
-template <typename T, typename U>
-__device__ __forceinline__ void scale_chunk(U *q, const T *p, unsigned long long count, unsigned chunk, float coef) {
+// scaled vectors to where they came from
+template <typename T, typename U> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], float coef) {
     constexpr int W = 16 / sizeof(T);
-    const int mis = (int)(((uintptr_t)p & 15) / sizeof(T));
-    const T *base = p - mis;
-    U *to = q - mis;
-    const unsigned long long lo = mis, hi = mis + count, at = (unsigned long long)chunk * CHUNK;
-    // the output's vectors: W elements of its own type, 16 bytes at most an access
+    // elements are counted from the 16-byte boundary; in the output's type its vectors may lie off theirs
+    U *to = reinterpret_cast<U *>(p.dst) - p.mis / (int)sizeof(T);
     const bool fits = ((uintptr_t)to & (sizeof(U) * W < 16 ? sizeof(U) * W - 1 : 15)) == 0;
-    if (at >= lo && at + CHUNK <= hi && fits) {
-        constexpr int N = CHUNK / (THREADS * W);
-        float v[N][W];
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_vec<T, W>(v[i], base + at + (size_t)(i * THREADS + threadIdx.x) * W);
+    for (int i = 0; i < VECTORS; ++i) {
+        const unsigned long long at = place(p, i), end = p.mis + p.bytes;
+        float v[W];
+        values<T, W>(v, q[i]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int j = 0; j < W; ++j) v[j] *= coef;
+        if (fits && inside(p, at)) store_vec<U, W>(to + at / sizeof(T), v);
+        else if (at < end && at + 16 > (unsigned)p.mis)
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[i][j] *= coef;
-            store_vec<U, W>(to + at + (size_t)(i * THREADS + threadIdx.x) * W, v[i]);
-        }
-    } else {
-        const unsigned long long end = at + CHUNK < hi ? at + CHUNK : hi;
-        for (unsigned long long e = (at > lo ? at : lo) + threadIdx.x; e < end; e += THREADS) to[e] = from_float<U>(to_float(base[e]) * coef);
+            for (int j = 0; j < W; ++j)
+                if (at + j * sizeof(T) >= (unsigned)p.mis && at + j * sizeof(T) < end) to[at / sizeof(T) + j] = from_float<U>(v[j]);
     }
 }
-template <typename T> __device__ __forceinline__ void scale_chunk_to(void *q, int type, const T *p, unsigned long long count, unsigned chunk, float coef) {
-    if (type == B2_F32) scale_chunk((float *)q, p, count, chunk, coef);
-    else if (type == B2_BF16) scale_chunk((__nv_bfloat16 *)q, p, count, chunk, coef);
-    else scale_chunk((__half *)q, p, count, chunk, coef);
+template <typename T> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], float coef) {
+    if (p.dst_type == B2_F32) put<T, float>(p, q, coef);
+    else if (p.dst_type == B2_BF16) put<T, __nv_bfloat16>(p, q, coef);
+    else put<T, __half>(p, q, coef);
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(THREADS) clip_kernel(const __grid_constant__ List<CAP> l, const double *__restrict__ partial, int n_partial, float max_norm,
-                                                       float *__restrict__ norm_out) {
+__global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant__ List<CAP> l, const double *__restrict__ partial, int n_partial, float max_norm,
+                                                          float *__restrict__ norm_out) {
     __shared__ double red[THREADS / 32];
+    const unsigned total = l.first[l.n];
+    const unsigned c0 = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x), c1 = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
+    int i = 0;
+    Piece now = {}, next;
+    uint4 q[VECTORS], r[VECTORS];
+    if (c0 < c1) {
+        // The first chunk is read before the wait: this kernel starts when all blocks of the one before have passed theirs, so what they
+        // read is complete.  Nothing is written before the wait: they may still be reading.
+        i = find_tensor(l, c1 - 1);
+        now = piece_of(l, i, c1 - 1);
+        fetch(q, now);
+    }
     grid_wait();
     const double norm = norm_of(partial, n_partial, red);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     // a norm that is no finite number says nothing about a scale: the values stay as they are
     const bool scale = norm > (double)max_norm && norm <= 1.7976931348623157e308;
     const float coef = scale ? (float)((double)max_norm / norm) : 1.0f;
-    const unsigned total = l.first[l.n];
-    const unsigned c0 = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x), c1 = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
-    if (c0 >= c1) return;
-    int i = find_tensor(l, c1 - 1);
+    next = now;
     for (unsigned c = c1; c-- > c0;) {
-        while (c < l.first[i]) --i;
-        if (!scale && l.src[i] == l.dst[i]) continue;
-        const unsigned k = c - l.first[i];
-        if (l.src_type[i] == B2_F32) scale_chunk_to(l.dst[i], l.dst_type[i], (const float *)l.src[i], l.count[i], k, coef);
-        else if (l.src_type[i] == B2_BF16) scale_chunk_to(l.dst[i], l.dst_type[i], (const __nv_bfloat16 *)l.src[i], l.count[i], k, coef);
-        else scale_chunk_to(l.dst[i], l.dst_type[i], (const __half *)l.src[i], l.count[i], k, coef);
+        if (c > c0) {
+            while (c - 1 < l.first[i]) --i;
+            next = piece_of(l, i, c - 1);
+            if (scale || next.src != next.dst) fetch(r, next);
+        }
+        if (scale || now.src != now.dst) {
+            if (now.src_type == B2_F32) put<float>(now, q, coef);
+            else if (now.src_type == B2_BF16) put<__nv_bfloat16>(now, q, coef);
+            else put<__half>(now, q, coef);
+        }
+        now = next;
+#pragma unroll
+        for (int j = 0; j < VECTORS; ++j) q[j] = r[j];
     }
 }
 
@@ -186,8 +238,7 @@ template <int CAP> bool fill(List<CAP> &l, const b2_tensor *src, const b2_tensor
     for (; *at < n && k < CAP; ++*at) {
         const b2_tensor &s = src[*at], &d = dst[*at];
         if (!s.count) continue;
-        const size_t mis = ((uintptr_t)s.data & 15) / type_size(s.type);
-        const unsigned long long c = (mis + s.count + CHUNK - 1) / CHUNK;
+        const unsigned long long c = (((uintptr_t)s.data & 15) + s.count * type_size(s.type) + CHUNK - 1) / CHUNK;
         if (k && chunks + c > 0xfffffffeull) break;
         chunks += c;
         l.src[k] = s.data;
@@ -202,8 +253,8 @@ template <int CAP> bool fill(List<CAP> &l, const b2_tensor *src, const b2_tensor
 }
 
 int grid_of(unsigned chunks) {
-    // blocks that are resident together (8 of 256 threads per multiprocessor), one chunk each at least
-    const unsigned most = (unsigned)(sm_count() * 8 < MAX_BLOCKS ? sm_count() * 8 : MAX_BLOCKS);
+    // blocks that are resident together (3 of 256 threads per multiprocessor), one chunk each at least
+    const unsigned most = (unsigned)(sm_count() * 3 < MAX_BLOCKS ? sm_count() * 3 : MAX_BLOCKS);
     return (int)(chunks < most ? chunks : most);
 }
 

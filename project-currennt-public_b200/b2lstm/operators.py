@@ -10,17 +10,22 @@ import ctypes as C
 from .lib import B2Error, _check, lib
 
 _CODES = {"float32": 0, "bfloat16": 1, "float16": 2}
-_types = {}
+_F32, _I32, _BYTES = ("float32",), ("int32",), ("uint8", "int8", "bool")
+_names = {}     # the name of a dtype, looked up once
+
+
+def _name(dtype):
+    name = _names.get(dtype)
+    if name is None:
+        name = _names[dtype] = str(dtype).split(".")[-1]
+    return name
 
 
 def _type(t):
     """element type code of a tensor"""
-    code = _types.get(t.dtype)
+    code = _CODES.get(_names.get(t.dtype) or _name(t.dtype))
     if code is None:
-        code = _CODES.get(str(t.dtype).split(".")[-1])
-        if code is None:
-            raise B2Error("element type %s (float32, bfloat16 or float16)" % t.dtype)
-        _types[t.dtype] = code
+        raise B2Error("element type %s (float32, bfloat16 or float16)" % t.dtype)
     return code
 
 
@@ -35,10 +40,11 @@ def _rows(t, name, rows=None, cols=None, like=None):
         raise B2Error("%s is not on the GPU" % name)
     if like is not None and t.dtype != like:
         raise B2Error("%s has the element type %s, not %s" % (name, t.dtype, like))
+    n, width = shape
     ld, unit = t.stride()
-    if (unit != 1 and shape[1] > 1) or (ld < shape[1] and shape[0] > 1):
+    if (unit != 1 and width > 1) or (ld < width and n > 1):
         raise B2Error("%s has the strides (%d, %d): its rows have to be contiguous and apart" % (name, ld, unit))
-    return t.data_ptr(), max(ld, shape[1])
+    return t.data_ptr(), ld if ld > width else width
 
 
 def _vector(t, name, n, dtype):
@@ -47,14 +53,11 @@ def _vector(t, name, n, dtype):
         return None
     if not t.is_cuda:
         raise B2Error("%s is not on the GPU" % name)
-    if str(t.dtype).split(".")[-1] not in dtype:
+    if (_names.get(t.dtype) or _name(t.dtype)) not in dtype:
         raise B2Error("%s has the element type %s, not %s" % (name, t.dtype, " or ".join(dtype)))
     if t.numel() != n or not t.is_contiguous():
         raise B2Error("%s has the shape %s and strides %s, not %d contiguous elements" % (name, tuple(t.shape), tuple(t.stride()), n))
     return t.data_ptr()
-
-
-_F32, _I32, _BYTES = ("float32",), ("int32",), ("uint8", "int8", "bool")
 
 
 def _workspace(t):
@@ -144,7 +147,7 @@ def _mask(mask, rows, vocab):
         return None, 0
     if len(mask.shape) == 1:
         return _vector(mask, "mask", vocab, _BYTES), 0
-    if str(mask.dtype).split(".")[-1] not in _BYTES:
+    if _name(mask.dtype) not in _BYTES:
         raise B2Error("mask has the element type %s" % mask.dtype)
     return _rows(mask, "mask", rows, vocab)
 

@@ -325,6 +325,13 @@ int b2_net_update_weights(b2_net *net, float learning_rate, float momentum);
  * reference's Optimizer constructor does (Optimizer.cu:421-457).  With a data-parallel communicator
  * attached the frame count is summed over the ranks. */
 int b2_net_set_optimizer(b2_net *net, int option);
+/* Clipping by the global norm (no counterpart in the reference): with max_norm > 0 every later update first scales the weightUpdates of all
+ * layers by min(1, max_norm / norm), norm = the L2 norm over all of them (b2_gradient_clip; after the sum over the ranks of a data-parallel
+ * job and over the fractions of batch learning, before the shaping options).  0, the default, switches it off.  A norm that is no finite
+ * number scales nothing: the update zeroes the entries that are not.  b2_net_gradient_norm: the norm of the last such update, before
+ * scaling (synchronises; B2_ERR_STATE before clipping was first switched on). */
+int b2_net_set_gradient_clipping(b2_net *net, float max_norm);
+int b2_net_gradient_norm(b2_net *net, float *norm);
 /* Optimizer::m_weightStats of one layer (AdaGrad: one float per weight; Adam: m and v interleaved),
  * the "optimizer_status_vector" of an autosave.  host_out may be NULL to ask for *count only. */
 int b2_net_get_optimizer_stats(b2_net *net, int layer, float *host_out, size_t capacity, size_t *count);

@@ -86,6 +86,8 @@ SIGNATURES = {
     "b2_net_forward": (C.c_int, [C.c_void_p, C.POINTER(C.c_double)]),
     "b2_net_backward": (C.c_int, [C.c_void_p]),
     "b2_net_update_weights": (C.c_int, [C.c_void_p, C.c_float, C.c_float]),
+    "b2_net_set_gradient_clipping": (C.c_int, [C.c_void_p, C.c_float]),
+    "b2_net_gradient_norm": (C.c_int, [C.c_void_p, C.POINTER(C.c_float)]),
     "b2_net_set_optimizer": (C.c_int, [C.c_void_p, C.c_int]),
     "b2_net_get_optimizer_stats": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.POINTER(C.c_size_t)]),
     "b2_net_accumulate_weight_updates": (C.c_int, [C.c_void_p, C.c_int]),
@@ -342,6 +344,16 @@ class Net:
 
     def update_weights(self, lr, momentum):
         _check(lib().b2_net_update_weights(self.h, lr, momentum))
+
+    def set_gradient_clipping(self, max_norm):
+        """scale the gradients of every later update down to this norm over all layers (0: off)"""
+        _check(lib().b2_net_set_gradient_clipping(self.h, max_norm))
+
+    def gradient_norm(self):
+        """norm of the last update's gradients before scaling"""
+        v = C.c_float()
+        _check(lib().b2_net_gradient_norm(self.h, C.byref(v)))
+        return v.value
 
     def train_step(self, lens, inputs, targets, lr, momentum, want_error=True):
         """inputs/targets: host arrays (numpy, or pinned torch CPU tensors via .numpy())."""

@@ -260,7 +260,7 @@ int SsePostOutputLayer::computeBackwardPass(int) {
 NeuralNetwork::~NeuralNetwork() {
     if (dp) dp_detach(*this);
     layers.clear();
-    cudaFree(ws); cudaFree(statusDev); cudaFree(fracLenDev);
+    cudaFree(ws); cudaFree(statusDev); cudaFree(fracLenDev); cudaFree(clipDev);
     for (int b = 0; b < 2; ++b) {
         cudaFree(inBuf[b]); cudaFree(tgBuf[b]); cudaFree(patBuf[b]); cudaFree(mapBuf[b]); cudaFree(lenBuf[b]);
         if (lenPinned[b]) cudaFreeHost(lenPinned[b]);
@@ -602,8 +602,33 @@ int NeuralNetwork::setOptimizerOption(int option) {
     return B2_OK;
 }
 
+// Gradients scaled down to a largest norm over all layers before every update; the summed ones of a data-parallel job, so that every rank
+// takes the same factor
+int NeuralNetwork::setGradientClipping(float maxNorm) {
+    if (!(maxNorm >= 0.0f)) { set_error("b2_net_set_gradient_clipping: the largest norm is %g", (double)maxNorm); return B2_ERR_BAD_ARG; }
+    if (maxNorm > 0.0f && !clipDev) {
+        B2_CUDA(cudaMalloc(&clipDev, 256 + b2_gradient_norm_workspace()));
+        B2_CUDA(cudaMemsetAsync(clipDev, 0, sizeof(float), stream));
+    }
+    maxGradientNorm = maxNorm;
+    return B2_OK;
+}
+int NeuralNetwork::readGradientNorm(float *norm) {
+    if (!clipDev) { set_error("b2_net_gradient_norm: gradients are not clipped"); return B2_ERR_STATE; }
+    B2_CUDA(cudaMemcpyAsync(norm, clipDev, sizeof(float), cudaMemcpyDeviceToHost, stream));
+    B2_CUDA(cudaStreamSynchronize(stream));
+    return B2_OK;
+}
+
 int NeuralNetwork::updateWeights(float lr, float mom) {
     ProfScope ps(*this, "sgd_update");
+    if (maxGradientNorm > 0.0f) {
+        std::vector<b2_tensor> grads;
+        for (size_t i = 0; i < layers.size(); ++i)
+            if (TrainableLayer *t = dynamic_cast<TrainableLayer *>(layers[i].get())) grads.push_back({t->weightUpdates(), t->numWeights(), B2_F32});
+        B2_TRY(b2_gradient_clip(grads.data(), nullptr, (int)grads.size(), maxGradientNorm, (float *)clipDev, (char *)clipDev + 256,
+                                b2_gradient_norm_workspace(), (b2_stream)stream));
+    }
     // option 4 (OPTIMIZATION_SGD_DECAY) updates like plain SGD; its schedule lives in the training run (b2_optimizer_train)
     const bool adjust = optOption > 0 && optOption != 4;
     if (adjust) {
@@ -801,6 +826,8 @@ int b2_net_update_weights_batch(b2_net *n, float lr, float mom) { return n ? n->
 int b2_net_backward_empty(b2_net *n) { return n ? n->net.computeBackwardPassEmpty() : B2_ERR_BAD_ARG; }
 int b2_net_train_step_empty(b2_net *n, float lr, float mom) { return n ? n->net.trainStepEmpty(lr, mom) : B2_ERR_BAD_ARG; }
 int b2_dp_world_size(const b2_net *n) { return n ? dp_world(n->net) : 1; }
+int b2_net_set_gradient_clipping(b2_net *n, float max_norm) { return n ? n->net.setGradientClipping(max_norm) : B2_ERR_BAD_ARG; }
+int b2_net_gradient_norm(b2_net *n, float *norm) { return n && norm ? n->net.readGradientNorm(norm) : B2_ERR_BAD_ARG; }
 int b2_net_set_optimizer(b2_net *n, int option) { return n ? n->net.setOptimizerOption(option) : B2_ERR_BAD_ARG; }
 int b2_net_get_optimizer_stats(b2_net *n, int i, float *host, size_t capacity, size_t *count) {
     TrainableLayer *t = trainable(n, i);

@@ -158,6 +158,8 @@ public:
     int computeForwardPass();
     int calculateError(double *hostError);
     int computeBackwardPass();
+    int setGradientClipping(float maxNorm);
+    int readGradientNorm(float *norm);
     int updateWeights(float lr, float mom);
     // data-parallel step of a rank that has no sequence in the current fraction: zero gradients into the sums, update
     int computeBackwardPassEmpty();
@@ -171,6 +173,8 @@ public:
     int optOption = 0;
     float adamBeta1Accum = 1.0f, adamBeta2Accum = 1.0f;
     float *fracLenDev = nullptr;
+    float maxGradientNorm = 0.0f;      // 0: gradients are not clipped
+    void *clipDev = nullptr;           // norm of the last update's gradients (first float), workspace from byte 256 on
     int synchronize();
 
     std::vector<std::unique_ptr<Layer> > layers;

@@ -751,3 +751,86 @@ def test_refusals(tm):
     assert L.b2_logprob_forward(x.data_ptr(), 0, -1, 16, 16, None, 0, 1.0, None, None, st.data_ptr(), None, 0, None, None, None) == -1
     assert L.b2_logprob_forward(x.data_ptr(), 0, 4, 16, 15, None, 0, 1.0, None, None, st.data_ptr(), None, 0, None, None, None) == -5
     assert L.b2_gradient_norm(None, 3, st.data_ptr(), ws.data_ptr(), ws.numel(), None) == -5
+
+
+# ---- large buffers, streams --------------------------------------------------------------------------------------------------------------------
+def test_offsets_beyond_32_bits(tm):
+    """rows 2^30 and more elements apart, a tensor of more than 2^32 elements: the last rows and elements are the ones that would go astray"""
+    torch, b2 = tm
+    ld, dim = (1 << 30) + 8, 72
+
+    def wide(rows, cols, seed, dtype=torch.bfloat16):
+        t = torch.empty(rows * ld, dtype=dtype, device="cuda").view(rows, ld)[:, :cols]
+        t.copy_(torch.randn(rows, cols, generator=torch.Generator().manual_seed(seed)).to(dtype))
+        return t
+
+    tok = torch.tensor([2, 0, 3, 3], dtype=torch.int32, device="cuda")
+    table, out = wide(4, dim, 1), wide(4, dim, 2)
+    b2.embedding_forward(out, table, tok, 2.0)
+    assert torch.equal(out.contiguous(), table.contiguous()[tok.long()] * 2)
+    ws = torch.empty(b2.embedding_backward_workspace(4, 4, dim), dtype=torch.uint8, device="cuda")
+    b2.embedding_backward(table, out, tok, 1.0, workspace=ws)
+    want = torch.zeros(4, dim, device="cuda").index_add_(0, tok.long(), out.float())
+    assert torch.equal(table.float(), want.to(torch.bfloat16).float())
+    # rows of logits, and their gradient in place
+    x, small = wide(4, 3000, 3), None
+    small = x.contiguous()
+    for a in (x, small):
+        r = _run_logprob(tm, a, tok.cpu().numpy(), None, 1.0, 5)
+        b2.logprob_backward(a, a, tok, r[1], torch.ones(4, device="cuda"))
+        if a is x:
+            first = r
+    assert all(torch.equal(p, q) for p, q in zip(first, r)) and torch.equal(x.contiguous(), small)
+    del table, out, x, small
+    # norms
+    f, y, h = wide(3, dim, 4), wide(3, dim, 5), wide(3, dim, 6)
+    st, st2 = torch.empty(3, 4, device="cuda"), torch.empty(3, 4, device="cuda")
+    fs, ys, hs = (t.contiguous() for t in (f, y, h))
+    b2.block_norm_forward(y, f, y, h, stats=st)
+    b2.block_norm_forward(ys, fs, ys, hs, stats=st2)
+    assert torch.equal(y.contiguous(), ys) and torch.equal(h.contiguous(), hs) and torch.equal(st, st2)
+    ws = torch.empty(b2.block_norm_backward_workspace(3, dim), dtype=torch.uint8, device="cuda")
+    b2.block_norm_backward(h, f, h, None, None, f, st, workspace=ws)
+    b2.block_norm_backward(hs, fs, hs, None, None, fs, st2, workspace=ws)
+    assert torch.equal(h.contiguous(), hs) and torch.equal(f.contiguous(), fs)
+    del f, y, h
+    big = torch.zeros((1 << 32) + 21, dtype=torch.bfloat16, device="cuda")
+    big[0], big[-1], big[1 << 31] = 2.0, 3.0, 6.0
+    norm, ws = torch.zeros(1, device="cuda"), torch.empty(b2.gradient_norm_workspace(), dtype=torch.uint8, device="cuda")
+    b2.gradient_clip(b2.TensorList([big]), 3.5, norm, workspace=ws)
+    assert norm.item() == 7.0 and big[0] == 1.0 and big[-1] == 1.5 and big[1 << 31] == 3.0 and big[1:1 << 31].sum() == 0
+
+
+def test_every_operator_runs_on_the_callers_stream(tm):
+    """work on a side stream, behind a kernel that keeps it busy and writes the inputs last: an operator that ran elsewhere would read them too early"""
+    torch, b2 = tm
+    side = torch.cuda.Stream()
+    n, vocab, dim = 5000, 3000, 96
+    g = torch.Generator().manual_seed(3)
+    src = {"table": torch.randn(vocab, dim, generator=g).cuda(), "x": torch.randn(n, dim, generator=g).cuda(), "logits": torch.randn(n, vocab, generator=g).cuda()}
+    tok = torch.randint(-1, vocab, (n,), generator=g).int().cuda()
+    ws = torch.empty(max(b2.embedding_backward_workspace(n, vocab, dim), b2.block_norm_backward_workspace(n, dim), b2.gradient_norm_workspace()), dtype=torch.uint8, device="cuda")
+
+    def run(late, handle):
+        t = {k: torch.zeros_like(v) for k, v in src.items()}
+        o = {k: torch.zeros(s, device="cuda") for k, s in dict(e=(n, dim), y=(n, dim), h=(n, dim), st=(n, 4), lp=(n,), lse=(n,), dt=(vocab, dim), dx=(n, dim), df=(n, dim),
+                                                               norm=(1,), dl=(n, vocab)).items()}
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side if handle else torch.cuda.current_stream()):
+            if late:
+                torch.cuda._sleep(20_000_000)
+            for k in src:
+                t[k].copy_(src[k])
+            b2.embedding_forward(o["e"], t["table"], tok, stream=handle)
+            b2.block_norm_forward(t["x"], o["e"], o["y"], o["h"], stats=o["st"], stream=handle)
+            b2.logprob_forward(t["logits"], tok, o["lp"], o["lse"], stream=handle)
+            b2.logprob_backward(o["dl"], t["logits"], tok, o["lse"], o["lp"], stream=handle)
+            b2.block_norm_backward(o["dx"], o["df"], o["h"], o["y"], o["y"], o["e"], o["st"], workspace=ws, stream=handle)
+            b2.embedding_backward(o["dt"], o["df"], tok, workspace=ws, stream=handle)
+            b2.gradient_clip(b2.TensorList([o["dt"], o["dx"], o["dl"]]), 1.0, o["norm"], workspace=ws, stream=handle)
+        torch.cuda.synchronize()
+        return o
+
+    want, got = run(False, None), run(True, side.cuda_stream)
+    for k in want:
+        assert torch.equal(want[k], got[k]), k

@@ -124,19 +124,6 @@ template <int W, int NV> struct Affine {
     }
 };
 
-// Copies of 16 bytes (the first `bytes` of them, zeros behind) into shared memory that nobody waits for before cp_wait
-__device__ __forceinline__ void cp_async(unsigned to, const void *from, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async(unsigned to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// until at most n (0 to 2) of the newest groups are under way
-__device__ __forceinline__ void cp_wait(int n) {
-    if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 2;" ::: "memory");
-}
-
 // Rows on their way into shared memory, `stages` of them, each with up to TENSORS tensors.  With whole vectors (W > 1) a thread copies the vectors that it
 // will read itself; rows that start anywhere (W = 1) are copied as the 16-byte pieces that hold them, by all their threads, and read element by
 // element, so that loads and stores stay coalesced.  Stages are byte offsets.

@@ -289,6 +289,7 @@ template <typename U, int W> __device__ __forceinline__ void put_row(U *to, cons
 }
 
 constexpr int SUM_THREADS = 128, MIN_GROUP = 8, MAX_PIECE = 64;
+constexpr int AHEAD = 12;                    // rows a thread has under way
 
 // A group of tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes W * tpr columns of a piece.  Every other block zeroes absent rows as long as
 // there are any: stores that nothing waits for, beside loads that the sums wait for.
@@ -297,6 +298,8 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
                                                                     int zero_blocks) {
     __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
     __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
+    constexpr bool RING = W * sizeof(T) == 16;
+    __shared__ uint4 ring[RING ? AHEAD : 1][SUM_THREADS];
     grid_wait();
     grid_release();
     const int both = 2 * min(sum_blocks, zero_blocks);
@@ -327,28 +330,51 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.0f;
     float *head = a.partial + (size_t)p * 2 * a.dim_pad + col;
-    for (int i = 0; i < n; i += 8) {
-        Vec<T, W> v[8];
-        unsigned k[8];
+    // another token, or padding: the one before is complete (what ends with the piece is seen to below)
+    const auto turn = [&](unsigned k) {
+        if (from_before) store_vec<float, W>(head, acc);
+        else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+        from_before = false;
+        cur = k;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            k[u] = i + u < n ? key[i + u] : 0xffffffffu;
-            if (k[u] < (unsigned)a.vocab) v[u] = *reinterpret_cast<const Vec<T, W> *>(dout + (long long)row[i + u] * a.ld_dout + col);
+        for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+    };
+    if constexpr (RING) {
+        // the next AHEAD rows are on their way into the thread's own slots
+        const unsigned slot = (unsigned)__cvta_generic_to_shared(&ring[0][threadIdx.x]);
+        const auto fetch = [&](int i, int stage) {
+            if (i < n && key[i] < (unsigned)a.vocab) cp_async(slot + stage * (SUM_THREADS * 16), dout + (long long)row[i] * a.ld_dout + col);
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(i, i);
+        for (int i = 0, stage = 0; i < n; ++i, stage = stage + 1 < AHEAD ? stage + 1 : 0) {
+            cp_wait<AHEAD - 1>();
+            const unsigned k = key[i];
+            if (k != cur) turn(k);
+            if (k >= (unsigned)a.vocab) break;             // padding to the end
+            float v[W];
+            load_vec<T, W>(v, reinterpret_cast<const T *>(&ring[stage][threadIdx.x]));
+            fetch(i + AHEAD, stage);
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[j] += v[j];
         }
+    } else {
+        for (int i = 0; i < n; i += AHEAD) {
+            Vec<T, W> v[AHEAD];
+            unsigned k[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            // another token, or padding: the one before is complete (what ends with the piece is seen to below)
-            if (k[u] != cur && i + u < n && cur < (unsigned)a.vocab) {
-                if (from_before) store_vec<float, W>(head, acc);
-                else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
-                from_before = false;
-                cur = k[u];
-#pragma unroll
-                for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+            for (int u = 0; u < AHEAD; ++u) {
+                k[u] = i + u < n ? key[i + u] : 0xffffffffu;
+                if (k[u] < (unsigned)a.vocab) v[u] = *reinterpret_cast<const Vec<T, W> *>(dout + (long long)row[i + u] * a.ld_dout + col);
             }
-            if (k[u] < (unsigned)a.vocab) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) acc[j] += to_float(v[u].v[j]);
+            for (int u = 0; u < AHEAD; ++u) {
+                if (k[u] != cur && i + u < n && cur < (unsigned)a.vocab) turn(k[u]);
+                if (k[u] < (unsigned)a.vocab) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) acc[j] += to_float(v[u].v[j]);
+                }
             }
         }
     }

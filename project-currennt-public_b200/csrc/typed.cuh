@@ -75,6 +75,21 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 __device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 
+// Copies of 16 bytes (the first `bytes` of them, zeros behind) into shared memory that nobody waits for before cp_wait
+__device__ __forceinline__ void cp_async(unsigned to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async(unsigned to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most N of the newest groups are under way
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// the same for n from 0 to 2
+__device__ __forceinline__ void cp_wait(int n) {
+    if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+
 // sums over a warp; every lane gets the result
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, forward_threads(NV * W)
     const int lane = warps == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const unsigned worker = warps == 1 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x, workers = warps == 1 ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
     const unsigned rows = (unsigned)a.rows, G = (unsigned)a.gate_rows;
-    const Ring<T, W, NV, FULL, 3> ring(ring_memory, tpr, lane, a.dim, stages);
+    const Ring<T, W, NV, FULL, 3, W == 1> ring(ring_memory, tpr, lane, a.dim, stages);
     typedef Cols<T, W, NV, FULL> C;
     clear_sums(red[0], 16);
     int phase = 0;
@@ -179,7 +179,7 @@ int forward(const b2_block_norm *d, const T *x, long long ld_x, const T *f, long
     const auto go = [&](auto kernel, auto vectors, int tpr) -> int {
         constexpr int NV = decltype(vectors)::value;
         const int threads = tpr == 32 ? 256 : tpr, each = threads / tpr, most = 208 * 1024, per_sm = forward_threads(NV * W) / threads > 0 ? forward_threads(NV * W) / threads : 1;
-        const int stage_bytes = Ring<T, W, NV, false, 3>::bytes(threads, tpr);
+        const int stage_bytes = Ring<T, W, NV, false, 3, W == 1>::bytes(threads, tpr);
         int stages = most / per_sm / stage_bytes;
         stages = stages > 4 ? 4 : stages < 1 ? 1 : stages;
         long long blocks = (long long)sm_count() * per_sm;
@@ -195,7 +195,7 @@ int forward(const b2_block_norm *d, const T *x, long long ld_x, const T *f, long
         constexpr int NV = decltype(vectors)::value;
         const auto sized = [&](auto threads) -> int {
             constexpr int TPR = decltype(threads)::value;
-            if constexpr (W > 1)
+            if constexpr (W * sizeof(T) == 16)
                 if (f && y && h && d->dim == NV * W * TPR) return go(block_norm_forward_kernel<T, W, NV, TPR, true>, vectors, TPR);
             return go(block_norm_forward_kernel<T, W, NV, TPR, false>, vectors, TPR);
         };
@@ -210,7 +210,7 @@ int forward(const b2_block_norm *d, const T *x, long long ld_x, const T *f, long
     const auto threads_for = [&](int nv) { const int t = (int)pow2_at_least((unsigned)(vecs + nv - 1) / nv); return t < 32 ? 32 : t; };
     if constexpr (W == 8)
         if (vecs > 64 && vecs <= 128) return pick(std::integral_constant<int, 4>(), 32);
-    if constexpr (W > 1)
+    if constexpr (W * sizeof(T) == 16)
         if (vecs <= 32) return pick(std::integral_constant<int, 1>(), 32);
     constexpr int NV = 16 / W;
     return pick(std::integral_constant<int, NV>(), threads_for(NV));
@@ -239,6 +239,8 @@ extern "C" int b2_block_norm_forward(const b2_block_norm *d, const void *x, long
         typedef B2_ELEM(t) T;
         constexpr int W = 16 / sizeof(T);
         if (w.w == W) return forward<T, W>(d, (const T *)x, ld_x, (const T *)f, ld_f, (T *)y, ld_y, (T *)h, ld_h, (cudaStream_t)stream);
+        if constexpr (W == 8)
+            if (w.w == 2) return forward<T, 2>(d, (const T *)x, ld_x, (const T *)f, ld_f, (T *)y, ld_y, (T *)h, ld_h, (cudaStream_t)stream);
         return forward<T, 1>(d, (const T *)x, ld_x, (const T *)f, ld_f, (T *)y, ld_y, (T *)h, ld_h, (cudaStream_t)stream);
     });
 }

@@ -124,15 +124,17 @@ template <int W, int NV> struct Affine {
     }
 };
 
-// Rows on their way into shared memory, `stages` of them, each with up to TENSORS tensors.  With whole vectors (W > 1) a thread copies the vectors that it
-// will read itself; rows that start anywhere (W = 1) are copied as the 16-byte pieces that hold them, by all their threads, and read element by
-// element, so that loads and stores stay coalesced.  Stages are byte offsets.
-template <typename T, int W, int NV, bool FULL, int TENSORS> struct Ring {
+// Rows on their way into shared memory, `stages` of them, each with up to TENSORS tensors.  A thread copies the vectors that it will read itself,
+// or (BYROW, for rows of single elements) all threads of a row copy the 16-byte pieces that hold it, and it is read element by element, so that
+// loads and stores stay coalesced; a piece may begin with bytes of what lies before the row, which nobody looks at.  Stages are byte offsets.
+template <typename T, int W, int NV, bool FULL, int TENSORS, bool BYROW> struct Ring {
+    static constexpr int VB = W * (int)sizeof(T);         // bytes of a vector
     char *base;
     unsigned base_addr;
     int tpr, lane, dim, pitch, mine, stage_bytes, stages;
     // bytes of a stage: TENSORS rows for every row group, then 16 bytes a warp for the caller's use
-    static __host__ __device__ int tensor_bytes(int threads, int tpr) { return W > 1 ? NV * threads * 16 : threads / tpr * (tpr * NV * (int)sizeof(T) + 32); }
+    static __host__ __device__ int row_bytes(int tpr) { return tpr * NV * (int)sizeof(T) + 32; }
+    static __host__ __device__ int tensor_bytes(int threads, int tpr) { return BYROW ? threads / tpr * row_bytes(tpr) : NV * threads * VB; }
     static __host__ __device__ int bytes(int threads, int tpr) { return TENSORS * tensor_bytes(threads, tpr) + threads / 32 * 16; }
     __device__ __forceinline__ Ring(char *ring, int tpr_, int lane_, int dim_, int stages_) {
         base = ring;
@@ -140,16 +142,16 @@ template <typename T, int W, int NV, bool FULL, int TENSORS> struct Ring {
         tpr = tpr_; lane = lane_; dim = dim_; stages = stages_;
         pitch = tensor_bytes(blockDim.x, tpr);
         stage_bytes = bytes(blockDim.x, tpr);
-        mine = W > 1 ? (int)threadIdx.x * 16 : (tpr == 32 ? (int)(threadIdx.x >> 5) : 0) * (tpr * NV * (int)sizeof(T) + 32);
+        mine = BYROW ? (tpr == 32 ? (int)(threadIdx.x >> 5) : 0) * row_bytes(tpr) : (int)threadIdx.x * VB;
     }
     __device__ __forceinline__ int column(int i) const { return (i * tpr + lane) * W; }   // of vector i
     __device__ __forceinline__ int next(int stage) const { return stage + stage_bytes < stages * stage_bytes ? stage + stage_bytes : 0; }
     __device__ __forceinline__ int spare(int stage) const { return stage + TENSORS * pitch + (int)(threadIdx.x >> 5) * 16; }
     __device__ __forceinline__ void copy(int stage, int what, const T *from) const {
-        if constexpr (W > 1) {
+        if constexpr (!BYROW) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (FULL || column(i) < dim) cp_async(base_addr + stage + mine + what * pitch + i * (int)blockDim.x * 16, from + column(i));
+                if (FULL || column(i) < dim) cp_async<VB>(base_addr + stage + mine + what * pitch + i * (int)blockDim.x * VB, from + column(i));
         } else {
             const int mis = (int)((uintptr_t)from & 15), bytes = mis + dim * (int)sizeof(T);
             const unsigned to = base_addr + stage + mine + what * pitch;
@@ -163,8 +165,8 @@ template <typename T, int W, int NV, bool FULL, int TENSORS> struct Ring {
 #pragma unroll
             for (int j = 0; j < W; ++j) v[i][j] = other;
             const char *at = base + stage + mine + what * pitch;
-            if constexpr (W > 1) {
-                if (FULL || column(i) < dim) load_vec<T, W>(v[i], reinterpret_cast<const T *>(at + i * (int)blockDim.x * 16));
+            if constexpr (!BYROW) {
+                if (FULL || column(i) < dim) load_vec<T, W>(v[i], reinterpret_cast<const T *>(at + i * (int)blockDim.x * VB));
             } else {
                 if (column(i) < dim) load_vec<T, W>(v[i], reinterpret_cast<const T *>(at + (int)((uintptr_t)from & 15)) + column(i));
             }
@@ -172,22 +174,27 @@ template <typename T, int W, int NV, bool FULL, int TENSORS> struct Ring {
     }
     // what a thread reads and another copied is there, and nobody is still reading what is copied over next
     __device__ __forceinline__ void barrier() const {
-        if (W == 1 && tpr > 32) __syncthreads();
+        if (BYROW && tpr > 32) __syncthreads();
         else __syncwarp();
     }
 };
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
-// widest vectors (16 bytes) only where every row of every tensor starts and ends on them
+// elements of an access that every row of every tensor starts and ends on: 16 bytes of them, else 2 of a 16-bit type, else 1
 struct Width {
-    int w;
-    int elem;
-    void rows(const void *p, long long ld) { if (p && (ld % w || !aligned_to(p, 16))) w = 1; }
-    void floats(const float *p) { if (!aligned_to(p, 16)) w = 1; }
+    int w, elem;
+    void fit(bool wide, bool two) {
+        if (w * elem == 16 && !wide) w = elem == 2 ? 2 : 1;
+        if (w == 2 && elem == 2 && !two) w = 1;
+    }
+    void rows(const void *p, long long ld) {
+        if (p) fit(ld % (16 / elem) == 0 && aligned_to(p, 16), ld % 2 == 0 && aligned_to(p, 4));
+    }
+    void floats(const float *p) { fit(aligned_to(p, 16), aligned_to(p, 8)); }
 };
 Width width_of(const b2_block_norm *d) {
     Width x = {16 / type_size(d->type), type_size(d->type)};
-    if (d->dim % x.w) x.w = 1;
+    x.fit(d->dim % x.w == 0, d->dim % 2 == 0);
     x.rows(d->gate, d->ld_gate);
     x.floats(d->w_pre); x.floats(d->b_pre); x.floats(d->w_post); x.floats(d->b_post);
     return x;

@@ -39,6 +39,9 @@ template <int W, int NV, bool FULL> struct Out {
     }
 };
 
+// fp32 elements are copied one by one here (48256 x 405: 117 us, by row 168 us; in the forward pass by row 61 us and one by one 74 us for 38400 x 511)
+template <typename T> __host__ __device__ constexpr bool by_row(int w) { return w == 1 && sizeof(T) == 2; }
+
 // A worker is a warp (TPR = 32) or a block of TPR threads.  per_group workers share a row of the gate (all workers, if there is one row or none), and
 // groups_at_once rows of the gate are worked on side by side.  BIAS: means are subtracted or the norms have a bias (without both, sums are saved).
 // FULL: dy, dh, f, dx and df are all there and the threads' columns are just the row's: a third of the instructions were tests of that.
@@ -74,7 +77,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 512 / (TPR == 32 ? 256 
     if (KEEP && a.w2) weights(w2, a.w2);
     const int group0 = worker / k.per_group, member = worker - group0 * k.per_group;
     RowWalk now = {group0 < k.groups_at_once ? group0 : G, member, G, (int)(a.rows / G), member, k.per_group, k.groups_at_once}, ahead = now;
-    const Ring<T, W, NV, FULL, 5> shared(ring, tpr, lane, a.dim, stages);
+    const Ring<T, W, NV, FULL, 5, by_row<T>(W)> shared(ring, tpr, lane, a.dim, stages);
     const auto take = [&](Pair (&v)[H], int stage, int what, const T *p, unsigned row, unsigned ld, float other) {
         float q[NV][W];
         shared.take(q, stage, what, p + (unsigned long long)row * ld, other);
@@ -91,7 +94,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 512 / (TPR == 32 ? 256 
         if (on) {
             const unsigned r = ahead.row();
             // the statistics by the warp's first lane
-            if ((threadIdx.x & 31) == 0) cp_async(shared.base_addr + shared.spare(stage), a.stats + r);
+            if ((threadIdx.x & 31) == 0) cp_async<16>(shared.base_addr + shared.spare(stage), a.stats + r);
             if (FULL || dh) { shared.copy(stage, 0, dh + (unsigned long long)r * k.ld_dh); shared.copy(stage, 1, y + (unsigned long long)r * k.ld_y); }
             if (FULL || dy) shared.copy(stage, 2, dy + (unsigned long long)r * k.ld_dy);
             if (FULL || f) shared.copy(stage, 3, f + (unsigned long long)r * k.ld_f);
@@ -286,15 +289,16 @@ template <typename T, int W>
 int backward(const b2_block_norm *d, T *dx, long long ld_dx, T *df, long long ld_df, T *dgate, long long ld_dgate, float *const (&dw)[4], const T *dy, long long ld_dy,
              const T *dh, long long ld_dh, const T *y, long long ld_y, const T *f, long long ld_f, float *ws, cudaStream_t st) {
     const NormArgs a = args_of(d);
-    const int per_thread = W > 1 ? W : 8;
+    const int per_thread = W * sizeof(T) == 16 ? W : 8;
     const BackPlan p = back_plan(d->rows, d->dim, per_thread, d->gate ? d->gate_rows : 0);
     BackArgs k = {(unsigned)ld_dx, (unsigned)ld_df, (unsigned)ld_dy, (unsigned)ld_dh, (unsigned)ld_y, (unsigned)ld_f, (unsigned)ld_dgate, dgate, nullptr, nullptr, (d->dim + 15) / 16 * 16, p.per_group, p.groups_at_once};
     const bool sums = dw[0] || dw[1] || dw[2] || dw[3], gate_sums = dgate && p.per_group > 1;
     if (sums) k.partial = ws;
     k.partial_gate = ws + (size_t)p.blocks * 4 * k.dim_pad;
     // the ring: up to 4 rows in what the blocks of a multiprocessor share
-    const int nv = W == 1 ? 8 : d->dim > p.tpr * W ? 2 : 1, here = 512 > p.threads ? 512 / p.threads : 1;
-    const int stage_bytes = nv == 2 ? Ring<T, W, 2, false, 5>::bytes(p.threads, p.tpr) : Ring<T, W, W == 1 ? 8 : 1, false, 5>::bytes(p.threads, p.tpr);
+    const int nv = W * sizeof(T) != 16 ? 8 / W : d->dim > p.tpr * W ? 2 : 1, here = 512 > p.threads ? 512 / p.threads : 1;
+    constexpr int ONE = W * sizeof(T) == 16 ? 1 : 8 / W;
+    const int stage_bytes = nv == ONE ? Ring<T, W, ONE, false, 5, by_row<T>(W)>::bytes(p.threads, p.tpr) : Ring<T, W, 2 * ONE, false, 5, by_row<T>(W)>::bytes(p.threads, p.tpr);
     const int most = 208 * 1024, join_bytes = p.tpr == 32 ? 8 * 32 * W * nv * 4 : 0;
     int stages = most / here / stage_bytes;
     stages = stages > 4 ? 4 : stages < 1 ? 1 : stages;
@@ -307,13 +311,13 @@ int backward(const b2_block_norm *d, T *dx, long long ld_dx, T *df, long long ld
         return B2_OK;
     };
     const bool bias = d->layer_norm || dw[1] || dw[3] || d->b_post;
-    const bool full = W > 1 && d->dim == p.tpr * W && dx && df && dy && dh && f;
+    const bool full = W * sizeof(T) == 16 && d->dim == p.tpr * W && dx && df && dy && dh && f;
     const auto pick = [&](auto b) {
         constexpr bool B = decltype(b)::value;
-        constexpr int NV = W == 1 ? 8 : 1;
+        constexpr int NV = W * sizeof(T) == 16 ? 1 : 8 / W;
         const auto sized = [&](auto threads) -> int {
             constexpr int TPR = decltype(threads)::value;
-            if constexpr (W > 1)
+            if constexpr (W * sizeof(T) == 16)
                 if (full) return go(block_norm_backward_kernel<T, W, 1, TPR, B, true>);
             if constexpr (W == 4 && TPR == 1024)
                 if (nv == 2) return go(block_norm_backward_kernel<T, W, 2, TPR, B, false>);
@@ -401,7 +405,10 @@ int b2_block_norm_backward(const b2_block_norm *d, void *dx, long long ld_dx, vo
             return backward<T, decltype(width)::value>(d, (T *)dx, ld_dx, (T *)df, ld_df, (T *)dgate, ld_dgate, dw, (const T *)dy, ld_dy, (const T *)dh, ld_dh, (const T *)y,
                                                        ld_y, (const T *)f, ld_f, (float *)workspace, (cudaStream_t)stream);
         };
-        return w.w == W ? go(std::integral_constant<int, W>()) : go(std::integral_constant<int, 1>());
+        if (w.w == W) return go(std::integral_constant<int, W>());
+        if constexpr (W == 8)
+            if (w.w == 2) return go(std::integral_constant<int, 2>());
+        return go(std::integral_constant<int, 1>());
     });
 }
 

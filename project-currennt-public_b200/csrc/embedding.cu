@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
         // the next AHEAD rows are on their way into the thread's own slots
         const unsigned slot = (unsigned)__cvta_generic_to_shared(&ring[0][threadIdx.x]);
         const auto fetch = [&](int i, int stage) {
-            if (i < n && key[i] < (unsigned)a.vocab) cp_async(slot + stage * (SUM_THREADS * 16), dout + (long long)row[i] * a.ld_dout + col);
+            if (i < n && key[i] < (unsigned)a.vocab) cp_async<16>(slot + stage * (SUM_THREADS * 16), dout + (long long)row[i] * a.ld_dout + col);
             cp_commit();
         };
 #pragma unroll

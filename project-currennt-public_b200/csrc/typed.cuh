@@ -79,7 +79,11 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2
 __device__ __forceinline__ void cp_async(unsigned to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async(unsigned to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+// BYTES (4, 8 or 16) of them
+template <int BYTES> __device__ __forceinline__ void cp_async(unsigned to, const void *from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // until at most N of the newest groups are under way
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

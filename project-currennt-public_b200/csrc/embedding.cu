@@ -291,15 +291,17 @@ template <typename U, int W> __device__ __forceinline__ void put_row(U *to, cons
 constexpr int SUM_THREADS = 128, MIN_GROUP = 8, MAX_PIECE = 64;
 constexpr int AHEAD = 12;                    // rows a thread has under way
 
-// A group of tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes W * tpr columns of a piece.  Every other block zeroes absent rows as long as
+// A group of tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes tpr times 16 bytes of a piece's rows.  Every other block zeroes absent rows as long as
 // there are any: stores that nothing waits for, beside loads that the sums wait for.
 template <typename T, typename U, int W>
 __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
                                                                     int zero_blocks) {
     __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
     __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
-    constexpr bool RING = W * sizeof(T) == 16;
-    __shared__ uint4 ring[RING ? AHEAD : 1][SUM_THREADS];
+    // a thread's columns: 16 bytes of a row, in as many vectors as the rows' alignment asks for
+    constexpr int NV = 16 / (W * (int)sizeof(T));
+    constexpr bool RING = W * sizeof(T) >= 4;
+    __shared__ uint4 ring[RING ? AHEAD * SUM_THREADS : 1];
     grid_wait();
     grid_release();
     const int both = 2 * min(sum_blocks, zero_blocks);
@@ -311,10 +313,10 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
         block -= both >> 1;
         if (zero_blocks > sum_blocks) { zero_rows(z, block, zero_blocks); return; }
     }
-    const int tiles = (a.dim + a.tpr * W - 1) / (a.tpr * W);
+    const int width = a.tpr * W * NV, tiles = (a.dim + width - 1) / width;
     const int group = threadIdx.x / a.tpr, lane = threadIdx.x & (a.tpr - 1);
     const long long unit = (long long)block * (SUM_THREADS / a.tpr) + group;
-    const int p = (int)(unit / tiles), col = ((int)(unit - (long long)p * tiles) * a.tpr + lane) * W;
+    const int p = (int)(unit / tiles), col0 = (int)(unit - (long long)p * tiles) * width + lane * W, step = a.tpr * W;   // vector i at col0 + i * step
     // the piece's keys and rows first: then the rows themselves can all be asked for at once
     const int i0 = p < a.pieces ? p * a.piece : a.n, n = min(a.n - i0, a.piece);
     unsigned *key = s_key + group * a.piece;
@@ -322,28 +324,46 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
     for (int i = lane; i < n; i += a.tpr) { key[i] = __ldg(a.keys + i0 + i); row[i] = __ldg(a.rows + i0 + i); }
     const unsigned before = n > 0 && i0 > 0 ? __ldg(a.keys + i0 - 1) : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? __ldg(a.keys + i0 + n) : 0xffffffffu;
     __syncthreads();
-    if (n <= 0 || col >= a.dim) return;
+    if (n <= 0 || col0 >= a.dim) return;
     unsigned cur = key[0];
     if (cur >= (unsigned)a.vocab) return;                  // nothing but padding from here on
     bool from_before = before == cur;
-    float acc[W];
+    float acc[NV][W];
+    const auto clear = [&]() {
 #pragma unroll
-    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-    float *head = a.partial + (size_t)p * 2 * a.dim_pad + col;
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[i][j] = 0.0f;
+    };
+    clear();
+    const auto save = [&](float *to) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (col0 + i * step < a.dim) store_vec<float, W>(to + col0 + i * step, acc[i]);
+    };
+    const auto put = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (col0 + i * step < a.dim) put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col0 + i * step, acc[i], a.scale, a.accumulate);
+    };
+    float *head = a.partial + (size_t)p * 2 * a.dim_pad;
     // another token, or padding: the one before is complete (what ends with the piece is seen to below)
     const auto turn = [&](unsigned k) {
-        if (from_before) store_vec<float, W>(head, acc);
-        else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+        if (from_before) save(head);
+        else put();
         from_before = false;
         cur = k;
-#pragma unroll
-        for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+        clear();
     };
     if constexpr (RING) {
         // the next AHEAD rows are on their way into the thread's own slots
-        const unsigned slot = (unsigned)__cvta_generic_to_shared(&ring[0][threadIdx.x]);
+        constexpr int VB = W * sizeof(T);
+        const unsigned slots = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * VB;
         const auto fetch = [&](int i, int stage) {
-            if (i < n && key[i] < (unsigned)a.vocab) cp_async<16>(slot + stage * (SUM_THREADS * 16), dout + (long long)row[i] * a.ld_dout + col);
+            if (i < n && key[i] < (unsigned)a.vocab)
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    if (col0 + v * step < a.dim) cp_async<VB>(slots + (stage * NV + v) * SUM_THREADS * VB, dout + (long long)row[i] * a.ld_dout + col0 + v * step);
             cp_commit();
         };
 #pragma unroll
@@ -353,85 +373,95 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
             const unsigned k = key[i];
             if (k != cur) turn(k);
             if (k >= (unsigned)a.vocab) break;             // padding to the end
-            float v[W];
-            load_vec<T, W>(v, reinterpret_cast<const T *>(&ring[stage][threadIdx.x]));
+            float x[NV][W];
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                load_vec<T, W>(x[v], reinterpret_cast<const T *>(reinterpret_cast<const char *>(ring) + (stage * NV + v) * SUM_THREADS * VB + threadIdx.x * VB));
             fetch(i + AHEAD, stage);
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[j] += v[j];
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < W; ++j) acc[v][j] += x[v][j];
         }
     } else {
-        for (int i = 0; i < n; i += AHEAD) {
-            Vec<T, W> v[AHEAD];
-            unsigned k[AHEAD];
+        constexpr int ROWS = 4;                            // 16-bit elements one by one: 32 loads under way
+        for (int i = 0; i < n; i += ROWS) {
+            T x[ROWS][NV];
+            unsigned k[ROWS];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
+            for (int u = 0; u < ROWS; ++u) {
                 k[u] = i + u < n ? key[i + u] : 0xffffffffu;
-                if (k[u] < (unsigned)a.vocab) v[u] = *reinterpret_cast<const Vec<T, W> *>(dout + (long long)row[i + u] * a.ld_dout + col);
+                if (k[u] < (unsigned)a.vocab)
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+                        if (col0 + v * step < a.dim) x[u][v] = dout[(long long)row[i + u] * a.ld_dout + col0 + v * step];
             }
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
+            for (int u = 0; u < ROWS; ++u) {
                 if (k[u] != cur && i + u < n && cur < (unsigned)a.vocab) turn(k[u]);
-                if (k[u] < (unsigned)a.vocab) {
+                if (k[u] < (unsigned)a.vocab)
 #pragma unroll
-                    for (int j = 0; j < W; ++j) acc[j] += to_float(v[u].v[j]);
-                }
+                    for (int v = 0; v < NV; ++v) acc[v][0] += to_float(x[u][v]);
             }
         }
     }
     if (cur >= (unsigned)a.vocab) return;
-    if (from_before) store_vec<float, W>(head, acc);
+    if (from_before) save(head);
     else if (behind == cur) {
-        store_vec<float, W>(head + a.dim_pad, acc);
-        if (col == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
-    } else put_row<U, W>(dtable + (long long)cur * a.ld_dtable + col, acc, a.scale, a.accumulate);
+        save(head + a.dim_pad);
+        if (col0 == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
+    } else put();
 }
 
 // Tokens that cross pieces: tail of the first piece plus the heads of those that follow.  A block is a.cols column vectors x 256 / a.cols
 // phases: a phase adds every so-many-th head, the phases' sums are added in order.
 template <typename U, int W>
 __global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dtable, const SumArgs a) {
-    __shared__ __align__(16) float part[256 * W];
+    constexpr int P = W < 4 ? 4 : W;                       // partial sums are aligned whatever the table is
+    __shared__ __align__(16) float part[256 * P];
     grid_wait();
     const unsigned n_list = *a.list_count;
-    const int phases = 256 / a.cols, x = threadIdx.x & (a.cols - 1), y = threadIdx.x / a.cols, col = ((int)blockIdx.y * a.cols + x) * W;
+    const int phases = 256 / a.cols, x = threadIdx.x & (a.cols - 1), y = threadIdx.x / a.cols, col = ((int)blockIdx.y * a.cols + x) * P;
     for (unsigned li = blockIdx.x; li < n_list; li += gridDim.x) {
         const int p = a.list[li];
         const unsigned key = __ldg(a.keys + (size_t)(p + 1) * a.piece);
-        float s[W];
+        float s[P];
 #pragma unroll
-        for (int j = 0; j < W; ++j) s[j] = 0.0f;
+        for (int j = 0; j < P; ++j) s[j] = 0.0f;
         if (col < a.dim) {
-            if (y == 0) load_vec<float, W>(s, a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col);
+            if (y == 0) load_vec<float, P>(s, a.partial + ((size_t)p * 2 + 1) * a.dim_pad + col);
             for (unsigned q = p + 1 + y; q < (unsigned)a.pieces; q += 4 * phases) {
-                float v[4][W];
+                float v[4][P];
                 unsigned k[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     // the head is fetched beside the key that tells whether it is one
                     const unsigned at = q + u * phases, in = min(at, (unsigned)a.pieces - 1);
                     k[u] = at < (unsigned)a.pieces ? __ldg(a.keys + (size_t)in * a.piece) : 0xffffffffu;
-                    load_vec<float, W>(v[u], a.partial + (size_t)in * 2 * a.dim_pad + col);
+                    load_vec<float, P>(v[u], a.partial + (size_t)in * 2 * a.dim_pad + col);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
                     if (k[u] == key) {
 #pragma unroll
-                        for (int j = 0; j < W; ++j) s[j] += v[u][j];
+                        for (int j = 0; j < P; ++j) s[j] += v[u][j];
                     }
                 if (k[3] != key) break;
             }
         }
-        store_vec<float, W>(part + threadIdx.x * W, s);
+        store_vec<float, P>(part + threadIdx.x * P, s);
         __syncthreads();
         if (y == 0 && col < a.dim) {
 #pragma unroll 7
             for (int i = 1; i < phases; ++i) {
-                float v[W];
-                load_vec<float, W>(v, part + (i * a.cols + x) * W);
+                float v[P];
+                load_vec<float, P>(v, part + (i * a.cols + x) * P);
 #pragma unroll
-                for (int j = 0; j < W; ++j) s[j] += v[j];
+                for (int j = 0; j < P; ++j) s[j] += v[j];
             }
-            put_row<U, W>(dtable + (long long)key * a.ld_dtable + col, s, a.scale, a.accumulate);
+#pragma unroll
+            for (int i = 0; i < P; i += W)
+                if (col + i < a.dim) put_row<U, W>(dtable + (long long)key * a.ld_dtable + col + i, *reinterpret_cast<const float(*)[W]>(s + i), a.scale, a.accumulate);
         }
         __syncthreads();
     }
@@ -455,7 +485,7 @@ Plan make_plan(long long n, int vocab, int dim) {
     tile = tile < 2048 ? 2048 : (tile + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
     p.tile = (int)tile;
     p.tiles = (int)((n + tile - 1) / tile);
-    // pieces: few rows give parallel groups, many rows few partial sums
+    // pieces: few rows give parallel groups, many rows few partial sums (32768 rows: 16 rows a piece 87 us, 32 77 us, 64 78 us)
     p.piece = n <= 4096 ? 8 : n <= 16384 ? 16 : n <= 262144 ? 32 : MAX_PIECE;
     p.pieces = (int)((n + p.piece - 1) / p.piece);
     p.dim_pad = (dim + 15) / 16 * 16;
@@ -506,15 +536,17 @@ int forward(U *out, long long ld_out, const T *table, long long ld_table, int vo
 template <typename T, typename U, int W>
 int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int zero_blocks, cudaStream_t st) {
     SumArgs a = base;
-    unsigned tpr = pow2_at_least((unsigned)((a.dim + W - 1) / W));
+    const int per_thread = 16 / (int)sizeof(T), P = W < 4 ? 4 : W;        // columns of a thread of the sums, and of the joins
+    unsigned tpr = pow2_at_least((unsigned)((a.dim + per_thread - 1) / per_thread));
     tpr = tpr > SUM_THREADS ? SUM_THREADS : tpr < MIN_GROUP ? MIN_GROUP : tpr;
     a.tpr = (int)tpr;
-    a.cols = tpr > 32 ? 32 : (int)tpr;
-    const long long tiles = (a.dim + (long long)tpr * W - 1) / ((long long)tpr * W), per = SUM_THREADS / tpr;
+    const unsigned cols = pow2_at_least((unsigned)((a.dim + P - 1) / P));
+    a.cols = cols > 32 ? 32 : (int)cols;
+    const long long tiles = (a.dim + (long long)tpr * per_thread - 1) / ((long long)tpr * per_thread), per = SUM_THREADS / tpr;
     const long long blocks = (a.pieces * tiles + per - 1) / per;
     if (blocks + zero_blocks > 0x7fffffffll) { set_error("b2_embedding_backward: %lld blocks", blocks); return B2_ERR_BAD_SHAPE; }
     B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks, zero_blocks));
-    const int join_tiles = (a.dim + a.cols * W - 1) / (a.cols * W), most = (sm_count() * 8 + join_tiles - 1) / join_tiles;
+    const int join_tiles = (a.dim + a.cols * P - 1) / (a.cols * P), most = (sm_count() * 8 + join_tiles - 1) / join_tiles;
     return launch_chained(embedding_join_kernel<U, W>, dim3((unsigned)(a.pieces < most ? a.pieces : most), (unsigned)join_tiles), dim3(256), 0, st, dtable, a);
 }
 

@@ -12,10 +12,16 @@
 //   dt = dy + r1 (w1 dh - [mean(w1 dh)] - u1 mean(w1 dh u1)),   dx = dt,   dn = a gate dt,   dgate = a dt n
 //   df = r2 (w2 dn - [mean(w2 dn)] - u2 mean(w2 dn u2)),   dw1 = sum dh u1, db1 = sum dh, dw2 = sum dn u2, db2 = sum dn   (over frames)
 //
-// Bound by memory: a row stays in registers between its loads and its stores, so every tensor is read once and written once.  A warp
-// takes a row where 4 vectors a lane hold it, a block otherwise.  The backward kernel has a fixed number of workers; a worker keeps
-// the same columns for all its rows, so the sums over frames stay in registers until the end, go to the workspace once, and are
-// added there in a fixed order by a second launch: no atomics, the same bits every time.
+// Bound by memory: a row stays in registers and shared memory between its loads and its stores, so every tensor is read once and written
+// once.  What stands against it is latency: a row is a chain of two sums over its threads (four with layer norm), so the rows that follow are on
+// their way into shared memory meanwhile; and instructions, so arithmetic is packed in the backward pass, the threads of a row are a constant,
+// and full rows are compiled without tests.  The backward kernel has a fixed number of workers; a worker keeps the same columns for all its rows,
+// so the sums over frames stay in registers until the end, go to the workspace once, and are added there in a fixed order by a second
+// launch: no atomics, the same bits every time.
+// Measured on a B200 (device time; share of the copy bandwidth): forward, layer norm, 38400 x 512 fp32 with a gate per sequence 52 us (all bytes counted
+// 93 %; a third of the frames are padding, of which only zeros are written), 38400 x 512 bf16 33 us, x 1024 64 us, 8192 x 4001 93 us
+// (single elements), 64 x 1024 bf16 3.3 us.  Backward, 16384 x 2048 bf16 with a gate per frame 95 us (87 %), with layer norm and biases 137 us
+// (its sums spill), 16384 x 2047 180 us, x 4096 249 us (one block a multiprocessor: its barriers are not hidden).
 #include "block_norm.cuh"
 
 namespace b2 {

@@ -13,8 +13,10 @@
 //      an earlier piece; "tail": it begins here and goes on).
 //   3. join: the pieces with a tail (a list, filled by atomics: its order changes no result) add the heads that follow.
 // A frequent token is thus spread over as many groups as it has pieces.  Without accumulation the rows of tokens that do not occur are
-// zeroed by extra blocks of the same launches: the table is written once, and the sort's launches, which occupy few
-// multiprocessors, hide behind that.
+// zeroed by extra blocks of the same launches, so that the table is written once.
+// Measured on a B200 (device time): lookup of 65536 x 1024 bf16 29 us (7.4 TB/s of what it reads and writes; repeated rows come from L2), of
+// 64 x 512 2 us, a launch.  Gradient of 32768 x 1024 bf16 in a table of 50000 rows 75 us against 42 us of bytes: the sort takes 19 us of latency
+// (four launches of 16 blocks), the sums with 209 MB 38 us (5.5 TB/s), the joins 10 us of latency.  1516 x 128 in 259 rows 11.5 us: three launches.
 #include <math.h>
 
 #include "typed.cuh"

@@ -8,10 +8,14 @@
 // rescales both.  Then lse = m + log S and H = log S - E / S, which needs no difference of large numbers.
 // The K largest: a warp keeps its best K as a sorted list, one entry a lane; a batch of values is looked at only if its maximum
 // passes the K-th entry, so that after the first batches insertions are rare (K log(n) of them for values in random order).
-// Rows of up to 1024 entries stay in the registers of one warp.  Longer rows take a block, or a thread-block cluster of up to 16 blocks
-// when there are few rows: its blocks hand their sums and lists to the first one through distributed shared memory, so that a row needs
-// neither a second launch nor a workspace.
-// Bound by memory for long rows: 4 to 5 issue slots and one ex2 an entry, against the 11 entries of 2 bytes that arrive per cycle and SM.
+// Rows of up to 1024 entries stay in the registers of 4 to 32 lanes.  Longer rows take a warp where the rows alone fill the device, a block of 4 or
+// 8 warps where they do not, or, when there are few, a thread-block cluster of up to 8 blocks, which hand their sums and lists to the first
+// one through distributed shared memory: a row needs neither a second launch nor a workspace.
+// Bound, for long rows of 16-bit logits, by memory and by the exponentials alike: 11.6 entries arrive per cycle and SM, and the special function
+// units return about 12 exponentials.  Measured on a B200 (device time): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth;
+// two bytes an entry), with four alternatives 162 us (the chains of the insertions, 20 a row), with 20 244 us; 38400 rows of 259 fp32 8.6 us (72 %);
+// 8 rows of 131072 with a mask and eight alternatives 11.4 us, without alternatives 6.8 us, a launch and two trips to memory of it.
+// Backward: one read, one write.  8192 rows of 32003 bf16 that start anywhere 167 us (96 %); 38400 of 259 fp32 18 us.
 #include <math.h>
 
 #include <cooperative_groups.h>

@@ -6,17 +6,20 @@
 //
 // Gradient: the rows are sorted by token (stable radix sort, so rows of one token keep their order), then summed in that order in
 // fp32: no atomics on values, the same bits every time.
-//   1. sort: digits of up to 9 bits; up to SMALL_SORT tokens one block does all passes in shared memory, otherwise two launches a pass
-//      (digit counts of every tile; ranks and scatter).  Tokens outside the table get the key `vocab` and end up last.
+//   1. sort: digits of up to 9 bits; up to SMALL_SORT tokens every block does all passes for itself in shared memory and goes on with the sums,
+//      otherwise two launches a pass (digit counts of every tile; ranks and scatter).  Tokens outside the table get the key `vocab` and end
+//      up last.
 //   2. sum: the sorted rows are cut into pieces of `piece` rows; a group of threads sums a piece column by column.  A token whose
 //      rows lie inside one piece is written at once; one that crosses a border leaves a partial sum per piece ("head": it began in
 //      an earlier piece; "tail": it begins here and goes on).
-//   3. join: the pieces with a tail (a list, filled by atomics: its order changes no result) add the heads that follow.
+//   3. join: the pieces with a tail (a list, filled by atomics: its order changes no result; few pieces are all looked at) add the heads that
+//      follow.
 // A frequent token is thus spread over as many groups as it has pieces.  Without accumulation the rows of tokens that do not occur are
 // zeroed by extra blocks of the same launches, so that the table is written once.
 // Measured on a B200 (device time): lookup of 65536 x 1024 bf16 29 us (7.4 TB/s of what it reads and writes; repeated rows come from L2), of
 // 64 x 512 2 us, a launch.  Gradient of 32768 x 1024 bf16 in a table of 50000 rows 75 us against 42 us of bytes: the sort takes 19 us of latency
-// (four launches of 16 blocks), the sums with 209 MB 38 us (5.5 TB/s), the joins 10 us of latency.  1516 x 128 in 259 rows 11.5 us: three launches.
+// (four launches of 16 blocks), the sums with 209 MB 38 us (5.5 TB/s), the joins 10 us of latency.  1516 x 128 in 259 rows 11.4 us: the sort 4.8, the sums 2.3 and a
+// second launch for the joins 2.5.
 #include <math.h>
 
 #include "typed.cuh"
@@ -96,34 +99,34 @@ __device__ __forceinline__ unsigned block_exclusive_scan(unsigned x, unsigned *w
     __syncthreads();
     return before;
 }
-// count[warp][digit] becomes the place of the first key of (digit, warp): digits in order, within a digit the warps in order, behind `base`
-// (thread d's own value, for digit d).
-__device__ __forceinline__ void places(unsigned *count, int digits, unsigned base) {
+// count[warp][digit] becomes the place of the first key of (digit, warp): digits in order, within a digit the warps in order.  before: what thread d adds for
+// digit d; total: its keys in all tiles, or a negative value for those counted here.
+__device__ __forceinline__ void places(unsigned *count, int digits, unsigned before, int total, unsigned *warp_tot) {
     const int d = threadIdx.x;
-    if (d < digits) {
+    unsigned c[SORT_WARPS], sum = 0;
 #pragma unroll
-        for (int w = 0; w < SORT_WARPS; ++w) { const unsigned c = count[w * digits + d]; count[w * digits + d] = base; base += c; }
+    for (int w = 0; w < SORT_WARPS; ++w) {
+        c[w] = d < digits ? count[w * digits + d] : 0;
+        sum += c[w];
     }
+    unsigned at = block_exclusive_scan(total < 0 ? sum : (unsigned)total, warp_tot) + before;
+    if (d < digits)
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; ++w) { count[w * digits + d] = at; at += c[w]; }
     __syncthreads();
 }
 
-// All passes for up to SMALL_SORT tokens.  Warp w ranks the keys [w * seg, (w + 1) * seg) in rounds of 32, counts kept per (digit, warp),
-// so equal digits stay in order.
-__global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__restrict__ tokens, int n, int vocab, int passes, int bits, unsigned *__restrict__ keys_out,
-                                                                  int *__restrict__ rows_out, unsigned *__restrict__ present, unsigned *__restrict__ list_count) {
-    extern __shared__ unsigned sm[];
+// All passes for up to SMALL_SORT tokens, in the block's shared memory: sm holds SMALL_WORDS words and the counts.  Warp w ranks the keys
+// [w * seg, (w + 1) * seg) in rounds of 32, counts kept per (digit, warp), so equal digits stay in order.  *keys and *rows are the sorted ones.
+constexpr int SMALL_WORDS = 3 * SMALL_SORT;
+__device__ __forceinline__ void sort_in_block(unsigned *sm, const int *__restrict__ tokens, int n, int vocab, int passes, int bits, const unsigned **keys, const unsigned short **rows) {
     unsigned *key[2] = {sm, sm + SMALL_SORT};
     unsigned short *row[2] = {(unsigned short *)(sm + 2 * SMALL_SORT), (unsigned short *)(sm + 2 * SMALL_SORT) + SMALL_SORT};
-    unsigned *count = sm + 3 * SMALL_SORT;                 // [SORT_WARPS][digits]
+    unsigned *count = sm + SMALL_WORDS;                    // [SORT_WARPS][digits]
     __shared__ unsigned warp_tot[SORT_WARPS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, digits = 1 << bits;
-    grid_wait();
-    if (threadIdx.x == 0) *list_count = 0;
-    for (int i = threadIdx.x; i < (vocab + 31) / 32; i += SORT_THREADS) present[i] = 0;
-    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { key[0][i] = key_of(tokens[i], vocab); row[0][i] = (unsigned short)i; }
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { key[0][i] = key_of(__ldg(tokens + i), vocab); row[0][i] = (unsigned short)i; }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += SORT_THREADS)
-        if (key[0][i] < (unsigned)vocab) atomicOr(present + (key[0][i] >> 5), 1u << (key[0][i] & 31));
     const int seg = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) & ~31;
     for (int p = 0; p < passes; ++p) {
         const unsigned *kin = key[p & 1];
@@ -148,11 +151,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__r
             __syncwarp();
         }
         __syncthreads();
-        unsigned total = 0;
-        if ((int)threadIdx.x < digits)
-#pragma unroll
-            for (int i = 0; i < SORT_WARPS; ++i) total += count[i * digits + threadIdx.x];
-        places(count, digits, block_exclusive_scan(total, warp_tot));
+        places(count, digits, 0, -1, warp_tot);
 #pragma unroll
         for (int k = 0; k < SMALL_SORT / SORT_THREADS; ++k) {
             const int i = w * seg + k * 32 + lane;
@@ -164,8 +163,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_small_kernel(const int *__r
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { keys_out[i] = key[passes & 1][i]; rows_out[i] = row[passes & 1][i]; }
-    grid_release();
+    *keys = key[passes & 1];
+    *rows = row[passes & 1];
 }
 
 struct SortArgs {
@@ -187,18 +186,23 @@ struct ZeroArgs {
 
 __device__ __forceinline__ unsigned sort_key(const SortArgs &a, int i) { return a.tokens ? key_of(a.tokens[i], a.vocab) : a.kin[i]; }
 
+// by a warp
+__device__ __forceinline__ void zero_row(const ZeroArgs &z, long long v) {
+    const int lane = threadIdx.x & 31;
+    char *p = (char *)z.dtable + v * z.ld_bytes;
+    if (z.unit == 16)
+        for (long long b = lane * 16; b < z.row_bytes; b += 512) *reinterpret_cast<uint4 *>(p + b) = make_uint4(0, 0, 0, 0);
+    else if (z.unit == 4)
+        for (long long b = lane * 4; b < z.row_bytes; b += 128) *reinterpret_cast<unsigned *>(p + b) = 0;
+    else
+        for (long long b = lane * 2; b < z.row_bytes; b += 64) *reinterpret_cast<unsigned short *>(p + b) = 0;
+}
 // one warp a row; block `blk` of `blks`
 __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int blk, int blks) {
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int warps = blockDim.x >> 5;
     for (long long v = (long long)z.v0 + (long long)blk * warps + (threadIdx.x >> 5); v < z.v1; v += (long long)blks * warps) {
         if (z.present[v >> 5] >> (v & 31) & 1) continue;
-        char *p = (char *)z.dtable + v * z.ld_bytes;
-        if (z.unit == 16)
-            for (long long b = lane * 16; b < z.row_bytes; b += 512) *reinterpret_cast<uint4 *>(p + b) = make_uint4(0, 0, 0, 0);
-        else if (z.unit == 4)
-            for (long long b = lane * 4; b < z.row_bytes; b += 128) *reinterpret_cast<unsigned *>(p + b) = 0;
-        else
-            for (long long b = lane * 2; b < z.row_bytes; b += 64) *reinterpret_cast<unsigned short *>(p + b) = 0;
+        zero_row(z, v);
     }
 }
 
@@ -248,8 +252,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const SortAr
     const int i0 = blockIdx.x * a.tile, i1 = min(a.n, i0 + a.tile), seg = a.tile / SORT_WARPS;
     const int s0 = i0 + w * seg, s1 = min(i1, s0 + seg);
     for (int i = s0 + lane; i < s1; i += 32) atomicAdd(count + w * digits + ((sort_key(a, i) >> a.shift) & (digits - 1)), 1u);
-    const unsigned base = block_exclusive_scan(total, warp_tot);   // its barriers stand behind the counts
-    places(count, digits, base + before);
+    __syncthreads();
+    places(count, digits, before, (int)total, warp_tot);
     for (int j = s0; j < s1; j += 32) {
         const int i = j + lane;
         const bool on = i < s1;
@@ -293,40 +297,15 @@ template <typename U, int W> __device__ __forceinline__ void put_row(U *to, cons
 constexpr int SUM_THREADS = 128, MIN_GROUP = 8, MAX_PIECE = 64;
 constexpr int AHEAD = 12;                    // rows a thread has under way
 
-// A group of tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes tpr times 16 bytes of a piece's rows.  Every other block zeroes absent rows as long as
-// there are any: stores that nothing waits for, beside loads that the sums wait for.
-template <typename T, typename U, int W>
-__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
-                                                                    int zero_blocks) {
-    __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
-    __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
-    // a thread's columns: 16 bytes of a row, in as many vectors as the rows' alignment asks for
-    constexpr int NV = 16 / (W * (int)sizeof(T));
+// A group of a.tpr threads (a power of two, MIN_GROUP to SUM_THREADS) takes a.tpr times 16 bytes of a piece's rows: a thread the columns col0 + i * step, NV
+// vectors of them, as the rows' alignment asks for.  key, row: the piece's n rows in shared memory; before, behind: the keys on either side;
+// ring: AHEAD times 16 bytes for each of the block's THREADS threads.
+template <typename T, int W> __host__ __device__ constexpr int sum_vectors() { return 16 / (W * (int)sizeof(T)); }
+template <typename T, typename U, int W, int THREADS, typename Row>
+__device__ __forceinline__ void sum_piece(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs &a, int p, int col0, int step, const unsigned *key, const Row *row,
+                                          int n, unsigned before, unsigned behind, uint4 *ring) {
+    constexpr int NV = sum_vectors<T, W>();
     constexpr bool RING = W * sizeof(T) >= 4;
-    __shared__ uint4 ring[RING ? AHEAD * SUM_THREADS : 1];
-    grid_wait();
-    grid_release();
-    const int both = 2 * min(sum_blocks, zero_blocks);
-    int block = blockIdx.x;
-    if (block < both) {
-        if (block & 1) { zero_rows(z, block >> 1, zero_blocks); return; }
-        block >>= 1;
-    } else {
-        block -= both >> 1;
-        if (zero_blocks > sum_blocks) { zero_rows(z, block, zero_blocks); return; }
-    }
-    const int width = a.tpr * W * NV, tiles = (a.dim + width - 1) / width;
-    const int group = threadIdx.x / a.tpr, lane = threadIdx.x & (a.tpr - 1);
-    const long long unit = (long long)block * (SUM_THREADS / a.tpr) + group;
-    const int p = (int)(unit / tiles), col0 = (int)(unit - (long long)p * tiles) * width + lane * W, step = a.tpr * W;   // vector i at col0 + i * step
-    // the piece's keys and rows first: then the rows themselves can all be asked for at once
-    const int i0 = p < a.pieces ? p * a.piece : a.n, n = min(a.n - i0, a.piece);
-    unsigned *key = s_key + group * a.piece;
-    int *row = s_row + group * a.piece;
-    for (int i = lane; i < n; i += a.tpr) { key[i] = __ldg(a.keys + i0 + i); row[i] = __ldg(a.rows + i0 + i); }
-    const unsigned before = n > 0 && i0 > 0 ? __ldg(a.keys + i0 - 1) : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? __ldg(a.keys + i0 + n) : 0xffffffffu;
-    __syncthreads();
-    if (n <= 0 || col0 >= a.dim) return;
     unsigned cur = key[0];
     if (cur >= (unsigned)a.vocab) return;                  // nothing but padding from here on
     bool from_before = before == cur;
@@ -365,7 +344,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
             if (i < n && key[i] < (unsigned)a.vocab)
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
-                    if (col0 + v * step < a.dim) cp_async<VB>(slots + (stage * NV + v) * SUM_THREADS * VB, dout + (long long)row[i] * a.ld_dout + col0 + v * step);
+                    if (col0 + v * step < a.dim) cp_async<VB>(slots + (stage * NV + v) * THREADS * VB, dout + (long long)row[i] * a.ld_dout + col0 + v * step);
             cp_commit();
         };
 #pragma unroll
@@ -378,7 +357,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
             float x[NV][W];
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                load_vec<T, W>(x[v], reinterpret_cast<const T *>(reinterpret_cast<const char *>(ring) + (stage * NV + v) * SUM_THREADS * VB + threadIdx.x * VB));
+                load_vec<T, W>(x[v], reinterpret_cast<const T *>(reinterpret_cast<const char *>(ring) + (stage * NV + v) * THREADS * VB + threadIdx.x * VB));
             fetch(i + AHEAD, stage);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -411,8 +390,73 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
     if (from_before) save(head);
     else if (behind == cur) {
         save(head + a.dim_pad);
-        if (col0 == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
+        if (a.list && col0 == 0) a.list[atomicAdd(a.list_count, 1u)] = p;
     } else put();
+}
+
+// Every other block zeroes absent rows as long as there are any: stores that nothing waits for, beside loads that the sums wait for.
+template <typename T, typename U, int W>
+__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
+                                                                    int zero_blocks) {
+    __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
+    __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
+    __shared__ uint4 ring[W * sizeof(T) >= 4 ? AHEAD * SUM_THREADS : 1];
+    grid_wait();
+    grid_release();
+    const int both = 2 * min(sum_blocks, zero_blocks);
+    int block = blockIdx.x;
+    if (block < both) {
+        if (block & 1) { zero_rows(z, block >> 1, zero_blocks); return; }
+        block >>= 1;
+    } else {
+        block -= both >> 1;
+        if (zero_blocks > sum_blocks) { zero_rows(z, block, zero_blocks); return; }
+    }
+    const int step = a.tpr * W, width = step * sum_vectors<T, W>(), tiles = (a.dim + width - 1) / width;
+    const int group = threadIdx.x / a.tpr, lane = threadIdx.x & (a.tpr - 1);
+    const long long unit = (long long)block * (SUM_THREADS / a.tpr) + group;
+    const int p = (int)(unit / tiles), col0 = (int)(unit - (long long)p * tiles) * width + lane * W;
+    // the piece's keys and rows first: then the rows themselves can all be asked for at once
+    const int i0 = p < a.pieces ? p * a.piece : a.n, n = min(a.n - i0, a.piece);
+    unsigned *key = s_key + group * a.piece;
+    int *row = s_row + group * a.piece;
+    for (int i = lane; i < n; i += a.tpr) { key[i] = __ldg(a.keys + i0 + i); row[i] = __ldg(a.rows + i0 + i); }
+    const unsigned before = n > 0 && i0 > 0 ? __ldg(a.keys + i0 - 1) : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? __ldg(a.keys + i0 + n) : 0xffffffffu;
+    __syncthreads();
+    if (n > 0 && col0 < a.dim) sum_piece<T, U, W, SUM_THREADS>(dtable, dout, a, p, col0, step, key, row, n, before, behind, ring);
+}
+
+// Sort and sums in one launch, for few tokens: every block sorts all of them by itself, which takes no longer than one block would, and then has its share of
+// the pieces' keys and rows in its own shared memory.  Block 0 leaves the keys for the joins.
+template <typename T, typename U, int W>
+__global__ void __launch_bounds__(SORT_THREADS) embedding_small_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const int *__restrict__ tokens, const SumArgs a,
+                                                                       const ZeroArgs z, int passes, int bits, unsigned *__restrict__ keys_out) {
+    extern __shared__ __align__(16) unsigned sm[];
+    grid_wait();
+    const unsigned *key;
+    const unsigned short *row;
+    sort_in_block(sm, tokens, a.n, a.vocab, passes, bits, &key, &row);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.n; i += SORT_THREADS) keys_out[i] = key[i];
+    // absent rows: a lane looks for each of 32 tokens among the keys
+    for (long long v0 = (long long)z.v0 + ((long long)blockIdx.x * SORT_WARPS + (threadIdx.x >> 5)) * 32; v0 < z.v1; v0 += (long long)gridDim.x * SORT_WARPS * 32) {
+        const unsigned v = (unsigned)v0 + (threadIdx.x & 31);
+        int lo = 0, hi = a.n;                              // the first key that is not below v
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (key[mid] < v) lo = mid + 1; else hi = mid;
+        }
+        unsigned absent = __ballot_sync(0xffffffffu, v < (unsigned)z.v1 && (lo == a.n || key[lo] != v));
+        for (; absent; absent &= absent - 1) zero_row(z, v0 + __ffs(absent) - 1);
+    }
+    const int step = a.tpr * W, width = step * sum_vectors<T, W>(), tiles = (a.dim + width - 1) / width, groups = SORT_THREADS / a.tpr;
+    const int group = threadIdx.x / a.tpr, lane = threadIdx.x & (a.tpr - 1);
+    uint4 *ring = reinterpret_cast<uint4 *>(sm + SMALL_WORDS);   // the counts are done with
+    for (int unit = blockIdx.x * groups + group; unit < a.pieces * tiles; unit += gridDim.x * groups) {
+        const int p = unit / tiles, col0 = (unit - p * tiles) * width + lane * W, i0 = p * a.piece, n = min(a.n - i0, a.piece);
+        if (col0 < a.dim)
+            sum_piece<T, U, W, SORT_THREADS>(dtable, dout, a, p, col0, step, key + i0, row + i0, n, i0 > 0 ? key[i0 - 1] : 0xffffffffu, i0 + n < a.n ? key[i0 + n] : 0xffffffffu, ring);
+    }
 }
 
 // Tokens that cross pieces: tail of the first piece plus the heads of those that follow.  A block is a.cols column vectors x 256 / a.cols
@@ -422,11 +466,14 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dta
     constexpr int P = W < 4 ? 4 : W;                       // partial sums are aligned whatever the table is
     __shared__ __align__(16) float part[256 * P];
     grid_wait();
-    const unsigned n_list = *a.list_count;
+    const unsigned n_list = a.list ? *a.list_count : a.pieces;
     const int phases = 256 / a.cols, x = threadIdx.x & (a.cols - 1), y = threadIdx.x / a.cols, col = ((int)blockIdx.y * a.cols + x) * P;
     for (unsigned li = blockIdx.x; li < n_list; li += gridDim.x) {
-        const int p = a.list[li];
+        const int p = a.list ? a.list[li] : (int)li;
+        if ((p + 1) * (long long)a.piece >= a.n) continue;
         const unsigned key = __ldg(a.keys + (size_t)(p + 1) * a.piece);
+        // without a list: does a token that begins in the piece go on behind it?
+        if (!a.list && (key >= (unsigned)a.vocab || __ldg(a.keys + (size_t)(p + 1) * a.piece - 1) != key || (p > 0 && __ldg(a.keys + (size_t)p * a.piece - 1) == key))) continue;
         float s[P];
 #pragma unroll
         for (int j = 0; j < P; ++j) s[j] = 0.0f;
@@ -536,7 +583,7 @@ int forward(U *out, long long ld_out, const T *table, long long ld_table, int vo
 }
 
 template <typename T, typename U, int W>
-int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int zero_blocks, cudaStream_t st) {
+int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int zero_blocks, const int *tokens, const Plan &plan, unsigned *keys, cudaStream_t st) {
     SumArgs a = base;
     const int per_thread = 16 / (int)sizeof(T), P = W < 4 ? 4 : W;        // columns of a thread of the sums, and of the joins
     unsigned tpr = pow2_at_least((unsigned)((a.dim + per_thread - 1) / per_thread));
@@ -546,8 +593,17 @@ int sums(U *dtable, const T *dout, const SumArgs &base, const ZeroArgs &z, int z
     a.cols = cols > 32 ? 32 : (int)cols;
     const long long tiles = (a.dim + (long long)tpr * per_thread - 1) / ((long long)tpr * per_thread), per = SUM_THREADS / tpr;
     const long long blocks = (a.pieces * tiles + per - 1) / per;
-    if (blocks + zero_blocks > 0x7fffffffll) { set_error("b2_embedding_backward: %lld blocks", blocks); return B2_ERR_BAD_SHAPE; }
-    B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks, zero_blocks));
+    if (a.n <= SMALL_SORT) {
+        const int sort_bytes = (1 << plan.bits) * SORT_WARPS * 4, ring_bytes = W * sizeof(T) >= 4 ? AHEAD * SORT_THREADS * 16 : 0;
+        const int smem = SMALL_WORDS * 4 + (sort_bytes > ring_bytes ? sort_bytes : ring_bytes);
+        B2_TRY(set_max_dynamic_smem((const void *)embedding_small_kernel<T, U, W>, SMALL_WORDS * 4 + AHEAD * SORT_THREADS * 16));
+        // as many blocks as have something to do, or as there are multiprocessors
+        const long long units = (a.pieces * tiles * tpr + SORT_THREADS - 1) / SORT_THREADS, rows = ((long long)z.v1 - z.v0 + 4 * SORT_WARPS - 1) / (4 * SORT_WARPS);
+        const long long want = units > rows ? units : rows;
+        B2_TRY(launch_chained(embedding_small_kernel<T, U, W>, dim3((unsigned)(want < sm_count() ? want : sm_count())), dim3(SORT_THREADS), smem, st, dtable, dout, tokens, a, z,
+                              plan.passes, plan.bits, keys));
+    } else if (blocks + zero_blocks > 0x7fffffffll) { set_error("b2_embedding_backward: %lld blocks", blocks); return B2_ERR_BAD_SHAPE; }
+    else B2_TRY(launch_chained(embedding_sum_kernel<T, U, W>, dim3((unsigned)(blocks + zero_blocks)), dim3(SUM_THREADS), 0, st, dtable, dout, a, z, (int)blocks, zero_blocks));
     const int join_tiles = (a.dim + a.cols * P - 1) / (a.cols * P), most = (sm_count() * 8 + join_tiles - 1) / join_tiles;
     return launch_chained(embedding_join_kernel<U, W>, dim3((unsigned)(a.pieces < most ? a.pieces : most), (unsigned)join_tiles), dim3(256), 0, st, dtable, a);
 }
@@ -561,11 +617,7 @@ int backward(U *dtable, long long ld_dtable, int vocab, int dim, const T *dout, 
     ZeroArgs z = {dtable, (long long)dim * (long long)sizeof(U), ld_dtable * (long long)sizeof(U), present, 0, accumulate ? 0 : vocab, 16};
     while (z.unit > 2 && (z.row_bytes % z.unit || z.ld_bytes % z.unit || !aligned_to(dtable, z.unit))) z.unit = z.unit == 16 ? 4 : 2;
     int last = 0;
-    if (n <= SMALL_SORT) {
-        const int smem = (3 * SMALL_SORT + (1 << p.bits) * SORT_WARPS) * 4;
-        B2_TRY(set_max_dynamic_smem((const void *)sort_small_kernel, (3 * SMALL_SORT + (1 << MAX_DIGIT_BITS) * SORT_WARPS) * 4));
-        B2_TRY(launch_chained(sort_small_kernel, dim3(1), dim3(SORT_THREADS), smem, st, tokens, (int)n, vocab, p.passes, p.bits, keys[0], rows[0], present, count));
-    } else {
+    if (n > SMALL_SORT) {
         B2_CUDA(cudaMemsetAsync(ws, 0, p.keys[0], st));                   // the list's length and the bits of the tokens that occur
         // rows that a launch of the sort zeroes besides: about as much as fits under its latency
         const long long share = (20ll << 20) / (z.row_bytes > 0 ? z.row_bytes : 1);
@@ -589,14 +641,14 @@ int backward(U *dtable, long long ld_dtable, int vocab, int dim, const T *dout, 
             a.kin = a.kout; a.rin = a.rout;
         }
     }
-    SumArgs a = {keys[last], rows[last], (float *)(ws + p.partial), (int *)(ws + p.list), count, ld_dout, ld_dtable, (int)n, vocab, dim, p.dim_pad, p.piece, p.pieces,
+    SumArgs a = {keys[last], rows[last], (float *)(ws + p.partial), n > SMALL_SORT ? (int *)(ws + p.list) : nullptr, count, ld_dout, ld_dtable, (int)n, vocab, dim, p.dim_pad, p.piece, p.pieces,
                  0, 0, accumulate ? 1 : 0, scale};
     const long long left = z.v1 - z.v0, zero_blocks = left > 0 ? (left + 3) / 4 < sm_count() * 16ll ? (left + 3) / 4 : sm_count() * 16ll : 0;
     const int w = common_width(16 / (int)sizeof(T), dim, dout, ld_dout, sizeof(T), dtable, ld_dtable, sizeof(U));
-    if (w == 8) return sums<T, U, (16 / sizeof(T))>(dtable, dout, a, z, (int)zero_blocks, st);
-    if (w >= 4) return sums<T, U, 4>(dtable, dout, a, z, (int)zero_blocks, st);
-    if (w >= 2) return sums<T, U, 2>(dtable, dout, a, z, (int)zero_blocks, st);
-    return sums<T, U, 1>(dtable, dout, a, z, (int)zero_blocks, st);
+    if (w == 8) return sums<T, U, (16 / sizeof(T))>(dtable, dout, a, z, (int)zero_blocks, tokens, p, keys[0], st);
+    if (w >= 4) return sums<T, U, 4>(dtable, dout, a, z, (int)zero_blocks, tokens, p, keys[0], st);
+    if (w >= 2) return sums<T, U, 2>(dtable, dout, a, z, (int)zero_blocks, tokens, p, keys[0], st);
+    return sums<T, U, 1>(dtable, dout, a, z, (int)zero_blocks, tokens, p, keys[0], st);
 }
 
 }  // namespace

@@ -663,8 +663,8 @@ int b2_embedding_forward(void *out, int out_type, long long ld_out, const void *
     if (bad_sizes("b2_embedding_forward", n, vocab, dim)) return B2_ERR_BAD_SHAPE;
     const int eo = type_size(out_type), et = type_size(table_type);
     if (!eo || !et) { set_error("b2_embedding_forward: unknown element type (output %d, table %d)", out_type, table_type); return B2_ERR_BAD_ARG; }
-    if (ld_out < dim || ld_table < dim) {
-        set_error("b2_embedding_forward: leading dimension too small (output %lld, table %lld for %d columns)", ld_out, ld_table, dim);
+    if (ld_out < dim || ld_table < dim || ld_out > MAX_LD || ld_table > MAX_LD) {
+        set_error("b2_embedding_forward: leading dimension too small or beyond 2^40 (output %lld, table %lld for %d columns)", ld_out, ld_table, dim);
         return B2_ERR_BAD_ARG;
     }
     if (!n) return B2_OK;
@@ -699,8 +699,8 @@ int b2_embedding_backward(void *dtable, int dtable_type, long long ld_dtable, in
     if (bad_sizes("b2_embedding_backward", n, vocab, dim)) return B2_ERR_BAD_SHAPE;
     const int et = type_size(dtable_type), ed = type_size(dout_type);
     if (!et || !ed) { set_error("b2_embedding_backward: unknown element type (table %d, output errors %d)", dtable_type, dout_type); return B2_ERR_BAD_ARG; }
-    if (ld_dtable < dim || ld_dout < dim) {
-        set_error("b2_embedding_backward: leading dimension too small (table %lld, output errors %lld for %d columns)", ld_dtable, ld_dout, dim);
+    if (ld_dtable < dim || ld_dout < dim || ld_dtable > MAX_LD || ld_dout > MAX_LD) {
+        set_error("b2_embedding_backward: leading dimension too small or beyond 2^40 (table %lld, output errors %lld for %d columns)", ld_dtable, ld_dout, dim);
         return B2_ERR_BAD_ARG;
     }
     if (!dtable || !aligned_to(dtable, et)) { set_error("b2_embedding_backward: the table's gradient is missing or not aligned to its elements"); return B2_ERR_BAD_ARG; }

@@ -282,7 +282,7 @@ int run(const b2_tensor *src, const b2_tensor *dst, int n, bool clip, float max_
 
 int dispatch(const char *who, const b2_tensor *src, const b2_tensor *dst, int n, bool clip, float max_norm, float *norm, void *ws, size_t ws_bytes,
              cudaStream_t st) {
-    if (!norm) { set_error("%s: null pointer for the norm", who); return B2_ERR_BAD_ARG; }
+    if (!norm || !aligned_to(norm, 4)) { set_error("%s: null pointer for the norm, or not aligned to 4 bytes", who); return B2_ERR_BAD_ARG; }
     if (!ws || !aligned_to(ws, 8)) { set_error("%s: the workspace is missing or not aligned to 8 bytes", who); return B2_ERR_BAD_ARG; }
     if (ws_bytes < b2_gradient_norm_workspace()) {
         set_error("%s: %zu bytes of workspace, %zu are needed", who, ws_bytes, b2_gradient_norm_workspace());

@@ -20,6 +20,8 @@
 
 #include <cooperative_groups.h>
 
+#include <initializer_list>
+
 #include "typed.cuh"
 
 namespace cg = cooperative_groups;
@@ -783,12 +785,18 @@ template <typename T, bool ENT, bool MASK> int backward(T *dlogits, const T *log
     return go(std::integral_constant<int, MASK ? 4 : 8>());
 }
 
+// vectors of 4-byte numbers, one a row
+bool misaligned(const char *who, std::initializer_list<const void *> all) {
+    for (const void *p : all)
+        if (!aligned_to(p, 4)) { set_error("%s: a vector of tokens or numbers is not aligned to 4 bytes", who); return true; }
+    return false;
+}
 int check(const char *who, const void *logits, int type, long long rows, int vocab, long long ld, const unsigned char *mask, long long ld_mask, float scale) {
     const int e = type_size(type);
     if (!e) { set_error("%s: unknown element type %d", who, type); return B2_ERR_BAD_ARG; }
     if (rows < 0 || vocab < 1 || vocab > (1 << 27)) { set_error("%s: %lld rows of %d logits (at most 2^27)", who, rows, vocab); return B2_ERR_BAD_SHAPE; }
-    if (ld < vocab || (mask && ld_mask != 0 && ld_mask < vocab)) {
-        set_error("%s: leading dimension too small (logits %lld, mask %lld for %d columns)", who, ld, ld_mask, vocab);
+    if (ld < vocab || ld > MAX_LD || (mask && ((ld_mask != 0 && ld_mask < vocab) || ld_mask > MAX_LD))) {
+        set_error("%s: leading dimension too small or beyond 2^40 (logits %lld, mask %lld for %d columns)", who, ld, ld_mask, vocab);
         return B2_ERR_BAD_ARG;
     }
     if (!(scale > 0.0f) || scale > 3.402823466e38f) { set_error("%s: the scale %g is not a positive number", who, (double)scale); return B2_ERR_BAD_ARG; }
@@ -809,6 +817,7 @@ int b2_logprob_forward(const void *logits, int type, long long rows, int vocab, 
     if (top < 0 || top > MAX_TOP) { set_error("b2_logprob_forward: %d alternatives (at most %d)", top, MAX_TOP); return B2_ERR_BAD_SHAPE; }
     if (!rows) return B2_OK;
     if (!lse || (logprob && !tokens_dev) || (top && (!top_tokens || !top_logprobs))) { set_error("b2_logprob_forward: null pointer"); return B2_ERR_BAD_ARG; }
+    if (misaligned("b2_logprob_forward", {tokens_dev, logprob, lse, entropy, top_tokens, top_logprobs})) return B2_ERR_BAD_ARG;
     const FwdArgs a = {mask, ld_mask, tokens_dev, logprob, lse, entropy, top_logprobs, top_tokens, rows, ld, vocab, top, scale};
     return with_type(type, [&](auto *t) { return forward((const B2_ELEM(t) *)logits, a, (cudaStream_t)stream); });
 }
@@ -817,11 +826,15 @@ int b2_logprob_backward(void *dlogits, long long ld_dlogits, const void *logits,
                         long long ld_mask, float scale, const int *tokens_dev, const float *lse, const float *dlogprob, const float *entropy, const float *dentropy,
                         b2_stream stream) {
     B2_TRY(check("b2_logprob_backward", logits, type, rows, vocab, ld, mask, ld_mask, scale));
-    if (ld_dlogits < vocab) { set_error("b2_logprob_backward: leading dimension too small (gradient %lld for %d columns)", ld_dlogits, vocab); return B2_ERR_BAD_ARG; }
+    if (ld_dlogits < vocab || ld_dlogits > MAX_LD) {
+        set_error("b2_logprob_backward: leading dimension too small or beyond 2^40 (gradient %lld for %d columns)", ld_dlogits, vocab);
+        return B2_ERR_BAD_ARG;
+    }
     if (!rows) return B2_OK;
     if (!dlogits || !aligned_to(dlogits, type_size(type))) { set_error("b2_logprob_backward: the gradient is missing or not aligned to its elements"); return B2_ERR_BAD_ARG; }
     if (!tokens_dev || !lse || (dentropy && !entropy)) { set_error("b2_logprob_backward: null pointer"); return B2_ERR_BAD_ARG; }
     if (dlogits == logits && ld_dlogits != ld) { set_error("b2_logprob_backward: in place with another leading dimension"); return B2_ERR_BAD_ARG; }
+    if (misaligned("b2_logprob_backward", {tokens_dev, lse, dlogprob, entropy, dentropy})) return B2_ERR_BAD_ARG;
     const BwdArgs a = {mask, ld_mask, tokens_dev, lse, dlogprob, entropy, dentropy, rows, ld, ld_dlogits, vocab, scale};
     return with_type(type, [&](auto *t) {
         typedef B2_ELEM(t) T;

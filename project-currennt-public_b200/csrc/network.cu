@@ -9,6 +9,7 @@
 #include <random>
 
 #include <mutex>
+#include <new>
 
 #include "network.hpp"
 
@@ -623,11 +624,12 @@ int NeuralNetwork::readGradientNorm(float *norm) {
 int NeuralNetwork::updateWeights(float lr, float mom) {
     ProfScope ps(*this, "sgd_update");
     if (maxGradientNorm > 0.0f) {
-        std::vector<b2_tensor> grads;
+        std::unique_ptr<b2_tensor[]> grads(new (std::nothrow) b2_tensor[layers.size()]);
+        if (!grads) { set_error("b2_net_update_weights: out of memory"); return B2_ERR_STATE; }
+        int count = 0;
         for (size_t i = 0; i < layers.size(); ++i)
-            if (TrainableLayer *t = dynamic_cast<TrainableLayer *>(layers[i].get())) grads.push_back({t->weightUpdates(), t->numWeights(), B2_F32});
-        B2_TRY(b2_gradient_clip(grads.data(), nullptr, (int)grads.size(), maxGradientNorm, (float *)clipDev, (char *)clipDev + 256,
-                                b2_gradient_norm_workspace(), (b2_stream)stream));
+            if (TrainableLayer *t = dynamic_cast<TrainableLayer *>(layers[i].get())) grads[count++] = {t->weightUpdates(), t->numWeights(), B2_F32};
+        B2_TRY(b2_gradient_clip(grads.get(), nullptr, count, maxGradientNorm, (float *)clipDev, (char *)clipDev + 256, b2_gradient_norm_workspace(), (b2_stream)stream));
     }
     // option 4 (OPTIMIZATION_SGD_DECAY) updates like plain SGD; its schedule lives in the training run (b2_optimizer_train)
     const bool adjust = optOption > 0 && optOption != 4;

@@ -30,6 +30,7 @@ template <typename T, int N> __device__ __forceinline__ void store_vec(T *p, con
     *reinterpret_cast<Vec<T, N> *>(p) = x;
 }
 
+constexpr long long MAX_LD = 1ll << 40;   // elements from row to row: 2^31 rows of them stay inside 64 bits
 inline int type_size(int type) { return type == B2_F32 ? 4 : (type == B2_BF16 || type == B2_F16) ? 2 : 0; }
 inline bool aligned_to(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 inline unsigned pow2_at_least(unsigned x) { unsigned p = 1; while (p < x) p <<= 1; return p; }

@@ -105,6 +105,20 @@ def test_tensor_lists():
     refused("error -1.*needed", b2lstm.gradient_clip, b2lstm.TensorList([Fake(3)]), 1.0, Fake(1), workspace=Fake(8, dtype="torch.uint8"))
 
 
+def test_addresses_and_distances_that_no_kernel_may_see():
+    L, at = b2lstm.lib(), 4096
+    assert L.b2_logprob_forward(at, 0, 4, 16, 16, None, 0, 1.0, at + 2, at, at, None, 0, None, None, None) == -5
+    assert L.b2_logprob_forward(at, 0, 4, 16, 16, None, 0, 1.0, at, at, at + 1, None, 0, None, None, None) == -5
+    assert L.b2_logprob_forward(at, 0, 4, 16, 1 << 41, None, 0, 1.0, at, at, at, None, 0, None, None, None) == -5
+    assert L.b2_logprob_forward(at, 0, 4, 16, 16, at, 1 << 41, 1.0, at, at, at, None, 0, None, None, None) == -5
+    assert L.b2_logprob_backward(at, 1 << 41, at, 0, 4, 16, 16, None, 0, 1.0, at, at, at, None, None, None) == -5
+    assert L.b2_logprob_backward(at, 16, at, 0, 4, 16, 16, None, 0, 1.0, at, at + 2, at, None, None, None) == -5
+    assert L.b2_embedding_forward(at, 0, 1 << 41, at, 0, 16, 4, 16, at, 4, 1.0, None) == -5
+    assert L.b2_embedding_forward(at, 0, 16, at, 0, 16, 4, 16, at + 1, 4, 1.0, None) == -5
+    assert L.b2_embedding_backward(at, 0, 16, 4, 16, at, 0, 1 << 41, at, 4, 1.0, 0, at, 1 << 20, None) == -5
+    assert L.b2_gradient_norm(None, 0, at + 2, at, 1 << 20, None) == -5
+
+
 def test_the_net_refuses_a_clipping_without_a_net():
     assert b2lstm.lib().b2_net_set_gradient_clipping(None, 1.0) == -5
     assert b2lstm.lib().b2_net_gradient_norm(None, C.byref(C.c_float())) == -5

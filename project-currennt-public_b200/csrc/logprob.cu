@@ -11,8 +11,8 @@
 // Rows of up to 1024 entries stay in the registers of 4 to 32 lanes.  Longer rows take a warp where the rows alone fill the device, a block of 4 or
 // 8 warps where they do not, or, when there are few, a thread-block cluster of up to 8 blocks, which hand their sums and lists to the first
 // one through distributed shared memory: a row needs neither a second launch nor a workspace.
-// Bound, for long rows of 16-bit logits, by memory and by the exponentials alike: 11.6 entries arrive per cycle and SM, and the special function
-// units return about 12 exponentials.  Measured on a B200 (device time): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth;
+// Bound, for long rows of 16-bit logits, by memory, with the exponentials close behind: 11.6 entries may arrive per cycle and SM, and the special
+// function units return 16 exponentials.  Measured on a B200 (device time): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth;
 // two bytes an entry), with four alternatives 162 us (the chains of the insertions, 20 a row), with 20 244 us; 38400 rows of 259 fp32 8.6 us (72 %);
 // 8 rows of 131072 with a mask and eight alternatives 11.4 us, without alternatives 6.8 us, a launch and two trips to memory of it.
 // Backward: one read, one write.  8192 rows of 32003 bf16 that start anywhere 167 us (96 %); 38400 of 259 fp32 18 us.

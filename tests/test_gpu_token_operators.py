@@ -634,6 +634,64 @@ def test_block_norm_backward_over_many_rows(tm, rows, dim, gate_rows):
         assert off <= (300 + math.sqrt(terms)) * u * 4, (k, off.item())
 
 
+@pytest.mark.parametrize("dim", [1, 45, 102, 127, 128, 129, 202, 255, 256, 257, 405])
+@pytest.mark.parametrize("t,ln,pad,shift", [("f32", True, 1, 1), ("f32", False, 2, 2), ("bf16", True, 1, 1), ("f16", False, 1, 1), ("bf16", False, 2, 2)])
+def test_block_norm_of_many_narrow_rows(tm, dim, t, ln, pad, shift):
+    """rows that no 16-byte access fits, more of them than the kernel for few rows takes: the columns a thread has change with the width.
+    The bounds are those of test_block_norm: a thread's terms are no more than there."""
+    torch, b2 = tm
+    rows, eps, a = 400000 // dim, 1e-5, 0.5
+    c = _norm_case(tm, rows, dim, t, ln, 0, pad, shift, padding=0.1)
+    real = (c["pat"].cpu().numpy() != 0)[:, None]
+    fy, y = _out(torch, (rows, dim), t, pad, shift)
+    fh, h = _out(torch, (rows, dim), t, pad, shift)
+    stats = torch.full((rows, 4), float("nan"), device="cuda")
+    kw = dict(w_pre=c["w1"], w_post=c["w2"], b_post=c["b2"], pat_types=c["pat"], layer_norm=ln, residual_scale=a)
+    b2.block_norm_forward(c["x"], c["f"], y, h, b_pre=c["b1"], eps=eps, stats=stats, **kw)
+    eps = float(np.float32(eps))
+    X, F, w1, w2 = (_host(c[n]) for n in ("x", "f", "w1", "w2"))
+    b1, b_2 = (_host(c[n]) if ln else np.zeros(dim) for n in ("b1", "b2"))
+    own = lambda v, rs: 60 * u * (np.abs((v - v.mean(1, keepdims=True) * ln) * rs[:, None]) + (np.abs(v).mean(1) * rs)[:, None] * ln)  # noqa: E731
+    m2, r2 = _norm64(F, ln, eps)
+    n = (F - m2[:, None]) * r2[:, None] * w2 + b_2
+    want = np.where(real, X + a * n, 0.0)
+    _close(_host(y), want, real * (4 * u * (np.abs(X) + np.abs(a * n)) + a * (own(F, r2) * np.abs(w2) + u * np.abs(b_2))) + U[t] * np.abs(want) + TINY[t])
+    Y = _host(y)
+    m1, r1 = _norm64(Y, ln, eps)
+    want = np.where(real, (Y - m1[:, None]) * r1[:, None] * w1 + b1, 0.0)
+    _close(_host(h), want, real * (own(Y, r1) * np.abs(w1) + 4 * u * (np.abs(want) + np.abs(b1))) + U[t] * np.abs(want) + TINY[t])
+    _untouched(torch, fy, y)
+    _untouched(torch, fh, h)
+
+    outs = {k: _out(torch, (rows, dim), t, pad, shift) for k in ("dx", "df")}
+    sums = {k: torch.full((dim,), float("nan"), device="cuda") if ln or k[1] == "w" else None for k in ("dw_pre", "db_pre", "dw_post", "db_post")}
+    ws = torch.full((b2.block_norm_backward_workspace(rows, dim, 0),), 0xA5, dtype=torch.uint8, device="cuda")
+    b2.block_norm_backward(outs["dx"][1], outs["df"][1], c["dy"], c["dh"], y, c["f"], stats, workspace=ws, **sums, **kw)
+    dy, dh = np.where(real, _host(c["dy"]), 0.0), np.where(real, _host(c["dh"]), 0.0)
+    m2, r2, m1, r1 = (_host(stats)[:, k:k + 1] for k in range(4))
+    v1, v2 = (Y - m1) * r1, (F - m2) * r2
+
+    def back(d, v, w, rs):
+        wd = d * w
+        g = rs * (wd - v * (wd * v).mean(1, keepdims=True) - (wd.mean(1, keepdims=True) if ln else 0.0))
+        size = rs * (np.abs(wd) + np.abs(v) * np.abs(wd * v).mean(1, keepdims=True) + (np.abs(wd).mean(1, keepdims=True) if ln else 0.0))
+        return g, size
+
+    g, size = back(dh, v1, w1, r1)
+    dt, M = dy + g, np.abs(dy) + size
+    dn, Mn = a * dt, a * M
+    dF, _ = back(dn, v2, w2, r2)
+    _, MF = back(Mn, np.abs(v2), np.abs(w2), r2)
+    _close(_host(outs["dx"][1]), np.where(real, dt, 0.0), real * 100 * u * M + U[t] * np.abs(dt) * real + TINY[t])
+    _close(_host(outs["df"][1]), np.where(real, dF, 0.0), real * 300 * u * MF + U[t] * np.abs(dF) * real + TINY[t])
+    for k, x, s in (("dw_pre", dh * v1, np.abs(dh * v1)), ("db_pre", dh, np.abs(dh)), ("dw_post", dn * v2, Mn * np.abs(v2)), ("db_post", dn, Mn)):
+        if sums[k] is not None:
+            # a worker adds at most rows / 148 of them in turn, the join 32 chains of at most 148
+            _close(_host(sums[k]), np.where(real, x, 0.0).sum(0), (300 + rows / 148 + 40) * u * np.where(real, s, 0.0).sum(0) + 1e-300)
+    for k in outs:
+        _untouched(torch, *outs[k])
+
+
 def test_block_norm_parts(tm):
     """without a block (first norm), without a norm behind (last block), in place, without statistics, gradients left out"""
     torch, b2 = tm

@@ -236,9 +236,9 @@ typedef struct {
 } b2_tensor;
 size_t b2_gradient_norm_workspace(void);
 int b2_gradient_norm(const b2_tensor *tensors, int n, float *norm_dev, void *workspace, size_t workspace_bytes, b2_stream stream);
-/* The same, and out = tensors * min(1, max_norm / norm), element by element; out[i] has tensors[i]'s count and may have another type.
- * out NULL: in place.  A norm that is NaN or infinite leaves the values as they are (the update of b2_net then zeroes the entries that are
- * no numbers).  Tensors must not overlap, save that out[i] may be tensors[i]. */
+/* The same, and out = tensors * min(1, max_norm / norm), element by element, norm being the float that is reported; out[i] has tensors[i]'s
+ * count and may have another type.  out NULL: in place.  A norm that is NaN or infinite (of finite values too, where it passes the largest
+ * float) leaves the values as they are (the update of b2_net then zeroes the entries that are no numbers).  Tensors must not overlap, save that out[i] may be tensors[i]. */
 int b2_gradient_clip(const b2_tensor *tensors, const b2_tensor *out, int n, float max_norm, float *norm_dev, void *workspace,
                      size_t workspace_bytes, b2_stream stream);
 

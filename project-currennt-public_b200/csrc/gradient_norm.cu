@@ -2,6 +2,7 @@
 //
 //   n = sqrt(sum_i sum_j x_ij^2),   out_ij = x_ij * (n > max ? max / n : 1)
 //
+// The factor is formed from the norm as it is reported, in fp32: who reads the norm can tell what was done, and repeat it.
 // The list travels as a kernel argument: no table in device memory, no copy, nothing kept between calls.  Every tensor is cut
 // into chunks of CHUNK bytes that start on 16-byte boundaries; a block takes a contiguous range of all chunks, so it looks up
 // its first tensor once.  Squares are summed in fp64: the square of any finite fp32 value is a normal fp64 number, so neither large
@@ -148,8 +149,16 @@ __device__ __forceinline__ double norm_of(const double *partial, int n, double *
     return sqrt(block_sum(s, red));
 }
 
+// What the values are multiplied by: one factor, or two where one would be subnormal and have lost bits (the second is 1 elsewhere)
+struct Factor { float a, b; };
+__device__ __forceinline__ Factor factor_of(float max_norm, float norm) {
+    const float c = max_norm / norm;
+    if (c >= 1.17549435e-38f) return {c, 1.0f};
+    const float root = (float)sqrt((double)max_norm / (double)norm);
+    return {root, root};
+}
 // scaled vectors to where they came from
-template <typename T, typename U> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], float coef) {
+template <typename T, typename U> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], const Factor &by) {
     constexpr int W = 16 / sizeof(T);
     // elements are counted from the 16-byte boundary; in the output's type its vectors may lie off theirs
     U *to = reinterpret_cast<U *>(p.dst) - p.mis / (int)sizeof(T);
@@ -160,7 +169,7 @@ template <typename T, typename U> __device__ __forceinline__ void put(const Piec
         float v[W];
         values<T, W>(v, q[i]);
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] *= coef;
+        for (int j = 0; j < W; ++j) v[j] = v[j] * by.a * by.b;
         if (fits && inside(p, at)) store_vec<U, W>(to + at / sizeof(T), v);
         else if (at < end && at + 16 > (unsigned)p.mis)
 #pragma unroll
@@ -168,10 +177,10 @@ template <typename T, typename U> __device__ __forceinline__ void put(const Piec
                 if (at + j * sizeof(T) >= (unsigned)p.mis && at + j * sizeof(T) < end) to[at / sizeof(T) + j] = from_float<U>(v[j]);
     }
 }
-template <typename T> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], float coef) {
-    if (p.dst_type == B2_F32) put<T, float>(p, q, coef);
-    else if (p.dst_type == B2_BF16) put<T, __nv_bfloat16>(p, q, coef);
-    else put<T, __half>(p, q, coef);
+template <typename T> __device__ __forceinline__ void put(const Piece &p, const uint4 (&q)[VECTORS], const Factor &by) {
+    if (p.dst_type == B2_F32) put<T, float>(p, q, by);
+    else if (p.dst_type == B2_BF16) put<T, __nv_bfloat16>(p, q, by);
+    else put<T, __half>(p, q, by);
 }
 
 template <int CAP>
@@ -191,11 +200,11 @@ __global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant_
         fetch(q, now);
     }
     grid_wait();
-    const double norm = norm_of(partial, n_partial, red);
-    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-    // a norm that is no finite number says nothing about a scale: the values stay as they are
-    const bool scale = norm > (double)max_norm && norm <= 1.7976931348623157e308;
-    const float coef = scale ? (float)((double)max_norm / norm) : 1.0f;
+    const float norm = (float)norm_of(partial, n_partial, red);
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+    // a norm that is no finite number, one beyond a float among them, says nothing about a scale: the values stay as they are
+    const bool scale = norm > max_norm && norm <= 3.402823466e38f;
+    const Factor by = scale ? factor_of(max_norm, norm) : Factor{1.0f, 1.0f};
     next = now;
     for (unsigned c = c1; c-- > c0;) {
         if (c > c0) {
@@ -204,9 +213,9 @@ __global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant_
             if (scale || next.src != next.dst) fetch(r, next);
         }
         if (scale || now.src != now.dst) {
-            if (now.src_type == B2_F32) put<float>(now, q, coef);
-            else if (now.src_type == B2_BF16) put<__nv_bfloat16>(now, q, coef);
-            else put<__half>(now, q, coef);
+            if (now.src_type == B2_F32) put<float>(now, q, by);
+            else if (now.src_type == B2_BF16) put<__nv_bfloat16>(now, q, by);
+            else put<__half>(now, q, by);
         }
         now = next;
 #pragma unroll

@@ -489,6 +489,36 @@ def test_gradient_norm_of_extreme_values(tm):
     assert (t == 0).all() and norm.item() == 10
 
 
+def test_gradient_clip_at_the_ends_of_the_floats(tm):
+    """a norm beyond the largest float is reported as infinite and scales nothing; a factor too small for a normal number loses nothing"""
+    torch, b2 = tm
+    ws, norm = torch.empty(b2.gradient_norm_workspace(), dtype=torch.uint8, device="cuda"), torch.zeros(1, device="cuda")
+    t = torch.full((10000,), 1e37, device="cuda")
+    out = torch.zeros_like(t)
+    b2.gradient_clip(b2.TensorList([t], [out]), 1.0, norm, workspace=ws)
+    assert norm.item() == math.inf and torch.equal(out, t)
+    for value, most in ((1e36, 1e-3), (3e36, 1e-20), (1e36, 1e-1), (1e-2, 3e-38), (1e30, 2.0)):
+        t = torch.full((10000,), value, device="cuda")
+        t[1::2] = -value / 3
+        ref = math.sqrt(float((_host(t) ** 2).sum()))
+        b2.gradient_clip(b2.TensorList([t], [out]), most, norm, workspace=ws)
+        assert abs(norm.item() - ref) <= 2 * u * ref
+        want = _host(t) * (float(np.float32(most)) / ref)
+        # the norm, its quotient (or the root of it, twice) and two products are rounded; numbers below the normal ones by their own unit
+        _close(_host(out), want, 6 * u * np.abs(want) + 2 * TINY["f32"])
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_gradient_clip_takes_its_factor_from_the_norm_it_reports(tm, t):
+    torch, b2 = tm
+    x = _rand(torch, (1, 70001), t, 5, 0.1)[0]
+    out, ws, norm = torch.empty(70001, device="cuda"), torch.empty(b2.gradient_norm_workspace(), dtype=torch.uint8, device="cuda"), torch.zeros(1, device="cuda")
+    for most in (0.37, 1.0, 3.3, 7.7, 11.1, 20.2):
+        b2.gradient_clip(b2.TensorList([x], [out]), most, norm, workspace=ws)
+        factor = np.float32(most) / norm.cpu().numpy()[0]
+        assert factor < 1 and np.array_equal(out.cpu().numpy(), x.float().cpu().numpy() * factor)
+
+
 # ---- norms around a block ------------------------------------------------------------------------------------------------------------------
 def _norm64(v, ln, eps):
     mean = v.mean(1) if ln else np.zeros(len(v))

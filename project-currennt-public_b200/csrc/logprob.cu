@@ -4,6 +4,8 @@
 //   H = -sum_j p_j log p_j,  p_j = e^(z_j - lse);   the K largest z_j by (value, lower index first)
 //   dx_j = s * (g * ([j = tok] - p_j) - h * p_j * (log p_j + H))       for gradients g of logprob and h of H
 //
+// z_j is the fp32 product everywhere: in the sums, for the given token, in the ranking and in the gradient.  A fused multiply-add would take the
+// unrounded one in the sums, and a likely token could end above log 1 by the rounding of a large z.  So S >= 1, and no log probability is above 0.
 // Forward, one pass: every thread keeps the largest value m it has met, S = sum e^(z - m) and E = sum e^(z - m) (z - m); a new maximum
 // rescales both.  Then lse = m + log S and H = log S - E / S, which needs no difference of large numbers.
 // The K largest: a warp keeps its best K as a sorted list, one entry a lane; a batch of values is looked at only if its maximum
@@ -36,6 +38,29 @@ constexpr int MAX_TOP = 32;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// z of two logits less what both subtract, z rounded.  Packed products and sums become one packed FMA in the assembler, rounding modifiers or not, and that
+// subtracts from the unrounded product; one that is an FMA already, with -0 for its addend, stays as it is.  The -0 is made from the scale, where it can not be
+// seen to be one.  With a scale that is a power of two the product needs no rounding, and the one FMA is right (8192 rows of 50001 with four alternatives: 180 us, with
+// two instructions 185 us).
+struct Exact {
+    Pair s, off;
+    __device__ __forceinline__ Pair operator()(float x, float y) const { return fma2(pair(x, y), s, off); }
+};
+struct Rounded {
+    Pair s, off, none;
+    __device__ __forceinline__ Rounded(Pair s_, Pair off_, float scale) : s(s_), off(off_) {
+        const float zero = __fmul_rn(scale, -0.0f);
+        none = pair(zero, zero);
+    }
+    __device__ __forceinline__ Pair operator()(float x, float y) const { return add2(fma2(pair(x, y), s, none), off); }
+};
+// f(function of two logits), the one that the scale asks for
+template <typename F> __device__ __forceinline__ void less_of(float scale, float minus, F &&f) {
+    const Pair s = pair(scale, scale), off = pair(-minus, -minus);
+    if ((__float_as_uint(scale) & 0x7fffffu) == 0) f(Exact{s, off});
+    else f(Rounded(s, off, scale));
+}
 
 // ---- running sums -----------------------------------------------------------------------------------------------------------------
 struct Sums { float m, s, e; };   // largest z, sum of e^(z - m), sum of e^(z - m) (z - m)
@@ -116,8 +141,8 @@ template <typename T> __device__ __forceinline__ unsigned larger_of(const uint4 
     return R::larger(R::larger(q.x, q.y), R::larger(q.z, q.w));
 }
 // The sums over U vectors of logits x; top: their largest x (NaN if one is NaN).  A pair of entries costs two conversions, one packed maximum
-// (by the caller), two packed FMAs, a packed product and sum, and two exponentials.  Where an entry is -inf the sum of w * d turns NaN and is taken
-// again with the differences held above -inf; SAFE does so at once.
+// (by the caller), two packed FMAs, a packed product and sum, and two exponentials, with a scale that is no power of two a packed sum more.  Where an
+// entry is -inf the sum of w * d turns NaN and is taken again with the differences held above -inf; SAFE does so at once.
 template <typename T, int U, bool SAFE> __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&q)[U], float top, float scale) {
     constexpr int W = 16 / sizeof(T);
     const float m = __fmul_rn(top, scale);
@@ -126,21 +151,23 @@ template <typename T, int U, bool SAFE> __device__ __forceinline__ void add_vect
     }
     if (a.m == neg_inf()) return;
     if (!SAFE) {
-        const Pair sc = pair(scale, scale), mm = pair(-a.m, -a.m), l2 = pair(LOG2E, LOG2E);
+        const Pair l2 = pair(LOG2E, LOG2E);
         Pair s = 0, e = 0;
+        less_of(scale, a.m, [&](const auto &less) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float x[W];
-            Raw<T>::values(x, q[u]);
+            for (int u = 0; u < U; ++u) {
+                float x[W];
+                Raw<T>::values(x, q[u]);
 #pragma unroll
-            for (int j = 0; j < W; j += 2) {
-                const Pair d = fma2(pair(x[j], x[j + 1]), sc, mm);
-                const float2 t = halves(mul2(d, l2));
-                const Pair w = pair(ex2(t.x), ex2(t.y));
-                s = add2(s, w);
-                e = fma2(w, d, e);
+                for (int j = 0; j < W; j += 2) {
+                    const Pair d = less(x[j], x[j + 1]);
+                    const float2 t = halves(mul2(d, l2));
+                    const Pair w = pair(ex2(t.x), ex2(t.y));
+                    s = add2(s, w);
+                    e = fma2(w, d, e);
+                }
             }
-        }
+        });
         const float2 sv = halves(s), ev = halves(e);
         const float en = ev.x + ev.y;
         if (en == en) {
@@ -156,7 +183,7 @@ template <typename T, int U, bool SAFE> __device__ __forceinline__ void add_vect
         Raw<T>::values(x, q[u]);
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-            const float d = max_nan(fmaf(x[j], scale, -a.m), -3.402823466e38f), w = ex2(d * LOG2E);
+            const float d = max_nan(__fmul_rn(x[j], scale) - a.m, -3.402823466e38f), w = ex2(d * LOG2E);
             s += w;
             e = fmaf(w, d, e);
         }
@@ -408,7 +435,8 @@ template <typename T, int G, int NV> __global__ void __launch_bounds__(256) logp
     for (int o = G / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(FULL, top, o));
     Sums t = {__fmul_rn(top, a.scale), 0.0f, 0.0f};
     if (t.m != neg_inf()) {
-        const Pair sc = pair(a.scale, a.scale), mm = pair(-t.m, -t.m), l2 = pair(LOG2E, LOG2E);
+        const Rounded less(pair(a.scale, a.scale), pair(-t.m, -t.m), a.scale);
+        const Pair l2 = pair(LOG2E, LOG2E);
         Pair s = 0, e = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -416,7 +444,7 @@ template <typename T, int G, int NV> __global__ void __launch_bounds__(256) logp
             Raw<T>::values(z, q[i]);
 #pragma unroll
             for (int j = 0; j < W; j += 2) {
-                const float2 v = halves(fma2(pair(z[j], z[j + 1]), sc, mm));
+                const float2 v = halves(less(z[j], z[j + 1]));
                 const Pair d = pair(max_nan(v.x, -3.402823466e38f), max_nan(v.y, -3.402823466e38f));   // as in add_values
                 const float2 y = halves(mul2(d, l2));
                 const Pair w = pair(ex2(y.x), ex2(y.y));
@@ -678,22 +706,24 @@ template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
     return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
 }
 // What a row's entries share: dx = p (c0 + c1 log p) with c0 = -s (g + h H), c1 = -s h, and s g more at the token.
-struct RowGrad { float neg_lse, c0, c1, at_token; int tok; };
+struct RowGrad { float lse, c0, c1, at_token; int tok; };
 // N entries from index i0 on
 template <typename T, int N, bool ENT> __device__ __forceinline__ void entry_grads(float (&o)[N], const float (&x)[N], const RowGrad &q, float scale, int i0) {
-    const Pair sc = pair(scale, scale), nl = pair(q.neg_lse, q.neg_lse), c0 = pair(q.c0, q.c0), c1 = pair(q.c1, q.c1);
+    const Pair c0 = pair(q.c0, q.c0), c1 = pair(q.c1, q.c1);
+    less_of(scale, q.lse, [&](const auto &less) {
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-        Pair lp = fma2(pair(x[j], x[j + 1]), sc, nl);
-        if (ENT) {
-            // below -1000 the probability is 0 whatever the logarithm is; -inf must not meet that 0
-            const float2 v = halves(lp);
-            lp = pair(max_nan(v.x, -1000.0f), max_nan(v.y, -1000.0f));
+        for (int j = 0; j < N; j += 2) {
+            Pair lp = less(x[j], x[j + 1]);
+            if (ENT) {
+                // below -1000 the probability is 0 whatever the logarithm is; -inf must not meet that 0
+                const float2 v = halves(lp);
+                lp = pair(max_nan(v.x, -1000.0f), max_nan(v.y, -1000.0f));
+            }
+            const float2 d = halves(mul2(exp_pair<T>(lp), ENT ? fma2(lp, c1, c0) : c0));
+            o[j] = d.x;
+            o[j + 1] = d.y;
         }
-        const float2 d = halves(mul2(exp_pair<T>(lp), ENT ? fma2(lp, c1, c0) : c0));
-        o[j] = d.x;
-        o[j + 1] = d.y;
-    }
+    });
     if ((unsigned)(q.tok - i0) < (unsigned)N)
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -722,7 +752,7 @@ __global__ void __launch_bounds__(256) logprob_backward_kernel(T *__restrict__ d
     RowGrad q;
     q.tok = __ldg(a.tokens + r);
     const float lse = __ldg(a.lse + r), g = a.dlogprob ? __ldg(a.dlogprob + r) : 0.0f, h = ENT ? __ldg(a.dentropy + r) : 0.0f;
-    q.neg_lse = -lse;
+    q.lse = lse;
     q.c0 = -a.scale * (ENT ? fmaf(h, __ldg(a.entropy + r), g) : g);
     q.c1 = -a.scale * h;
     q.at_token = a.scale * g;

@@ -307,6 +307,67 @@ def test_logprob_forward_of_special_rows(tm, vocab):
     assert np.array_equal(tt.cpu().numpy(), w_tt)
 
 
+# a row a group of lanes, a warp, a block of 8, of 4 and of 1 warps, and a cluster
+ROW_KERNELS = [(64, 40), (64, 3000), (700, 1500), (2500, 1500), (3, 70001)]
+
+
+@pytest.mark.parametrize("rows,vocab", ROW_KERNELS)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("top", [0, 3])
+def test_a_certain_token_has_the_log_probability_0(tm, rows, vocab, t, top):
+    """one token allowed, its logit large and the scale no power of two: z is one number everywhere, so z - lse is 0 and so are entropy and gradient"""
+    torch, b2 = tm
+    x = _rand(torch, (rows, vocab), t, 3, 4.0)
+    tok = np.random.default_rng(vocab).integers(0, vocab, rows)
+    at = torch.from_numpy(tok).cuda()
+    r = torch.arange(rows, device="cuda")
+    x[r, at] = (torch.rand(rows, generator=torch.Generator().manual_seed(4)) * 7000 - 2000).cuda().to(x.dtype)
+    mask = torch.zeros(rows, vocab, dtype=torch.uint8, device="cuda")
+    mask[r, at] = 1
+    lp, lse, H, tt, tl = _run_logprob(tm, x, tok, mask, 0.7, top)
+    assert (lp == 0).all() and (H == 0).all() and torch.equal(lse, x[r, at].float() * np.float32(0.7))
+    if top:
+        assert torch.equal(tt[:, 0].long(), at) and (tl[:, 0] == 0).all() and (tt[:, 1:] == -1).all()
+    d = torch.full_like(x, 9.0)
+    b2.logprob_backward(d, x, torch.from_numpy(tok).int().cuda(), lse, torch.ones(rows, device="cuda"), mask=mask, scale=0.7)
+    assert (d == 0).all()
+
+
+@pytest.mark.parametrize("rows,vocab", ROW_KERNELS)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("top", [0, 4])
+@pytest.mark.parametrize("masked", [False, True])
+def test_logprob_of_large_logits_close_together(tm, rows, vocab, t, top, masked):
+    """logits near 9000 a few apart: what is lost must follow from their differences, not from their size"""
+    torch, b2 = tm
+    x = _rand(torch, (rows, vocab), t, 6, 2.0)
+    x.copy_((x.float().clamp(-8, 8) + 9000).to(x.dtype))
+    tok = np.random.default_rng(vocab).integers(0, vocab, rows)
+    mask = None
+    if masked:
+        m = (np.random.default_rng(7).random(vocab) < 0.7).astype(np.uint8)
+        m[[0, vocab - 1]] = 1
+        mask = torch.from_numpy(m).cuda()
+    lp, lse, H, tt, tl = _run_logprob(tm, x, tok, mask, 0.7, top)
+    z = (x.float().cpu().numpy() * np.float32(0.7)).astype(np.float64)
+    if masked:
+        z = np.where(m != 0, z, -np.inf)
+    best = z.max(1, keepdims=True)
+    S = np.exp(z - best).sum(1)
+    # z - m is exact to a rounding of itself: bf16 logits near 9000 are 64 apart (scaled 45), the others within 16 + 8.  The exponential is off by 4 u and by 3 u |d| of its argument
+    # (weights e^d |d| <= 1/e beyond 1), sums of 100 partial steps, log S and the difference by a rounding each
+    want = np.where(z[np.arange(rows), tok] == -np.inf, -np.inf, z[np.arange(rows), tok] - best[:, 0] - np.log(S))
+    size = np.where(np.isfinite(want), np.abs(want), 0.0)
+    _close(_host(lp), want, u * (200 + 2 * size))
+    assert (lp <= 0).all()
+    if top:
+        order = np.argsort(-z, axis=1, kind="stable")[:, :top]
+        assert np.array_equal(tt.cpu().numpy(), order)
+        w = np.take_along_axis(z, order, 1) - best - np.log(S)[:, None]
+        _close(_host(tl), w, u * (200 + 2 * np.abs(w)))
+        assert (tl <= 0).all()
+
+
 def test_logprob_forward_marks_tokens_beyond_the_vocabulary(tm):
     torch, b2 = tm
     for vocab in (10, 3000):

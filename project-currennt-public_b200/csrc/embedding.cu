@@ -119,13 +119,13 @@ __device__ __forceinline__ void places(unsigned *count, int digits, unsigned bef
 // All passes for up to SMALL_SORT tokens, in the block's shared memory: sm holds SMALL_WORDS words and the counts.  Warp w ranks the keys
 // [w * seg, (w + 1) * seg) in rounds of 32, counts kept per (digit, warp), so equal digits stay in order.  *keys and *rows are the sorted ones.
 constexpr int SMALL_WORDS = 3 * SMALL_SORT;
-__device__ __forceinline__ void sort_in_block(unsigned *sm, const int *__restrict__ tokens, int n, int vocab, int passes, int bits, const unsigned **keys, const unsigned short **rows) {
+__device__ __forceinline__ void sort_in_block(unsigned *sm, const int *tokens, int n, int vocab, int passes, int bits, const unsigned **keys, const unsigned short **rows) {
     unsigned *key[2] = {sm, sm + SMALL_SORT};
     unsigned short *row[2] = {(unsigned short *)(sm + 2 * SMALL_SORT), (unsigned short *)(sm + 2 * SMALL_SORT) + SMALL_SORT};
     unsigned *count = sm + SMALL_WORDS;                    // [SORT_WARPS][digits]
     __shared__ unsigned warp_tot[SORT_WARPS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, digits = 1 << bits;
-    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { key[0][i] = key_of(__ldg(tokens + i), vocab); row[0][i] = (unsigned short)i; }
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) { key[0][i] = key_of(tokens[i], vocab); row[0][i] = (unsigned short)i; }
     __syncthreads();
     const int seg = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) & ~31;
     for (int p = 0; p < passes; ++p) {
@@ -302,7 +302,7 @@ constexpr int AHEAD = 12;                    // rows a thread has under way
 // ring: AHEAD times 16 bytes for each of the block's THREADS threads.
 template <typename T, int W> __host__ __device__ constexpr int sum_vectors() { return 16 / (W * (int)sizeof(T)); }
 template <typename T, typename U, int W, int THREADS, typename Row>
-__device__ __forceinline__ void sum_piece(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs &a, int p, int col0, int step, const unsigned *key, const Row *row,
+__device__ __forceinline__ void sum_piece(U *__restrict__ dtable, const T *dout, const SumArgs &a, int p, int col0, int step, const unsigned *key, const Row *row,
                                           int n, unsigned before, unsigned behind, uint4 *ring) {
     constexpr int NV = sum_vectors<T, W>();
     constexpr bool RING = W * sizeof(T) >= 4;
@@ -396,7 +396,7 @@ __device__ __forceinline__ void sum_piece(U *__restrict__ dtable, const T *__res
 
 // Every other block zeroes absent rows as long as there are any: stores that nothing waits for, beside loads that the sums wait for.
 template <typename T, typename U, int W>
-__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
+__global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restrict__ dtable, const T *dout, const SumArgs a, const ZeroArgs z, int sum_blocks,
                                                                     int zero_blocks) {
     __shared__ unsigned s_key[SUM_THREADS / MIN_GROUP * MAX_PIECE];
     __shared__ int s_row[SUM_THREADS / MIN_GROUP * MAX_PIECE];
@@ -420,8 +420,8 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
     const int i0 = p < a.pieces ? p * a.piece : a.n, n = min(a.n - i0, a.piece);
     unsigned *key = s_key + group * a.piece;
     int *row = s_row + group * a.piece;
-    for (int i = lane; i < n; i += a.tpr) { key[i] = __ldg(a.keys + i0 + i); row[i] = __ldg(a.rows + i0 + i); }
-    const unsigned before = n > 0 && i0 > 0 ? __ldg(a.keys + i0 - 1) : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? __ldg(a.keys + i0 + n) : 0xffffffffu;
+    for (int i = lane; i < n; i += a.tpr) { key[i] = a.keys[i0 + i]; row[i] = a.rows[i0 + i]; }
+    const unsigned before = n > 0 && i0 > 0 ? a.keys[i0 - 1] : 0xffffffffu, behind = n > 0 && i0 + n < a.n ? a.keys[i0 + n] : 0xffffffffu;
     __syncthreads();
     if (n > 0 && col0 < a.dim) sum_piece<T, U, W, SUM_THREADS>(dtable, dout, a, p, col0, step, key, row, n, before, behind, ring);
 }
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(U *__restric
 // Sort and sums in one launch, for few tokens: every block sorts all of them by itself, which takes no longer than one block would, and then has its share of
 // the pieces' keys and rows in its own shared memory.  Block 0 leaves the keys for the joins.
 template <typename T, typename U, int W>
-__global__ void __launch_bounds__(SORT_THREADS) embedding_small_kernel(U *__restrict__ dtable, const T *__restrict__ dout, const int *__restrict__ tokens, const SumArgs a,
+__global__ void __launch_bounds__(SORT_THREADS) embedding_small_kernel(U *__restrict__ dtable, const T *dout, const int *tokens, const SumArgs a,
                                                                        const ZeroArgs z, int passes, int bits, unsigned *__restrict__ keys_out) {
     extern __shared__ __align__(16) unsigned sm[];
     grid_wait();
@@ -471,9 +471,9 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dta
     for (unsigned li = blockIdx.x; li < n_list; li += gridDim.x) {
         const int p = a.list ? a.list[li] : (int)li;
         if ((p + 1) * (long long)a.piece >= a.n) continue;
-        const unsigned key = __ldg(a.keys + (size_t)(p + 1) * a.piece);
+        const unsigned key = a.keys[(size_t)(p + 1) * a.piece], last = a.keys[(size_t)(p + 1) * a.piece - 1], before = p > 0 ? a.keys[(size_t)p * a.piece - 1] : 0xffffffffu;
         // without a list: does a token that begins in the piece go on behind it?
-        if (!a.list && (key >= (unsigned)a.vocab || __ldg(a.keys + (size_t)(p + 1) * a.piece - 1) != key || (p > 0 && __ldg(a.keys + (size_t)p * a.piece - 1) == key))) continue;
+        if (!a.list && (key >= (unsigned)a.vocab || last != key || before == key)) continue;
         float s[P];
 #pragma unroll
         for (int j = 0; j < P; ++j) s[j] = 0.0f;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(U *__restrict__ dta
                 for (int u = 0; u < 4; ++u) {
                     // the head is fetched beside the key that tells whether it is one
                     const unsigned at = q + u * phases, in = min(at, (unsigned)a.pieces - 1);
-                    k[u] = at < (unsigned)a.pieces ? __ldg(a.keys + (size_t)in * a.piece) : 0xffffffffu;
+                    k[u] = at < (unsigned)a.pieces ? a.keys[(size_t)in * a.piece] : 0xffffffffu;
                     load_vec<float, P>(v[u], a.partial + (size_t)in * 2 * a.dim_pad + col);
                 }
 #pragma unroll

@@ -184,7 +184,7 @@ template <typename T> __device__ __forceinline__ void put(const Piece &p, const 
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant__ List<CAP> l, const double *__restrict__ partial, int n_partial, float max_norm,
+__global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant__ List<CAP> l, const double *partial, int n_partial, float max_norm,
                                                           float *__restrict__ norm_out) {
     __shared__ double red[THREADS / 32];
     const unsigned total = l.first[l.n];
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant_
     }
 }
 
-__global__ void __launch_bounds__(THREADS) norm_kernel(const double *__restrict__ partial, int n_partial, float *__restrict__ norm_out) {
+__global__ void __launch_bounds__(THREADS) norm_kernel(const double *partial, int n_partial, float *__restrict__ norm_out) {
     __shared__ double red[THREADS / 32];
     grid_wait();
     const double norm = norm_of(partial, n_partial, red);

@@ -48,7 +48,8 @@ template <typename F> int with_type(int type, F &&f) {
 #define B2_ELEM(p) std::remove_pointer_t<decltype(p)>
 
 // A launch that may start while the kernel before it on the stream drains; the kernel calls grid_wait() before it touches
-// what that one wrote (and before it writes what that one reads).
+// what that one wrote (and before it writes what that one reads).  Behind the wait it reads by plain loads: __ldg and loads through
+// `const ... *__restrict__` are for memory that nobody writes while the kernel runs, and may be moved above it.
 template <typename... KArgs, typename... Args>
 int launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
     cudaLaunchConfig_t cfg = {};

@@ -983,3 +983,43 @@ def test_every_operator_runs_on_the_callers_stream(tm):
     want, got = run(False, None), run(True, side.cuda_stream)
     for k in want:
         assert torch.equal(want[k], got[k]), k
+
+
+@pytest.mark.parametrize("n,vocab", [(600, 259), (5000, 259), (6000, 60000)])
+def test_calls_that_follow_each_other_closely(tm, n, vocab):
+    """the launches of a call overlap with those before: other inputs in the same buffers and workspace every time, nothing waited for between"""
+    torch, b2 = tm
+    dim, calls = 40, 24
+    g = torch.Generator().manual_seed(n)
+    toks = torch.randint(-1, vocab, (calls, n), generator=g).int().cuda()
+    grads = torch.randn(calls, n, dim, generator=g).cuda()
+    sizes = [70001, 5, 300000]
+    lists = [[(torch.randn(s, generator=g) * (k + 1)).cuda() for s in sizes] for k in range(calls)]
+    new = lambda: torch.empty(b2.embedding_backward_workspace(n, vocab, dim), dtype=torch.uint8, device="cuda")  # noqa: E731
+    small = lambda: torch.empty(b2.gradient_norm_workspace(), dtype=torch.uint8, device="cuda")  # noqa: E731
+    tok, dout, ts = torch.empty_like(toks[0]), torch.empty_like(grads[0]), [torch.empty(s, device="cuda") for s in sizes]
+    ws, ws2, tables = new(), small(), torch.empty(calls, vocab, dim, device="cuda")
+    outs, norms = [[torch.empty(s, device="cuda") for s in sizes] for _ in range(calls)], torch.empty(calls, 1, device="cuda")
+    tl = [b2.TensorList(ts, o) for o in outs]
+    torch.cuda.synchronize()
+    for k in range(calls):
+        tok.copy_(toks[k])
+        dout.copy_(grads[k])
+        b2.embedding_backward(tables[k], dout, tok, 1.0, workspace=ws)
+        for a, b in zip(ts, lists[k]):
+            a.copy_(b)
+        b2.gradient_clip(tl[k], 100.0, norms[k], workspace=ws2)
+    torch.cuda.synchronize()
+    for k in range(calls):
+        want, norm = torch.empty(vocab, dim, device="cuda"), torch.empty(1, device="cuda")
+        b2.embedding_backward(want, grads[k], toks[k], 1.0, workspace=new())
+        alone = [torch.empty(s, device="cuda") for s in sizes]
+        b2.gradient_clip(b2.TensorList(lists[k], alone), 100.0, norm, workspace=small())
+        torch.cuda.synchronize()
+        assert torch.equal(want, tables[k]) and torch.equal(norm, norms[k]) and all(torch.equal(a, b) for a, b in zip(alone, outs[k])), k
+        ref = math.sqrt(math.fsum(float((t.double() ** 2).sum()) for t in lists[k]))
+        assert abs(norm.item() - ref) <= 2 * u * ref
+        real = toks[k] >= 0
+        plain = torch.zeros(vocab, dim, device="cuda", dtype=torch.float64).index_add_(0, toks[k][real].long(), grads[k][real].double())
+        mass = torch.zeros(vocab, dim, device="cuda", dtype=torch.float64).index_add_(0, toks[k][real].long(), grads[k][real].double().abs())
+        assert ((want.double() - plain).abs() <= (n + 1) * u * mass).all()

@@ -350,7 +350,7 @@ using namespace b2;
 extern "C" {
 
 size_t b2_block_norm_backward_workspace(long long rows, int dim, long long gate_rows) {
-    if (rows < 1 || rows > 0x7fffffffll || dim < 1 || dim > MAX_DIM || gate_rows < 0) return 0;
+    if (rows < 1 || rows > 0x7fffffffll || dim < 1 || dim > MAX_DIM || gate_rows < 0 || (gate_rows && rows % gate_rows)) return 0;
     // enough for any type and alignment
     size_t most = 0;
     for (int per_thread = 4; per_thread <= 8; per_thread *= 2) {

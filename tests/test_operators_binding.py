@@ -122,3 +122,10 @@ def test_addresses_and_distances_that_no_kernel_may_see():
 def test_the_net_refuses_a_clipping_without_a_net():
     assert b2lstm.lib().b2_net_set_gradient_clipping(None, 1.0) == -5
     assert b2lstm.lib().b2_net_gradient_norm(None, C.byref(C.c_float())) == -5
+
+
+def test_the_workspace_of_sizes_that_the_norm_gradient_refuses():
+    """a gate with more rows than there are frames, or with rows that the frames are no multiple of (the plan of such a call would divide by zero)"""
+    size = b2lstm.block_norm_backward_workspace
+    assert size(4, 8, 100) == 0 and size(5, 8, 3) == 0 and size(1, 8, 2 ** 40) == 0
+    assert size(6, 8, 3) > 0 and size(6, 8, 6) > 0 and size(6, 8) > 0

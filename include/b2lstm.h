@@ -48,6 +48,9 @@ enum {
 const char *b2_last_error_string(void);
 /* Library build id, e.g. "b2lstm 0.1 sm_100a". */
 const char *b2_version(void);
+/* Ordinal of the CUDA device that this thread's calls go to (the current device), -1 where there is none.  Buffers and streams of a call have to
+ * belong to it. */
+int b2_current_device(void);
 
 /* ------------------------------------------------------------------------------------------
  * helpers::Matrix<Gpu>::assignProduct / addProduct          (helpers/Matrix.cu:354-377,

@@ -29,6 +29,7 @@ _ip = C.POINTER(C.c_int)
 SIGNATURES = {
     "b2_last_error_string": (C.c_char_p, []),
     "b2_version": (C.c_char_p, []),
+    "b2_current_device": (C.c_int, []),
     "b2_matrix_multiply": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "b2_matrix_multiply_noalloc": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int,

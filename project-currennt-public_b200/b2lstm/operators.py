@@ -1,5 +1,6 @@
 """The operators of a token model around the recurrent layers (include/b2lstm.h: b2_embedding_*, b2_block_norm_*, b2_logprob_*,
-b2_gradient_*), on tensors: any object with data_ptr(), shape, stride(), dtype and is_cuda, e.g. torch CUDA tensors.
+b2_gradient_*), on tensors: any object with data_ptr(), shape, stride(), dtype and is_cuda, e.g. torch CUDA tensors.  Calls go to the current
+CUDA device; tensors that say where they are (get_device()) are refused if that is another one.
 
 Shapes, element types and leading dimensions come from the tensors and are checked on the way (csrc/binding.cpp); the library checks the rest.  Rows may lie
 apart (a slice of a wider tensor), channels have to be contiguous.  Outputs are the caller's tensors.  `stream` is a raw stream handle
@@ -14,7 +15,7 @@ try:
 except ImportError:             # not built: the first call says so
     _tensors = None
 
-_BOUND = ("b2_last_error_string", "b2_embedding_forward", "b2_embedding_backward", "b2_block_norm_forward", "b2_block_norm_backward", "b2_logprob_forward",
+_BOUND = ("b2_last_error_string", "b2_current_device", "b2_embedding_forward", "b2_embedding_backward", "b2_block_norm_forward", "b2_block_norm_backward", "b2_logprob_forward",
           "b2_logprob_backward", "b2_gradient_norm", "b2_gradient_clip")
 _ready = None
 
@@ -91,6 +92,10 @@ class TensorList:
         if self.out is not None and len(self.out) != self.n:
             raise B2Error("%d tensors and %d outputs" % (self.n, len(self.out)))
         self._in, self._out = self._array(self.tensors), None if out is None else self._array(self.out)
+        devices = {t.get_device() for t in self.tensors + (self.out or []) if hasattr(t, "get_device")}
+        if len(devices) > 1:
+            raise B2Error("the tensors are on the devices %s" % sorted(devices))
+        self._device = devices.pop() if devices else -1
         self._at, self._out_at = C.addressof(self._in), 0 if out is None else C.addressof(self._out)
 
     @staticmethod
@@ -112,9 +117,9 @@ def gradient_norm_workspace():
 
 def gradient_norm(tensors, norm, workspace=None, stream=None):
     """norm (float32 [1]) = the L2 norm over all elements of a TensorList"""
-    (_ready or _ops()).gradient_norm(tensors._at, tensors.n, norm, workspace, stream)
+    (_ready or _ops()).gradient_norm(tensors._at, tensors.n, tensors._device, norm, workspace, stream)
 
 
 def gradient_clip(tensors, max_norm, norm, workspace=None, stream=None):
     """The same, and the tensors scaled by min(1, max_norm / norm), in place or into the list's outputs"""
-    (_ready or _ops()).gradient_clip(tensors._at, tensors._out_at, tensors.n, max_norm, norm, workspace, stream)
+    (_ready or _ops()).gradient_clip(tensors._at, tensors._out_at, tensors.n, tensors._device, max_norm, norm, workspace, stream)

@@ -1,7 +1,7 @@
 // The tensor side of the Python binding of the token operators (b2lstm/operators.py): reads addresses, shapes, strides and element types
 // from tensor objects, checks them, and calls the library.  A call of an operator on a handful of frames is as long as its host work;
 // done attribute by attribute in Python that was half of it.  Knows no tensor library: a tensor is any object with data_ptr(), shape,
-// stride(), numel(), is_contiguous(), dtype and is_cuda.  The library's functions come as addresses (bind), so this file links against nothing.
+// stride(), numel(), is_contiguous(), dtype and is_cuda; one that has get_device() too has to be on the device that the call goes to.  The library's functions come as addresses (bind), so this file links against nothing.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -17,6 +17,7 @@ enum { INT32 = 16, BYTE = 17, OTHER = 18 };
 
 struct Api {
     decltype(&b2_last_error_string) last_error;
+    decltype(&b2_current_device) current_device;
     decltype(&b2_embedding_forward) embedding_forward;
     decltype(&b2_embedding_backward) embedding_backward;
     decltype(&b2_block_norm_forward) block_norm_forward;
@@ -27,7 +28,7 @@ struct Api {
     decltype(&b2_gradient_clip) gradient_clip;
 } api;
 
-PyObject *s_shape, *s_stride, *s_dtype, *s_is_cuda, *s_data_ptr, *s_numel, *s_is_contiguous;
+PyObject *s_shape, *s_stride, *s_dtype, *s_is_cuda, *s_get_device, *s_data_ptr, *s_numel, *s_is_contiguous;
 
 // an owned reference
 struct Ref {
@@ -67,7 +68,18 @@ int type_of(const Ref &dtype) {
     return code;
 }
 
+thread_local int t_device;         // of the call under way on this thread
+// Kernels run on the current device: memory of another one is out of their reach, or a fault.
 bool on_gpu(PyObject *t, const char *name) {
+    Ref at(PyObject_CallMethodNoArgs(t, s_get_device));
+    if (at) {
+        const long device = PyLong_AsLong(at.p);
+        if (device == -1 && PyErr_Occurred()) return false;
+        if (device < 0) return refuse("%s is not on the GPU", name);
+        return device == t_device ? true : refuse("%s is on device %ld, the current one is %d", name, device, t_device);
+    }
+    if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return false;
+    PyErr_Clear();
     Ref cuda(PyObject_GetAttr(t, s_is_cuda));
     if (!cuda) return false;
     const int yes = PyObject_IsTrue(cuda.p);
@@ -160,7 +172,12 @@ PyObject *done(int rc) {
     refuse("b2lstm error %d: %s", rc, api.last_error());
     return nullptr;
 }
-bool arguments(Py_ssize_t n, Py_ssize_t want) { return n == want ? true : refuse("%zd arguments instead of %zd", n, want); }
+// the beginning of every call
+bool arguments(Py_ssize_t n, Py_ssize_t want) {
+    if (n != want) return refuse("%zd arguments instead of %zd", n, want);
+    t_device = api.current_device();
+    return true;
+}
 
 // a table's rows are an int in the library
 bool few_rows(const Matrix &m) { return m.rows <= 0x7fffffff ? true : refuse("a table of %lld rows", m.rows); }
@@ -300,35 +317,41 @@ PyObject *logprob_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
                               (const float *)g, (const float *)entropy, (const float *)h, st));
 }
 
-// address of the list, its length, norm, workspace, stream
+// a list's tensors, all on one device (-1: not known)
+bool list_on_gpu(PyObject *device) {
+    const long d = PyLong_AsLong(device);
+    if (d == -1 && PyErr_Occurred()) return false;
+    return d < 0 || d == t_device ? true : refuse("the tensors are on device %ld, the current one is %d", d, t_device);
+}
+// address of the list, its length, its device, norm, workspace, stream
 PyObject *gradient_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     void *norm, *ws;
     size_t bytes;
     b2_stream st;
-    if (!arguments(n, 5)) return nullptr;
+    if (!arguments(n, 6)) return nullptr;
     const b2_tensor *list = (const b2_tensor *)PyLong_AsVoidPtr(a[0]);
     const int len = (int)PyLong_AsLong(a[1]);
-    if (PyErr_Occurred() || !vector(a[2], "norm", 1, B2_F32, &norm) || !workspace(a[3], &ws, &bytes) || !stream_of(a[4], &st)) return nullptr;
+    if (PyErr_Occurred() || !list_on_gpu(a[2]) || !vector(a[3], "norm", 1, B2_F32, &norm) || !workspace(a[4], &ws, &bytes) || !stream_of(a[5], &st)) return nullptr;
     CALL(api.gradient_norm(list, len, (float *)norm, ws, bytes, st));
 }
-// address of the list, of the outputs' (0: in place), length, max_norm, norm, workspace, stream
+// address of the list, of the outputs' (0: in place), length, device, max_norm, norm, workspace, stream
 PyObject *gradient_clip(PyObject *, PyObject *const *a, Py_ssize_t n) {
     void *norm, *ws;
     size_t bytes;
     float most;
     b2_stream st;
-    if (!arguments(n, 7)) return nullptr;
+    if (!arguments(n, 8)) return nullptr;
     const b2_tensor *list = (const b2_tensor *)PyLong_AsVoidPtr(a[0]), *out = (const b2_tensor *)PyLong_AsVoidPtr(a[1]);
     const int len = (int)PyLong_AsLong(a[2]);
-    if (PyErr_Occurred() || !number(a[3], &most) || !vector(a[4], "norm", 1, B2_F32, &norm) || !workspace(a[5], &ws, &bytes) || !stream_of(a[6], &st)) return nullptr;
+    if (PyErr_Occurred() || !list_on_gpu(a[3]) || !number(a[4], &most) || !vector(a[5], "norm", 1, B2_F32, &norm) || !workspace(a[6], &ws, &bytes) || !stream_of(a[7], &st)) return nullptr;
     CALL(api.gradient_clip(list, out, len, most, (float *)norm, ws, bytes, st));
 }
 
 // bind({name: address}, B2Error)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!arguments(n, 2)) return nullptr;
+    if (n != 2) { refuse("%zd arguments instead of 2", n); return nullptr; }
     const struct { const char *name; void **to; } all[] = {
-        {"b2_last_error_string", (void **)&api.last_error}, {"b2_embedding_forward", (void **)&api.embedding_forward},
+        {"b2_last_error_string", (void **)&api.last_error}, {"b2_current_device", (void **)&api.current_device}, {"b2_embedding_forward", (void **)&api.embedding_forward},
         {"b2_embedding_backward", (void **)&api.embedding_backward}, {"b2_block_norm_forward", (void **)&api.block_norm_forward},
         {"b2_block_norm_backward", (void **)&api.block_norm_backward}, {"b2_logprob_forward", (void **)&api.logprob_forward},
         {"b2_logprob_backward", (void **)&api.logprob_backward}, {"b2_gradient_norm", (void **)&api.gradient_norm}, {"b2_gradient_clip", (void **)&api.gradient_clip}};
@@ -352,7 +375,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", "tensor side of the tok
 }  // namespace
 
 PyMODINIT_FUNC PyInit__tensors(void) {
-    const struct { PyObject **to; const char *text; } names[] = {{&s_shape, "shape"}, {&s_stride, "stride"}, {&s_dtype, "dtype"}, {&s_is_cuda, "is_cuda"},
+    const struct { PyObject **to; const char *text; } names[] = {{&s_shape, "shape"}, {&s_stride, "stride"}, {&s_dtype, "dtype"}, {&s_is_cuda, "is_cuda"}, {&s_get_device, "get_device"},
                                                                  {&s_data_ptr, "data_ptr"}, {&s_numel, "numel"}, {&s_is_contiguous, "is_contiguous"}};
     for (const auto &n : names)
         if (!(*n.to = PyUnicode_InternFromString(n.text))) return nullptr;

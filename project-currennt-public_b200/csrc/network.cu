@@ -707,6 +707,7 @@ b2::NeuralNetwork *b2_net_impl(b2_net *n) { return &n->net; }
 
 const char *b2_last_error_string(void) { return b2::last_error(); }
 const char *b2_version(void) { return "b2lstm 0.1 sm_100a"; }
+int b2_current_device(void) { return current_device(); }
 
 int b2_matrix_multiply(float *C, int ldc, const float *A, int lda, int transA, const float *B, int ldb, int transB,
                        int m, int n, int k, int accumulate, int force_ffma, b2_stream stream) {

@@ -129,3 +129,45 @@ def test_the_workspace_of_sizes_that_the_norm_gradient_refuses():
     size = b2lstm.block_norm_backward_workspace
     assert size(4, 8, 100) == 0 and size(5, 8, 3) == 0 and size(1, 8, 2 ** 40) == 0
     assert size(6, 8, 3) > 0 and size(6, 8, 6) > 0 and size(6, 8) > 0
+
+
+class FakeOn(Fake):
+    """one that knows its device, as torch's tensors do"""
+
+    def __init__(self, device, *shape, **k):
+        super().__init__(*shape, **k)
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+def test_tensors_of_another_device():
+    from b2lstm import operators
+    assert b2lstm.lib().b2_current_device() >= -1
+    ops, library = operators._ops(), b2lstm.lib()
+    real = {name: C.cast(getattr(library, name), C.c_void_p).value for name in operators._BOUND}
+    current = C.CFUNCTYPE(C.c_int)(lambda: 1)                     # as if device 1 was the current one
+    on = lambda d, *s, **k: FakeOn(d, *s, **k)  # noqa: E731
+    i32, ws = dict(dtype="torch.int32"), dict(dtype="torch.uint8")
+    try:
+        ops.bind(dict(real, b2_current_device=C.cast(current, C.c_void_p).value), b2lstm.B2Error)
+        refused("out is on device 0, the current one is 1", b2lstm.embedding_forward, on(0, 4, 8), on(1, 10, 8), on(1, 4, **i32))
+        refused("table is on device 2", b2lstm.embedding_forward, on(1, 4, 8), on(2, 10, 8), on(1, 4, **i32))
+        refused("tokens is on device 0", b2lstm.embedding_forward, on(1, 4, 8), on(1, 10, 8), on(0, 4, **i32))
+        refused("workspace is on device 0", b2lstm.embedding_backward, on(1, 10, 8), on(1, 4, 8), on(1, 4, **i32), workspace=on(0, 1 << 20, **ws))
+        refused("not on the GPU", b2lstm.embedding_forward, on(-1, 4, 8), on(1, 10, 8), on(1, 4, **i32))
+        refused("lse is on device 0", b2lstm.logprob_forward, on(1, 4, 8), on(1, 4, **i32), on(1, 4), on(0, 4))
+        refused("mask is on device 0", b2lstm.logprob_forward, on(1, 4, 8), on(1, 4, **i32), on(1, 4), on(1, 4), mask=on(0, 8, dtype="torch.bool"))
+        refused("h is on device 0", b2lstm.block_norm_forward, on(1, 4, 16), None, None, on(0, 4, 16))
+        refused("devices .0, 1.", b2lstm.TensorList, [on(0, 3), on(1, 3)])
+        refused("devices .0, 1.", b2lstm.TensorList, [on(1, 3)], [on(0, 3, address=8192)])
+        refused("tensors are on device 0, the current one is 1", b2lstm.gradient_norm, b2lstm.TensorList([on(0, 3)]), on(1, 1), workspace=on(1, 1 << 16, **ws))
+        refused("norm is on device 0", b2lstm.gradient_clip, b2lstm.TensorList([on(1, 3)]), 1.0, on(0, 1), workspace=on(1, 1 << 16, **ws))
+        # on the current device the calls go on, to the next thing that is wrong
+        refused("error -5.*aligned", b2lstm.embedding_forward, on(1, 4, 8), on(1, 10, 8, address=4098), on(1, 4, **i32))
+        refused("error -1.*needed", b2lstm.gradient_clip, b2lstm.TensorList([on(1, 3)]), 1.0, on(1, 1), workspace=on(1, 8, **ws))
+        # one that does not say where it is, is taken at its word
+        refused("error -5.*aligned", b2lstm.embedding_forward, Fake(4, 8), Fake(10, 8, address=4098), TOK)
+    finally:
+        ops.bind(real, b2lstm.B2Error)

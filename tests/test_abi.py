@@ -59,3 +59,24 @@ def test_missing_library_fails_loudly(monkeypatch, tmp_path):
     monkeypatch.setattr(L, "library_path", lambda: str(tmp_path / "libb2lstm.so"))
     with pytest.raises(b2lstm.B2Error):
         L.lib()
+
+
+def _make(*args):
+    import subprocess
+    csrc = os.path.join(ROOT, "project-currennt-public_b200", "csrc")
+    return subprocess.run(["make", "-n", "-B", "-C", csrc, *args], capture_output=True, text=True, timeout=60)
+
+
+def test_the_library_is_built_where_there_is_no_python_to_build_for(tmp_path):
+    """make's default target, dry: without an interpreter, or with one that has no headers, the library and not the binding"""
+    bare = tmp_path / "python"
+    bare.write_text("#!/bin/sh\necho %s\n" % (tmp_path / "include"))
+    bare.chmod(0o755)
+    for python in (str(tmp_path / "none"), str(bare)):
+        r = _make("PYTHON=" + python)
+        assert r.returncode == 0 and "-o ../libb2lstm.so" in r.stdout and "_tensors.so" not in r.stdout
+    import sys
+    import sysconfig
+    r = _make("PYTHON=" + sys.executable)
+    headers = os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h"))
+    assert r.returncode == 0 and "-o ../libb2lstm.so" in r.stdout and ("-o ../b2lstm/_tensors.so" in r.stdout) == headers

@@ -732,7 +732,7 @@ template <typename T, int N, bool ENT> __device__ __forceinline__ void entry_gra
 
 // tpr threads a row, each up to U vectors apart by tpr; a long row takes several blocks.  Bound by memory (5 to 6 issue slots an entry).
 template <typename T, bool ENT, bool MASK, int U>
-__global__ void __launch_bounds__(256) logprob_backward_kernel(T *__restrict__ dlogits, const T *logits, const BwdArgs a, int tpr, int segs) {
+__global__ void __launch_bounds__(256) logprob_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int tpr, int segs) {
     constexpr int W = 16 / sizeof(T);
     const int per_block = 256 / tpr;
     // a row of several segments takes whole blocks (tpr = 256)

@@ -60,3 +60,11 @@ def test_chained_kernels_read_by_plain_loads(path):
             assert "grid_wait()" in body, name
         assert "__ldg(" not in body, name
         assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", body), name
+
+
+@pytest.mark.parametrize("path,kernel", [("logprob.cu", "logprob_backward_kernel"), ("block_norm.cu", "block_norm_few_kernel"), ("block_norm.cu", "block_norm_forward_kernel"),
+                                         ("block_norm_back.cu", "block_norm_backward_kernel"), ("gradient_norm.cu", "clip_kernel")])
+def test_what_may_be_in_place_is_not_declared_apart(path, kernel):
+    """the header lets outputs of these take the place of an input: a __restrict__ of the tensors' type would promise that they do not"""
+    head = _functions(open(os.path.join(CSRC, path)).read())[kernel].split("{", 1)[0]
+    assert not re.search(r"\bT\s*\*\s*__restrict__", head)

@@ -204,7 +204,7 @@ int b2_block_norm_forward(const b2_block_norm *desc, const void *x, long long ld
                           void *h, long long ld_h, b2_stream stream);
 /* Gradients from dy (of y, may be NULL: 0) and dh (of h, NULL where the forward pass had no h) with y (x where there was no f) and f of the
  * forward pass.  Outputs may be NULL, and are OVERWRITTEN: dx, df, dgate (gate_rows rows) in the tensors' type, the sums over frames dw_pre,
- * db_pre, dw_post, db_post (dim floats each).  dx and df may take the place of an input that has the same leading dimension.
+ * db_pre, dw_post, db_post (dim floats each).  dx and df may take the place of an input with as many rows and the same leading dimension.
  * workspace: aligned to 16 bytes; gate_rows 0 without a gate; its size is 0 for sizes that the gradient refuses. */
 size_t b2_block_norm_backward_workspace(long long rows, int dim, long long gate_rows);
 int b2_block_norm_backward(const b2_block_norm *desc, void *dx, long long ld_dx, void *df, long long ld_df, void *dgate, long long ld_dgate,

@@ -399,6 +399,10 @@ int b2_block_norm_backward(const b2_block_norm *d, void *dx, long long ld_dx, vo
             set_error("%s: a gradient takes the place of an input with another leading dimension", who);
             return B2_ERR_BAD_ARG;
         }
+    if (d->gate && (dx == d->gate || df == d->gate) && (d->gate_rows != d->rows || (dx == d->gate ? ld_dx : ld_df) != d->ld_gate)) {
+        set_error("%s: a gradient takes the place of the gate, which has other rows", who);
+        return B2_ERR_BAD_ARG;
+    }
     if (dx && dx == df) { set_error("%s: dx and df are the same", who); return B2_ERR_BAD_ARG; }
     Width w = width_of(d);
     w.rows(dx, ld_dx); w.rows(df, ld_df); w.rows(dgate, ld_dgate); w.rows(dy, ld_dy); w.rows(dh, ld_dh); w.rows(y, ld_y); w.rows(f, ld_f);

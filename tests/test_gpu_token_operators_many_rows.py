@@ -348,3 +348,21 @@ def test_block_norm_parts_of_many_rows(tm, t, dim):  # noqa: F811
     only = torch.empty_like(g)
     b2.block_norm_backward(None, None, dy, dh, y, f, st, dgate=only, w_pre=w1, workspace=ws, **kw)
     assert torch.equal(only, dg)
+
+
+@pytest.mark.parametrize("t,dim", [("bf16", 512), ("f16", 333), ("f32", 2000)])
+def test_block_norm_gradients_in_place_of_a_gate_for_every_frame(tm, t, dim):  # noqa: F811
+    torch, b2 = tm
+    rows = 5000
+    y, f, dy, dh = (_randn(torch, rows, dim, t, i, s) for i, s in enumerate((2.0, 0.7, 0.3, 0.4)))
+    g = _randn(torch, rows, dim, t, 8)
+    st = torch.rand(rows, 4, device="cuda")
+    ws = torch.empty(b2.block_norm_backward_workspace(rows, dim, rows), dtype=torch.uint8, device="cuda")
+    run = lambda dx, df, gate, dgate: b2.block_norm_backward(dx, df, dy, dh, y, f, st, gate=gate, dgate=dgate, workspace=ws)  # noqa: E731
+    dx, df, dg = (torch.empty_like(y) for _ in range(3))
+    run(dx, df, g, dg)
+    a, b, c, other = g.clone(), g.clone(), g.clone(), torch.empty_like(y)
+    run(a, other, a, None)
+    run(other, b, b, None)
+    run(other, torch.empty_like(y), c, c)
+    assert torch.equal(a, dx) and torch.equal(b, df) and torch.equal(c, dg)

@@ -171,3 +171,14 @@ def test_tensors_of_another_device():
         refused("error -5.*aligned", b2lstm.embedding_forward, Fake(4, 8), Fake(10, 8, address=4098), TOK)
     finally:
         ops.bind(real, b2lstm.B2Error)
+
+
+def test_a_norm_gradient_in_place_of_a_gate_for_several_frames():
+    """other frames still read the gate's rows: refused, and accepted where every frame has its own"""
+    x, o, st, ws = Fake(4, 16), Fake(4, 16, address=8192), Fake(4, 4, address=16384), dict(workspace=Fake(1 << 24, dtype="torch.uint8"))
+    gate = Fake(2, 16, address=1 << 20)
+    for at in (0, 1):
+        outs = [Fake(4, 16, address=1 << 21), Fake(4, 16, address=1 << 22)]
+        outs[at] = Fake(4, 16, address=1 << 20)
+        refused("error -5.*place of the gate", b2lstm.block_norm_backward, *outs, x, None, None, o, st, gate=gate, **ws)
+        refused("error -5.*place of the gate", b2lstm.block_norm_backward, *outs, x, None, None, o, st, gate=Fake(4, 16, address=1 << 20, stride=(24, 1)), **ws)

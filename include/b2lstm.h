@@ -157,7 +157,9 @@ size_t b2_lstm_state_bytes(const b2_lstm *layer);
  * All of them work on the caller's device buffers, on the caller's stream, without allocating, synchronising or keeping anything between
  * calls; scratch, where one is needed, comes from the caller (the matching _workspace function tells its size; its contents need no
  * set-up and may be overwritten between calls).  Calls that share a workspace have to be ordered, by one stream for instance.  Arithmetic
- * is fp32 whatever the tensors' type, results are rounded once, sums are added in a fixed order (the same bits every time).
+ * is fp32 whatever the tensors' type, results are rounded once, sums are added in a fixed order: the same call gives the same bits every
+ * time.  The order follows the sizes of the call, so a row among more rows or fewer may come out in another last place.
+ * Buffers and streams have to be of the current device (b2_current_device).
  * Rows are the frames of a fraction, row t*P + p for frame t of sequence p; row r of a tensor starts ld elements behind row r - 1.  Any
  * address that is a multiple of the element size is accepted; 16-byte aligned rows are the fastest.
  * Padding frames have the token -1 (any negative one) or the pattern type 0: their results and gradients are zero.

@@ -3,8 +3,9 @@ b2_gradient_*), on tensors: any object with data_ptr(), shape, stride(), dtype a
 CUDA device; tensors that say where they are (get_device()) are refused if that is another one.
 
 Shapes, element types and leading dimensions come from the tensors and are checked on the way (csrc/binding.cpp); the library checks the rest.  Rows may lie
-apart (a slice of a wider tensor), channels have to be contiguous.  Outputs are the caller's tensors.  `stream` is a raw stream handle
-(None: the default stream); `workspace` a uint8 tensor of at least as many bytes as the matching _workspace function tells.
+apart (a slice of a wider tensor), channels have to be contiguous.  Outputs are the caller's tensors.  `stream` is a raw stream handle,
+None the legacy default stream, as everywhere in this package: under torch.cuda.stream(s) that is not the stream the tensors are made on, and the call is not
+ordered with them unless it is given s.cuda_stream; `workspace` a uint8 tensor of at least as many bytes as the matching _workspace function tells.
 """
 import ctypes as C
 

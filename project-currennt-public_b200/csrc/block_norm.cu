@@ -14,14 +14,17 @@
 //
 // Bound by memory: a row stays in registers and shared memory between its loads and its stores, so every tensor is read once and written
 // once.  What stands against it is latency: a row is a chain of two sums over its threads (four with layer norm), so the rows that follow are on
-// their way into shared memory meanwhile; and instructions, so arithmetic is packed in the backward pass, the threads of a row are a constant,
-// and full rows are compiled without tests.  The backward kernel has a fixed number of workers; a worker keeps the same columns for all its rows,
-// so the sums over frames stay in registers until the end, go to the workspace once, and are added there in a fixed order by a second
-// launch: no atomics, the same bits every time.
-// Measured on a B200 (device time; share of the copy bandwidth): forward, layer norm, 38400 x 512 fp32 with a gate per sequence 52 us (all bytes counted
-// 93 %; a third of the frames are padding, of which only zeros are written), 38400 x 512 bf16 33 us, x 1024 64 us, 8192 x 4001 93 us
-// (single elements), 64 x 1024 bf16 3.3 us.  Backward, 16384 x 2048 bf16 with a gate per frame 95 us (87 %), with layer norm and biases 137 us
-// (its sums spill), 16384 x 2047 180 us, x 4096 249 us (one block a multiprocessor: its barriers are not hidden).
+// their way into shared memory meanwhile, as many as fit (see the forward kernel); and instructions, so arithmetic is packed in the backward
+// pass, the threads of a row are a constant, and full rows are compiled without tests.  The backward kernel has a fixed number of workers; a worker
+// keeps the same columns for all its rows, so the sums over frames stay in registers until the end, go to the workspace once, and are added there in a
+// fixed order by a second launch: no atomics, the same bits every time.
+// Measured on a B200 (device time of a pass among passes over the same buffers, a third of the frames padding in the forward pass; share of the copy
+// bandwidth; with buffers that change 1 to 10 % more, and boxes differ by 4 %): forward, layer norm, 38400 x 512 fp32 with a gate per sequence 52 us
+// (all bytes counted 92 %, of padding only zeros are written), 38400 x 512 bf16 33 us, x 1024 64 us, 8192 x 4001 without a gate 93 us (43 %; single
+// elements), 64 x 1024 bf16 3.5 us.  Backward, 16384 x 2048 bf16 with a gate per frame 95 us (86 %), with layer norm and biases 137 us (60 %), 16384 x 2047
+// 179 us, x 4096 250 us (one block a multiprocessor: its barriers are not hidden).
+// Rows that no 16-byte access fits reach 17 to 58 %: they come into shared memory in 16-byte pieces (16-bit types), but every element is read from there and
+// stored by an access of its own.
 #include "block_norm.cuh"
 
 namespace b2 {
@@ -74,7 +77,9 @@ __global__ void __launch_bounds__(512) block_norm_few_kernel(const NormArgs a, c
 }
 
 // Many rows: workers (a warp, or a block of tpr threads) take rows one after another; the next `stages` - 1 rows are on their way while one is worked
-// on, since a row is a chain of two to four sums over its threads that would leave the memory idle.  FULL: x, f, y, h are all there and the
+// on, since a row is a chain of two to four sums over its threads that would leave the memory idle.  What the blocks of a multiprocessor may have of its
+// shared memory gives 2 to 4 stages, but one only for fp32 rows of 129 to 4096 columns in 16-byte vectors and of 257 to 4096 single elements: there
+// nothing is ahead, and the other workers' rows cover for it (38400 x 512 fp32: 92 % of the copy bandwidth).  FULL: x, f, y, h are all there and the
 // threads' columns are just the row's.
 __host__ __device__ constexpr int forward_threads(int per_thread) { return per_thread > 16 ? 512 : 768; }   // a multiprocessor's, by their registers
 // TPR, the threads of a row (32: a warp, 8 rows a block), is a constant, which makes the offsets of a row's columns constants too: with single
@@ -174,7 +179,7 @@ template <typename T, int W>
 int forward(const b2_block_norm *d, const T *x, long long ld_x, const T *f, long long ld_f, T *y, long long ld_y, T *h, long long ld_h, cudaStream_t st) {
     const NormArgs a = args_of(d);
     const int vecs = (d->dim + W - 1) / W;
-    // few rows (64 x 1024 bf16: 3.3 us, with the kernel for many rows 4.3 us)
+    // few rows (64 x 1024 bf16: 3.5 us, with the kernel for many rows 4.3 us)
     if ((double)d->rows * vecs <= 512.0 * sm_count() && vecs <= 512) {
         const int t = (int)pow2_at_least((unsigned)vecs), tpr = t < 32 ? 32 : t;
         block_norm_few_kernel<T, W><<<tpr == 32 ? (unsigned)((d->rows + 7) / 8) : (unsigned)d->rows, tpr == 32 ? 256 : tpr, 0, st>>>(a, x, ld_x, f, ld_f, y, ld_y, h, ld_h, tpr);

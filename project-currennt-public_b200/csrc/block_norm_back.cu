@@ -39,18 +39,20 @@ template <int W, int NV, bool FULL> struct Out {
     }
 };
 
-// fp32 elements are copied one by one here (48256 x 405: 117 us, by row 168 us; in the forward pass by row 61 us and one by one 74 us for 38400 x 511)
+// fp32 elements are copied one by one here (48256 x 405, RMS: 117 us, by row 168 us; in the forward pass by row 61 us and one by one 74 us for 38400 x 511)
 template <typename T> __host__ __device__ constexpr bool by_row(int w) { return w == 1 && sizeof(T) == 2; }
 
 // A worker is a warp (TPR = 32) or a block of TPR threads.  per_group workers share a row of the gate (all workers, if there is one row or none), and
 // groups_at_once rows of the gate are worked on side by side.  BIAS: means are subtracted or the norms have a bias (without both, sums are saved).
 // FULL: dy, dh, f, dx and df are all there and the threads' columns are just the row's: a third of the instructions were tests of that.
-// As in the forward kernel, the next `stages` - 1 rows are on their way into shared memory while one is worked on.
+// As in the forward kernel, the next `stages` - 1 rows (up to three, as many as fit) are on their way into shared memory while one is worked on.
 template <typename T, int W, int NV, int TPR, bool BIAS, bool FULL>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 512 / (TPR == 32 ? 256 : TPR) > 0 ? 512 / (TPR == 32 ? 256 : TPR) : 1)
     block_norm_backward_kernel(const NormArgs a, const BackArgs k, T *dx, T *df, const T *dy, const T *dh, const T *y, const T *f, int stages) {
     constexpr int S = BIAS ? 2 : 1, N = NV * W, H = N / 2;   // a thread's columns, as pairs
-    constexpr bool KEEP = TPR <= 256 && !BIAS;          // the weights stay in registers
+    // The weights stay in registers; elsewhere they are loaded again for every row, which for 2048 channels with two weights and a bias is 24 KB of fp32, as much as
+    // the row itself (16384 x 2048 bf16 with layer norm and biases 137 us, without 95 us).  Above 4096 columns of 16 bits a thread has 64 registers and spills.
+    constexpr bool KEEP = TPR <= 256 && !BIAS;
     __shared__ float4 red[2 * S][8];
     extern __shared__ __align__(16) char ring[];
     constexpr int tpr = TPR, warps = TPR / 32;

@@ -16,10 +16,11 @@
 //      follow.
 // A frequent token is thus spread over as many groups as it has pieces.  Without accumulation the rows of tokens that do not occur are
 // zeroed by extra blocks of the same launches, so that the table is written once.
-// Measured on a B200 (device time): lookup of 65536 x 1024 bf16 29 us (7.4 TB/s of what it reads and writes; repeated rows come from L2), of
-// 64 x 512 2 us, a launch.  Gradient of 32768 x 1024 bf16 in a table of 50000 rows 75 us against 42 us of bytes: the sort takes 19 us of latency
-// (four launches of 16 blocks), the sums with 209 MB 38 us (5.5 TB/s), the joins 10 us of latency.  1516 x 128 in 259 rows 11.4 us: the sort 4.8, the sums 2.3 and a
-// second launch for the joins 2.5.
+// Measured on a B200 (device time of a pass among passes over the same buffers; with buffers that change 3 to 14 % more): lookup of 65536 x 1024 bf16 29.6 us
+// (7.5 TB/s of what it reads and writes; repeated rows come from L2), x 1023, single elements, 68 us, of 64 x 512 2 us, a launch.  Gradient of
+// 32768 x 1024 bf16 in a table of 50000 rows 75 to 77 us against 42 us of bytes: the sort takes 19 us of latency (four launches of 16 blocks), the sums
+// with 209 MB 38 us (5.5 TB/s), the joins 10 us of latency.  In a table of 259 rows the same batch takes 41 us against 10.5: two launches of the sort, sums into
+// partial rows and joins over long runs of pieces.  1516 x 128 in 259 rows 11.3 us: the sort 4.8, the sums 2.3 and a second launch for the joins 2.5.
 #include <math.h>
 
 #include "typed.cuh"
@@ -79,7 +80,7 @@ constexpr int SMALL_SORT = 4096;             // tokens one block sorts in shared
 
 __device__ __forceinline__ unsigned key_of(int tok, int vocab) { return (tok >= 0 && tok < vocab) ? (unsigned)tok : (unsigned)vocab; }
 
-// How many of the warp's earlier lanes hold the same digit, and whether this lane is the last of them.
+// the lanes, of those active, that hold the same digit as this one
 __device__ __forceinline__ unsigned same_digit(unsigned active, unsigned digit) { return __match_any_sync(active, digit); }
 
 // Exclusive prefix sum over one value a thread; all threads of the block call it.

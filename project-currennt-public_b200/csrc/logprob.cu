@@ -14,10 +14,12 @@
 // 8 warps where they do not, or, when there are few, a thread-block cluster of up to 8 blocks, which hand their sums and lists to the first
 // one through distributed shared memory: a row needs neither a second launch nor a workspace.
 // Bound, for long rows of 16-bit logits, by memory, with the exponentials close behind: 11.6 entries may arrive per cycle and SM, and the special
-// function units return 16 exponentials.  Measured on a B200 (device time): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth;
-// two bytes an entry), with four alternatives 162 us (the chains of the insertions, 20 a row), with 20 244 us; 38400 rows of 259 fp32 8.6 us (72 %);
-// 8 rows of 131072 with a mask and eight alternatives 11.4 us, without alternatives 6.8 us, a launch and two trips to memory of it.
-// Backward: one read, one write.  8192 rows of 32003 bf16 that start anywhere 167 us (96 %); 38400 of 259 fp32 18 us.
+// function units return 16 exponentials.  Measured on a B200 (device time of a pass among passes over the same buffers; with buffers that change 3 to 8 % more,
+// and boxes differ by 5 %): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth; two bytes an entry), with four alternatives
+// 165 us (the chains of the insertions, 20 a row), with 20 246 us; 38400 rows of 259 fp32 9 us (69 %); 8 rows of 131072 with a mask and eight
+// alternatives 11.6 us, without alternatives 6.8 us, a launch and two trips to memory of it.  A mask makes long rows slow: 8192 rows of 32003 bf16 with a
+// shared one 308 us (26 %), bytes are tested one by one and the registers spill.
+// Backward: one read, one write.  8192 rows of 32003 bf16 that start anywhere 168 to 170 us (95 %), with a shared mask 281 us (57 %); 38400 of 259 fp32 18 us.
 #include <math.h>
 
 #include <cooperative_groups.h>
@@ -35,13 +37,15 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int MAX_TOP = 32;
 
+// The hardware's exponential, whatever the logits' type: its error of 2^-22 goes into a sum whose own roundings are as large (38400 rows of 259 fp32: 4.2e-8 off in
+// the mean, a plain form with expf 4.1e-8).  Results below 2^-126 are 0.
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
 // z of two logits less what both subtract, z rounded.  Packed products and sums become one packed FMA in the assembler, rounding modifiers or not, and that
 // subtracts from the unrounded product; one that is an FMA already, with -0 for its addend, stays as it is.  The -0 is made from the scale, where it can not be
-// seen to be one.  With a scale that is a power of two the product needs no rounding, and the one FMA is right (8192 rows of 50001 with four alternatives: 180 us, with
+// seen to be one.  With a scale that is a power of two the product needs no rounding, and the one FMA is right (8192 rows of 50001 with four alternatives: 180 us a pass, with
 // two instructions 185 us).
 struct Exact {
     Pair s, off;
@@ -680,7 +684,8 @@ template <typename T> int forward(const T *logits, const FwdArgs &a, cudaStream_
         return B2_OK;
     }
     // What a warp does once a row (its first list, the joins) is the less the fewer warps a row has: one where the rows alone fill the device
-    // (8192 rows of 50001: 175 us, with four warps 251 us), four for some rows (1200 rows of 200000: 119 us, with one warp 153 us)
+    // (8192 rows of 50001, four alternatives: 165 us, with four warps 231, with eight 340), four for some rows (1200 rows of 200000: 112 us, with one warp 147, with
+    // eight 133)
     const auto go = [&](auto threads) -> int {
         constexpr int N = decltype(threads)::value;
         if (a.top) return a.mask ? launch_rows<T, N, true, true>(logits, a, st) : launch_rows<T, N, true, false>(logits, a, st);
@@ -700,7 +705,8 @@ struct BwdArgs {
     int vocab;
     float scale;
 };
-// fp32 gradients with the exponential of the full accuracy, 16-bit ones with the hardware's: its error of 2^-22 is lost in their rounding
+// fp32 gradients with the exponential of the full accuracy, 16-bit ones with the hardware's: its error of 2^-22 is lost in their rounding (and a probability
+// below 2^-126 is 0)
 template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
     const float2 v = halves(sizeof(T) == 4 ? x : mul2(x, pair(LOG2E, LOG2E)));
     return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
@@ -809,8 +815,8 @@ template <typename T, bool ENT, bool MASK> int backward(T *dlogits, const T *log
         B2_CUDA(cudaGetLastError());
         return B2_OK;
     };
-    // Vectors of a thread: 2 where the rows do not fill the device (16 rows of 32003: 2.7 us, with 8 4.0 us), else 8 (8192 rows: 167 us, with 4 172 us,
-    // with 2 211 us), with a mask 4 (300 us, with 8 337 us)
+    // Vectors of a thread: 2 where the rows do not fill the device (16 rows of 32003: 2.5 us, with 8 3.9 us), else 8 (8192 rows: 167 us, with 4 171 us,
+    // with 2 191 us), with a mask 4 (shared: 280 us, with 8 347 us, with 2 303 us; a mask a row: 310, 366, 305 us)
     if ((double)a.rows * vecs < 4096.0 * sm_count()) return go(std::integral_constant<int, 2>());
     return go(std::integral_constant<int, MASK ? 4 : 8>());
 }

@@ -19,7 +19,7 @@
 // keeps the same columns for all its rows, so the sums over frames stay in registers until the end, go to the workspace once, and are added there in a
 // fixed order by a second launch: no atomics, the same bits every time.
 // Measured on a B200 (device time of a pass among passes over the same buffers, a third of the frames padding in the forward pass; share of the copy
-// bandwidth; with buffers that change 1 to 10 % more, and boxes differ by 4 %): forward, layer norm, 38400 x 512 fp32 with a gate per sequence 52 us
+// bandwidth; with buffers that change 1 to 10 % more, and cards differ by 4 %): forward, layer norm, 38400 x 512 fp32 with a gate per sequence 52 us
 // (all bytes counted 92 %, of padding only zeros are written), 38400 x 512 bf16 33 us, x 1024 64 us, 8192 x 4001 without a gate 93 us (43 %; single
 // elements), 64 x 1024 bf16 3.5 us.  Backward, 16384 x 2048 bf16 with a gate per frame 95 us (86 %), with layer norm and biases 137 us (60 %), 16384 x 2047
 // 179 us, x 4096 250 us (one block a multiprocessor: its barriers are not hidden).

@@ -15,7 +15,7 @@
 // one through distributed shared memory: a row needs neither a second launch nor a workspace.
 // Bound, for long rows of 16-bit logits, by memory, with the exponentials close behind: 11.6 entries may arrive per cycle and SM, and the special
 // function units return 16 exponentials.  Measured on a B200 (device time of a pass among passes over the same buffers; with buffers that change 3 to 8 % more,
-// and boxes differ by 5 %): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth; two bytes an entry), with four alternatives
+// and cards differ by 5 %): 8192 rows of 50001 bf16 with entropy 138 us (91 % of the copy bandwidth; two bytes an entry), with four alternatives
 // 165 us (the chains of the insertions, 20 a row), with 20 246 us; 38400 rows of 259 fp32 9 us (69 %); 8 rows of 131072 with a mask and eight
 // alternatives 11.6 us, without alternatives 6.8 us, a launch and two trips to memory of it.  A mask makes long rows slow: 8192 rows of 32003 bf16 with a
 // shared one 308 us (26 %), bytes are tested one by one and the registers spill.

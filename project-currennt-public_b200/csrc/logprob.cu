@@ -26,45 +26,14 @@
 
 #include <initializer_list>
 
-#include "typed.cuh"
+#include "logits.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace b2 {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr unsigned FULL = 0xffffffffu;
 constexpr int MAX_TOP = 32;
-
-// The hardware's exponential, whatever the logits' type: its error of 2^-22 goes into a sum whose own roundings are as large (38400 rows of 259 fp32: 4.2e-8 off in
-// the mean, a plain form with expf 4.1e-8).  Results below 2^-126 are 0.
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
-__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
-
-// z of two logits less what both subtract, z rounded.  Packed products and sums become one packed FMA in the assembler, rounding modifiers or not, and that
-// subtracts from the unrounded product; one that is an FMA already, with -0 for its addend, stays as it is.  The -0 is made from the scale, where it can not be
-// seen to be one.  With a scale that is a power of two the product needs no rounding, and the one FMA is right (8192 rows of 50001 with four alternatives: 180 us a pass, with
-// two instructions 185 us).
-struct Exact {
-    Pair s, off;
-    __device__ __forceinline__ Pair operator()(float x, float y) const { return fma2(pair(x, y), s, off); }
-};
-struct Rounded {
-    Pair s, off, none;
-    __device__ __forceinline__ Rounded(Pair s_, Pair off_, float scale) : s(s_), off(off_) {
-        const float zero = __fmul_rn(scale, -0.0f);
-        none = pair(zero, zero);
-    }
-    __device__ __forceinline__ Pair operator()(float x, float y) const { return add2(fma2(pair(x, y), s, none), off); }
-};
-// f(function of two logits), the one that the scale asks for
-template <typename F> __device__ __forceinline__ void less_of(float scale, float minus, F &&f) {
-    const Pair s = pair(scale, scale), off = pair(-minus, -minus);
-    if ((__float_as_uint(scale) & 0x7fffffu) == 0) f(Exact{s, off});
-    else f(Rounded(s, off, scale));
-}
 
 // ---- running sums -----------------------------------------------------------------------------------------------------------------
 struct Sums { float m, s, e; };   // largest z, sum of e^(z - m), sum of e^(z - m) (z - m)
@@ -110,40 +79,6 @@ template <int N> __device__ __forceinline__ void add_values(Sums &a, const float
     a.e += e;
 }
 
-// ---- vectors of 16 bytes as they were loaded ------------------------------------------------------------------------------------------
-template <typename T> struct Raw;
-template <> struct Raw<float> {
-    static constexpr unsigned NONE = 0xff800000u;      // -inf in every place of a word
-    static __device__ __forceinline__ void values(float (&z)[4], const uint4 &q) {
-        z[0] = __uint_as_float(q.x); z[1] = __uint_as_float(q.y); z[2] = __uint_as_float(q.z); z[3] = __uint_as_float(q.w);
-    }
-    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
-    static __device__ __forceinline__ float largest(unsigned a) { return __uint_as_float(a); }
-};
-template <> struct Raw<__nv_bfloat16> {
-    static constexpr unsigned NONE = 0xff80ff80u;
-    static __device__ __forceinline__ float2 two(unsigned a) { return make_float2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)); }
-    static __device__ __forceinline__ void values(float (&z)[8], const uint4 &q) {
-        const float2 a = two(q.x), b = two(q.y), c = two(q.z), d = two(q.w);
-        z[0] = a.x; z[1] = a.y; z[2] = b.x; z[3] = b.y; z[4] = c.x; z[5] = c.y; z[6] = d.x; z[7] = d.y;
-    }
-    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { unsigned y; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b)); return y; }
-    static __device__ __forceinline__ float largest(unsigned a) { const float2 v = two(a); return max_nan(v.x, v.y); }
-};
-template <> struct Raw<__half> {
-    static constexpr unsigned NONE = 0xfc00fc00u;
-    static __device__ __forceinline__ float2 two(unsigned a) { return __half22float2(*reinterpret_cast<const __half2 *>(&a)); }
-    static __device__ __forceinline__ void values(float (&z)[8], const uint4 &q) {
-        const float2 a = two(q.x), b = two(q.y), c = two(q.z), d = two(q.w);
-        z[0] = a.x; z[1] = a.y; z[2] = b.x; z[3] = b.y; z[4] = c.x; z[5] = c.y; z[6] = d.x; z[7] = d.y;
-    }
-    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { unsigned y; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b)); return y; }
-    static __device__ __forceinline__ float largest(unsigned a) { const float2 v = two(a); return max_nan(v.x, v.y); }
-};
-template <typename T> __device__ __forceinline__ unsigned larger_of(const uint4 &q) {
-    typedef Raw<T> R;
-    return R::larger(R::larger(q.x, q.y), R::larger(q.z, q.w));
-}
 // The sums over U vectors of logits x; top: their largest x (NaN if one is NaN).  A pair of entries costs two conversions, one packed maximum
 // (by the caller), two packed FMAs, a packed product and sum, and two exponentials, with a scale that is no power of two a packed sum more.  Where an
 // entry is -inf the sum of w * d turns NaN and is taken again with the differences held above -inf; SAFE does so at once.
@@ -197,17 +132,6 @@ template <typename T, int U, bool SAFE> __device__ __forceinline__ void add_vect
 }
 
 // ---- the K largest ------------------------------------------------------------------------------------------------------------------
-// An entry is one 64-bit key: the value as an ordered integer above, the complement of its index below; larger is better.  0 is no entry.
-typedef unsigned long long Key;
-__device__ __forceinline__ unsigned ordered(float z) {
-    const unsigned b = __float_as_uint(z + 0.0f);           // -0 counts as 0
-    return z != z ? FULL : (b ^ ((b >> 31) ? FULL : 0x80000000u));
-}
-__device__ __forceinline__ float ordered_value(unsigned o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : FULL)); }
-__device__ __forceinline__ Key make_key(float z, int index) { return ((Key)ordered(z) << 32) | (unsigned)~index; }
-__device__ __forceinline__ float key_value(Key k) { return ordered_value((unsigned)(k >> 32)); }
-__device__ __forceinline__ int key_index(Key k) { return (int)~(unsigned)k; }
-
 // Lane l holds the l-th best of the warp, descending.  A value is of interest if it is not below `limit` (the K-th best, or a bound known
 // from elsewhere) and above `floor`: the K-th best of the batches before the current one, whose indices are all lower, so that an equal
 // value loses against it.

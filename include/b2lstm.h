@@ -21,7 +21,7 @@
  *   b2_net_*      layer stack + minibatch step          <-> NeuralNetwork + Optimizer::_processDataSet
  *   b2_dp_*       gradient all-reduce across GPUs (no counterpart: the reference is single-GPU)
  * and, beside the layers, the operators of models over tokens (no counterpart: the reference has real-valued inputs and targets):
- *   b2_embedding_*, b2_block_norm_*, b2_logprob_*, b2_gradient_*
+ *   b2_embedding_*, b2_block_norm_*, b2_logprob_*, b2_gradient_*, b2_distill_*, b2_beam_*, b2_int8_*
  */
 #ifndef B2LSTM_H
 #define B2LSTM_H
@@ -246,6 +246,69 @@ int b2_gradient_norm(const b2_tensor *tensors, int n, float *norm_dev, void *wor
  * float) leaves the values as they are (the update of b2_net then zeroes the entries that are no numbers).  Tensors must not overlap, save that out[i] may be tensors[i]. */
 int b2_gradient_clip(const b2_tensor *tensors, const b2_tensor *out, int n, float max_norm, float *norm_dev, void *workspace,
                      size_t workspace_bytes, b2_stream stream);
+
+/* Learning from a teacher: the divergence of the rows of logits x from a teacher that is known by its `top` (1 to 128) most likely tokens and their
+ * log probabilities, [rows][top], as b2_logprob_forward leaves them.  With z = scale * x, lse = log sum exp z and p = exp(z - lse):
+ *   lse_rest NULL: the listed tokens are all there is, q = exp(top_logprobs) over their sum (top_logprobs may then be logits):
+ *       loss = sum q (log q - log p)
+ *   else:         q = exp(top_logprobs); the rest of the vocabulary is one more outcome, with q_rest = 1 - sum q (0 where that is below 2^-20: log
+ *       probabilities in fp32 say no more) and p_rest = exp(lse_rest - lse), lse_rest = log sum exp z over the tokens that are not listed:
+ *       loss = sum q (log q - log p) + q_rest (log q_rest - log p_rest)
+ * A temperature T is scale = 1 / T here and in the teacher's b2_logprob_forward.  A place of the list with a negative token is empty, and so is one whose
+ * token stands further ahead in its row; a row with nothing but empty places (and, with lse_rest NULL, one whose listed tokens all have the log probability
+ * -inf) has the loss 0.  A token that is not below vocab, NaN or +inf among the logits or a listed log probability that is NaN or +inf: NaN.  A listed token
+ * with q > 0 and the logit -inf: +inf; so is a rest with q_rest > 0 and p_rest 0.  loss, lse and lse_rest (NULL: see above) are floats, one a row; lse -inf:
+ * nothing above -inf in the row. */
+int b2_distill_forward(const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *top_tokens,
+                       const float *top_logprobs, int top, float *loss, float *lse, float *lse_rest, b2_stream stream);
+/* The gradient of sum(dloss * loss) with respect to the logits, in their type; lse and lse_rest as the forward pass left them:
+ *   dlogits = dloss * scale * (p - q),  and off the list, with lse_rest:  dloss * scale * (p - q_rest * exp(z - lse_rest))
+ * Rows without a listed token get zeros, those with one that is not below vocab NaN.  With accumulate non-zero it is added to dlogits (rows of zeros leave it
+ * as it is); else dlogits may take the place of the logits. */
+int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits, int type, long long rows, int vocab, long long ld, float scale,
+                        const int *top_tokens, const float *top_logprobs, int top, const float *lse, const float *lse_rest, const float *dloss,
+                        int accumulate, b2_stream stream);
+
+/* A step of beam search: the `top` (1 to 64) best continuations of `groups` sequences with `beams` (1 to 64) beams each.  Row g * beams + b of the
+ * logits, vocab (at most 2^26) columns, belongs to beam b of sequence g; scores [groups * beams] are the beams' log probabilities so far.  With z = scale * x
+ * where the token is allowed (mask as for b2_logprob_forward) and -inf elsewhere, the continuation of beam b by token v has the
+ *   score = scores[b] + z[v] - log sum exp z
+ * and they are ranked by weights[b] * score, in 64 bits, equal ones by beam, logit (larger first) and token.  weights (NULL: 1) are a length penalty's factors,
+ * above 0.  A beam with finished[b] (NULL: none) non-zero is at its end: it has one continuation, end_token with the score it has; its logits are not
+ * looked at.  No continuations: beams whose score is -inf or NaN or whose weight is no positive finite number, rows with NaN or +inf among the allowed logits,
+ * tokens that are not allowed or have z = -inf.  top_scores, top_beams (below beams) and top_tokens are [groups][top], best first; -inf, -1 and -1 where
+ * there are fewer.  workspace: aligned to 16 bytes; its size is 0 for sizes that the call refuses. */
+size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top);
+int b2_beam_select(const void *logits, int type, long long groups, int beams, int vocab, long long ld, const unsigned char *mask, long long ld_mask,
+                   float scale, const float *scores, const unsigned char *finished, const float *weights, int end_token, int top, float *top_scores,
+                   int *top_beams, int *top_tokens, void *workspace, size_t workspace_bytes, b2_stream stream);
+/* The beams that go on take their states and histories along:
+ *   out[o][g * beams + b][:] = data[o][g * beams + parents[g * beams + b]][:]   for all o < outer
+ * in n tensors [outer][groups * beams][row_bytes], contiguous, of any element type; zeros for a parent that is negative or not below beams (1 to 64).  outer 1: a
+ * state of the beams; outer T: frames or tokens of T steps, time-major.  out NULL or data: in place; else the two must not overlap, nor may tensors.  The list
+ * is read during the call only. */
+typedef struct {
+    void *data, *out;
+    long long outer;
+    long long row_bytes;
+} b2_state;
+int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long groups, int beams, b2_stream stream);
+
+/* Rows in 8-bit integers: scales[r] = max |x[r]| / 127 and q[r][:] = x[r][:] * (127 / max |x[r]|), the quotients rounded to fp32, the product rounded once, to
+ * the nearest integer (the even one of two).  A row of zeros (or of nothing above 2^-118) has the scale 0 and zeros; one that holds NaN or an infinity the
+ * scale NaN and zeros. */
+int b2_int8_quantize(signed char *q, long long ld_q, float *scales, const void *x, int type, long long rows, int dim, long long ld_x, b2_stream stream);
+/* Products in 8-bit integers with a scale for each row and each channel, as for the output matrix of a model that is answered with:
+ *   out[r][c] = x_scales[r] * w_scales[c] * sum_k x[r][k] * w[c][k] + bias[c]
+ * w is [channels][dim], bias (channels floats) may be NULL.  The sums are exact (dim at most 131071); each is rounded to fp32, then the product, the sum with
+ * the bias and the conversion to out_type are.  x_type B2_F32, B2_BF16 or B2_F16: x is quantised in the call as b2_int8_quantize does (x_scales is NULL,
+ * workspace aligned to 16 bytes); B2_I8: x and x_scales are given and no workspace is needed.  8-bit integers start at a multiple of 16 bytes, and so does each
+ * of their rows (ld_w, and ld_x with B2_I8). */
+enum { B2_I8 = 3 };
+size_t b2_int8_product_workspace(long long rows, int channels, int dim);
+int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, int x_type, long long ld_x, const float *x_scales, const signed char *w,
+                    long long ld_w, const float *w_scales, const float *bias, long long rows, int channels, int dim, void *workspace,
+                    size_t workspace_bytes, b2_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * NeuralNetwork + Optimizer::_processDataSet + SteepestDescentOptimizer

@@ -50,6 +50,17 @@ SIGNATURES = {
     "b2_gradient_norm_workspace": (C.c_size_t, []),
     "b2_gradient_norm": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "b2_gradient_clip": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b2_distill_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_float, C.c_void_p, C.c_void_p, C.c_int] + [C.c_void_p] * 4),
+    "b2_distill_backward": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_float, C.c_void_p, C.c_void_p,
+                                      C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "b2_beam_select_workspace": (C.c_size_t, [C.c_longlong, C.c_int, C.c_int, C.c_int]),
+    "b2_beam_select": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_float, C.c_void_p, C.c_void_p,
+                                 C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b2_beam_reorder": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p]),
+    "b2_int8_quantize": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p]),
+    "b2_int8_product_workspace": (C.c_size_t, [C.c_longlong, C.c_int, C.c_int]),
+    "b2_int8_product": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p,
+                                  C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "b2_lstm_num_weights": (C.c_size_t, [C.c_void_p]),
     "b2_lstm_create": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "b2_lstm_destroy": (None, [C.c_void_p]),

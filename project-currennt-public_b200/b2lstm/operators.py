@@ -1,5 +1,5 @@
 """The operators of a token model around the recurrent layers (include/b2lstm.h: b2_embedding_*, b2_block_norm_*, b2_logprob_*,
-b2_gradient_*), on tensors: any object with data_ptr(), shape, stride(), dtype and is_cuda, e.g. torch CUDA tensors.  Calls go to the current
+b2_gradient_*, b2_distill_*, b2_beam_*, b2_int8_*), on tensors: any object with data_ptr(), shape, stride(), dtype and is_cuda, e.g. torch CUDA tensors.  Calls go to the current
 CUDA device; tensors that say where they are (get_device()) are refused if that is another one.
 
 Shapes, element types and leading dimensions come from the tensors and are checked on the way (csrc/binding.cpp); the library checks the rest.  Rows may lie
@@ -17,7 +17,8 @@ except ImportError:             # not built: the first call says so
     _tensors = None
 
 _BOUND = ("b2_last_error_string", "b2_current_device", "b2_embedding_forward", "b2_embedding_backward", "b2_block_norm_forward", "b2_block_norm_backward", "b2_logprob_forward",
-          "b2_logprob_backward", "b2_gradient_norm", "b2_gradient_clip")
+          "b2_logprob_backward", "b2_gradient_norm", "b2_gradient_clip", "b2_distill_forward", "b2_distill_backward", "b2_beam_select", "b2_beam_reorder",
+          "b2_int8_quantize", "b2_int8_product")
 _ready = None
 
 
@@ -124,3 +125,91 @@ def gradient_norm(tensors, norm, workspace=None, stream=None):
 def gradient_clip(tensors, max_norm, norm, workspace=None, stream=None):
     """The same, and the tensors scaled by min(1, max_norm / norm), in place or into the list's outputs"""
     (_ready or _ops()).gradient_clip(tensors._at, tensors._out_at, tensors.n, tensors._device, max_norm, norm, workspace, stream)
+
+
+def distill_forward(logits, top_tokens, top_logprobs, loss, lse, lse_rest=None, scale=1.0, stream=None):
+    """Divergence of the rows of logits [rows, vocab] from a teacher's most likely tokens: top_tokens int32 and top_logprobs float32 [rows, top] as
+    logprob_forward leaves them, loss and lse float32 [rows].  With lse_rest (float32 [rows]) the rest of the vocabulary counts as one more outcome."""
+    (_ready or _ops()).distill_forward(logits, top_tokens, top_logprobs, loss, lse, lse_rest, scale, stream)
+
+
+def distill_backward(dlogits, logits, top_tokens, top_logprobs, lse, dloss, lse_rest=None, scale=1.0, accumulate=False, stream=None):
+    """The gradient of sum(dloss * loss) with respect to the logits (added to dlogits with accumulate; dlogits may else be logits)"""
+    (_ready or _ops()).distill_backward(dlogits, logits, top_tokens, top_logprobs, lse, lse_rest, dloss, scale, accumulate, stream)
+
+
+def beam_select_workspace(groups, beams, vocab, top):
+    return int(lib().b2_beam_select_workspace(groups, beams, vocab, top))
+
+
+def beam_select(logits, scores, top_scores, top_beams, top_tokens, finished=None, weights=None, end_token=0, mask=None, scale=1.0, workspace=None,
+                stream=None):
+    """The best continuations of the beams of each sequence: logits [groups * beams, vocab], scores float32 [groups * beams], results [groups, top]
+    (scores float32; the beam each one continues and its token int32).  finished uint8 or bool, weights float32 [groups * beams]; mask as for
+    logprob_forward."""
+    (_ready or _ops()).beam_select(logits, scores, top_scores, top_beams, top_tokens, finished, weights, end_token, mask, scale, workspace, stream)
+
+
+class _State(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("outer", C.c_longlong), ("row_bytes", C.c_longlong)]
+
+
+class StateList:
+    """What the beams of a search carry along, as one argument, built once: contiguous tensors of any element types, the axis of each that runs over
+    the beams of all sequences (an int for all, or one for each), and, where they are not reordered in place, the tensors that take the
+    reordered ones.  Holds references to them."""
+
+    def __init__(self, tensors, axes=0, out=None):
+        self.tensors, self.out = list(tensors), None if out is None else list(out)
+        self.n = len(self.tensors)
+        axes = [axes] * self.n if isinstance(axes, int) else list(axes)
+        if len(axes) != self.n or (self.out is not None and len(self.out) != self.n):
+            raise B2Error("%d tensors, %d axes and %s outputs" % (self.n, len(axes), "no" if out is None else len(self.out)))
+        self._in, rows = (_State * self.n)(), set()
+        for i, t in enumerate(self.tensors):
+            to = t if self.out is None else self.out[i]
+            shape = tuple(t.shape)
+            for x in (t, to):
+                if not x.is_cuda or not x.is_contiguous():
+                    raise B2Error("tensor %d is not a contiguous tensor on the GPU" % i)
+            if tuple(to.shape) != shape or to.dtype != t.dtype:
+                raise B2Error("output %d has the shape %s and the element type %s, not %s and %s" % (i, tuple(to.shape), to.dtype, shape, t.dtype))
+            if not 0 <= axes[i] < len(shape):
+                raise B2Error("tensor %d has the shape %s: no axis %d" % (i, shape, axes[i]))
+            outer, inner = 1, t.element_size()
+            for n in shape[:axes[i]]:
+                outer *= n
+            for n in shape[axes[i] + 1:]:
+                inner *= n
+            rows.add(shape[axes[i]])
+            self._in[i] = _State(t.data_ptr(), to.data_ptr(), outer, inner)
+        if len(rows) > 1:
+            raise B2Error("the tensors have %s beams" % sorted(rows))
+        devices = {t.get_device() for t in self.tensors + (self.out or []) if hasattr(t, "get_device")}
+        if len(devices) > 1:
+            raise B2Error("the tensors are on the devices %s" % sorted(devices))
+        self.rows = rows.pop() if rows else -1
+        self._device = devices.pop() if devices else -1
+        self._at = C.addressof(self._in)
+
+
+def beam_reorder(states, parents, stream=None):
+    """The tensors of a StateList by parents (int32 [groups, beams]): row g * beams + b becomes row g * beams + parents[g, b], zeros for a parent that is
+    no beam"""
+    (_ready or _ops()).beam_reorder(states._at, states.n, states._device, states.rows, parents, stream)
+
+
+def int8_quantize(q, scales, x, stream=None):
+    """q (int8) = x over scales, scales (float32 [rows]) = the largest magnitudes of the rows of x over 127.  int8_product wants rows of int8 that start at
+    multiples of 16 bytes: torch.empty(rows, (dim + 15) // 16 * 16, dtype=torch.int8)[:, :dim]"""
+    (_ready or _ops()).int8_quantize(q, scales, x, stream)
+
+
+def int8_product_workspace(rows, channels, dim):
+    return int(lib().b2_int8_product_workspace(rows, channels, dim))
+
+
+def int8_product(out, x, w, w_scales, bias=None, x_scales=None, workspace=None, stream=None):
+    """out [rows, channels] = x [rows, dim] times w [channels, dim] (int8, w_scales float32 [channels]) in 8-bit integers, plus bias (float32 [channels]); x is
+    quantised in the call (with a workspace), or int8 with its x_scales (float32 [rows])"""
+    (_ready or _ops()).int8_product(out, x, x_scales, w, w_scales, bias, workspace, stream)

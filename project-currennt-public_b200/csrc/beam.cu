@@ -1,0 +1,534 @@
+// A step of beam search: the K best continuations of a sequence's beams over all tokens, and the beams' states by the beams that go on.
+//
+//   score(b, v) = score_b + z_bv - lse_b,  z = s * x where token v is allowed, -inf elsewhere;   rank = weight_b * score(b, v)
+//
+// Within a beam the ranks are in the order of z, so the K best of a beam are its K largest logits, and the beam's log sum is not needed to find them.
+// First kernel: a block takes a slice of a beam's row into registers, all loads at once, one trip to memory.  Groups of neighbouring lanes give 64 maxima;
+// the K-th largest of them is a bound that at least K entries of the slice reach, and that hardly more do (16 of 12500: 20 to 25).  The entries that
+// reach it go to shared memory and are counted into their places.  The maximum gives the sum of exponentials its reference, so nothing is ever rescaled.
+// Second kernel, started while the first one drains: a block joins the sums and the lists of a sequence's beams, the ranks in 64 bits (scores of different
+// beams meet, and 32 bits would make ties of what the beams' logits tell apart).
+#include <math.h>
+
+#include "logits.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int MAX_BEAMS = 64, MAX_BEST = 64, MOST_VOCAB = 1 << 26;
+constexpr int SLICE_VECS = 4;        // vectors of 16 bytes a thread holds
+
+struct Part { float m, s; };         // largest z of a slice, sum of e^(z - m)
+
+struct SelectArgs {
+    const unsigned char *mask; long long ld_mask;
+    const float *scores; const unsigned char *finished; const float *weights;
+    long long groups, ld;
+    int beams, vocab, top, end_token, slices, slice;     // slice: vectors of a slice
+    float scale;
+    Part *parts; Key *lists;                             // [row][slice], [row][slice][top]
+    float *best; int *from, *tokens;
+};
+// whether beam `row` has continuations of its own (finished ones have their one without looking at the logits)
+__device__ __forceinline__ bool runs(const SelectArgs &a, long long row) {
+    const float s = a.scores[row], w = a.weights ? a.weights[row] : 1.0f;
+    return s > neg_inf() && s < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000) && !(a.finished && a.finished[row]);
+}
+
+template <typename T, int THREADS, bool MASK>
+__global__ void __launch_bounds__(THREADS) beam_rows_kernel(const T *logits, const SelectArgs a) {
+    constexpr int W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, GROUP = THREADS / 64, CAP = 512;
+    __shared__ float maxima[64], tops[WARPS], sums[WARPS];
+    __shared__ Key found[CAP];
+    __shared__ float bound;
+    __shared__ int count;
+    __shared__ Key winner[WARPS];
+    grid_release();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const long long row = blockIdx.x / (unsigned)a.slices;
+    const int part = (int)(blockIdx.x % (unsigned)a.slices);
+    if (!runs(a, row)) return;
+    Part *const to = a.parts + row * a.slices + part;
+    Key *const list = a.lists + (row * a.slices + part) * a.top;
+    const T *x = logits + row * a.ld;
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const unsigned char *mk = MASK ? a.mask + row * a.ld_mask : nullptr;
+    const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
+    const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
+    uint4 q[U];
+    Vec<unsigned char, W> on[MASK ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = v0 + t + u * THREADS, i0 = v * W - mis;
+        const bool inside = v < v1, whole = i0 >= 0 && i0 + W <= a.vocab;
+        q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+        if (inside && whole) q[u] = *reinterpret_cast<const uint4 *>(x + i0);
+        else if (inside) {
+            T e[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < a.vocab ? x[i0 + j] : from_float<T>(neg_inf());
+            memcpy(&q[u], e, 16);
+        }
+        if (MASK) {
+            if (inside && whole && mask_vec) on[u] = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
+            else
+#pragma unroll
+                for (int j = 0; j < W; ++j) on[u].v[j] = inside && i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
+        }
+    }
+    if (MASK)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            T e[W];
+            memcpy(e, &q[u], 16);
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (!on[u].v[j]) e[j] = from_float<T>(neg_inf());
+            memcpy(&q[u], e, 16);
+        }
+    unsigned big = larger_of<T>(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) big = Raw<T>::larger(big, larger_of<T>(q[u]));
+    const float mine = __fmul_rn(Raw<T>::largest(big), a.scale);
+    float most = mine;
+#pragma unroll
+    for (int o = 1; o < GROUP && o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+    if (t % GROUP == 0) maxima[t / GROUP] = most;
+#pragma unroll
+    for (int o = GROUP; o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+    if (lane == 0) tops[warp] = most;
+    if (t == 0) count = 0;
+    __syncthreads();
+    most = tops[lane % WARPS];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+    if (t < 64) {
+        // the place of this group's maximum among the 64
+        const Key k = make_key(maxima[t], t);
+        int before = 0;
+#pragma unroll 8
+        for (int i = 0; i < 64; ++i) before += make_key(maxima[i], i) > k;
+        if (before == a.top - 1) bound = maxima[t];
+    }
+    float s = 0.0f;
+    if (most != neg_inf()) {
+        const Pair l2 = pair(LOG2E, LOG2E);
+        Pair p = 0;
+        less_of(a.scale, most, [&](const auto &less) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float z[W];
+                Raw<T>::values(z, q[u]);
+#pragma unroll
+                for (int j = 0; j < W; j += 2) {
+                    const float2 d = halves(mul2(less(z[j], z[j + 1]), l2));
+                    p = add2(p, pair(ex2(d.x), ex2(d.y)));
+                }
+            }
+        });
+        const float2 h = halves(p);
+        s = h.x + h.y;
+    }
+    s = warp_sum(s);
+    if (lane == 0) sums[warp] = s;
+    __syncthreads();
+    const float limit = bound;
+    if (mine >= limit && mine > neg_inf())
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float z[W];
+            Raw<T>::values(z, q[u]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float v = __fmul_rn(z[j], a.scale);
+                if (v >= limit && v > neg_inf()) {
+                    const int at = atomicAdd(&count, 1);
+                    if (at < CAP) found[at] = make_key(v, (v0 + t + u * THREADS) * W - mis + j);
+                }
+            }
+        }
+    __syncthreads();
+    const int n = count;
+    if (n <= CAP) {
+        for (int i = t; i < n; i += THREADS) {
+            const Key k = found[i];
+            int before = 0;
+            for (int j = 0; j < n; ++j) before += found[j] > k;
+            if (before < a.top) list[before] = k;
+        }
+        for (int i = n + t; i < a.top; i += THREADS) list[i] = 0;
+    } else {
+        // many equal ones: the next best in turn
+        Key last = ~0ull;
+        for (int i = 0; i < a.top; ++i) {
+            Key k = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float z[W];
+                Raw<T>::values(z, q[u]);
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const float v = __fmul_rn(z[j], a.scale);
+                    const Key e = make_key(v, (v0 + t + u * THREADS) * W - mis + j);
+                    if (v > neg_inf() && e < last && e > k) k = e;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const Key other = __shfl_xor_sync(FULL, k, o);
+                if (other > k) k = other;
+            }
+            if (lane == 0) winner[warp] = k;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                if (winner[w] > k) k = winner[w];
+            if (t == 0) list[i] = k;
+            last = k;
+            __syncthreads();
+        }
+    }
+    if (t == 0) {
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) all += sums[w];
+        *to = {most, all};
+    }
+}
+
+// A continuation in the order of ranks: the rank, then beam (lower first), logit (larger), token (lower) in one word
+struct Cand { double rank; unsigned long long tie; };
+__device__ __forceinline__ bool better(const Cand &a, const Cand &b) { return a.rank > b.rank || (a.rank == b.rank && a.tie > b.tie); }
+__device__ __forceinline__ Cand no_cand() { return {-INFINITY, 0}; }
+__device__ __forceinline__ unsigned long long tie_of(int beam, float z, int token) {
+    return ((unsigned long long)(MAX_BEAMS - 1 - beam) << 58) | ((unsigned long long)ordered(z) << 26) | (unsigned)(MOST_VOCAB - 1 - token);
+}
+__device__ __forceinline__ int beam_of(unsigned long long tie) { return MAX_BEAMS - 1 - (int)(tie >> 58); }
+__device__ __forceinline__ float logit_of(unsigned long long tie) { return ordered_value((unsigned)(tie >> 26)); }
+__device__ __forceinline__ int token_of(unsigned long long tie) { return MOST_VOCAB - 1 - (int)(tie & (MOST_VOCAB - 1)); }
+
+// one block a sequence
+constexpr int JOIN_WARPS = 8;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) beam_join_kernel(const SelectArgs a) {
+    __shared__ double off[MAX_BEAMS], weight[MAX_BEAMS];
+    __shared__ bool ended[MAX_BEAMS];
+    __shared__ Cand stage[JOIN_WARPS][MAX_BEST];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long g = blockIdx.x;
+    grid_wait();
+    // score_b - lse_b of the beams; NaN: no continuations
+    for (int b = warp; b < a.beams; b += JOIN_WARPS) {
+        const long long row = g * a.beams + b;
+        const float score = a.scores[row], w = a.weights ? a.weights[row] : 1.0f;
+        const bool end = a.finished && a.finished[row];
+        const bool fit = score > neg_inf() && score < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000);
+        double o = nan("");
+        if (fit && end) o = (double)score;
+        else if (fit) {
+            float m = neg_inf();
+            for (int i = lane; i < a.slices; i += 32) m = max_nan(m, a.parts[row * a.slices + i].m);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, x));
+            double s = 0.0;
+            if (m != neg_inf())
+                for (int i = lane; i < a.slices; i += 32) {
+                    const Part p = a.parts[row * a.slices + i];
+                    if (p.m != neg_inf()) s += (double)p.s * exp((double)p.m - (double)m);
+                }
+            s = warp_sum(s);
+            o = m == neg_inf() ? nan("") : (double)score - (double)m - log(s);
+        }
+        if (lane == 0) { off[b] = o; weight[b] = (double)w; ended[b] = end; }
+    }
+    __syncthreads();
+    // every warp merges its share of the sorted lists: lane l has the heads of the lists l, l + 32, ... of the share, and gives the best of them
+    const int lists = a.beams * a.slices, share = (lists + JOIN_WARPS - 1) / JOIN_WARPS, warps = (lists + share - 1) / share;
+    const auto entry = [&](int l, int i) -> Cand {
+        const int b = l / a.slices;
+        const double o = off[b];
+        if (o != o || i >= a.top) return no_cand();
+        if (ended[b]) return l % a.slices == 0 && i == 0 ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
+        const Key k = a.lists[((g * a.beams + b) * (long long)a.slices + l % a.slices) * a.top + i];
+        if (!k) return no_cand();
+        const float z = key_value(k);
+        return {weight[b] * (o + (double)z), tie_of(b, z, key_index(k))};
+    };
+    if (warp < warps) {
+        const int l0 = warp * share, l1 = min(lists, l0 + share);
+        // a lane with several lists merges them on the fly: per list a position
+        constexpr int HELD = 4;
+        if (share <= 32 * HELD) {
+            Cand head[HELD];
+            int at[HELD];
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                const int l = l0 + lane + 32 * h;
+                at[h] = 0;
+                head[h] = l < l1 ? entry(l, 0) : no_cand();
+            }
+            for (int k = 0; k < a.top; ++k) {
+                Cand c = head[0];
+                int which = 0;
+#pragma unroll
+                for (int h = 1; h < HELD; ++h)
+                    if (better(head[h], c)) { c = head[h]; which = h; }
+                Cand top = c;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
+                    if (better(other, top)) top = other;
+                }
+                if (lane == 0) stage[warp][k] = top;
+                if (top.tie == 0) {                              // none is left
+                    for (int i = k + 1 + lane; i < a.top; i += 32) stage[warp][i] = no_cand();
+                    break;
+                }
+                if (c.tie == top.tie && c.rank == top.rank)
+#pragma unroll
+                    for (int h = 0; h < HELD; ++h)
+                        if (h == which) head[h] = entry(l0 + lane + 32 * h, ++at[h]);
+            }
+        } else {
+            // very many lists: the best entry behind the last one, by looking at all
+            Cand last = {INFINITY, ~0ull};
+            for (int k = 0; k < a.top; ++k) {
+                Cand top = no_cand();
+                for (int l = l0 + lane; l < l1; l += 32)
+                    for (int i = 0; i < a.top; ++i) {
+                        const Cand c = entry(l, i);
+                        if (c.tie == 0) break;
+                        if (better(last, c)) {
+                            if (better(c, top)) top = c;
+                            break;
+                        }
+                    }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
+                    if (better(other, top)) top = other;
+                }
+                if (lane == 0) stage[warp][k] = top;
+                last = top;
+                if (top.tie == 0) {
+                    for (int i = k + 1 + lane; i < a.top; i += 32) stage[warp][i] = no_cand();
+                    break;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    // the warps' lists
+    int at = 0;
+    Cand head = lane < warps ? stage[lane][0] : no_cand();
+    for (int k = 0; k < a.top; ++k) {
+        Cand top = head;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
+            if (better(other, top)) top = other;
+        }
+        if (lane == 0) {
+            const long long i = g * a.top + k;
+            const bool none = top.tie == 0;
+            const int b = none ? 0 : beam_of(top.tie);
+            a.best[i] = none ? neg_inf() : ended[b] ? (float)off[b] : (float)(off[b] + (double)logit_of(top.tie));
+            a.from[i] = none ? -1 : b;
+            a.tokens[i] = none ? -1 : token_of(top.tie);
+        }
+        if (head.tie != 0 && head.tie == top.tie && head.rank == top.rank) {
+            ++at;
+            head = at < a.top ? stage[lane][at] : no_cand();
+        }
+    }
+}
+
+// slices of a row: vectors in each, a multiple of nothing; the last one may be shorter
+constexpr int SLICE_THREADS = 512;
+int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
+int slices_of(int vocab, int type) { return (vectors_of(vocab, type) + SLICE_THREADS * SLICE_VECS - 1) / (SLICE_THREADS * SLICE_VECS); }
+
+template <typename T> int select(const T *logits, SelectArgs a, int type, cudaStream_t st) {
+    const int vecs = vectors_of(a.vocab, type);
+    a.slices = slices_of(a.vocab, type);
+    a.slice = (vecs + a.slices - 1) / a.slices;
+    const long long blocks = a.groups * a.beams * a.slices;
+    if (blocks > 0x7fffffffll) { set_error("b2_beam_select: %lld rows of %d", a.groups * a.beams, a.vocab); return B2_ERR_BAD_SHAPE; }
+    if (a.mask) beam_rows_kernel<T, SLICE_THREADS, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    else beam_rows_kernel<T, SLICE_THREADS, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(32 * JOIN_WARPS), 0, st, a);
+}
+
+bool sizes_fit(long long groups, int beams, int vocab, int top) {
+    return groups >= 0 && groups <= 0x7fffffff / MAX_BEAMS && beams >= 1 && beams <= MAX_BEAMS && vocab >= 1 && vocab <= MOST_VOCAB && top >= 1 && top <= MAX_BEST;
+}
+
+// ---- reordering -----------------------------------------------------------------------------------------------------------------------
+constexpr int MAX_STATES = 32;       // of a launch; more take several
+struct StateArgs {
+    b2_state s[MAX_STATES];
+    int n, beams;
+    long long groups;
+    const int *parents;
+    unsigned first[MAX_STATES + 1];  // of the blocks of tensor i
+};
+// A thread moves a column of N bytes (of the same place in a sequence's beams) for all beams of a sequence: it alone reads and writes it, so that a state may
+// be reordered in place without a barrier.  HELD beams at a time are in registers; in place all are.
+template <int N> struct Bytes;
+template <> struct Bytes<16> { typedef uint4 T; };
+template <> struct Bytes<8> { typedef uint2 T; };
+template <> struct Bytes<4> { typedef unsigned T; };
+template <> struct Bytes<2> { typedef unsigned short T; };
+template <> struct Bytes<1> { typedef unsigned char T; };
+template <typename V> __device__ __forceinline__ V zero_of() { V v; memset(&v, 0, sizeof(V)); return v; }
+
+constexpr int MOVE_THREADS = 128;
+template <int N, int HELD> __device__ __forceinline__ void move(const b2_state &s, const int *parent, long long group, int beams, long long groups, long long o, long long column) {
+    typedef typename Bytes<N>::T V;
+    const long long base = (o * groups + group) * beams * s.row_bytes + column * N;
+    const char *in = (const char *)s.data + base;
+    char *out = (char *)s.out + base;
+    const bool place = s.data == s.out;
+    for (int b0 = 0; b0 < beams; b0 += HELD) {
+        V v[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int b = b0 + i;
+            if (b >= beams) break;
+            const int p = parent[b];
+            v[i] = p < 0 || (place && p == b) ? zero_of<V>() : *reinterpret_cast<const V *>(in + p * s.row_bytes);
+        }
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int b = b0 + i;
+            if (b >= beams) break;
+            if (!(place && parent[b] == b)) *reinterpret_cast<V *>(out + b * s.row_bytes) = v[i];
+        }
+    }
+}
+// HELD: beams in registers; a block's threads have neighbouring columns of one sequence and one outer index
+template <int HELD> __global__ void __launch_bounds__(MOVE_THREADS) beam_reorder_kernel(const __grid_constant__ StateArgs a) {
+    __shared__ int parent[MAX_BEAMS];
+    int i = 0;
+    while (i + 1 < a.n && blockIdx.x >= a.first[i + 1]) ++i;
+    const b2_state &s = a.s[i];
+    unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & 15;
+    const int width = at == 0 ? 16 : (at & 7) == 0 ? 8 : (at & 3) == 0 ? 4 : (at & 1) == 0 ? 2 : 1;
+    const long long columns = s.row_bytes / width, chunks = (columns + MOVE_THREADS - 1) / MOVE_THREADS;
+    // blocks of a tensor: [outer][group][chunk]
+    const long long k = blockIdx.x - a.first[i];
+    const long long chunk = k % chunks, group = k / chunks % a.groups, o = k / chunks / a.groups;
+    if ((int)threadIdx.x < a.beams) {
+        const int p = a.parents[group * a.beams + threadIdx.x];
+        parent[threadIdx.x] = p >= 0 && p < a.beams ? p : -1;
+    }
+    __syncthreads();
+    const long long column = chunk * MOVE_THREADS + threadIdx.x;
+    if (column >= columns) return;
+    switch (width) {
+        case 16: return move<16, HELD>(s, parent, group, a.beams, a.groups, o, column);
+        case 8: return move<8, HELD>(s, parent, group, a.beams, a.groups, o, column);
+        case 4: return move<4, HELD>(s, parent, group, a.beams, a.groups, o, column);
+        case 2: return move<2, HELD>(s, parent, group, a.beams, a.groups, o, column);
+        default: return move<1, HELD>(s, parent, group, a.beams, a.groups, o, column);
+    }
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top) {
+    if (!sizes_fit(groups, beams, vocab, top)) return 0;
+    const size_t slices = (size_t)slices_of(vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
+    return slices * (sizeof(Part) + (size_t)top * sizeof(Key));
+}
+
+int b2_beam_select(const void *logits, int type, long long groups, int beams, int vocab, long long ld, const unsigned char *mask, long long ld_mask, float scale,
+                   const float *scores, const unsigned char *finished, const float *weights, int end_token, int top, float *top_scores, int *top_beams, int *top_tokens,
+                   void *workspace, size_t workspace_bytes, b2_stream stream) {
+    const int e = type_size(type);
+    if (!e) { set_error("b2_beam_select: unknown element type %d", type); return B2_ERR_BAD_ARG; }
+    if (!sizes_fit(groups, beams, vocab, top)) {
+        set_error("b2_beam_select: %lld sequences, %d beams (1 to %d), %d logits (at most 2^26), %d continuations (1 to %d)", groups, beams, MAX_BEAMS, vocab, top, MAX_BEST);
+        return B2_ERR_BAD_SHAPE;
+    }
+    if (ld < vocab || ld > MAX_LD || (mask && ((ld_mask != 0 && ld_mask < vocab) || ld_mask > MAX_LD))) {
+        set_error("b2_beam_select: leading dimension too small or beyond 2^40 (logits %lld, mask %lld for %d columns)", ld, ld_mask, vocab);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!(scale > 0.0f) || scale > 3.402823466e38f) { set_error("b2_beam_select: the scale %g is not a positive number", (double)scale); return B2_ERR_BAD_ARG; }
+    if (finished && (end_token < 0 || end_token >= vocab)) { set_error("b2_beam_select: end_token %d of %d", end_token, vocab); return B2_ERR_BAD_ARG; }
+    if (!groups) return B2_OK;
+    if (!logits || !aligned_to(logits, e)) { set_error("b2_beam_select: the logits are missing or not aligned to their elements"); return B2_ERR_BAD_ARG; }
+    if (!scores || !top_scores || !top_beams || !top_tokens || !workspace) { set_error("b2_beam_select: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(scores, 4) || !aligned_to(weights, 4) || !aligned_to(top_scores, 4) || !aligned_to(top_beams, 4) || !aligned_to(top_tokens, 4)) {
+        set_error("b2_beam_select: a vector of tokens or numbers is not aligned to 4 bytes");
+        return B2_ERR_BAD_ARG;
+    }
+    if (!aligned_to(workspace, 16)) { set_error("b2_beam_select: the workspace is not aligned to 16 bytes"); return B2_ERR_BAD_ARG; }
+    const size_t need = b2_beam_select_workspace(groups, beams, vocab, top);
+    if (workspace_bytes < need) { set_error("b2_beam_select: a workspace of %zu bytes, %zu are needed", workspace_bytes, need); return B2_ERR_BAD_SHAPE; }
+    SelectArgs a = {};
+    a.mask = mask; a.ld_mask = ld_mask; a.scores = scores; a.finished = finished; a.weights = weights;
+    a.groups = groups; a.ld = ld; a.beams = beams; a.vocab = vocab; a.top = top; a.end_token = end_token; a.scale = scale;
+    a.lists = (Key *)workspace;
+    a.parts = (Part *)(a.lists + (size_t)slices_of(vocab, type) * (size_t)groups * beams * top);
+    a.best = top_scores; a.from = top_beams; a.tokens = top_tokens;
+    return with_type(type, [&](auto *t) { return select((const B2_ELEM(t) *)logits, a, type, (cudaStream_t)stream); });
+}
+
+int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long groups, int beams, b2_stream stream) {
+    if (n < 0 || groups < 0 || groups > (1ll << 31) || beams < 1 || beams > MAX_BEAMS) {
+        set_error("b2_beam_reorder: %d tensors, %lld sequences of %d beams (1 to %d)", n, groups, beams, MAX_BEAMS);
+        return B2_ERR_BAD_SHAPE;
+    }
+    if (!n || !groups) return B2_OK;
+    if (!states || !parents || !aligned_to(parents, 4)) { set_error("b2_beam_reorder: null pointer, or parents that are not aligned to 4 bytes"); return B2_ERR_BAD_ARG; }
+    for (int i = 0; i < n; ++i) {
+        const b2_state &s = states[i];
+        if (s.outer < 0 || s.row_bytes < 0 || s.outer > MAX_LD || s.row_bytes > MAX_LD) { set_error("b2_beam_reorder: tensor %d: %lld x rows of %lld bytes", i, s.outer, s.row_bytes); return B2_ERR_BAD_SHAPE; }
+        const double bytes = (double)s.outer * (double)groups * beams * (double)s.row_bytes;
+        if (bytes > 1e15) { set_error("b2_beam_reorder: tensor %d: %lld x rows of %lld bytes", i, s.outer, s.row_bytes); return B2_ERR_BAD_SHAPE; }
+        if (!s.outer || !s.row_bytes) continue;
+        if (!s.data) { set_error("b2_beam_reorder: null pointer (tensor %d)", i); return B2_ERR_BAD_ARG; }
+        const char *p = (const char *)s.data, *q = (const char *)s.out, *end = p + (long long)bytes;
+        if (q && q != p && q < end && p < q + (long long)bytes) { set_error("b2_beam_reorder: tensor %d and its output overlap", i); return B2_ERR_BAD_ARG; }
+    }
+    int i = 0;
+    while (i < n) {
+        StateArgs a;
+        a.n = 0; a.beams = beams; a.groups = groups; a.parents = parents;
+        unsigned long long blocks = 0;
+        for (; i < n && a.n < MAX_STATES; ++i) {
+            b2_state s = states[i];
+            if (!s.outer || !s.row_bytes) continue;
+            if (!s.out) s.out = s.data;
+            const unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & 15;
+            const int width = at == 0 ? 16 : (at & 7) == 0 ? 8 : (at & 3) == 0 ? 4 : (at & 1) == 0 ? 2 : 1;
+            const double more = (double)s.outer * (double)groups * (double)((s.row_bytes / width + MOVE_THREADS - 1) / MOVE_THREADS);
+            if (more > 2147483647.0) { set_error("b2_beam_reorder: tensor %d is too large", i); return B2_ERR_BAD_SHAPE; }
+            if (blocks + (unsigned long long)more > 2147483647ull) break;
+            a.s[a.n] = s;
+            a.first[a.n++] = (unsigned)blocks;
+            blocks += (unsigned long long)more;
+        }
+        a.first[a.n] = (unsigned)blocks;
+        if (!blocks) continue;
+        const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, MOVE_THREADS, 0, (cudaStream_t)stream>>>(a); };
+        if (beams <= 4) go(beam_reorder_kernel<4>);
+        else if (beams <= 8) go(beam_reorder_kernel<8>);
+        else if (beams <= 16) go(beam_reorder_kernel<16>);
+        else go(beam_reorder_kernel<MAX_BEAMS>);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+    }
+    return B2_OK;
+}
+
+}  // extern "C"

@@ -13,7 +13,7 @@ namespace {
 
 PyObject *g_error = nullptr;      // b2lstm.B2Error
 PyObject *g_types = nullptr;      // dtype object -> code
-enum { INT32 = 16, BYTE = 17, OTHER = 18 };
+enum { INT32 = 16, BYTE = 17, INT8 = 18, OTHER = 19 };     // BYTE: uint8 and bool, and int8 where bytes are meant
 
 struct Api {
     decltype(&b2_last_error_string) last_error;
@@ -26,6 +26,12 @@ struct Api {
     decltype(&b2_logprob_backward) logprob_backward;
     decltype(&b2_gradient_norm) gradient_norm;
     decltype(&b2_gradient_clip) gradient_clip;
+    decltype(&b2_distill_forward) distill_forward;
+    decltype(&b2_distill_backward) distill_backward;
+    decltype(&b2_beam_select) beam_select;
+    decltype(&b2_beam_reorder) beam_reorder;
+    decltype(&b2_int8_quantize) int8_quantize;
+    decltype(&b2_int8_product) int8_product;
 } api;
 
 PyObject *s_shape, *s_stride, *s_dtype, *s_is_cuda, *s_get_device, *s_data_ptr, *s_numel, *s_is_contiguous;
@@ -59,7 +65,7 @@ int type_of(const Ref &dtype) {
     if (!s) return -1;
     const char *dot = strrchr(s, '.'), *name = dot ? dot + 1 : s;
     static const struct { const char *name; int code; } known_names[] = {{"float32", B2_F32}, {"bfloat16", B2_BF16}, {"float16", B2_F16}, {"int32", INT32},
-                                                                         {"uint8", BYTE}, {"int8", BYTE}, {"bool", BYTE}};
+                                                                         {"uint8", BYTE}, {"int8", INT8}, {"bool", BYTE}};
     int code = OTHER;
     for (const auto &k : known_names)
         if (!strcmp(name, k.name)) code = k.code;
@@ -94,6 +100,8 @@ bool address(PyObject *t, void **out) {
 }
 
 struct Matrix { void *p = nullptr; long long ld = 0, rows = 0, cols = 0; int type = OTHER; };
+// whether an element type is what is asked for: a code, or -1: fp32, bf16 or fp16
+bool fits(int type, int like) { return like < 0 ? type <= B2_F16 : type == like || (like == BYTE && type == INT8); }
 // rows, cols: what they have to be (-1: anything); like: the element type it has to have (-1: fp32, bf16 or fp16; BYTE)
 bool matrix(PyObject *t, const char *name, long long rows, long long cols, int like, Matrix &m) {
     m = Matrix();
@@ -109,7 +117,7 @@ bool matrix(PyObject *t, const char *name, long long rows, long long cols, int l
     Ref dtype(PyObject_GetAttr(t, s_dtype));
     m.type = type_of(dtype);
     if (m.type < 0) return false;
-    if (like < 0 ? m.type > B2_F16 : m.type != like) return refuse("%s has the element type %S", name, dtype.p);
+    if (!fits(m.type, like)) return refuse("%s has the element type %S", name, dtype.p);
     Ref stride(PyObject_CallMethodNoArgs(t, s_stride));
     if (!stride) return false;
     if (!PyTuple_Check(stride.p) || PyTuple_GET_SIZE(stride.p) != 2) return refuse("%s has the strides %S", name, stride.p);
@@ -128,7 +136,7 @@ bool vector(PyObject *t, const char *name, long long n, int like, void **out) {
     Ref dtype(PyObject_GetAttr(t, s_dtype));
     const int type = type_of(dtype);
     if (type < 0) return false;
-    if (type != like) return refuse("%s has the element type %S, not %s", name, dtype.p, like == B2_F32 ? "float32" : like == INT32 ? "int32" : "uint8, int8 or bool");
+    if (!fits(type, like)) return refuse("%s has the element type %S, not %s", name, dtype.p, like == B2_F32 ? "float32" : like == INT32 ? "int32" : "uint8, int8 or bool");
     Ref count(PyObject_CallMethodNoArgs(t, s_numel)), whole(PyObject_CallMethodNoArgs(t, s_is_contiguous));
     if (!count || !whole) return false;
     const long long have = PyLong_AsLongLong(count.p);
@@ -150,7 +158,7 @@ bool workspace(PyObject *t, void **p, size_t *bytes) {
     const int ok = PyObject_IsTrue(whole.p);
     if (PyErr_Occurred()) return false;
     if (!ok || type == OTHER) return refuse("the workspace is not a contiguous tensor of bytes");
-    *bytes = (size_t)n * (type == B2_F32 || type == INT32 ? 4 : type == BYTE ? 1 : 2);
+    *bytes = (size_t)n * (type == B2_F32 || type == INT32 ? 4 : type == BYTE || type == INT8 ? 1 : 2);
     return address(t, p);
 }
 bool number(PyObject *o, float *out) { const double v = PyFloat_AsDouble(o); *out = (float)v; return !(v == -1.0 && PyErr_Occurred()); }
@@ -347,6 +355,121 @@ PyObject *gradient_clip(PyObject *, PyObject *const *a, Py_ssize_t n) {
     CALL(api.gradient_clip(list, out, len, most, (float *)norm, ws, bytes, st));
 }
 
+// the columns of a list [rows, top] that is not None
+bool width_of(PyObject *t, const char *name, long long *out) {
+    Ref shape(PyObject_GetAttr(t, s_shape));
+    if (!shape) return false;
+    if (!PyTuple_Check(shape.p) || PyTuple_GET_SIZE(shape.p) != 2) return refuse("%s has the shape %S, not (rows, columns)", name, shape.p);
+    *out = PyLong_AsLongLong(PyTuple_GET_ITEM(shape.p, 1));
+    if (PyErr_Occurred()) return false;
+    if (*out > 1 << 20) *out = 1 << 20;
+    return true;
+}
+// logits, top_tokens, top_logprobs, loss, lse, lse_rest, scale, stream
+PyObject *distill_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Matrix x;
+    void *tokens, *lp, *loss, *lse, *rest;
+    long long top;
+    float scale;
+    b2_stream st;
+    if (!arguments(n, 8) || !matrix(a[0], "logits", -1, -1, -1, x)) return nullptr;
+    for (int i = 0; i < 5; ++i)
+        if (a[i] == Py_None) { refuse("null pointer: all but lse_rest are needed"); return nullptr; }
+    if (!width_of(a[1], "top_tokens", &top) || !vector(a[1], "top_tokens", x.rows * top, INT32, &tokens) || !vector(a[2], "top_logprobs", x.rows * top, B2_F32, &lp) ||
+        !vector(a[3], "loss", x.rows, B2_F32, &loss) || !vector(a[4], "lse", x.rows, B2_F32, &lse) || !vector(a[5], "lse_rest", x.rows, B2_F32, &rest) ||
+        !number(a[6], &scale) || !stream_of(a[7], &st))
+        return nullptr;
+    CALL(api.distill_forward(x.p, x.type, x.rows, (int)x.cols, x.ld, scale, (const int *)tokens, (const float *)lp, (int)top, (float *)loss, (float *)lse, (float *)rest, st));
+}
+// dlogits, logits, top_tokens, top_logprobs, lse, lse_rest, dloss, scale, accumulate, stream
+PyObject *distill_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Matrix d, x;
+    void *tokens, *lp, *lse, *rest, *g;
+    long long top;
+    float scale;
+    int add;
+    b2_stream st;
+    if (!arguments(n, 10) || !matrix(a[1], "logits", -1, -1, -1, x)) return nullptr;
+    for (int i = 0; i < 7; ++i)
+        if (i != 5 && a[i] == Py_None) { refuse("null pointer: all but lse_rest are needed"); return nullptr; }
+    if (!matrix(a[0], "dlogits", x.rows, x.cols, x.type, d) || !width_of(a[2], "top_tokens", &top) || !vector(a[2], "top_tokens", x.rows * top, INT32, &tokens) ||
+        !vector(a[3], "top_logprobs", x.rows * top, B2_F32, &lp) || !vector(a[4], "lse", x.rows, B2_F32, &lse) || !vector(a[5], "lse_rest", x.rows, B2_F32, &rest) ||
+        !vector(a[6], "dloss", x.rows, B2_F32, &g) || !number(a[7], &scale) || !flag(a[8], &add) || !stream_of(a[9], &st))
+        return nullptr;
+    CALL(api.distill_backward(d.p, d.ld, x.p, x.type, x.rows, (int)x.cols, x.ld, scale, (const int *)tokens, (const float *)lp, (int)top, (const float *)lse,
+                              (const float *)rest, (const float *)g, add, st));
+}
+// logits, scores, top_scores, top_beams, top_tokens, finished, weights, end_token, mask, scale, workspace, stream
+PyObject *beam_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Matrix x, mask;
+    void *scores, *best, *from, *tokens, *finished, *weights, *ws;
+    size_t bytes;
+    long long top, groups;
+    float scale;
+    b2_stream st;
+    if (!arguments(n, 12) || !matrix(a[0], "logits", -1, -1, -1, x)) return nullptr;
+    for (int i = 0; i < 5; ++i)
+        if (a[i] == Py_None) { refuse("null pointer: logits, scores and results are needed"); return nullptr; }
+    if (!width_of(a[2], "top_scores", &top) || !count_of(a[2], "top_scores", &groups)) return nullptr;
+    groups = top > 0 ? groups / top : 0;
+    if (groups < 1 ? x.rows > 0 : x.rows % groups != 0) { refuse("%lld rows of logits for %lld sequences", x.rows, groups); return nullptr; }
+    const long long beams = groups ? x.rows / groups : 1;
+    const long end = PyLong_AsLong(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (beams > 1 << 20 || end != (int)end) { refuse("%lld beams a sequence, end_token %ld", beams, end); return nullptr; }
+    if (!mask_of(a[8], x.rows, x.cols, mask) || !vector(a[1], "scores", x.rows, B2_F32, &scores) || !vector(a[2], "top_scores", groups * top, B2_F32, &best) ||
+        !vector(a[3], "top_beams", groups * top, INT32, &from) || !vector(a[4], "top_tokens", groups * top, INT32, &tokens) ||
+        !vector(a[5], "finished", x.rows, BYTE, &finished) || !vector(a[6], "weights", x.rows, B2_F32, &weights) || !number(a[9], &scale) ||
+        !workspace(a[10], &ws, &bytes) || !stream_of(a[11], &st))
+        return nullptr;
+    CALL(api.beam_select(x.p, x.type, groups, (int)beams, (int)x.cols, x.ld, (const unsigned char *)mask.p, mask.ld, scale, (const float *)scores,
+                         (const unsigned char *)finished, (const float *)weights, (int)end, (int)top, (float *)best, (int *)from, (int *)tokens, ws, bytes, st));
+}
+// address of the list, its length, its device, its beams (-1: an empty list), parents, stream
+PyObject *beam_reorder(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    void *parents;
+    long long count, beams;
+    b2_stream st;
+    if (!arguments(n, 6)) return nullptr;
+    const b2_state *list = (const b2_state *)PyLong_AsVoidPtr(a[0]);
+    const int len = (int)PyLong_AsLong(a[1]);
+    const long long rows = PyLong_AsLongLong(a[3]);
+    if (PyErr_Occurred() || !list_on_gpu(a[2]) || !width_of(a[4], "parents", &beams) || !count_of(a[4], "parents", &count) ||
+        !vector(a[4], "parents", count, INT32, &parents) || !stream_of(a[5], &st))
+        return nullptr;
+    if (rows >= 0 && count != rows) { refuse("%lld parents for %lld beams", count, rows); return nullptr; }
+    CALL(api.beam_reorder(list, len, (const int *)parents, beams > 0 ? count / beams : 0, (int)beams, st));
+}
+// q, scales, x, stream
+PyObject *int8_quantize(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Matrix q, x;
+    void *scales;
+    b2_stream st;
+    if (!arguments(n, 4)) return nullptr;
+    for (int i = 0; i < 3; ++i)
+        if (a[i] == Py_None) { refuse("null pointer: q, scales and x are needed"); return nullptr; }
+    if (!matrix(a[2], "x", -1, -1, -1, x) || !matrix(a[0], "q", x.rows, x.cols, INT8, q) || !vector(a[1], "scales", x.rows, B2_F32, &scales) || !stream_of(a[3], &st)) return nullptr;
+    CALL(api.int8_quantize((signed char *)q.p, q.ld, (float *)scales, x.p, x.type, x.rows, (int)x.cols, x.ld, st));
+}
+// out, x, x_scales, w, w_scales, bias, workspace, stream
+PyObject *int8_product(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Matrix out, x, w;
+    void *xs, *wsc, *bias, *ws;
+    size_t bytes;
+    b2_stream st;
+    if (!arguments(n, 8)) return nullptr;
+    for (int i = 0; i < 5; ++i)
+        if (i != 2 && a[i] == Py_None) { refuse("null pointer: out, x, w and w_scales are needed"); return nullptr; }
+    const bool given = a[2] != Py_None;
+    if (!matrix(a[3], "w", -1, -1, INT8, w)) return nullptr;
+    if (w.rows > 0x7fffffff) { refuse("w has %lld channels", w.rows); return nullptr; }
+    if (!matrix(a[1], "x", -1, w.cols, given ? INT8 : -1, x) || !matrix(a[0], "out", x.rows, w.rows, -1, out) || !vector(a[2], "x_scales", x.rows, B2_F32, &xs) ||
+        !vector(a[4], "w_scales", w.rows, B2_F32, &wsc) || !vector(a[5], "bias", w.rows, B2_F32, &bias) || !workspace(a[6], &ws, &bytes) || !stream_of(a[7], &st))
+        return nullptr;
+    CALL(api.int8_product(out.p, out.type, out.ld, x.p, given ? (int)B2_I8 : x.type, x.ld, (const float *)xs, (const signed char *)w.p, w.ld, (const float *)wsc,
+                          (const float *)bias, x.rows, (int)w.rows, (int)w.cols, ws, bytes, st));
+}
+
 // bind({name: address}, B2Error)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 2) { refuse("%zd arguments instead of 2", n); return nullptr; }
@@ -354,7 +477,9 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
         {"b2_last_error_string", (void **)&api.last_error}, {"b2_current_device", (void **)&api.current_device}, {"b2_embedding_forward", (void **)&api.embedding_forward},
         {"b2_embedding_backward", (void **)&api.embedding_backward}, {"b2_block_norm_forward", (void **)&api.block_norm_forward},
         {"b2_block_norm_backward", (void **)&api.block_norm_backward}, {"b2_logprob_forward", (void **)&api.logprob_forward},
-        {"b2_logprob_backward", (void **)&api.logprob_backward}, {"b2_gradient_norm", (void **)&api.gradient_norm}, {"b2_gradient_clip", (void **)&api.gradient_clip}};
+        {"b2_logprob_backward", (void **)&api.logprob_backward}, {"b2_gradient_norm", (void **)&api.gradient_norm}, {"b2_gradient_clip", (void **)&api.gradient_clip},
+        {"b2_distill_forward", (void **)&api.distill_forward}, {"b2_distill_backward", (void **)&api.distill_backward}, {"b2_beam_select", (void **)&api.beam_select},
+        {"b2_beam_reorder", (void **)&api.beam_reorder}, {"b2_int8_quantize", (void **)&api.int8_quantize}, {"b2_int8_product", (void **)&api.int8_product}};
     for (const auto &f : all) {
         PyObject *p = PyDict_GetItemString(a[0], f.name);
         if (!p) { refuse("%s is missing", f.name); return nullptr; }
@@ -369,7 +494,8 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(embedding_forward), METHOD(embedding_backward), METHOD(block_norm_forward), METHOD(block_norm_backward),
-                         METHOD(logprob_forward), METHOD(logprob_backward), METHOD(gradient_norm), METHOD(gradient_clip), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(logprob_forward), METHOD(logprob_backward), METHOD(gradient_norm), METHOD(gradient_clip),
+                         METHOD(distill_forward), METHOD(distill_backward), METHOD(beam_select), METHOD(beam_reorder), METHOD(int8_quantize), METHOD(int8_product), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", "tensor side of the token operators' binding", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

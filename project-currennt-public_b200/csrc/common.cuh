@@ -104,6 +104,8 @@ int gemm_tc(float *C, long ldc, const SplitOperand &A, const SplitOperand &B, in
 // (contiguous index, other index) coordinates and writes split z to C + c_off + z*c_split_stride.
 struct TcBatch { int a_in, a_out, b_in, b_out; long long c_off; };
 struct TcPlan;
+// tensor map over rows of bytes (`inner` of them, rows ld bytes apart), boxes of one 128-byte swizzle row x box_rows; outside: zeros (gemm_tc.cu)
+int make_byte_map(struct CUtensorMap_st *map, const void *base, long long inner, long long outer, long long ld, int box_rows);
 int tc_plan_create(TcPlan **out, const SplitOperand &A, long a_inner, long a_outer, const SplitOperand &B, long b_inner,
                    long b_outer, int m, int n, int k, int splits, int kseg_len, int kseg_stride, long ldc);
 int tc_plan_launch(const TcPlan *p, float *C, const TcBatch *batches, int nbatch, long long c_split_stride, int *status,

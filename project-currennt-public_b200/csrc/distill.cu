@@ -1,0 +1,520 @@
+// Divergence of rows of logits from a teacher that is known by its K most likely tokens i_k and their log probabilities t_k, and its gradient.
+//
+//   z = s * x,  lse = log sum_j e^z_j,  p = e^(z - lse)
+//   without a rest:  q = e^t / sum e^t                          L = sum_k q_k (log q_k - log p_k)
+//   with a rest:     q = e^t, q_r = 1 - sum q, p_r = sum of p off the list      L = sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r)
+//   dL/dx_j = s (p_j - q_k) at i_k, s (p_j - q_r e^(z_j - lse_r)) = s e^(z_j - lse_r) (p_r - q_r) elsewhere (without a rest s p_j)
+//
+// Forward: p_r is a sum of its own, over the tokens that are not listed.  As 1 - sum p_k it would lose all its digits where the listed tokens hold most
+// of the mass, which is what a good student does.  A row passes through shared memory in pieces of 2 KB that each warp copies ahead for itself; a lane holds
+// up to four places of the list, and when a piece is there the lanes whose tokens lie in it take their logits out and leave -inf behind.  So the sum over the
+// rest needs no test at any entry, and nothing is read twice.
+// Backward: one read, one write; a block prepares the list while its logits are on the way, writes the gradient of unlisted tokens everywhere, and then
+// that of the listed ones over it.  Only one exponential an entry: the rest's probabilities given that it is the rest, times the row's factor p_r - q_r.
+#include <math.h>
+
+#include "logits.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int MAX_LIST = 128;
+constexpr float LEAST_REST = 9.5367431640625e-7f;      // 2^-20
+
+// The places of a row's list that a lane holds: place s * 32 + lane.  tok -1: empty, or listed further ahead
+template <int SLOTS> struct List {
+    int tok[SLOTS];
+    float lp[SLOTS];
+    __device__ __forceinline__ void load(const int *tokens, const float *lps, long long r, int top) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int k = s * 32 + lane;
+            tok[s] = k < top ? tokens[r * top + k] : -1;
+            lp[s] = k < top ? lps[r * top + k] : neg_inf();
+        }
+    }
+    // empties the places whose token is negative or stands further ahead; true where a token is not below vocab or a log probability is NaN or +inf
+    __device__ __forceinline__ bool settle(int vocab) {
+        const int lane = threadIdx.x & 31;
+        bool wrong = false, twice[SLOTS];
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            twice[s] = (__ffs(__match_any_sync(FULL, tok[s])) - 1) != lane;
+#pragma unroll
+            for (int e = 0; e < s; ++e)
+#pragma unroll 8
+                for (int i = 0; i < 32; ++i) twice[s] |= __shfl_sync(FULL, tok[e], i) == tok[s];
+        }
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            if (twice[s]) tok[s] = -1;
+            if (tok[s] < 0) { tok[s] = -1; lp[s] = neg_inf(); }
+            else if (tok[s] >= vocab || !(lp[s] < __int_as_float(0x7f800000))) wrong = true;
+        }
+        return __any_sync(FULL, wrong);
+    }
+    __device__ __forceinline__ bool any() const {
+        bool one = false;
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) one |= tok[s] >= 0;
+        return __any_sync(FULL, one);
+    }
+};
+// The teacher's probabilities (q of the lane's places, the rest's, what log q is less than lp); false: the row says nothing
+template <int SLOTS, bool REST> __device__ __forceinline__ bool teacher(const List<SLOTS> &list, float (&q)[SLOTS], float &rest, float &minus) {
+    float most = neg_inf(), sum = 0.0f;
+    rest = minus = 0.0f;
+    if (!REST) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) most = fmaxf(most, list.lp[s]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, o));
+        if (most == neg_inf()) {
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) q[s] = 0.0f;
+            return false;
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) sum += q[s] = expf(REST ? list.lp[s] : list.lp[s] - most);
+    sum = warp_sum(sum);
+    if (REST) {
+        rest = 1.0f - sum;
+        if (rest < LEAST_REST) rest = 0.0f;
+        return list.any();
+    }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) q[s] *= inv;
+    minus = most + logf(sum);
+    return true;
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------------
+struct Sum { float m, s; };      // largest z, sum of e^(z - m)
+__device__ __forceinline__ void rise(Sum &a, float m) {
+    if (a.m != neg_inf()) {
+        const float r = ex2((a.m - m) * LOG2E);
+        a.s = r == 0.0f ? 0.0f : r * a.s;
+    }
+    a.m = m;
+}
+__device__ __forceinline__ Sum join(Sum a, Sum b) {
+    const float m = max_nan(a.m, b.m);
+    if (m == neg_inf()) return a;
+    if (b.m != neg_inf()) rise(b, m); else b.s = 0.0f;
+    rise(a, m);
+    return {m, a.s + b.s};
+}
+__device__ __forceinline__ Sum warp_join(Sum a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = join(a, {__shfl_xor_sync(FULL, a.m, o), __shfl_xor_sync(FULL, a.s, o)});
+    return a;
+}
+template <typename T, int U> __device__ __forceinline__ void add_vectors(Sum &a, const uint4 (&q)[U], float scale) {
+    constexpr int W = 16 / sizeof(T);
+    unsigned big = larger_of<T>(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) big = Raw<T>::larger(big, larger_of<T>(q[u]));
+    const float m = __fmul_rn(Raw<T>::largest(big), scale);
+    if (!(m <= a.m)) rise(a, m);
+    if (a.m == neg_inf()) return;
+    const Pair l2 = pair(LOG2E, LOG2E);
+    Pair s = 0;
+    less_of(scale, a.m, [&](const auto &less) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[W];
+            Raw<T>::values(x, q[u]);
+#pragma unroll
+            for (int j = 0; j < W; j += 2) {
+                const float2 t = halves(mul2(less(x[j], x[j + 1]), l2));
+                s = add2(s, pair(ex2(t.x), ex2(t.y)));
+            }
+        }
+    });
+    const float2 v = halves(s);
+    a.s += v.x + v.y;
+}
+
+struct FwdArgs {
+    const int *tokens; const float *lps;
+    float *loss, *lse, *lse_rest;
+    long long rows, ld;
+    int vocab, top;
+    float scale;
+};
+constexpr int PIECE = 128, RING = 3;      // vectors of 16 bytes in a piece (4 a lane), pieces in a warp's ring
+
+// A row's place among the 16-byte boundaries: `head` entries before the first one, nv vectors, the rest behind
+struct Row {
+    int head, nv, pieces;
+    template <typename T> __device__ __forceinline__ Row(const T *x, int vocab) {
+        constexpr int W = 16 / sizeof(T);
+        head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);
+        if (head > vocab) head = vocab;
+        nv = (vocab - head) / W;
+        pieces = (nv + PIECE - 1) / PIECE;
+    }
+};
+
+// WARPS warps a row (1: a block has 8 rows under way), each with the row's pieces w, w + WARPS, ...
+template <typename T, int WARPS, int SLOTS, bool REST>
+__global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, const FwdArgs a) {
+    constexpr int W = 16 / sizeof(T);
+    extern __shared__ uint4 rings[];
+    uint4 (*ring)[PIECE] = reinterpret_cast<uint4 (*)[PIECE]>(rings) + (threadIdx.x >> 5) * RING;
+    __shared__ float edges[8][32], picked[WARPS > 1 ? MAX_LIST : 1];
+    __shared__ Sum sums[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = WARPS > 1 ? warp : 0;
+    const long long team = WARPS > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + warp, teams = WARPS > 1 ? gridDim.x : (long long)gridDim.x * 8;
+
+    // what is copied next: piece ic of row ir
+    long long ir = team;
+    int ic = w, slot = 0;
+    const auto issue = [&](int to) {
+        while (ir < a.rows) {
+            const T *x = logits + ir * a.ld;
+            const Row g(x, a.vocab);
+            if (ic < g.pieces) {
+                const int n = min(PIECE, g.nv - ic * PIECE);
+                const uint4 *from = reinterpret_cast<const uint4 *>(x + g.head) + ic * PIECE;
+                const unsigned at = (unsigned)__cvta_generic_to_shared(&ring[to][0]);
+#pragma unroll
+                for (int u = 0; u < PIECE / 32; ++u)
+                    if (lane + 32 * u < n) cp_async<16>(at + 16 * (lane + 32 * u), from + lane + 32 * u);
+                ic += WARPS;
+                break;
+            }
+            ic = w;
+            ir += teams;
+        }
+        cp_commit();
+    };
+    List<SLOTS> list, next;
+    float edge = 0.0f;
+    const auto ahead = [&](long long r) {
+        if (r >= a.rows) return;
+        next.load(a.tokens, a.lps, r, a.top);
+        const T *x = logits + r * a.ld;
+        const Row g(x, a.vocab);
+        const int behind = a.vocab - g.head - g.nv * W;
+        edge = w == 0 && lane < g.head + behind ? to_float(x[lane < g.head ? lane : lane + g.nv * W]) : neg_inf();
+    };
+    for (int i = 0; i < RING - 1; ++i) issue(i);
+    ahead(team);
+    for (long long r = team; r < a.rows; r += teams) {
+        const T *x = logits + r * a.ld;
+        const Row g(x, a.vocab);
+        list = next;
+        float z_edge = edge;
+        ahead(r + teams);
+        const bool wrong = list.settle(a.vocab);
+        float z[SLOTS];
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) z[s] = neg_inf();
+        Sum t = {neg_inf(), 0.0f};
+        if (w == 0) {
+            // the entries outside the vectors
+            edges[warp][lane] = z_edge;
+            __syncwarp();
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) {
+                const int at = list.tok[s] < g.head ? list.tok[s] : list.tok[s] >= g.head + g.nv * W ? list.tok[s] - g.nv * W : -1;
+                if (at >= 0 && at < 32 && list.tok[s] < a.vocab) {
+                    z[s] = __fmul_rn(edges[warp][at], a.scale);
+                    if (REST) edges[warp][at] = neg_inf();
+                }
+            }
+            __syncwarp();
+            z_edge = edges[warp][lane];
+            __syncwarp();
+            if (!(z_edge <= neg_inf())) t = {__fmul_rn(z_edge, a.scale), 1.0f};
+            // +inf as e^(inf - inf)
+            if (t.m == __int_as_float(0x7f800000)) t.m = t.s = nanf("");
+        }
+        for (int c = w; c < g.pieces; c += WARPS) {
+            cp_wait<RING - 2>();
+            __syncwarp();
+            issue((slot + RING - 1) % RING);
+            T *piece = reinterpret_cast<T *>(&ring[slot][0]);
+            const int first = g.head + c * PIECE * W, n = min(PIECE, g.nv - c * PIECE);
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+                if ((unsigned)(list.tok[s] - first) < (unsigned)(n * W)) {
+                    z[s] = __fmul_rn(to_float(piece[list.tok[s] - first]), a.scale);
+                    if (REST) piece[list.tok[s] - first] = from_float<T>(neg_inf());
+                }
+            if (REST) __syncwarp();
+            uint4 q[PIECE / 32];
+#pragma unroll
+            for (int u = 0; u < PIECE / 32; ++u)
+                q[u] = lane + 32 * u < n ? ring[slot][lane + 32 * u] : make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+            __syncwarp();
+            add_vectors<T, PIECE / 32>(t, q, a.scale);
+            slot = (slot + 1) % RING;
+        }
+        t = warp_join(t);
+        if (WARPS > 1) {
+            if (lane == 0) sums[warp] = t;
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+                if (list.tok[s] >= 0 && list.tok[s] < a.vocab) {
+                    const int at = list.tok[s];
+                    const bool outside = at < g.head || at >= g.head + g.nv * W;
+                    if (outside ? w == 0 : (at - g.head) / (PIECE * W) % WARPS == w) picked[s * 32 + lane] = z[s];
+                }
+            __syncthreads();
+            if (w == 0) {
+                t = warp_join(lane < WARPS ? sums[lane] : Sum{neg_inf(), 0.0f});
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+                    if (list.tok[s] >= 0 && list.tok[s] < a.vocab) z[s] = picked[s * 32 + lane];
+            }
+            __syncthreads();
+            if (w != 0) continue;
+        }
+        // the row's results
+        float q[SLOTS], q_rest, minus;
+        const bool known = teacher<SLOTS, REST>(list, q, q_rest, minus);
+        Sum all = t;
+        if (REST) {
+            Sum mine = {neg_inf(), 0.0f};
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+                if (!(z[s] <= neg_inf())) mine = join(mine, z[s] == __int_as_float(0x7f800000) ? Sum{nanf(""), 1.0f} : Sum{z[s], 1.0f});
+            all = join(t, warp_join(mine));
+        }
+        const float log_all = logf(all.s), log_rest = logf(t.s);
+        float part = 0.0f;
+        const float inf = __int_as_float(0x7f800000);
+        if (all.m != neg_inf()) {
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+                if (q[s] > 0.0f) part += q[s] * ((list.lp[s] - minus) - ((z[s] - all.m) - log_all));
+        } else {
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+                if (q[s] > 0.0f) part = inf;
+        }
+        part = warp_sum(part);
+        if (lane == 0) {
+            const float lse = all.m == neg_inf() ? neg_inf() : all.m + log_all;
+            if (REST && q_rest > 0.0f) part += t.m == neg_inf() ? inf : q_rest * (logf(q_rest) - (((t.m - all.m) + log_rest) - log_all));
+            a.loss[r] = wrong || (known && lse != lse) ? nanf("") : known ? part : 0.0f;
+            a.lse[r] = lse;
+            if (REST) a.lse_rest[r] = t.m == neg_inf() ? neg_inf() : t.m + log_rest;
+        }
+    }
+    cp_wait<0>();
+}
+
+template <typename T, int WARPS, int SLOTS> int launch_forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    const long long teams = WARPS > 1 ? a.rows : (a.rows + 7) / 8, most = 3ll * sm_count();      // what runs at a time
+    const unsigned blocks = (unsigned)(teams < most ? teams : most);
+    constexpr int BYTES = 8 * RING * PIECE * 16;
+    const auto go = [&](auto kernel) -> int {
+        B2_TRY(set_max_dynamic_smem((const void *)kernel, BYTES));
+        kernel<<<blocks, 256, BYTES, st>>>(logits, a);
+        return B2_OK;
+    };
+    if (a.lse_rest) B2_TRY(go(distill_forward_kernel<T, WARPS, SLOTS, true>)); else B2_TRY(go(distill_forward_kernel<T, WARPS, SLOTS, false>));
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
+template <typename T, int WARPS> int forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    if (a.top <= 32) return launch_forward<T, WARPS, 1>(logits, a, st);
+    if (a.top <= 64) return launch_forward<T, WARPS, 2>(logits, a, st);
+    return launch_forward<T, WARPS, 4>(logits, a, st);
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------------------------
+struct BwdArgs {
+    const int *tokens; const float *lps;
+    const float *lse, *lse_rest, *dloss;
+    long long rows, ld, ld_out;
+    int vocab, top;
+    float scale;
+};
+struct RowGrad { float base, factor; int what; };      // what: 0 zeros, 1 gradient, 2 NaN
+
+// TEAM threads a row (32: a warp; 256: a block, several of them for a long row), each up to U vectors apart by TEAM
+template <typename T, int TEAM, int U, int SLOTS, bool REST, bool ADD>
+__global__ void __launch_bounds__(256) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
+    constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
+    __shared__ RowGrad shared[TEAMS];
+    const int lane = threadIdx.x & 31, team = threadIdx.x / TEAM, at = threadIdx.x % TEAM;
+    const long long r = TEAM == 256 ? (long long)(blockIdx.x / (unsigned)segs) : (long long)blockIdx.x * TEAMS + team;
+    const int seg = TEAM == 256 ? (int)(blockIdx.x % (unsigned)segs) : 0;
+    if (r >= a.rows) return;                                   // TEAM 256: the block as a whole
+    const T *x = logits + r * a.ld;
+    T *d = dlogits + r * a.ld_out;
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const bool out_vec = (((uintptr_t)(d - mis)) & 15) == 0;
+    const int first = seg * TEAM * U + at;
+    // the entries of this block
+    const int lo = max(0, seg * TEAM * U * W - mis), hi = TEAM == 256 ? min(a.vocab, (seg + 1) * TEAM * U * W - mis) : a.vocab;
+    const auto whole = [&](int v) { return v * W >= mis && (v + 1) * W <= mis + a.vocab; };
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (whole(first + u * TEAM)) raw[u] = *reinterpret_cast<const uint4 *>(x - mis + (size_t)(first + u * TEAM) * W);
+
+    List<SLOTS> list;
+    float own[SLOTS];
+    RowGrad g = {0.0f, 0.0f, 0};
+    if (at < 32) {
+        list.load(a.tokens, a.lps, r, a.top);
+        const float lse = a.lse[r], rest = REST ? a.lse_rest[r] : 0.0f, weight = a.dloss[r] * a.scale;
+        float z[SLOTS], old[SLOTS];
+        const bool wrong = list.settle(a.vocab);
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const bool here = list.tok[s] >= lo && list.tok[s] < hi;
+            z[s] = here ? __fmul_rn(to_float(x[list.tok[s]]), a.scale) : 0.0f;
+            old[s] = ADD && here ? to_float(d[list.tok[s]]) : 0.0f;
+        }
+        float q[SLOTS], q_rest, minus;
+        const bool known = teacher<SLOTS, REST>(list, q, q_rest, minus);
+        if (wrong) g.what = 2;
+        else if (known && lse != neg_inf()) g.what = 1;
+        // e^(z - base) * factor off the list; where the rest has no mass all of its logits are -inf
+        const bool split = REST && rest != neg_inf();
+        g.base = split ? rest : lse;
+        g.factor = weight * (split ? expf(rest - lse) - q_rest : 1.0f);
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) own[s] = old[s] + weight * (expf(z[s] - lse) - q[s]);
+        if (lane == 0) shared[team] = g;
+    }
+    if (TEAM == 256) __syncthreads(); else __syncwarp();
+    g = shared[team];
+    if (g.what == 0 && ADD) return;
+    const float none = g.what == 2 ? nanf("") : 0.0f;
+    const Pair factor = pair(g.factor, g.factor);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = first + u * TEAM, i0 = v * W - mis;
+        if (i0 >= a.vocab) break;
+        const bool inside = whole(v);
+        float z[W], o[W], old[W];
+        if (inside) Raw<T>::values(z, raw[u]);
+        else
+#pragma unroll
+            for (int j = 0; j < W; ++j) z[j] = i0 + j >= 0 && i0 + j < a.vocab ? to_float(x[i0 + j]) : 0.0f;
+        if (ADD) {
+            if (inside && out_vec) load_vec<T, W>(old, d + i0);
+            else
+#pragma unroll
+                for (int j = 0; j < W; ++j) old[j] = i0 + j >= 0 && i0 + j < a.vocab ? to_float(d[i0 + j]) : 0.0f;
+        }
+        if (g.what == 1) {
+            less_of(a.scale, g.base, [&](const auto &less) {
+#pragma unroll
+                for (int j = 0; j < W; j += 2) {
+                    const float2 t = halves(mul2(exp_pair<T>(less(z[j], z[j + 1])), factor));
+                    o[j] = ADD ? old[j] + t.x : t.x;
+                    o[j + 1] = ADD ? old[j + 1] + t.y : t.y;
+                }
+            });
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) o[j] = none;
+        }
+        if (inside && out_vec) store_vec<T, W>(d + i0, o);
+        else
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (i0 + j >= 0 && i0 + j < a.vocab) d[i0 + j] = from_float<T>(o[j]);
+    }
+    if (g.what != 1) return;
+    if (TEAM == 256) __syncthreads(); else __syncwarp();
+    if (at < 32)
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (list.tok[s] >= lo && list.tok[s] < hi) d[list.tok[s]] = from_float<T>(own[s]);
+}
+
+template <typename T, int TEAM, int U, int SLOTS> int launch_backward(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    const int vecs = (a.vocab + W - 1) / W + 1;               // one more: a row may start inside a vector
+    const int segs = TEAM == 256 ? (vecs + TEAM * U - 1) / (TEAM * U) : 1;
+    const long long blocks = TEAM == 256 ? a.rows * segs : (a.rows + 7) / 8;
+    if (blocks > 0x7fffffffll) { set_error("b2_distill_backward: %lld rows of %d", a.rows, a.vocab); return B2_ERR_BAD_SHAPE; }
+    const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, st>>>(dlogits, logits, a, segs); };
+    if (a.lse_rest) { if (add) go(distill_backward_kernel<T, TEAM, U, SLOTS, true, true>); else go(distill_backward_kernel<T, TEAM, U, SLOTS, true, false>); }
+    else { if (add) go(distill_backward_kernel<T, TEAM, U, SLOTS, false, true>); else go(distill_backward_kernel<T, TEAM, U, SLOTS, false, false>); }
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
+template <typename T, int TEAM, int U> int backward_of(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
+    if (a.top <= 32) return launch_backward<T, TEAM, U, 1>(dlogits, logits, a, add, st);
+    if (a.top <= 64) return launch_backward<T, TEAM, U, 2>(dlogits, logits, a, add, st);
+    return launch_backward<T, TEAM, U, 4>(dlogits, logits, a, add, st);
+}
+template <typename T> int backward(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    const int vecs = (a.vocab + W - 1) / W + 1;
+    if (vecs <= 32 * 4) return backward_of<T, 32, 4>(dlogits, logits, a, add, st);
+    if ((double)a.rows * vecs < 4096.0 * sm_count()) return backward_of<T, 256, 2>(dlogits, logits, a, add, st);
+    return backward_of<T, 256, 8>(dlogits, logits, a, add, st);
+}
+
+int check(const char *who, const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *tokens, const float *lps, int top) {
+    const int e = type_size(type);
+    if (!e) { set_error("%s: unknown element type %d", who, type); return B2_ERR_BAD_ARG; }
+    if (rows < 0 || vocab < 1 || vocab > (1 << 27)) { set_error("%s: %lld rows of %d logits (at most 2^27)", who, rows, vocab); return B2_ERR_BAD_SHAPE; }
+    if (top < 1 || top > MAX_LIST) { set_error("%s: %d listed tokens (1 to %d)", who, top, MAX_LIST); return B2_ERR_BAD_SHAPE; }
+    if (ld < vocab || ld > MAX_LD) { set_error("%s: leading dimension %lld too small or beyond 2^40 (%d columns)", who, ld, vocab); return B2_ERR_BAD_ARG; }
+    if (!(scale > 0.0f) || scale > 3.402823466e38f) { set_error("%s: the scale %g is not a positive number", who, (double)scale); return B2_ERR_BAD_ARG; }
+    if (rows && (!logits || !aligned_to(logits, e))) { set_error("%s: the logits are missing or not aligned to their elements", who); return B2_ERR_BAD_ARG; }
+    if (rows && (!tokens || !lps || !aligned_to(tokens, 4) || !aligned_to(lps, 4))) {
+        set_error("%s: the teacher's tokens or log probabilities are missing or not aligned to 4 bytes", who);
+        return B2_ERR_BAD_ARG;
+    }
+    return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_distill_forward(const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *top_tokens, const float *top_logprobs, int top,
+                       float *loss, float *lse, float *lse_rest, b2_stream stream) {
+    B2_TRY(check("b2_distill_forward", logits, type, rows, vocab, ld, scale, top_tokens, top_logprobs, top));
+    if (!rows) return B2_OK;
+    if (!loss || !lse) { set_error("b2_distill_forward: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(loss, 4) || !aligned_to(lse, 4) || !aligned_to(lse_rest, 4)) { set_error("b2_distill_forward: a vector of numbers is not aligned to 4 bytes"); return B2_ERR_BAD_ARG; }
+    const FwdArgs a = {top_tokens, top_logprobs, loss, lse, lse_rest, rows, ld, vocab, top, scale};
+    return with_type(type, [&](auto *t) {
+        typedef B2_ELEM(t) T;
+        const T *x = (const T *)logits;
+        return a.rows >= 16 * sm_count() || a.vocab <= 2048 ? forward<T, 1>(x, a, (cudaStream_t)stream) : forward<T, 8>(x, a, (cudaStream_t)stream);
+    });
+}
+
+int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *top_tokens,
+                        const float *top_logprobs, int top, const float *lse, const float *lse_rest, const float *dloss, int accumulate, b2_stream stream) {
+    B2_TRY(check("b2_distill_backward", logits, type, rows, vocab, ld, scale, top_tokens, top_logprobs, top));
+    if (ld_dlogits < vocab || ld_dlogits > MAX_LD) {
+        set_error("b2_distill_backward: leading dimension %lld of the gradient too small or beyond 2^40 (%d columns)", ld_dlogits, vocab);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!rows) return B2_OK;
+    if (!dlogits || !aligned_to(dlogits, type_size(type))) { set_error("b2_distill_backward: the gradient is missing or not aligned to its elements"); return B2_ERR_BAD_ARG; }
+    if (!lse || !dloss) { set_error("b2_distill_backward: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(lse, 4) || !aligned_to(lse_rest, 4) || !aligned_to(dloss, 4)) { set_error("b2_distill_backward: a vector of numbers is not aligned to 4 bytes"); return B2_ERR_BAD_ARG; }
+    if (dlogits == logits && (ld_dlogits != ld || accumulate)) { set_error("b2_distill_backward: in place with another leading dimension, or added to the logits"); return B2_ERR_BAD_ARG; }
+    const BwdArgs a = {top_tokens, top_logprobs, lse, lse_rest, dloss, rows, ld, ld_dlogits, vocab, top, scale};
+    return with_type(type, [&](auto *t) {
+        typedef B2_ELEM(t) T;
+        return backward<T>((T *)dlogits, (const T *)logits, a, accumulate != 0, (cudaStream_t)stream);
+    });
+}
+
+}  // extern "C"

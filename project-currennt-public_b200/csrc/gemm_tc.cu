@@ -658,6 +658,25 @@ int make_map(CUtensorMap *map, const float *base, long inner, long outer, long l
     return B2_OK;
 }
 
+}  // namespace
+
+int make_byte_map(CUtensorMap *map, const void *base, long long inner, long long outer, long long ld, int box_rows) {
+    B2_TRY(get_encode());
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d) for rows of %lld bytes, %lld of them %lld apart", (int)r, inner, outer, ld);
+        return B2_ERR_CUDA;
+    }
+    return B2_OK;
+}
+
+namespace {
+
 // one block per SM (the kernel loops over its share of the tiles), fewer when there is less work
 int persistent_grid(int items) {
     const int sms = sm_count();

@@ -1,0 +1,373 @@
+// Products in 8-bit integers with a scale for each row of the activations and each channel of the weights, and the quantisation of rows.
+//
+//   quantise:  s_r = max_k |x_rk| / 127,  q_rk = rint(x_rk * (127 / max |x_r|))         one FMA with 1.5 * 2^23: the product is rounded once, to an integer
+//   product:   out_rc = s_r * s_c * sum_k q_rk w_ck + bias_c                             exact 32-bit sums
+//
+// The product runs on the tensor cores (tcgen05.mma kind::i8): channels are the rows of a tile (128 tensor-memory lanes), activations its columns, so that a warp
+// of the epilogue, which has 32 lanes of one column, stores 32 neighbouring channels of one row of out, whatever its alignment.  The number of columns follows
+// the rows of x: few rows stream the weights once through a deep ring, many rows reuse them.
+#include <cuda.h>
+#include <math.h>
+
+#include "ptx.cuh"
+#include "typed.cuh"
+
+namespace b2 {
+namespace {
+
+// ---- quantisation ---------------------------------------------------------------------------------------------------------------------
+constexpr float TINY_ROW = 3.00926553810506e-36f;       // 2^-118: 127 over less leaves the floats
+
+template <typename T> __device__ __forceinline__ float largest_magnitude(const uint4 &q) {
+    float m = 0.0f;
+    if constexpr (sizeof(T) == 4) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+        unsigned b = 0;      // magnitudes of floats are in the order of their bits, NaN above all
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b = max(b, w[i] & 0x7fffffffu);
+        m = __uint_as_float(b);
+    } else {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+        unsigned b = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b = __vmaxu2(b, w[i] & 0x7fff7fffu);
+        const unsigned short h = (unsigned short)max(b & 0xffffu, b >> 16);
+        T v;
+        memcpy(&v, &h, 2);
+        m = to_float(v);
+    }
+    return m;
+}
+__device__ __forceinline__ float larger_magnitude(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+__device__ __forceinline__ unsigned char quantised(float x, float inv) { return (unsigned char)__float_as_uint(fmaf(x, inv, 12582912.0f)); }
+
+// TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice
+template <typename T, int TEAM, int U, bool KEPT>
+__global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long long ld_q, float *scales, const T *x0, long long rows, int dim, long long ld_x) {
+    constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
+    __shared__ float most[8];
+    const int team = threadIdx.x / TEAM, at = threadIdx.x % TEAM, lane = threadIdx.x & 31;
+    const long long r = (long long)blockIdx.x * TEAMS + team;
+    grid_release();
+    if (r >= rows) return;
+    const T *x = x0 + r * ld_x;
+    unsigned char *to = reinterpret_cast<unsigned char *>(q) + r * ld_q;
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T)), vecs = (mis + dim + W - 1) / W;
+    const bool out_vec = (((uintptr_t)(to - mis)) & (W - 1)) == 0;
+    const auto load = [&](int v) -> uint4 {
+        const int i0 = v * W - mis;
+        if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(x + i0);
+        T e[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? x[i0 + j] : from_float<T>(0.0f);
+        uint4 o;
+        memcpy(&o, e, 16);
+        return o;
+    };
+    uint4 held[KEPT ? U : 1];
+    float m = 0.0f;
+    if (KEPT) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) held[u] = at + u * TEAM < vecs ? load(at + u * TEAM) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) m = larger_magnitude(m, largest_magnitude<T>(held[u]));
+    } else
+        for (int v = at; v < vecs; v += TEAM) m = larger_magnitude(m, largest_magnitude<T>(load(v)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (TEAM == 256) {
+        if (lane == 0) most[threadIdx.x >> 5] = m;
+        __syncthreads();
+        m = most[lane & 7];
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    const bool finite = m < __int_as_float(0x7f800000), some = finite && m > TINY_ROW;
+    const float inv = some ? __fdiv_rn(127.0f, m) : 0.0f;
+    if (at == 0) scales[r] = !finite ? nanf("") : some ? __fdiv_rn(m, 127.0f) : 0.0f;
+    const auto store = [&](int v, const uint4 &h) {
+        const int i0 = v * W - mis;
+        T e[W];
+        memcpy(e, &h, 16);
+        Vec<unsigned char, W> o;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o.v[j] = finite ? quantised(to_float(e[j]), inv) : 0;
+        if (out_vec && i0 >= 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
+        else
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (i0 + j >= 0 && i0 + j < dim) to[i0 + j] = o.v[j];
+    };
+    if (KEPT) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at + u * TEAM < vecs) store(at + u * TEAM, held[u]);
+    } else
+        for (int v = at; v < vecs; v += TEAM) store(v, load(v));
+}
+
+template <typename T> int quantize(signed char *q, long long ld_q, float *scales, const T *x, long long rows, int dim, long long ld_x, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    const int vecs = (dim + W - 1) / W + 1;                  // one more: a row may start inside a vector
+    const auto go = [&](auto kernel, int teams) -> int {
+        const long long blocks = (rows + teams - 1) / teams;
+        if (blocks > 0x7fffffffll) { set_error("b2_int8_quantize: %lld rows", rows); return B2_ERR_BAD_SHAPE; }
+        kernel<<<(unsigned)blocks, 256, 0, st>>>(q, ld_q, scales, x, rows, dim, ld_x);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+        return B2_OK;
+    };
+    if (vecs <= 32 * 5) return go(int8_quantize_kernel<T, 32, 5, true>, 8);
+    if (vecs <= 256 * 4) return go(int8_quantize_kernel<T, 256, 4, true>, 1);
+    if (vecs <= 256 * 9) return go(int8_quantize_kernel<T, 256, 9, true>, 1);
+    return go(int8_quantize_kernel<T, 256, 1, false>, 1);
+}
+
+// ---- product --------------------------------------------------------------------------------------------------------------------------
+constexpr int BM = 128, BK = 128;                 // channels of a tile, positions of a slab (one swizzle row of 128 bytes)
+constexpr int A_BYTES = BM * BK;
+constexpr int THREADS = 320;                      // warp 0 copies, 1 multiplies, 2 to 9 store
+constexpr long long WAIT_CYCLES = 4000000000LL;   // about two seconds
+template <int BN> struct Shape {
+    static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
+    static constexpr int STAGES = BN >= 256 ? 4 : BN >= 128 ? 6 : 8;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // slack: the swizzle wants 1024-byte alignment
+    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+};
+struct ProductArgs {
+    const float *x_scales, *w_scales, *bias;
+    long long ld_out, rows;
+    int channels, slabs;
+    unsigned row_tiles, channel_tiles;
+    int chained;
+};
+
+template <int BN, typename O>
+__global__ void __launch_bounds__(THREADS, 1)
+int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
+    using namespace ptx;
+    typedef Shape<BN> S;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 5];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int fail;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
+    const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(S::STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * S::STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * S::STAGES + 2 + b); };
+    const uint32_t idle = bar0 + 8u * (uint32_t)(2 * S::STAGES + 4);
+    const unsigned tiles = a.row_tiles * a.channel_tiles;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 8); }
+        mbar_init(idle, 1);
+        fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) tmem_alloc(smem_u32((const void *)&tmem_slot), S::TMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned i = 0;
+            bool ok = true;
+            const auto wait_x = [&](unsigned k) {
+                if (k == 0 && a.chained) { grid_wait(); fence_async_global(); }
+            };
+            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                const int r0 = (int)(tile % a.row_tiles) * BN, c0 = (int)(tile / a.row_tiles) * BM;
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % S::STAGES);
+                    if (!mbar_wait_bounded<false>(empty(s), ((i / S::STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    const uint32_t at = ring + (uint32_t)s * S::STAGE_BYTES;
+                    mbar_expect_tx(full(s), S::STAGE_BYTES);
+                    tma_load_2d(at, &map_w, k * BK, c0, full(s));
+                    // the activations are what the launch before this one may still be writing
+                    wait_x(i);
+                    tma_load_2d(at + A_BYTES, &map_x, k * BK, r0, full(s));
+                }
+            }
+            if (!ok)      // copies under way end before the block does
+                for (unsigned j = i > (unsigned)S::STAGES ? i - S::STAGES : 0; j < i; ++j) {
+                    volatile int never = 0;
+                    mbar_wait_bounded<false>(full((int)(j % S::STAGES)), (j / S::STAGES) & 1u, &never, WAIT_CYCLES);
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc_s8(BM, BN);
+            unsigned i = 0, n = 0;
+            bool ok = true;
+            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+                const uint32_t d = tmem + (n & 1u) * BN;
+                if (!mbar_wait_bounded<false>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                tc_fence_after();
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % S::STAGES);
+                    if (!mbar_wait_bounded<false>(full(s), (i / S::STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = ring + (uint32_t)s * S::STAGE_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 32; ++kk)
+                        mma_s8(d, desc_kmajor_sw128(at + kk * 32, 1024), desc_kmajor_sw128(at + A_BYTES + kk * 32, 1024), idesc, (k | kk) ? 1u : 0u);
+                    mma_commit(empty(s));
+                }
+                if (ok) mma_commit(acc_full((int)(n & 1u)));
+            }
+            if (!ok) {
+                volatile int never = 0;
+                mma_commit(idle);
+                mbar_wait_bounded<false>(idle, 0, &never, WAIT_CYCLES);
+            }
+        }
+    } else {
+        // A warp reads the tensor-memory lanes 32 * (warp % 4) on; warps 2 to 5 take the first half of the columns, 6 to 9 the second
+        constexpr int HALF = BN / 2, STEP = HALF < 16 ? 8 : 16;
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        unsigned n = 0;
+        bool ok = true;
+        if (a.chained) grid_wait();
+        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+            const long long r0 = (long long)(tile % a.row_tiles) * BN + half * HALF;
+            const int c = (int)(tile / a.row_tiles) * BM + 32 * quarter + lane;
+            const bool real = c < a.channels;
+            const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
+            // a tile that its block gave up on shows as NaN
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
+            if (!ok && lane == 0) fail = 1;
+            tc_fence_after();
+            for (int j0 = 0; j0 < HALF; j0 += STEP) {
+                if (r0 + j0 >= a.rows) break;
+                uint32_t v[16];
+                if (ok) {
+                    if constexpr (STEP == 16) tmem_ld16(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF + j0, v);
+                    else tmem_ld8(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF + j0, v);
+                    tmem_ld_wait();
+                }
+                const float xs = lane < STEP && r0 + j0 + lane < a.rows ? a.x_scales[r0 + j0 + lane] : 0.0f;
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) {
+                    const float s = __shfl_sync(0xffffffffu, xs, j);
+                    if (real && r0 + j0 + j < a.rows) {
+                        const float y = ok ? fmaf((float)(int)v[j], s * ws, bias) : nanf("");
+                        out[(r0 + j0 + j) * a.ld_out + c] = from_float<O>(y);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty((int)(n & 1u)));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, S::TMEM);
+}
+
+template <int BN, typename O> int launch_product(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
+    typedef Shape<BN> S;
+    const auto kernel = int8_product_kernel<BN, O>;
+    B2_TRY(set_max_dynamic_smem((const void *)kernel, S::SMEM));
+    const long long tiles = (long long)a.row_tiles * a.channel_tiles;
+    const unsigned blocks = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+    if (a.chained) return launch_chained(int8_product_kernel<BN, O>, dim3(blocks), dim3(THREADS), S::SMEM, st, mw, mx, out, a);
+    kernel<<<blocks, THREADS, S::SMEM, st>>>(mw, mx, out, a);
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
+
+size_t pitch_of(int dim) { return ((size_t)dim + 15) & ~(size_t)15; }
+bool sizes_fit(long long rows, int channels, int dim) { return rows >= 0 && rows <= 0x7fffff00ll && channels >= 1 && channels <= 0x7fffff00 && dim >= 1 && dim <= 131071; }
+
+template <typename O> int product(O *out, const signed char *x, long long ld_x, const signed char *w, long long ld_w, int dim, ProductArgs a, cudaStream_t st) {
+    const auto go = [&](auto columns) -> int {
+        constexpr int BN = decltype(columns)::value;
+        CUtensorMap mw, mx;
+        B2_TRY(make_byte_map(&mw, w, dim, a.channels, ld_w, BM));
+        B2_TRY(make_byte_map(&mx, x, dim, a.rows, ld_x, BN));
+        a.row_tiles = (unsigned)((a.rows + BN - 1) / BN);
+        a.channel_tiles = (unsigned)((a.channels + BM - 1) / BM);
+        if ((double)a.row_tiles * a.channel_tiles > 4e9) { set_error("b2_int8_product: %lld rows of %d channels", a.rows, a.channels); return B2_ERR_BAD_SHAPE; }
+        return launch_product<BN, O>(mw, mx, out, a, st);
+    };
+    if (a.rows <= 16) return go(std::integral_constant<int, 16>());
+    if (a.rows <= 32) return go(std::integral_constant<int, 32>());
+    if (a.rows <= 64) return go(std::integral_constant<int, 64>());
+    if (a.rows <= 128) return go(std::integral_constant<int, 128>());
+    return go(std::integral_constant<int, 256>());
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_int8_quantize(signed char *q, long long ld_q, float *scales, const void *x, int type, long long rows, int dim, long long ld_x, b2_stream stream) {
+    const int e = type_size(type);
+    if (!e) { set_error("b2_int8_quantize: unknown element type %d", type); return B2_ERR_BAD_ARG; }
+    if (rows < 0 || dim < 1 || dim > (1 << 27)) { set_error("b2_int8_quantize: %lld rows of %d (at most 2^27)", rows, dim); return B2_ERR_BAD_SHAPE; }
+    if (ld_q < dim || ld_x < dim || ld_q > MAX_LD || ld_x > MAX_LD) {
+        set_error("b2_int8_quantize: leading dimension too small or beyond 2^40 (integers %lld, input %lld for %d columns)", ld_q, ld_x, dim);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!rows) return B2_OK;
+    if (!q || !scales || !x) { set_error("b2_int8_quantize: null pointer"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(x, e) || !aligned_to(scales, 4)) { set_error("b2_int8_quantize: the input or the scales are not aligned to their elements"); return B2_ERR_BAD_ARG; }
+    return with_type(type, [&](auto *t) { return quantize(q, ld_q, scales, (const B2_ELEM(t) *)x, rows, dim, ld_x, (cudaStream_t)stream); });
+}
+
+size_t b2_int8_product_workspace(long long rows, int channels, int dim) {
+    if (!sizes_fit(rows, channels, dim)) return 0;
+    return (size_t)rows * pitch_of(dim) + (size_t)rows * sizeof(float);
+}
+
+int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, int x_type, long long ld_x, const float *x_scales, const signed char *w, long long ld_w,
+                    const float *w_scales, const float *bias, long long rows, int channels, int dim, void *workspace, size_t workspace_bytes, b2_stream stream) {
+    const int eo = type_size(out_type), ex = x_type == B2_I8 ? 1 : type_size(x_type);
+    if (!eo || !ex) { set_error("b2_int8_product: unknown element type %d or %d", out_type, x_type); return B2_ERR_BAD_ARG; }
+    if (!sizes_fit(rows, channels, dim)) { set_error("b2_int8_product: %lld rows, %d channels, %d positions (at most 131071)", rows, channels, dim); return B2_ERR_BAD_SHAPE; }
+    if (ld_out < channels || ld_x < dim || ld_w < dim || ld_out > MAX_LD || ld_x > (1ll << 39) || ld_w > (1ll << 39)) {      // a tensor map's rows lie up to 2^40 bytes apart
+        set_error("b2_int8_product: leading dimension too small or too large (out %lld for %d columns, x %lld and w %lld for %d)", ld_out, channels, ld_x, ld_w, dim);
+        return B2_ERR_BAD_ARG;
+    }
+    if (!rows) return B2_OK;
+    if (!out || !x || !w || !w_scales || (x_type == B2_I8 && !x_scales)) { set_error("b2_int8_product: null pointer"); return B2_ERR_BAD_ARG; }
+    if (x_type != B2_I8 && x_scales) { set_error("b2_int8_product: scales of rows that are quantised in the call"); return B2_ERR_BAD_ARG; }
+    if (!aligned_to(out, eo) || !aligned_to(x, ex) || !aligned_to(x_scales, 4) || !aligned_to(w_scales, 4) || !aligned_to(bias, 4)) {
+        set_error("b2_int8_product: a tensor is not aligned to its elements");
+        return B2_ERR_BAD_ARG;
+    }
+    if (!aligned_to(w, 16) || ld_w % 16 || (x_type == B2_I8 && (!aligned_to(x, 16) || ld_x % 16))) {
+        set_error("b2_int8_product: rows of 8-bit integers that do not start at multiples of 16 bytes");
+        return B2_ERR_BAD_ARG;
+    }
+    ProductArgs a = {};
+    a.x_scales = x_scales; a.w_scales = w_scales; a.bias = bias;
+    a.ld_out = ld_out; a.rows = rows; a.channels = channels; a.slabs = (dim + BK - 1) / BK;
+    const signed char *xq = (const signed char *)x;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (x_type != B2_I8) {
+        const size_t need = b2_int8_product_workspace(rows, channels, dim);
+        if (!workspace || !aligned_to(workspace, 16)) { set_error("b2_int8_product: the workspace is missing or not aligned to 16 bytes"); return B2_ERR_BAD_ARG; }
+        if (workspace_bytes < need) { set_error("b2_int8_product: a workspace of %zu bytes, %zu are needed", workspace_bytes, need); return B2_ERR_BAD_SHAPE; }
+        signed char *q = (signed char *)workspace;
+        float *scales = (float *)(q + (size_t)rows * pitch_of(dim));
+        B2_TRY(with_type(x_type, [&](auto *t) { return quantize(q, (long long)pitch_of(dim), scales, (const B2_ELEM(t) *)x, rows, dim, ld_x, st); }));
+        xq = q;
+        ld_x = (long long)pitch_of(dim);
+        a.x_scales = scales;
+        a.chained = 1;
+    }
+    return with_type(out_type, [&](auto *t) { return product((B2_ELEM(t) *)out, xq, ld_x, w, ld_w, dim, a, st); });
+}
+
+}  // extern "C"

@@ -37,6 +37,13 @@ template <typename F> __device__ __forceinline__ void less_of(float scale, float
     else f(Rounded(s, off, scale));
 }
 
+// fp32 gradients with the exponential of the full accuracy, 16-bit ones with the hardware's: its error of 2^-22 is lost in their rounding (and a probability
+// below 2^-126 is 0)
+template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
+    const float2 v = halves(sizeof(T) == 4 ? x : mul2(x, pair(LOG2E, LOG2E)));
+    return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
+}
+
 // ---- vectors of 16 bytes as they were loaded ------------------------------------------------------------------------------------------
 template <typename T> struct Raw;
 template <> struct Raw<float> {

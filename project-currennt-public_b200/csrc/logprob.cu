@@ -629,12 +629,6 @@ struct BwdArgs {
     int vocab;
     float scale;
 };
-// fp32 gradients with the exponential of the full accuracy, 16-bit ones with the hardware's: its error of 2^-22 is lost in their rounding (and a probability
-// below 2^-126 is 0)
-template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
-    const float2 v = halves(sizeof(T) == 4 ? x : mul2(x, pair(LOG2E, LOG2E)));
-    return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
-}
 // What a row's entries share: dx = p (c0 + c1 log p) with c0 = -s (g + h H), c1 = -s h, and s g more at the token.
 struct RowGrad { float lse, c0, c1, at_token; int tok; };
 // N entries from index i0 on

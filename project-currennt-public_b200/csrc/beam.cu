@@ -16,7 +16,7 @@ namespace b2 {
 namespace {
 
 constexpr int MAX_BEAMS = 64, MAX_BEST = 64, MOST_VOCAB = 1 << 26;
-constexpr int SLICE_VECS = 4;        // vectors of 16 bytes a thread holds
+constexpr int SLICE_THREADS = 256, SLICE_VECS = 8;        // threads of a slice, vectors of 16 bytes each holds
 
 struct Part { float m, s; };         // largest z of a slice, sum of e^(z - m)
 
@@ -36,9 +36,10 @@ __device__ __forceinline__ bool runs(const SelectArgs &a, long long row) {
 }
 
 template <typename T, int THREADS, bool MASK>
-__global__ void __launch_bounds__(THREADS) beam_rows_kernel(const T *logits, const SelectArgs a) {
+__global__ void __launch_bounds__(THREADS, 3) beam_rows_kernel(const T *logits, const SelectArgs a) {
     constexpr int W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, GROUP = THREADS / 64, CAP = 512;
-    __shared__ float maxima[64], tops[WARPS], sums[WARPS];
+    __shared__ __align__(16) float maxima[64];
+    __shared__ float tops[WARPS], sums[WARPS];
     __shared__ Key found[CAP];
     __shared__ float bound;
     __shared__ int count;
@@ -97,18 +98,22 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const T *logits, con
 #pragma unroll
     for (int o = GROUP; o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
     if (lane == 0) tops[warp] = most;
-    if (t == 0) count = 0;
+    if (t == 0) { count = 0; bound = neg_inf(); }
     __syncthreads();
     most = tops[lane % WARPS];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
     if (t < 64) {
-        // the place of this group's maximum among the 64
-        const Key k = make_key(maxima[t], t);
+        // the place of this group's maximum among the 64 (NaN: the row has no continuations)
+        const float mine64 = maxima[t];
         int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) before += make_key(maxima[i], i) > k;
-        if (before == a.top - 1) bound = maxima[t];
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+            const float4 m = *reinterpret_cast<const float4 *>(&maxima[i]);
+            before += (m.x > mine64 || (m.x == mine64 && i < t)) + (m.y > mine64 || (m.y == mine64 && i + 1 < t)) + (m.z > mine64 || (m.z == mine64 && i + 2 < t)) +
+                      (m.w > mine64 || (m.w == mine64 && i + 3 < t));
+        }
+        if (before == a.top - 1) bound = mine64;
     }
     float s = 0.0f;
     if (most != neg_inf()) {
@@ -132,6 +137,9 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const T *logits, con
     s = warp_sum(s);
     if (lane == 0) sums[warp] = s;
     __syncthreads();
+    // the logits are taken apart again below: kept apart over the barrier, they do not fit into the registers
+#pragma unroll
+    for (int u = 0; u < U; ++u) asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
     const float limit = bound;
     if (mine >= limit && mine > neg_inf())
 #pragma unroll
@@ -162,6 +170,8 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const T *logits, con
         Key last = ~0ull;
         for (int i = 0; i < a.top; ++i) {
             Key k = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float z[W];
@@ -207,144 +217,137 @@ __device__ __forceinline__ int beam_of(unsigned long long tie) { return MAX_BEAM
 __device__ __forceinline__ float logit_of(unsigned long long tie) { return ordered_value((unsigned)(tie >> 26)); }
 __device__ __forceinline__ int token_of(unsigned long long tie) { return MOST_VOCAB - 1 - (int)(tie & (MOST_VOCAB - 1)); }
 
-// one block a sequence
-constexpr int JOIN_WARPS = 8;
-__global__ void __launch_bounds__(32 * JOIN_WARPS) beam_join_kernel(const SelectArgs a) {
+// One block a sequence.  A slice's list is sorted, so the first few entries of every list, 2 K of them together, hold a bound that K continuations reach: the K-th best of
+// them.  All entries that reach it are counted into their places.
+constexpr int JOIN_THREADS = 256, AHEAD = 4, MOST_HEADS = 1024, MOST_FOUND = 1024;
+__global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArgs a) {
     __shared__ double off[MAX_BEAMS], weight[MAX_BEAMS];
     __shared__ bool ended[MAX_BEAMS];
-    __shared__ Cand stage[JOIN_WARPS][MAX_BEST];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ __align__(16) double heads[MOST_HEADS];
+    __shared__ Cand found[MOST_FOUND];
+    __shared__ double bound;
+    __shared__ int count;
+    __shared__ Cand winner[JOIN_THREADS / 32];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const long long g = blockIdx.x;
+    const int lists = a.beams * a.slices, entries = lists * a.top;
+    const Key *const keys = a.lists + g * entries;
     grid_wait();
+    Key ahead[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = t + i * JOIN_THREADS < entries ? keys[t + i * JOIN_THREADS] : 0;
+    const int deep = min(a.top, (2 * a.top + lists - 1) / lists), n_heads = lists * deep;
+    Key head = 0;
+    if (t < n_heads) head = keys[t / deep * a.top + t % deep];
     // score_b - lse_b of the beams; NaN: no continuations
-    for (int b = warp; b < a.beams; b += JOIN_WARPS) {
+    for (int b = warp; b < a.beams; b += JOIN_THREADS / 32) {
         const long long row = g * a.beams + b;
         const float score = a.scores[row], w = a.weights ? a.weights[row] : 1.0f;
         const bool end = a.finished && a.finished[row];
+        Part p = {neg_inf(), 0.0f};
+        if (lane < a.slices) p = a.parts[row * a.slices + lane];
         const bool fit = score > neg_inf() && score < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000);
         double o = nan("");
         if (fit && end) o = (double)score;
         else if (fit) {
-            float m = neg_inf();
-            for (int i = lane; i < a.slices; i += 32) m = max_nan(m, a.parts[row * a.slices + i].m);
+            float m = p.m;
+            for (int i = lane + 32; i < a.slices; i += 32) m = max_nan(m, a.parts[row * a.slices + i].m);
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, x));
-            double s = 0.0;
-            if (m != neg_inf())
-                for (int i = lane; i < a.slices; i += 32) {
-                    const Part p = a.parts[row * a.slices + i];
-                    if (p.m != neg_inf()) s += (double)p.s * exp((double)p.m - (double)m);
-                }
+            // a slice's sum has the error of 32 bits already: the factors need no more
+            double s = p.m != neg_inf() ? (double)(p.s * expf(p.m - m)) : 0.0;
+            for (int i = lane + 32; i < a.slices; i += 32) {
+                const Part q = a.parts[row * a.slices + i];
+                if (q.m != neg_inf()) s += (double)(q.s * expf(q.m - m));
+            }
             s = warp_sum(s);
             o = m == neg_inf() ? nan("") : (double)score - (double)m - log(s);
         }
         if (lane == 0) { off[b] = o; weight[b] = (double)w; ended[b] = end; }
     }
+    if (t == 0) { count = 0; bound = -INFINITY; }
     __syncthreads();
-    // every warp merges its share of the sorted lists: lane l has the heads of the lists l, l + 32, ... of the share, and gives the best of them
-    const int lists = a.beams * a.slices, share = (lists + JOIN_WARPS - 1) / JOIN_WARPS, warps = (lists + share - 1) / share;
-    const auto entry = [&](int l, int i) -> Cand {
-        const int b = l / a.slices;
+    const auto cand = [&](int i, Key k) -> Cand {
+        const int l = i / a.top, b = l / a.slices;
         const double o = off[b];
-        if (o != o || i >= a.top) return no_cand();
-        if (ended[b]) return l % a.slices == 0 && i == 0 ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
-        const Key k = a.lists[((g * a.beams + b) * (long long)a.slices + l % a.slices) * a.top + i];
+        if (o != o) return no_cand();
+        if (ended[b]) return i == b * a.slices * a.top ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
         if (!k) return no_cand();
         const float z = key_value(k);
         return {weight[b] * (o + (double)z), tie_of(b, z, key_index(k))};
     };
-    if (warp < warps) {
-        const int l0 = warp * share, l1 = min(lists, l0 + share);
-        // a lane with several lists merges them on the fly: per list a position
-        constexpr int HELD = 4;
-        if (share <= 32 * HELD) {
-            Cand head[HELD];
-            int at[HELD];
-#pragma unroll
-            for (int h = 0; h < HELD; ++h) {
-                const int l = l0 + lane + 32 * h;
-                at[h] = 0;
-                head[h] = l < l1 ? entry(l, 0) : no_cand();
-            }
-            for (int k = 0; k < a.top; ++k) {
-                Cand c = head[0];
-                int which = 0;
-#pragma unroll
-                for (int h = 1; h < HELD; ++h)
-                    if (better(head[h], c)) { c = head[h]; which = h; }
-                Cand top = c;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
-                    if (better(other, top)) top = other;
-                }
-                if (lane == 0) stage[warp][k] = top;
-                if (top.tie == 0) {                              // none is left
-                    for (int i = k + 1 + lane; i < a.top; i += 32) stage[warp][i] = no_cand();
-                    break;
-                }
-                if (c.tie == top.tie && c.rank == top.rank)
-#pragma unroll
-                    for (int h = 0; h < HELD; ++h)
-                        if (h == which) head[h] = entry(l0 + lane + 32 * h, ++at[h]);
-            }
-        } else {
-            // very many lists: the best entry behind the last one, by looking at all
-            Cand last = {INFINITY, ~0ull};
-            for (int k = 0; k < a.top; ++k) {
-                Cand top = no_cand();
-                for (int l = l0 + lane; l < l1; l += 32)
-                    for (int i = 0; i < a.top; ++i) {
-                        const Cand c = entry(l, i);
-                        if (c.tie == 0) break;
-                        if (better(last, c)) {
-                            if (better(c, top)) top = c;
-                            break;
-                        }
-                    }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
-                    if (better(other, top)) top = other;
-                }
-                if (lane == 0) stage[warp][k] = top;
-                last = top;
-                if (top.tie == 0) {
-                    for (int i = k + 1 + lane; i < a.top; i += 32) stage[warp][i] = no_cand();
-                    break;
-                }
-            }
+    const bool few = n_heads <= MOST_HEADS;
+    if (few) {
+        for (int i = t; i < n_heads; i += JOIN_THREADS) {
+            const int at = i / deep * a.top + i % deep;
+            heads[i] = cand(at, i < JOIN_THREADS ? head : keys[at]).rank;
         }
+        __syncthreads();
+        for (int i = t; i < n_heads; i += JOIN_THREADS) {
+            const double mine = heads[i];
+            int before = 0;
+#pragma unroll 8
+            for (int j = 0; j < n_heads; ++j) before += heads[j] > mine || (heads[j] == mine && j < i);
+            if (before == a.top - 1) bound = mine;
+        }
+        __syncthreads();
+        const double limit = bound;
+        const auto offer = [&](int i, Key k) {
+            const Cand c = cand(i, k);
+            if (c.tie != 0 && c.rank >= limit) {
+                const int at = atomicAdd(&count, 1);
+                if (at < MOST_FOUND) found[at] = c;
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (t + i * JOIN_THREADS < entries) offer(t + i * JOIN_THREADS, ahead[i]);
+        for (int i = t + AHEAD * JOIN_THREADS; i < entries; i += JOIN_THREADS) offer(i, keys[i]);
+        __syncthreads();
     }
-    __syncthreads();
-    if (warp != 0) return;
-    // the warps' lists
-    int at = 0;
-    Cand head = lane < warps ? stage[lane][0] : no_cand();
-    for (int k = 0; k < a.top; ++k) {
-        Cand top = head;
+    const auto write = [&](int place, const Cand &c) {
+        const long long i = g * a.top + place;
+        const bool none = c.tie == 0;
+        const int b = none ? 0 : beam_of(c.tie);
+        a.best[i] = none ? neg_inf() : ended[b] ? (float)off[b] : (float)(off[b] + (double)logit_of(c.tie));
+        a.from[i] = none ? -1 : b;
+        a.tokens[i] = none ? -1 : token_of(c.tie);
+    };
+    const int n = count;
+    if (few && n <= MOST_FOUND) {
+        for (int i = t; i < n; i += JOIN_THREADS) {
+            const Cand c = found[i];
+            int before = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) before += better(found[j], c);
+            if (before < a.top) write(before, c);
+        }
+        for (int i = n + t; i < a.top; i += JOIN_THREADS) write(i, no_cand());
+        return;
+    }
+    // very many slices, or many equal ranks: the next best in turn
+    Cand last = {INFINITY, ~0ull};
+    for (int place = 0; place < a.top; ++place) {
+        Cand top = no_cand();
+        for (int i = t; i < entries; i += JOIN_THREADS) {
+            const Cand c = cand(i, keys[i]);
+            if (c.tie != 0 && better(last, c) && better(c, top)) top = c;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
             if (better(other, top)) top = other;
         }
-        if (lane == 0) {
-            const long long i = g * a.top + k;
-            const bool none = top.tie == 0;
-            const int b = none ? 0 : beam_of(top.tie);
-            a.best[i] = none ? neg_inf() : ended[b] ? (float)off[b] : (float)(off[b] + (double)logit_of(top.tie));
-            a.from[i] = none ? -1 : b;
-            a.tokens[i] = none ? -1 : token_of(top.tie);
-        }
-        if (head.tie != 0 && head.tie == top.tie && head.rank == top.rank) {
-            ++at;
-            head = at < a.top ? stage[lane][at] : no_cand();
-        }
+        if (lane == 0) winner[warp] = top;
+        __syncthreads();
+        for (int w = 0; w < JOIN_THREADS / 32; ++w)
+            if (better(winner[w], top)) top = winner[w];
+        if (t == 0) write(place, top);
+        if (top.tie != 0) last = top; else last = no_cand();
+        __syncthreads();
     }
 }
 
-// slices of a row: vectors in each, a multiple of nothing; the last one may be shorter
-constexpr int SLICE_THREADS = 512;
 int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
 int slices_of(int vocab, int type) { return (vectors_of(vocab, type) + SLICE_THREADS * SLICE_VECS - 1) / (SLICE_THREADS * SLICE_VECS); }
 
@@ -358,7 +361,7 @@ template <typename T> int select(const T *logits, SelectArgs a, int type, cudaSt
     else beam_rows_kernel<T, SLICE_THREADS, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
     count_launch();
     B2_CUDA(cudaGetLastError());
-    return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(32 * JOIN_WARPS), 0, st, a);
+    return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(JOIN_THREADS), 0, st, a);
 }
 
 bool sizes_fit(long long groups, int beams, int vocab, int top) {
@@ -375,7 +378,7 @@ struct StateArgs {
     unsigned first[MAX_STATES + 1];  // of the blocks of tensor i
 };
 // A thread moves a column of N bytes (of the same place in a sequence's beams) for all beams of a sequence: it alone reads and writes it, so that a state may
-// be reordered in place without a barrier.  HELD beams at a time are in registers; in place all are.
+// be reordered in place without a barrier.  HELD beams at a time are in registers; in place all are (narrower columns then, if there are more than MOST_HELD).
 template <int N> struct Bytes;
 template <> struct Bytes<16> { typedef uint4 T; };
 template <> struct Bytes<8> { typedef uint2 T; };
@@ -384,10 +387,9 @@ template <> struct Bytes<2> { typedef unsigned short T; };
 template <> struct Bytes<1> { typedef unsigned char T; };
 template <typename V> __device__ __forceinline__ V zero_of() { V v; memset(&v, 0, sizeof(V)); return v; }
 
-constexpr int MOVE_THREADS = 128;
-template <int N, int HELD> __device__ __forceinline__ void move(const b2_state &s, const int *parent, long long group, int beams, long long groups, long long o, long long column) {
+constexpr int MOVE_THREADS = 128, MOST_HELD = 16;
+template <int N, int HELD> __device__ __forceinline__ void move(const b2_state &s, const int *parent, int beams, long long base) {
     typedef typename Bytes<N>::T V;
-    const long long base = (o * groups + group) * beams * s.row_bytes + column * N;
     const char *in = (const char *)s.data + base;
     char *out = (char *)s.out + base;
     const bool place = s.data == s.out;
@@ -395,45 +397,51 @@ template <int N, int HELD> __device__ __forceinline__ void move(const b2_state &
         V v[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const int b = b0 + i;
-            if (b >= beams) break;
-            const int p = parent[b];
-            v[i] = p < 0 || (place && p == b) ? zero_of<V>() : *reinterpret_cast<const V *>(in + p * s.row_bytes);
+            if (b0 + i >= beams) break;
+            const int p = parent[b0 + i];
+            v[i] = p < 0 || (place && p == b0 + i) ? zero_of<V>() : *reinterpret_cast<const V *>(in + p * s.row_bytes);
         }
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const int b = b0 + i;
-            if (b >= beams) break;
-            if (!(place && parent[b] == b)) *reinterpret_cast<V *>(out + b * s.row_bytes) = v[i];
+            if (b0 + i >= beams) break;
+            if (!(place && parent[b0 + i] == b0 + i)) *reinterpret_cast<V *>(out + (b0 + i) * s.row_bytes) = v[i];
         }
     }
 }
-// HELD: beams in registers; a block's threads have neighbouring columns of one sequence and one outer index
+// bytes of a column: what the addresses and the rows allow, and 4 where more than MOST_HELD beams have to be in registers at once
+__host__ __device__ __forceinline__ int column_width(const b2_state &s, int beams) {
+    const unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & (s.data == s.out && beams > MOST_HELD ? 3 : 15);
+    return at & 1 ? 1 : at & 2 ? 2 : at & 4 ? 4 : at & 8 ? 8 : s.data == s.out && beams > MOST_HELD ? 4 : 16;
+}
+// a block's threads have columns of one sequence, those of all outer indices one after the other
 template <int HELD> __global__ void __launch_bounds__(MOVE_THREADS) beam_reorder_kernel(const __grid_constant__ StateArgs a) {
     __shared__ int parent[MAX_BEAMS];
     int i = 0;
     while (i + 1 < a.n && blockIdx.x >= a.first[i + 1]) ++i;
     const b2_state &s = a.s[i];
-    unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & 15;
-    const int width = at == 0 ? 16 : (at & 7) == 0 ? 8 : (at & 3) == 0 ? 4 : (at & 1) == 0 ? 2 : 1;
-    const long long columns = s.row_bytes / width, chunks = (columns + MOVE_THREADS - 1) / MOVE_THREADS;
-    // blocks of a tensor: [outer][group][chunk]
-    const long long k = blockIdx.x - a.first[i];
-    const long long chunk = k % chunks, group = k / chunks % a.groups, o = k / chunks / a.groups;
+    const int width = column_width(s, a.beams);
+    const unsigned groups = (unsigned)a.groups, k = blockIdx.x - a.first[i], group = k % groups;     // blocks of a tensor: [chunk][group]
     if ((int)threadIdx.x < a.beams) {
-        const int p = a.parents[group * a.beams + threadIdx.x];
+        const int p = a.parents[(long long)group * a.beams + threadIdx.x];
         parent[threadIdx.x] = p >= 0 && p < a.beams ? p : -1;
     }
-    __syncthreads();
-    const long long column = chunk * MOVE_THREADS + threadIdx.x;
-    if (column >= columns) return;
-    switch (width) {
-        case 16: return move<16, HELD>(s, parent, group, a.beams, a.groups, o, column);
-        case 8: return move<8, HELD>(s, parent, group, a.beams, a.groups, o, column);
-        case 4: return move<4, HELD>(s, parent, group, a.beams, a.groups, o, column);
-        case 2: return move<2, HELD>(s, parent, group, a.beams, a.groups, o, column);
-        default: return move<1, HELD>(s, parent, group, a.beams, a.groups, o, column);
+    const long long columns = s.row_bytes / width, at = (long long)(k / groups) * MOVE_THREADS + threadIdx.x;
+    long long o, column;
+    if (columns * s.outer <= 0x7fffffff) {
+        o = (unsigned)at / (unsigned)columns;
+        column = (unsigned)at % (unsigned)columns;
+    } else {
+        o = at / columns;
+        column = at % columns;
     }
+    __syncthreads();
+    if (o >= s.outer) return;
+    const long long base = (o * a.groups + group) * a.beams * s.row_bytes + column * width;
+    if (HELD <= MOST_HELD && width == 16) return move<16, HELD <= MOST_HELD ? HELD : 1>(s, parent, a.beams, base);
+    if (HELD <= MOST_HELD && width == 8) return move<8, HELD <= MOST_HELD ? HELD : 1>(s, parent, a.beams, base);
+    if (width == 4) return move<4, HELD>(s, parent, a.beams, base);
+    if (width == 2) return move<2, HELD>(s, parent, a.beams, base);
+    return move<1, HELD>(s, parent, a.beams, base);
 }
 
 }  // namespace
@@ -484,7 +492,7 @@ int b2_beam_select(const void *logits, int type, long long groups, int beams, in
 }
 
 int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long groups, int beams, b2_stream stream) {
-    if (n < 0 || groups < 0 || groups > (1ll << 31) || beams < 1 || beams > MAX_BEAMS) {
+    if (n < 0 || groups < 0 || groups > 0x7fffffff / MAX_BEAMS || beams < 1 || beams > MAX_BEAMS) {
         set_error("b2_beam_reorder: %d tensors, %lld sequences of %d beams (1 to %d)", n, groups, beams, MAX_BEAMS);
         return B2_ERR_BAD_SHAPE;
     }
@@ -500,33 +508,35 @@ int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long
         const char *p = (const char *)s.data, *q = (const char *)s.out, *end = p + (long long)bytes;
         if (q && q != p && q < end && p < q + (long long)bytes) { set_error("b2_beam_reorder: tensor %d and its output overlap", i); return B2_ERR_BAD_ARG; }
     }
-    int i = 0;
-    while (i < n) {
-        StateArgs a;
-        a.n = 0; a.beams = beams; a.groups = groups; a.parents = parents;
-        unsigned long long blocks = 0;
-        for (; i < n && a.n < MAX_STATES; ++i) {
-            b2_state s = states[i];
-            if (!s.outer || !s.row_bytes) continue;
-            if (!s.out) s.out = s.data;
-            const unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & 15;
-            const int width = at == 0 ? 16 : (at & 7) == 0 ? 8 : (at & 3) == 0 ? 4 : (at & 1) == 0 ? 2 : 1;
-            const double more = (double)s.outer * (double)groups * (double)((s.row_bytes / width + MOVE_THREADS - 1) / MOVE_THREADS);
-            if (more > 2147483647.0) { set_error("b2_beam_reorder: tensor %d is too large", i); return B2_ERR_BAD_SHAPE; }
-            if (blocks + (unsigned long long)more > 2147483647ull) break;
-            a.s[a.n] = s;
-            a.first[a.n++] = (unsigned)blocks;
-            blocks += (unsigned long long)more;
+    // in place, more than MOST_HELD beams are in registers at once, in narrow columns: a launch of their own
+    for (int pass = 0; pass < 2; ++pass) {
+        int i = 0;
+        while (i < n) {
+            StateArgs a;
+            a.n = 0; a.beams = beams; a.groups = groups; a.parents = parents;
+            unsigned long long blocks = 0;
+            for (; i < n && a.n < MAX_STATES; ++i) {
+                b2_state s = states[i];
+                if (!s.outer || !s.row_bytes) continue;
+                if (!s.out) s.out = s.data;
+                if ((s.out == s.data && beams > MOST_HELD) != (pass == 1)) continue;
+                const double more = (double)groups * ceil((double)s.outer * (double)(s.row_bytes / column_width(s, beams)) / MOVE_THREADS);
+                if (more > 2147483647.0) { set_error("b2_beam_reorder: tensor %d is too large", i); return B2_ERR_BAD_SHAPE; }
+                if (blocks + (unsigned long long)more > 2147483647ull) break;
+                a.s[a.n] = s;
+                a.first[a.n++] = (unsigned)blocks;
+                blocks += (unsigned long long)more;
+            }
+            a.first[a.n] = (unsigned)blocks;
+            if (!blocks) continue;
+            const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, MOVE_THREADS, 0, (cudaStream_t)stream>>>(a); };
+            if (pass) go(beam_reorder_kernel<MAX_BEAMS>);
+            else if (beams <= 4) go(beam_reorder_kernel<4>);
+            else if (beams <= 8) go(beam_reorder_kernel<8>);
+            else go(beam_reorder_kernel<MOST_HELD>);
+            count_launch();
+            B2_CUDA(cudaGetLastError());
         }
-        a.first[a.n] = (unsigned)blocks;
-        if (!blocks) continue;
-        const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, MOVE_THREADS, 0, (cudaStream_t)stream>>>(a); };
-        if (beams <= 4) go(beam_reorder_kernel<4>);
-        else if (beams <= 8) go(beam_reorder_kernel<8>);
-        else if (beams <= 16) go(beam_reorder_kernel<16>);
-        else go(beam_reorder_kernel<MAX_BEAMS>);
-        count_launch();
-        B2_CUDA(cudaGetLastError());
     }
     return B2_OK;
 }

@@ -9,6 +9,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "ptx.cuh"
 #include "typed.cuh"
 
@@ -39,7 +41,26 @@ template <typename T> __device__ __forceinline__ float largest_magnitude(const u
     return m;
 }
 __device__ __forceinline__ float larger_magnitude(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
-__device__ __forceinline__ unsigned char quantised(float x, float inv) { return (unsigned char)__float_as_uint(fmaf(x, inv, 12582912.0f)); }
+// A row's scale and the factor of its values, from its largest magnitude
+struct RowScale {
+    float scale, inv;
+    bool finite;
+    __device__ __forceinline__ explicit RowScale(float most) {
+        finite = most < __int_as_float(0x7f800000);
+        const bool some = finite && most > TINY_ROW;
+        inv = some ? __fdiv_rn(127.0f, most) : 0.0f;
+        scale = !finite ? nanf("") : some ? __fdiv_rn(most, 127.0f) : 0.0f;
+    }
+    template <typename T> __device__ __forceinline__ Vec<unsigned char, 16 / sizeof(T)> quantised(const uint4 &h) const {
+        constexpr int W = 16 / sizeof(T);
+        T e[W];
+        memcpy(e, &h, 16);
+        Vec<unsigned char, W> o;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o.v[j] = finite ? (unsigned char)__float_as_uint(fmaf(to_float(e[j]), inv, 12582912.0f)) : 0;
+        return o;
+    }
+};
 
 // TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice
 template <typename T, int TEAM, int U, bool KEPT>
@@ -82,16 +103,11 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
     }
-    const bool finite = m < __int_as_float(0x7f800000), some = finite && m > TINY_ROW;
-    const float inv = some ? __fdiv_rn(127.0f, m) : 0.0f;
-    if (at == 0) scales[r] = !finite ? nanf("") : some ? __fdiv_rn(m, 127.0f) : 0.0f;
+    const RowScale s(m);
+    if (at == 0) scales[r] = s.scale;
     const auto store = [&](int v, const uint4 &h) {
         const int i0 = v * W - mis;
-        T e[W];
-        memcpy(e, &h, 16);
-        Vec<unsigned char, W> o;
-#pragma unroll
-        for (int j = 0; j < W; ++j) o.v[j] = finite ? quantised(to_float(e[j]), inv) : 0;
+        const Vec<unsigned char, W> o = s.template quantised<T>(h);
         if (out_vec && i0 >= 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
         else
 #pragma unroll
@@ -118,22 +134,17 @@ template <typename T> int quantize(signed char *q, long long ld_q, float *scales
         return B2_OK;
     };
     if (vecs <= 32 * 5) return go(int8_quantize_kernel<T, 32, 5, true>, 8);
+    if (vecs <= 32 * 9) return go(int8_quantize_kernel<T, 32, 9, true>, 8);
     if (vecs <= 256 * 4) return go(int8_quantize_kernel<T, 256, 4, true>, 1);
     if (vecs <= 256 * 9) return go(int8_quantize_kernel<T, 256, 9, true>, 1);
     return go(int8_quantize_kernel<T, 256, 1, false>, 1);
 }
 
 // ---- product --------------------------------------------------------------------------------------------------------------------------
-constexpr int BM = 128, BK = 128;                 // channels of a tile, positions of a slab (one swizzle row of 128 bytes)
+constexpr int BM = 128, BK = 128;                 // channels of a block's tile, positions of a slab (one swizzle row of 128 bytes)
 constexpr int A_BYTES = BM * BK;
 constexpr int THREADS = 320;                      // warp 0 copies, 1 multiplies, 2 to 9 store
 constexpr long long WAIT_CYCLES = 4000000000LL;   // about two seconds
-template <int BN> struct Shape {
-    static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
-    static constexpr int STAGES = BN >= 256 ? 4 : BN >= 128 ? 6 : 8;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // slack: the swizzle wants 1024-byte alignment
-    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
-};
 struct ProductArgs {
     const float *x_scales, *w_scales, *bias;
     long long ld_out, rows;
@@ -142,6 +153,54 @@ struct ProductArgs {
     int chained;
 };
 
+// N columns (rows r0 on of out) of a thread's tensor-memory lane (channel c; real: there is one) to out.  xs: their scales in shared memory, 16-byte aligned
+template <int N, typename O>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, float ws, float bias, bool real, bool ok, O *out, long long ld, long long r0, long long rows, int c) {
+    constexpr int STEP = N < 32 ? N : 32;
+    const long long left = rows - r0;
+    O *p = out + r0 * ld + c;
+#pragma unroll 1
+    for (int j0 = 0; j0 < N; j0 += STEP) {
+        if (j0 >= left) break;
+        uint32_t v[STEP];
+        if constexpr (STEP == 32) ptx::tmem_ld32(taddr + j0, v);
+        else if constexpr (STEP == 16) ptx::tmem_ld16(taddr + j0, v);
+        else ptx::tmem_ld8(taddr + j0, v);
+        ptx::tmem_ld_wait();
+        const auto put = [&](bool all) {
+#pragma unroll
+            for (int j = 0; j < STEP; j += 4) {
+                const float4 s = *reinterpret_cast<const float4 *>(xs + j0 + j);
+                const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // a tile that its block gave up on shows as NaN
+                    const float y = ok ? fmaf((float)(int)v[j + i], f[i] * ws, bias) : nanf("");
+                    if (real && (all || j0 + j + i < left)) *p = from_float<O>(y);
+                    p += ld;
+                }
+            }
+        };
+        if (j0 + STEP <= left) put(true); else put(false);
+    }
+}
+// a warp's copy of the scales of N rows from r0 on
+template <int N> __device__ __forceinline__ void load_scales(float *xs, const float *x_scales, long long r0, long long rows) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < N; j += 32)
+        if (j + lane < N) xs[j + lane] = r0 + j + lane < rows ? x_scales[r0 + j + lane] : 0.0f;
+    __syncwarp();
+}
+
+// Up to 128 rows: a block's tile has BN columns, the weights stream through the ring
+template <int BN> struct Shape {
+    static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
+    static constexpr int STAGES = BN >= 128 ? 6 : 8;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // slack: the swizzle wants 1024-byte alignment
+    static constexpr int TMEM = 2 * BN;
+};
 template <int BN, typename O>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
@@ -149,6 +208,7 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     typedef Shape<BN> S;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 5];
+    __shared__ __align__(16) float scales[8][BN / 2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int fail;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -177,21 +237,33 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         if (lane == 0) {
             unsigned i = 0;
             bool ok = true;
-            const auto wait_x = [&](unsigned k) {
-                if (k == 0 && a.chained) { grid_wait(); fence_async_global(); }
+            const unsigned mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * (unsigned)a.slabs;     // slabs of this block
+            const auto of = [&](unsigned k, int &r0, int &c0, int &at) {
+                const unsigned tile = blockIdx.x + k / (unsigned)a.slabs * gridDim.x;
+                r0 = (int)(tile % a.row_tiles) * BN;
+                c0 = (int)(tile / a.row_tiles) * BM;
+                at = (int)(k % (unsigned)a.slabs) * BK;
             };
-            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-                const int r0 = (int)(tile % a.row_tiles) * BN, c0 = (int)(tile / a.row_tiles) * BM;
-                for (int k = 0; k < a.slabs; ++k, ++i) {
-                    const int s = (int)(i % S::STAGES);
-                    if (!mbar_wait_bounded<false>(empty(s), ((i / S::STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                    const uint32_t at = ring + (uint32_t)s * S::STAGE_BYTES;
-                    mbar_expect_tx(full(s), S::STAGE_BYTES);
-                    tma_load_2d(at, &map_w, k * BK, c0, full(s));
-                    // the activations are what the launch before this one may still be writing
-                    wait_x(i);
-                    tma_load_2d(at + A_BYTES, &map_x, k * BK, r0, full(s));
-                }
+            int r0, c0, at;
+            // The first slabs' weights are on the way before the activations, which the launch before this one may still be writing
+            const unsigned first = min(mine, (unsigned)S::STAGES);
+            for (i = 0; i < first; ++i) {
+                of(i, r0, c0, at);
+                mbar_expect_tx(full((int)i), S::STAGE_BYTES);
+                tma_load_2d(ring + i * S::STAGE_BYTES, &map_w, at, c0, full((int)i));
+            }
+            if (a.chained) { grid_wait(); fence_async_global(); }
+            for (i = 0; i < first; ++i) {
+                of(i, r0, c0, at);
+                tma_load_2d(ring + i * S::STAGE_BYTES + A_BYTES, &map_x, at, r0, full((int)i));
+            }
+            for (; i < mine; ++i) {
+                const int s = (int)(i % S::STAGES);
+                if (!mbar_wait_bounded<false>(empty(s), ((i / S::STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                of(i, r0, c0, at);
+                mbar_expect_tx(full(s), S::STAGE_BYTES);
+                tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES, &map_w, at, c0, full(s));
+                tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES + A_BYTES, &map_x, at, r0, full(s));
             }
             if (!ok)      // copies under way end before the block does
                 for (unsigned j = i > (unsigned)S::STAGES ? i - S::STAGES : 0; j < i; ++j) {
@@ -228,7 +300,7 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
     } else {
         // A warp reads the tensor-memory lanes 32 * (warp % 4) on; warps 2 to 5 take the first half of the columns, 6 to 9 the second
-        constexpr int HALF = BN / 2, STEP = HALF < 16 ? 8 : 16;
+        constexpr int HALF = BN / 2;
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         unsigned n = 0;
         bool ok = true;
@@ -238,28 +310,11 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             const int c = (int)(tile / a.row_tiles) * BM + 32 * quarter + lane;
             const bool real = c < a.channels;
             const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
-            // a tile that its block gave up on shows as NaN
+            load_scales<HALF>(scales[warp - 2], a.x_scales, r0, a.rows);
             ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
             if (!ok && lane == 0) fail = 1;
             tc_fence_after();
-            for (int j0 = 0; j0 < HALF; j0 += STEP) {
-                if (r0 + j0 >= a.rows) break;
-                uint32_t v[16];
-                if (ok) {
-                    if constexpr (STEP == 16) tmem_ld16(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF + j0, v);
-                    else tmem_ld8(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF + j0, v);
-                    tmem_ld_wait();
-                }
-                const float xs = lane < STEP && r0 + j0 + lane < a.rows ? a.x_scales[r0 + j0 + lane] : 0.0f;
-#pragma unroll
-                for (int j = 0; j < STEP; ++j) {
-                    const float s = __shfl_sync(0xffffffffu, xs, j);
-                    if (real && r0 + j0 + j < a.rows) {
-                        const float y = ok ? fmaf((float)(int)v[j], s * ws, bias) : nanf("");
-                        out[(r0 + j0 + j) * a.ld_out + c] = from_float<O>(y);
-                    }
-                }
-            }
+            store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales[warp - 2], ws, bias, real, ok, out, a.ld_out, r0, a.rows, c);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty((int)(n & 1u)));
@@ -268,6 +323,300 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem, S::TMEM);
+}
+
+// Few rows of activations that are no integers yet: every block quantises them for itself, into the layout of the tensor cores' operand, while its
+// first slabs of weights are on the way.  One launch, and the activations pass through no memory.
+constexpr int ROWS_STAGES = 8, ROWS_X_BYTES = 80 * 1024;
+template <int BN> constexpr int rows_smem(int slabs) { return ROWS_STAGES * A_BYTES + slabs * BN * BK + 1024; }
+template <int BN, typename T, typename O>
+__global__ void __launch_bounds__(THREADS, 1)
+int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long long ld_x, int dim, O *out, const ProductArgs a) {
+    using namespace ptx;
+    constexpr int STAGES = ROWS_STAGES, W = 16 / sizeof(T), TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES + 6];
+    __shared__ __align__(16) float scales[BN];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int fail;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars), operand = ring + STAGES * A_BYTES;
+    const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
+    const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4), x_full = bar0 + 8u * (uint32_t)(2 * STAGES + 5);
+    const unsigned tiles = a.channel_tiles;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 8); }
+        mbar_init(idle, 1);
+        mbar_init(x_full, 8);
+        fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) tmem_alloc(smem_u32((const void *)&tmem_slot), TMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned i = 0;
+            bool ok = true;
+            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % STAGES);
+                    if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    mbar_expect_tx(full(s), A_BYTES);
+                    tma_load_2d(ring + (uint32_t)s * A_BYTES, &map_w, k * BK, (int)tile * BM, full(s));
+                }
+            if (!ok)
+                for (unsigned j = i > (unsigned)STAGES ? i - STAGES : 0; j < i; ++j) {
+                    volatile int never = 0;
+                    mbar_wait_bounded<false>(full((int)(j % STAGES)), (j / STAGES) & 1u, &never, WAIT_CYCLES);
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc_s8(BM, BN);
+            unsigned i = 0, n = 0;
+            bool ok = mbar_wait_bounded<false>(x_full, 0, &fail, WAIT_CYCLES);
+            if (!ok) fail = 1;
+            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+                const uint32_t d = tmem + (n & 1u) * BN;
+                if (!mbar_wait_bounded<false>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                tc_fence_after();
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % STAGES);
+                    if (!mbar_wait_bounded<false>(full(s), (i / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = ring + (uint32_t)s * A_BYTES, b = operand + (uint32_t)k * (BN * BK);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 32; ++kk) mma_s8(d, desc_kmajor_sw128(at + kk * 32, 1024), desc_kmajor_sw128(b + kk * 32, 1024), idesc, (k | kk) ? 1u : 0u);
+                    mma_commit(empty(s));
+                }
+                if (ok) mma_commit(acc_full((int)(n & 1u)));
+            }
+            if (!ok) {
+                volatile int never = 0;
+                mma_commit(idle);
+                mbar_wait_bounded<false>(idle, 0, &never, WAIT_CYCLES);
+            }
+        }
+    } else {
+        // the rows of x: a warp's rows w, w + 8, ...; columns without a row, and positions behind the last one, meet zeros of the weights or are not stored
+        const int w = warp - 2;
+        unsigned char *const to = smem_raw + (operand - smem_u32(smem_raw));
+        for (int r = w; r < BN && r < a.rows; r += 8) {
+            const T *row = x + r * ld_x;
+            const int mis = (int)(((uintptr_t)row & 15) / sizeof(T)), vecs = (mis + dim + W - 1) / W;
+            const auto load = [&](int v) -> uint4 {
+                const int i0 = v * W - mis;
+                if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(row + i0);
+                T e[W];
+#pragma unroll
+                for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? row[i0 + j] : from_float<T>(0.0f);
+                uint4 o;
+                memcpy(&o, e, 16);
+                return o;
+            };
+            constexpr int U = 8;
+            uint4 held[U];
+            float m = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) held[u] = lane + 32 * u < vecs ? load(lane + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) m = larger_magnitude(m, largest_magnitude<T>(held[u]));
+            for (int v = lane + 32 * U; v < vecs; v += 32) m = larger_magnitude(m, largest_magnitude<T>(load(v)));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const RowScale s(m);
+            if (lane == 0) scales[r] = s.scale;
+            const auto store = [&](int v, const uint4 &h) {
+                const int i0 = v * W - mis;
+                const Vec<unsigned char, W> o = s.template quantised<T>(h);
+                // slab, row of 128 bytes, 16-byte chunk with its index xor the row's
+                const auto place = [&](int k) { return (k / BK) * (BN * BK) + r * BK + ((((k % BK) >> 4) ^ (r & 7)) << 4) + (k & 15); };
+                if (mis == 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + place(i0)) = o;
+                else
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (i0 + j >= 0 && i0 + j < dim) to[place(i0 + j)] = o.v[j];
+            };
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (lane + 32 * u < vecs) store(lane + 32 * u, held[u]);
+            for (int v = lane + 32 * U; v < vecs; v += 32) store(v, load(v));
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_full);
+        bar_named(1, 256);                   // the scales
+        constexpr int HALF = BN / 2;
+        const int quarter = warp & 3, half = w >> 2;
+        unsigned n = 0;
+        bool ok = true;
+        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+            const int c = (int)tile * BM + 32 * quarter + lane;
+            const bool real = c < a.channels;
+            const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
+            if (!ok && lane == 0) fail = 1;
+            tc_fence_after();
+            store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales + half * HALF, ws, bias, real, ok, out, a.ld_out, half * HALF, a.rows, c);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty((int)(n & 1u)));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, TMEM);
+}
+
+// Many rows: a pair of blocks (cta_group::2) has a tile of 256 channels, 128 in each block, and 256 rows, of which each block holds 128 in its shared memory.  A
+// slab so costs a block 32 KB of copies and 32 KB of operand reads for 512 cycles of multiplication; by itself, with the same tile, it would be 48 and 48.
+constexpr int PAIR_BN = 256, PAIR_STAGE = A_BYTES + PAIR_BN / 2 * BK, PAIR_STAGES = 6, PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024, PAIR_TMEM = 512;
+template <typename O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
+    using namespace ptx;
+    constexpr int BN = PAIR_BN, STAGES = PAIR_STAGES;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES + 5];
+    __shared__ __align__(16) float scales[8][BN / 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int fail;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
+    // full and acc_empty: the even block's count; empty, acc_full: each block has its own
+    const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
+    const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4);
+    const unsigned tiles = a.row_tiles * a.channel_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 16); }
+        mbar_init(idle, 1);
+        fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32((const void *)&tmem_slot), PAIR_TMEM);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned i = 0;
+            bool ok = true;
+            if (a.chained) { grid_wait(); fence_async_global(); }
+            for (unsigned tile = pair; tile < tiles && ok; tile += pairs) {
+                const int r0 = (int)(tile % a.row_tiles) * BN + (int)rank * (BN / 2), c0 = (int)(tile / a.row_tiles) * (2 * BM) + (int)rank * BM;
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % STAGES);
+                    if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    const uint32_t at = ring + (uint32_t)s * PAIR_STAGE, bar = map_to_rank(full(s), 0);
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * PAIR_STAGE);
+                    tma_load_2d_pair(at, &map_w, k * BK, c0, bar);
+                    tma_load_2d_pair(at + A_BYTES, &map_x, k * BK, r0, bar);
+                }
+            }
+            if (!ok && rank == 0)      // copies under way end before the blocks do
+                for (unsigned j = i > (unsigned)STAGES ? i - STAGES : 0; j < i; ++j) {
+                    volatile int never = 0;
+                    mbar_wait_bounded<false>(full((int)(j % STAGES)), (j / STAGES) & 1u, &never, WAIT_CYCLES);
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = idesc_s8(2 * BM, BN);
+            unsigned i = 0, n = 0;
+            bool ok = true;
+            for (unsigned tile = pair; tile < tiles && ok; tile += pairs, ++n) {
+                const uint32_t d = tmem + (n & 1u) * BN;
+                if (!mbar_wait_bounded<true>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                tc_fence_after();
+                for (int k = 0; k < a.slabs; ++k, ++i) {
+                    const int s = (int)(i % STAGES);
+                    if (!mbar_wait_bounded<true>(full(s), (i / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = ring + (uint32_t)s * PAIR_STAGE;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 32; ++kk)
+                        mma_s8_pair(d, desc_kmajor_sw128(at + kk * 32, 1024), desc_kmajor_sw128(at + A_BYTES + kk * 32, 1024), idesc, (k | kk) ? 1u : 0u);
+                    mma_commit_pair(empty(s));
+                }
+                if (ok) mma_commit_pair(acc_full((int)(n & 1u)));
+            }
+            if (!ok) {
+                volatile int never = 0;
+                mma_commit_pair(idle);
+                mbar_wait_bounded<false>(idle, 0, &never, WAIT_CYCLES);
+            }
+        }
+    } else {
+        constexpr int HALF = BN / 2;
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        unsigned n = 0;
+        bool ok = true;
+        if (a.chained) grid_wait();
+        for (unsigned tile = pair; tile < tiles; tile += pairs, ++n) {
+            const long long r0 = (long long)(tile % a.row_tiles) * BN + half * HALF;
+            const int c = (int)(tile / a.row_tiles) * (2 * BM) + (int)rank * BM + 32 * quarter + lane;
+            const bool real = c < a.channels;
+            const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
+            load_scales<HALF>(scales[warp - 2], a.x_scales, r0, a.rows);
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
+            if (!ok && lane == 0) fail = 1;
+            tc_fence_after();
+            store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales[warp - 2], ws, bias, real, ok, out, a.ld_out, r0, a.rows, c);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(acc_empty((int)(n & 1u)), 0));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();          // neither block leaves while the other's arrivals and copies may still reach it
+    if (warp == 1) tmem_dealloc_pair(tmem, PAIR_TMEM);
+}
+
+// pairs of blocks that run side by side, by device
+int pair_count(const void *kernel, int *out) {
+    static std::mutex mu;
+    static int known[MAX_DEVICES];      // of all element types: a block has its SM to itself
+    const int dev = current_device();
+    if (dev < 0) { set_error("no current CUDA device (or an ordinal beyond %d)", MAX_DEVICES - 1); return B2_ERR_CUDA; }
+    std::lock_guard<std::mutex> lk(mu);
+    int &n = known[dev];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * (unsigned)(sm_count() / 2 > 0 ? sm_count() / 2 : 1));
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = PAIR_SMEM;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
+        if (clusters < 1) { set_error("b2_int8_product: no pair of blocks fits on the device"); return B2_ERR_CUDA; }
+        n = clusters;
+    }
+    *out = n;
+    return B2_OK;
 }
 
 template <int BN, typename O> int launch_product(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
@@ -282,6 +631,19 @@ template <int BN, typename O> int launch_product(const CUtensorMap &mw, const CU
     B2_CUDA(cudaGetLastError());
     return B2_OK;
 }
+template <typename O> int launch_pairs(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
+    const auto kernel = int8_pair_kernel<O>;
+    B2_TRY(set_max_dynamic_smem((const void *)kernel, PAIR_SMEM));
+    int pairs;
+    B2_TRY(pair_count((const void *)kernel, &pairs));
+    const long long tiles = (long long)a.row_tiles * a.channel_tiles;
+    const unsigned blocks = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
+    if (a.chained) return launch_chained(int8_pair_kernel<O>, dim3(blocks), dim3(THREADS), PAIR_SMEM, st, mw, mx, out, a);
+    kernel<<<blocks, THREADS, PAIR_SMEM, st>>>(mw, mx, out, a);
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
+}
 
 size_t pitch_of(int dim) { return ((size_t)dim + 15) & ~(size_t)15; }
 bool sizes_fit(long long rows, int channels, int dim) { return rows >= 0 && rows <= 0x7fffff00ll && channels >= 1 && channels <= 0x7fffff00 && dim >= 1 && dim <= 131071; }
@@ -289,19 +651,39 @@ bool sizes_fit(long long rows, int channels, int dim) { return rows >= 0 && rows
 template <typename O> int product(O *out, const signed char *x, long long ld_x, const signed char *w, long long ld_w, int dim, ProductArgs a, cudaStream_t st) {
     const auto go = [&](auto columns) -> int {
         constexpr int BN = decltype(columns)::value;
+        constexpr bool PAIR = BN == PAIR_BN;
         CUtensorMap mw, mx;
         B2_TRY(make_byte_map(&mw, w, dim, a.channels, ld_w, BM));
-        B2_TRY(make_byte_map(&mx, x, dim, a.rows, ld_x, BN));
+        B2_TRY(make_byte_map(&mx, x, dim, a.rows, ld_x, PAIR ? BN / 2 : BN));
         a.row_tiles = (unsigned)((a.rows + BN - 1) / BN);
-        a.channel_tiles = (unsigned)((a.channels + BM - 1) / BM);
+        a.channel_tiles = (unsigned)((a.channels + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM));
         if ((double)a.row_tiles * a.channel_tiles > 4e9) { set_error("b2_int8_product: %lld rows of %d channels", a.rows, a.channels); return B2_ERR_BAD_SHAPE; }
-        return launch_product<BN, O>(mw, mx, out, a, st);
+        if constexpr (PAIR) return launch_pairs<O>(mw, mx, out, a, st);
+        else return launch_product<BN, O>(mw, mx, out, a, st);
     };
     if (a.rows <= 16) return go(std::integral_constant<int, 16>());
     if (a.rows <= 32) return go(std::integral_constant<int, 32>());
     if (a.rows <= 64) return go(std::integral_constant<int, 64>());
     if (a.rows <= 128) return go(std::integral_constant<int, 128>());
-    return go(std::integral_constant<int, 256>());
+    return go(std::integral_constant<int, PAIR_BN>());
+}
+// whether the call runs as one launch that quantises in every block
+bool few_rows(long long rows, int dim) { return rows <= 32 && (rows <= 16 ? 16 : 32) * (((long long)dim + BK - 1) / BK * BK) <= ROWS_X_BYTES; }
+template <typename T, typename O> int product_of_few(O *out, const T *x, long long ld_x, const signed char *w, long long ld_w, int dim, ProductArgs a, cudaStream_t st) {
+    CUtensorMap mw;
+    B2_TRY(make_byte_map(&mw, w, dim, a.channels, ld_w, BM));
+    a.row_tiles = 1;
+    a.channel_tiles = (unsigned)((a.channels + BM - 1) / BM);
+    const unsigned blocks = (unsigned)((long long)a.channel_tiles < sm_count() ? (int)a.channel_tiles : sm_count());
+    const auto go = [&](auto kernel, int bytes) -> int {
+        B2_TRY(set_max_dynamic_smem((const void *)kernel, ROWS_STAGES * A_BYTES + ROWS_X_BYTES + 1024));
+        kernel<<<blocks, THREADS, bytes, st>>>(mw, x, ld_x, dim, out, a);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+        return B2_OK;
+    };
+    if (a.rows <= 16) return go(int8_rows_kernel<16, T, O>, rows_smem<16>(a.slabs));
+    return go(int8_rows_kernel<32, T, O>, rows_smem<32>(a.slabs));
 }
 
 }  // namespace
@@ -359,6 +741,11 @@ int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, in
         const size_t need = b2_int8_product_workspace(rows, channels, dim);
         if (!workspace || !aligned_to(workspace, 16)) { set_error("b2_int8_product: the workspace is missing or not aligned to 16 bytes"); return B2_ERR_BAD_ARG; }
         if (workspace_bytes < need) { set_error("b2_int8_product: a workspace of %zu bytes, %zu are needed", workspace_bytes, need); return B2_ERR_BAD_SHAPE; }
+        if (few_rows(rows, dim))
+            return with_type(x_type, [&](auto *t) {
+                const B2_ELEM(t) *in = (const B2_ELEM(t) *)x;
+                return with_type(out_type, [&](auto *o) { return product_of_few((B2_ELEM(o) *)out, in, ld_x, w, ld_w, dim, a, st); });
+            });
         signed char *q = (signed char *)workspace;
         float *scales = (float *)(q + (size_t)rows * pitch_of(dim));
         B2_TRY(with_type(x_type, [&](auto *t) { return quantize(q, (long long)pitch_of(dim), scales, (const B2_ELEM(t) *)x, rows, dim, ld_x, st); }));

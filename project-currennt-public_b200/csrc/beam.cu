@@ -35,27 +35,40 @@ __device__ __forceinline__ bool runs(const SelectArgs &a, long long row) {
     return s > neg_inf() && s < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000) && !(a.finished && a.finished[row]);
 }
 
-template <typename T, int THREADS, bool MASK>
-__global__ void __launch_bounds__(THREADS, 3) beam_rows_kernel(const T *logits, const SelectArgs a) {
-    constexpr int W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, GROUP = THREADS / 64, CAP = 512;
+// -inf in the places of q whose bytes of `on` are 0
+template <typename T> __device__ __forceinline__ void rule_out(uint4 &q, const Vec<unsigned char, 16 / sizeof(T)> &on) {
+    unsigned w[4] = {q.x, q.y, q.z, q.w}, bytes[4 / sizeof(T) + 1];
+    memcpy(bytes, &on, sizeof(on));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        unsigned off;                                     // all ones in the places that go
+        if constexpr (sizeof(T) == 4) off = __byte_perm(__vcmpeq4(bytes[0], 0), 0, 0x1111 * i);
+        else off = __byte_perm(__vcmpeq4(bytes[i / 2], 0), 0, i & 1 ? 0x3322 : 0x1100);
+        w[i] = (w[i] & ~off) | (Raw<T>::NONE & off);
+    }
+    q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, bool MASK>
+__global__ void __launch_bounds__(SLICE_THREADS, 3) beam_rows_kernel(const T *logits, const SelectArgs a) {
+    constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, GROUP = THREADS / 64, CAP = 256;
     __shared__ __align__(16) float maxima[64];
     __shared__ float tops[WARPS], sums[WARPS];
-    __shared__ Key found[CAP];
+    __shared__ __align__(16) T hits[CAP][W];            // vectors that hold an entry of interest
+    __shared__ int hit_at[CAP];                           // where they are in the row
+    __shared__ Key found[CAP], winner[WARPS];
     __shared__ float bound;
-    __shared__ int count;
-    __shared__ Key winner[WARPS];
+    __shared__ int n_hits, count;
     grid_release();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const long long row = blockIdx.x / (unsigned)a.slices;
     const int part = (int)(blockIdx.x % (unsigned)a.slices);
-    if (!runs(a, row)) return;
-    Part *const to = a.parts + row * a.slices + part;
-    Key *const list = a.lists + (row * a.slices + part) * a.top;
     const T *x = logits + row * a.ld;
     const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
     const unsigned char *mk = MASK ? a.mask + row * a.ld_mask : nullptr;
     const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
     const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
+    if (!runs(a, row)) return;
     uint4 q[U];
     Vec<unsigned char, W> on[MASK ? U : 1];
 #pragma unroll
@@ -64,56 +77,59 @@ __global__ void __launch_bounds__(THREADS, 3) beam_rows_kernel(const T *logits, 
         const bool inside = v < v1, whole = i0 >= 0 && i0 + W <= a.vocab;
         q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
         if (inside && whole) q[u] = *reinterpret_cast<const uint4 *>(x + i0);
-        else if (inside) {
-            T e[W];
+        if (MASK && inside && whole && mask_vec) on[u] = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
+    }
+    // the ends of the row, and masks whose bytes lie across the vectors
+    if (v0 * W < mis || (v1 - 1) * W - mis + W > a.vocab || (MASK && !mask_vec)) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < a.vocab ? x[i0 + j] : from_float<T>(neg_inf());
-            memcpy(&q[u], e, 16);
-        }
-        if (MASK) {
-            if (inside && whole && mask_vec) on[u] = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
-            else
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + t + u * THREADS, i0 = v * W - mis;
+            const bool whole = i0 >= 0 && i0 + W <= a.vocab;
+            if (v < v1 && !whole) {
+                T e[W];
 #pragma unroll
-                for (int j = 0; j < W; ++j) on[u].v[j] = inside && i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
+                for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < a.vocab ? x[i0 + j] : from_float<T>(neg_inf());
+                memcpy(&q[u], e, 16);
+            }
+            if (MASK && v < v1 && !(whole && mask_vec))
+#pragma unroll
+                for (int j = 0; j < W; ++j) on[u].v[j] = i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
         }
     }
     if (MASK)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            T e[W];
-            memcpy(e, &q[u], 16);
+        for (int u = 0; u < U; ++u)
+            if (v0 + t + u * THREADS < v1) rule_out<T>(q[u], on[u]);
+    unsigned big[U];
 #pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (!on[u].v[j]) e[j] = from_float<T>(neg_inf());
-            memcpy(&q[u], e, 16);
-        }
-    unsigned big = larger_of<T>(q[0]);
+    for (int u = 0; u < U; ++u) big[u] = larger_of<T>(q[u]);
+    unsigned biggest = big[0];
 #pragma unroll
-    for (int u = 1; u < U; ++u) big = Raw<T>::larger(big, larger_of<T>(q[u]));
-    const float mine = __fmul_rn(Raw<T>::largest(big), a.scale);
+    for (int u = 1; u < U; ++u) biggest = Raw<T>::larger(biggest, big[u]);
+    const float mine = __fmul_rn(Raw<T>::largest(biggest), a.scale);
     float most = mine;
 #pragma unroll
-    for (int o = 1; o < GROUP && o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+    for (int o = 1; o < GROUP; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
     if (t % GROUP == 0) maxima[t / GROUP] = most;
 #pragma unroll
     for (int o = GROUP; o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
     if (lane == 0) tops[warp] = most;
-    if (t == 0) { count = 0; bound = neg_inf(); }
+    if (t == 0) { n_hits = count = 0; bound = neg_inf(); }
     __syncthreads();
     most = tops[lane % WARPS];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+    for (int o = WARPS / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
     if (t < 64) {
         // the place of this group's maximum among the 64 (NaN: the row has no continuations)
-        const float mine64 = maxima[t];
+        const float group = maxima[t];
         int before = 0;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 64; i += 4) {
             const float4 m = *reinterpret_cast<const float4 *>(&maxima[i]);
-            before += (m.x > mine64 || (m.x == mine64 && i < t)) + (m.y > mine64 || (m.y == mine64 && i + 1 < t)) + (m.z > mine64 || (m.z == mine64 && i + 2 < t)) +
-                      (m.w > mine64 || (m.w == mine64 && i + 3 < t));
+            before += (m.x > group || (m.x == group && i < t)) + (m.y > group || (m.y == group && i + 1 < t)) + (m.z > group || (m.z == group && i + 2 < t)) +
+                      (m.w > group || (m.w == group && i + 3 < t));
         }
-        if (before == a.top - 1) bound = mine64;
+        if (before == a.top - 1) bound = group;
     }
     float s = 0.0f;
     if (most != neg_inf()) {
@@ -137,72 +153,72 @@ __global__ void __launch_bounds__(THREADS, 3) beam_rows_kernel(const T *logits, 
     s = warp_sum(s);
     if (lane == 0) sums[warp] = s;
     __syncthreads();
-    // the logits are taken apart again below: kept apart over the barrier, they do not fit into the registers
-#pragma unroll
-    for (int u = 0; u < U; ++u) asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
-    const float limit = bound;
-    if (mine >= limit && mine > neg_inf())
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float z[W];
-            Raw<T>::values(z, q[u]);
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const float v = __fmul_rn(z[j], a.scale);
-                if (v >= limit && v > neg_inf()) {
-                    const int at = atomicAdd(&count, 1);
-                    if (at < CAP) found[at] = make_key(v, (v0 + t + u * THREADS) * W - mis + j);
-                }
-            }
-        }
-    __syncthreads();
-    const int n = count;
-    if (n <= CAP) {
-        for (int i = t; i < n; i += THREADS) {
-            const Key k = found[i];
-            int before = 0;
-            for (int j = 0; j < n; ++j) before += found[j] > k;
-            if (before < a.top) list[before] = k;
-        }
-        for (int i = n + t; i < a.top; i += THREADS) list[i] = 0;
-    } else {
-        // many equal ones: the next best in turn
-        Key last = ~0ull;
-        for (int i = 0; i < a.top; ++i) {
-            Key k = 0;
-#pragma unroll
-            for (int u = 0; u < U; ++u) asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float z[W];
-                Raw<T>::values(z, q[u]);
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const float v = __fmul_rn(z[j], a.scale);
-                    const Key e = make_key(v, (v0 + t + u * THREADS) * W - mis + j);
-                    if (v > neg_inf() && e < last && e > k) k = e;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const Key other = __shfl_xor_sync(FULL, k, o);
-                if (other > k) k = other;
-            }
-            if (lane == 0) winner[warp] = k;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-                if (winner[w] > k) k = winner[w];
-            if (t == 0) list[i] = k;
-            last = k;
-            __syncthreads();
-        }
-    }
     if (t == 0) {
         float all = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) all += sums[w];
-        *to = {most, all};
+        a.parts[row * a.slices + part] = {most, all};
+    }
+    Key *const list = a.lists + (row * a.slices + part) * a.top;
+    const float limit = bound;
+    if (mine >= limit)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float m = __fmul_rn(Raw<T>::largest(big[u]), a.scale);
+            if (m >= limit && m > neg_inf()) {
+                const int at = atomicAdd(&n_hits, 1);
+                if (at < CAP) {
+                    *reinterpret_cast<uint4 *>(&hits[at][0]) = q[u];
+                    hit_at[at] = (v0 + t + u * THREADS) * W - mis;
+                }
+            }
+        }
+    __syncthreads();
+    const int h = n_hits;
+    if (h <= CAP)
+        for (int i = t; i < h * W; i += THREADS) {
+            const float z = __fmul_rn(to_float(hits[i / W][i % W]), a.scale);
+            if (z >= limit && z > neg_inf()) {
+                const int at = atomicAdd(&count, 1);
+                if (at < CAP) found[at] = make_key(z, hit_at[i / W] + i % W);
+            }
+        }
+    __syncthreads();
+    const int n = count;
+    if (h <= CAP && n <= CAP) {
+        if (t < n) {
+            const Key k = found[t];
+            int before = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) before += found[j] > k;
+            if (before < a.top) list[before] = k;
+        } else if (t < a.top) list[t] = 0;
+        return;
+    }
+    // many that reach the bound, as in a row of equal logits: the next best in turn
+    const int i0 = max(v0 * W - mis, 0), i1 = min(v1 * W - mis, a.vocab);
+    Key last = ~0ull;
+    for (int i = 0; i < a.top; ++i) {
+        Key k = 0;
+        for (int e = i0 + t; e < i1; e += THREADS) {
+            const float z = __fmul_rn(to_float(x[e]), a.scale);
+            if (!(z >= limit) || z == neg_inf() || (MASK && !mk[e])) continue;
+            const Key c = make_key(z, e);
+            if (c < last && c > k) k = c;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const Key other = __shfl_xor_sync(FULL, k, o);
+            if (other > k) k = other;
+        }
+        if (lane == 0) winner[warp] = k;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+            if (winner[w] > k) k = winner[w];
+        if (t == 0) list[i] = k;
+        last = k;
+        __syncthreads();
     }
 }
 
@@ -357,8 +373,8 @@ template <typename T> int select(const T *logits, SelectArgs a, int type, cudaSt
     a.slice = (vecs + a.slices - 1) / a.slices;
     const long long blocks = a.groups * a.beams * a.slices;
     if (blocks > 0x7fffffffll) { set_error("b2_beam_select: %lld rows of %d", a.groups * a.beams, a.vocab); return B2_ERR_BAD_SHAPE; }
-    if (a.mask) beam_rows_kernel<T, SLICE_THREADS, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
-    else beam_rows_kernel<T, SLICE_THREADS, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    if (a.mask) beam_rows_kernel<T, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    else beam_rows_kernel<T, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
     count_launch();
     B2_CUDA(cudaGetLastError());
     return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(JOIN_THREADS), 0, st, a);

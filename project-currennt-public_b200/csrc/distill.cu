@@ -149,13 +149,12 @@ constexpr int PIECE = 128, RING = 3;      // vectors of 16 bytes in a piece (4 a
 
 // A row's place among the 16-byte boundaries: `head` entries before the first one, nv vectors, the rest behind
 struct Row {
-    int head, nv, pieces;
+    int head, nv;
     template <typename T> __device__ __forceinline__ Row(const T *x, int vocab) {
         constexpr int W = 16 / sizeof(T);
         head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);
         if (head > vocab) head = vocab;
         nv = (vocab - head) / W;
-        pieces = (nv + PIECE - 1) / PIECE;
     }
 };
 
@@ -170,28 +169,39 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = WARPS > 1 ? warp : 0;
     const long long team = WARPS > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + warp, teams = WARPS > 1 ? gridDim.x : (long long)gridDim.x * 8;
 
-    // what is copied next: piece ic of row ir
+    // what is copied next: the vectors src on of row ir, `ahead_left` of which are left for this warp and those behind it
     long long ir = team;
-    int ic = w, slot = 0;
+    int slot = 0, ahead_left = 0;
+    const uint4 *src = nullptr;
+    const auto enter = [&]() {
+        if (ir >= a.rows) return;
+        const T *x = logits + ir * a.ld;
+        const Row g(x, a.vocab);
+        src = reinterpret_cast<const uint4 *>(x + g.head) + w * PIECE + lane;
+        ahead_left = g.nv - w * PIECE;
+    };
+    const unsigned ring0 = (unsigned)__cvta_generic_to_shared(&ring[0][lane]);
     const auto issue = [&](int to) {
-        while (ir < a.rows) {
-            const T *x = logits + ir * a.ld;
-            const Row g(x, a.vocab);
-            if (ic < g.pieces) {
-                const int n = min(PIECE, g.nv - ic * PIECE);
-                const uint4 *from = reinterpret_cast<const uint4 *>(x + g.head) + ic * PIECE;
-                const unsigned at = (unsigned)__cvta_generic_to_shared(&ring[to][0]);
+        while (ahead_left <= 0 && ir < a.rows) {
+            ir += teams;
+            enter();
+        }
+        if (ahead_left > 0) {
+            const unsigned at = ring0 + to * (PIECE * 16);
+            if (ahead_left >= PIECE) {
+#pragma unroll
+                for (int u = 0; u < PIECE / 32; ++u) cp_async<16>(at + 512 * u, src + 32 * u);
+            } else {
 #pragma unroll
                 for (int u = 0; u < PIECE / 32; ++u)
-                    if (lane + 32 * u < n) cp_async<16>(at + 16 * (lane + 32 * u), from + lane + 32 * u);
-                ic += WARPS;
-                break;
+                    if (lane + 32 * u < ahead_left) cp_async<16>(at + 512 * u, src + 32 * u);
             }
-            ic = w;
-            ir += teams;
+            src += WARPS * PIECE;
+            ahead_left -= WARPS * PIECE;
         }
         cp_commit();
     };
+    enter();
     List<SLOTS> list, next;
     float edge = 0.0f;
     const auto ahead = [&](long long r) {
@@ -234,26 +244,32 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
             // +inf as e^(inf - inf)
             if (t.m == __int_as_float(0x7f800000)) t.m = t.s = nanf("");
         }
-        for (int c = w; c < g.pieces; c += WARPS) {
+        int first = g.head + w * PIECE * W;
+        for (int left = g.nv - w * PIECE; left > 0; left -= WARPS * PIECE, first += WARPS * PIECE * W) {
             cp_wait<RING - 2>();
             __syncwarp();
-            issue((slot + RING - 1) % RING);
+            issue(slot == 0 ? RING - 1 : slot - 1);
             T *piece = reinterpret_cast<T *>(&ring[slot][0]);
-            const int first = g.head + c * PIECE * W, n = min(PIECE, g.nv - c * PIECE);
+            const unsigned n = (unsigned)min(PIECE, left) * W;
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s)
-                if ((unsigned)(list.tok[s] - first) < (unsigned)(n * W)) {
+                if ((unsigned)(list.tok[s] - first) < n) {
                     z[s] = __fmul_rn(to_float(piece[list.tok[s] - first]), a.scale);
                     if (REST) piece[list.tok[s] - first] = from_float<T>(neg_inf());
                 }
             if (REST) __syncwarp();
             uint4 q[PIECE / 32];
+            if (left >= PIECE) {
 #pragma unroll
-            for (int u = 0; u < PIECE / 32; ++u)
-                q[u] = lane + 32 * u < n ? ring[slot][lane + 32 * u] : make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+                for (int u = 0; u < PIECE / 32; ++u) q[u] = ring[slot][lane + 32 * u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < PIECE / 32; ++u)
+                    q[u] = lane + 32 * u < left ? ring[slot][lane + 32 * u] : make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+            }
             __syncwarp();
             add_vectors<T, PIECE / 32>(t, q, a.scale);
-            slot = (slot + 1) % RING;
+            slot = slot == RING - 1 ? 0 : slot + 1;
         }
         t = warp_join(t);
         if (WARPS > 1) {
@@ -342,7 +358,7 @@ struct RowGrad { float base, factor; int what; };      // what: 0 zeros, 1 gradi
 
 // TEAM threads a row (32: a warp; 256: a block, several of them for a long row), each up to U vectors apart by TEAM
 template <typename T, int TEAM, int U, int SLOTS, bool REST, bool ADD>
-__global__ void __launch_bounds__(256) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
+__global__ void __launch_bounds__(256, U <= 4 ? 5 : 3) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
     constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
     __shared__ RowGrad shared[TEAMS];
     const int lane = threadIdx.x & 31, team = threadIdx.x / TEAM, at = threadIdx.x % TEAM;
@@ -357,25 +373,30 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(T *dlogits, const
     // the entries of this block
     const int lo = max(0, seg * TEAM * U * W - mis), hi = TEAM == 256 ? min(a.vocab, (seg + 1) * TEAM * U * W - mis) : a.vocab;
     const auto whole = [&](int v) { return v * W >= mis && (v + 1) * W <= mis + a.vocab; };
+    // the list first: everything waits for it
+    List<SLOTS> list;
+    float lse = 0.0f, rest = 0.0f, weight = 0.0f;
+    if (at < 32) {
+        list.load(a.tokens, a.lps, r, a.top);
+        lse = a.lse[r];
+        rest = REST ? a.lse_rest[r] : 0.0f;
+        weight = a.dloss[r] * a.scale;
+    }
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (whole(first + u * TEAM)) raw[u] = *reinterpret_cast<const uint4 *>(x - mis + (size_t)(first + u * TEAM) * W);
-
-    List<SLOTS> list;
     float own[SLOTS];
     RowGrad g = {0.0f, 0.0f, 0};
     if (at < 32) {
-        list.load(a.tokens, a.lps, r, a.top);
-        const float lse = a.lse[r], rest = REST ? a.lse_rest[r] : 0.0f, weight = a.dloss[r] * a.scale;
         float z[SLOTS], old[SLOTS];
-        const bool wrong = list.settle(a.vocab);
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const bool here = list.tok[s] >= lo && list.tok[s] < hi;
-            z[s] = here ? __fmul_rn(to_float(x[list.tok[s]]), a.scale) : 0.0f;
+            z[s] = here ? to_float(x[list.tok[s]]) : 0.0f;
             old[s] = ADD && here ? to_float(d[list.tok[s]]) : 0.0f;
         }
+        const bool wrong = list.settle(a.vocab);
         float q[SLOTS], q_rest, minus;
         const bool known = teacher<SLOTS, REST>(list, q, q_rest, minus);
         if (wrong) g.what = 2;
@@ -385,7 +406,7 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(T *dlogits, const
         g.base = split ? rest : lse;
         g.factor = weight * (split ? expf(rest - lse) - q_rest : 1.0f);
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) own[s] = old[s] + weight * (expf(z[s] - lse) - q[s]);
+        for (int s = 0; s < SLOTS; ++s) own[s] = old[s] + weight * (expf(__fmul_rn(z[s], a.scale) - lse) - q[s]);
         if (lane == 0) shared[team] = g;
     }
     if (TEAM == 256) __syncthreads(); else __syncwarp();
@@ -459,7 +480,7 @@ template <typename T> int backward(T *dlogits, const T *logits, const BwdArgs &a
     const int vecs = (a.vocab + W - 1) / W + 1;
     if (vecs <= 32 * 4) return backward_of<T, 32, 4>(dlogits, logits, a, add, st);
     if ((double)a.rows * vecs < 4096.0 * sm_count()) return backward_of<T, 256, 2>(dlogits, logits, a, add, st);
-    return backward_of<T, 256, 8>(dlogits, logits, a, add, st);
+    return backward_of<T, 256, 4>(dlogits, logits, a, add, st);
 }
 
 int check(const char *who, const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *tokens, const float *lps, int top) {

@@ -347,6 +347,7 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
     const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
     const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4), x_full = bar0 + 8u * (uint32_t)(2 * STAGES + 5);
     const unsigned tiles = a.channel_tiles;
+    const unsigned mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * (unsigned)a.slabs, first = min(mine, (unsigned)STAGES);      // slabs of this block
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 8); }
@@ -355,6 +356,11 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
         fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
+        // the first slabs are on the way before the block is set up
+        for (unsigned i = 0; i < first; ++i) {
+            mbar_expect_tx(full((int)i), A_BYTES);
+            tma_load_2d(ring + i * A_BYTES, &map_w, (int)(i % (unsigned)a.slabs) * BK, (int)(blockIdx.x + i / (unsigned)a.slabs * gridDim.x) * BM, full((int)i));
+        }
     }
     if (warp == 1) tmem_alloc(smem_u32((const void *)&tmem_slot), TMEM);
     tc_fence_before();
@@ -364,15 +370,14 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
 
     if (warp == 0) {
         if (lane == 0) {
-            unsigned i = 0;
+            unsigned i = first;
             bool ok = true;
-            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
-                for (int k = 0; k < a.slabs; ++k, ++i) {
-                    const int s = (int)(i % STAGES);
-                    if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                    mbar_expect_tx(full(s), A_BYTES);
-                    tma_load_2d(ring + (uint32_t)s * A_BYTES, &map_w, k * BK, (int)tile * BM, full(s));
-                }
+            for (; i < mine; ++i) {
+                const int s = (int)(i % STAGES);
+                if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                mbar_expect_tx(full(s), A_BYTES);
+                tma_load_2d(ring + (uint32_t)s * A_BYTES, &map_w, (int)(i % (unsigned)a.slabs) * BK, (int)(blockIdx.x + i / (unsigned)a.slabs * gridDim.x) * BM, full(s));
+            }
             if (!ok)
                 for (unsigned j = i > (unsigned)STAGES ? i - STAGES : 0; j < i; ++j) {
                     volatile int never = 0;
@@ -582,7 +587,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales[warp - 2], ws, bias, real, ok, out, a.ld_out, r0, a.rows, c);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(acc_empty((int)(n & 1u)), 0));
+            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(acc_empty((int)(n & 1u)), 0));
         }
     }
     tc_fence_before();

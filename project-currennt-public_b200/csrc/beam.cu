@@ -16,7 +16,7 @@ namespace b2 {
 namespace {
 
 constexpr int MAX_BEAMS = 64, MAX_BEST = 64, MOST_VOCAB = 1 << 26;
-constexpr int SLICE_THREADS = 256, SLICE_VECS = 8;        // threads of a slice, vectors of 16 bytes each holds
+constexpr int SLICE_THREADS = 256, SLICE_VECS = 8;        // threads of a slice, vectors of 16 bytes each holds at most
 
 struct Part { float m, s; };         // largest z of a slice, sum of e^(z - m)
 
@@ -35,29 +35,32 @@ __device__ __forceinline__ bool runs(const SelectArgs &a, long long row) {
     return s > neg_inf() && s < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000) && !(a.finished && a.finished[row]);
 }
 
+// bytes of x as the selector's digits tell; 8 and above: the sign of byte digit - 8, all over
+template <unsigned S> __device__ __forceinline__ unsigned signs(unsigned x) { unsigned y; asm("prmt.b32 %0, %1, 0, %2;" : "=r"(y) : "r"(x), "n"(S)); return y; }
 // -inf in the places of q whose bytes of `on` are 0
 template <typename T> __device__ __forceinline__ void rule_out(uint4 &q, const Vec<unsigned char, 16 / sizeof(T)> &on) {
     unsigned w[4] = {q.x, q.y, q.z, q.w}, bytes[4 / sizeof(T) + 1];
     memcpy(bytes, &on, sizeof(on));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        unsigned off;                                     // all ones in the places that go
-        if constexpr (sizeof(T) == 4) off = __byte_perm(__vcmpeq4(bytes[0], 0), 0, 0x1111 * i);
-        else off = __byte_perm(__vcmpeq4(bytes[i / 2], 0), 0, i & 1 ? 0x3322 : 0x1100);
-        w[i] = (w[i] & ~off) | (Raw<T>::NONE & off);
+    for (int i = 0; i < 4 / (int)sizeof(T); ++i) bytes[i] |= (bytes[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu;     // the sign of a byte that is not 0
+    unsigned keep[4];                                     // a sign all over an entry's bytes
+    if constexpr (sizeof(T) == 4) {
+        keep[0] = signs<0x8888>(bytes[0]); keep[1] = signs<0x9999>(bytes[0]); keep[2] = signs<0xaaaa>(bytes[0]); keep[3] = signs<0xbbbb>(bytes[0]);
+    } else {
+        keep[0] = signs<0x9988>(bytes[0]); keep[1] = signs<0xbbaa>(bytes[0]); keep[2] = signs<0x9988>(bytes[1]); keep[3] = signs<0xbbaa>(bytes[1]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] & keep[i]) | (Raw<T>::NONE & ~keep[i]);
     q = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, bool MASK>
-__global__ void __launch_bounds__(SLICE_THREADS, 3) beam_rows_kernel(const T *logits, const SelectArgs a) {
-    constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, GROUP = THREADS / 64, CAP = 256;
-    __shared__ __align__(16) float maxima[64];
-    __shared__ float tops[WARPS], sums[WARPS];
+template <typename T, int U, bool MASK>
+__global__ void __launch_bounds__(SLICE_THREADS, U > 6 ? 3 : 4) beam_rows_kernel(const T *logits, const SelectArgs a) {
+    constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), WARPS = THREADS / 32, CAP = 256;
+    __shared__ float tops[WARPS], bounds[WARPS], sums[WARPS];
     __shared__ __align__(16) T hits[CAP][W];            // vectors that hold an entry of interest
     __shared__ int hit_at[CAP];                           // where they are in the row
     __shared__ Key found[CAP], winner[WARPS];
-    __shared__ float bound;
     __shared__ int n_hits, count;
     grid_release();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -107,29 +110,23 @@ __global__ void __launch_bounds__(SLICE_THREADS, 3) beam_rows_kernel(const T *lo
 #pragma unroll
     for (int u = 1; u < U; ++u) biggest = Raw<T>::larger(biggest, big[u]);
     const float mine = __fmul_rn(Raw<T>::largest(biggest), a.scale);
-    float most = mine;
-#pragma unroll
-    for (int o = 1; o < GROUP; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
-    if (t % GROUP == 0) maxima[t / GROUP] = most;
-#pragma unroll
-    for (int o = GROUP; o < 32; o <<= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
-    if (lane == 0) tops[warp] = most;
-    if (t == 0) { n_hits = count = 0; bound = neg_inf(); }
+    // The warp's largest, and what its ceil(top / WARPS) first lanes reach: the least of these over the warps is a bound that `top` entries of the slice reach
+    unsigned order = ordered(mine), least = 0;
+    float most = neg_inf();
+    for (int i = 0; i < a.top; i += WARPS) {
+        least = __reduce_max_sync(FULL, order);
+        if (i == 0) most = ordered_value(least);
+        if (lane == __ffs(__ballot_sync(FULL, order == least)) - 1) order = 0;
+    }
+    if (lane == 0) { tops[warp] = most; bounds[warp] = least ? ordered_value(least) : neg_inf(); }
+    if (t == 0) n_hits = count = 0;
     __syncthreads();
     most = tops[lane % WARPS];
+    float limit = bounds[lane % WARPS];
 #pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(FULL, most, o));
-    if (t < 64) {
-        // the place of this group's maximum among the 64 (NaN: the row has no continuations)
-        const float group = maxima[t];
-        int before = 0;
-#pragma unroll 4
-        for (int i = 0; i < 64; i += 4) {
-            const float4 m = *reinterpret_cast<const float4 *>(&maxima[i]);
-            before += (m.x > group || (m.x == group && i < t)) + (m.y > group || (m.y == group && i + 1 < t)) + (m.z > group || (m.z == group && i + 2 < t)) +
-                      (m.w > group || (m.w == group && i + 3 < t));
-        }
-        if (before == a.top - 1) bound = group;
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+        most = max_nan(most, __shfl_xor_sync(FULL, most, o));
+        limit = fminf(limit, __shfl_xor_sync(FULL, limit, o));
     }
     float s = 0.0f;
     if (most != neg_inf()) {
@@ -152,15 +149,7 @@ __global__ void __launch_bounds__(SLICE_THREADS, 3) beam_rows_kernel(const T *lo
     }
     s = warp_sum(s);
     if (lane == 0) sums[warp] = s;
-    __syncthreads();
-    if (t == 0) {
-        float all = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) all += sums[w];
-        a.parts[row * a.slices + part] = {most, all};
-    }
     Key *const list = a.lists + (row * a.slices + part) * a.top;
-    const float limit = bound;
     if (mine >= limit)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -174,6 +163,12 @@ __global__ void __launch_bounds__(SLICE_THREADS, 3) beam_rows_kernel(const T *lo
             }
         }
     __syncthreads();
+    if (t == 0) {
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) all += sums[w];
+        a.parts[row * a.slices + part] = {most, all};
+    }
     const int h = n_hits;
     if (h <= CAP)
         for (int i = t; i < h * W; i += THREADS) {
@@ -249,12 +244,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
     const int lists = a.beams * a.slices, entries = lists * a.top;
     const Key *const keys = a.lists + g * entries;
     grid_wait();
+    // a warp has the lists w, w + 8, ..., a lane their entries l and l + 32
+    constexpr int WARPS = JOIN_THREADS / 32;
+    const int deep = min(a.top, (2 * a.top + lists - 1) / lists), n_heads = lists * deep;
     Key ahead[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ahead[i] = t + i * JOIN_THREADS < entries ? keys[t + i * JOIN_THREADS] : 0;
-    const int deep = min(a.top, (2 * a.top + lists - 1) / lists), n_heads = lists * deep;
-    Key head = 0;
-    if (t < n_heads) head = keys[t / deep * a.top + t % deep];
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = warp + i * WARPS < lists && lane < a.top ? keys[(warp + i * WARPS) * a.top + lane] : 0;
     // score_b - lse_b of the beams; NaN: no continuations
     for (int b = warp; b < a.beams; b += JOIN_THREADS / 32) {
         const long long row = g * a.beams + b;
@@ -283,21 +278,28 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
     }
     if (t == 0) { count = 0; bound = -INFINITY; }
     __syncthreads();
-    const auto cand = [&](int i, Key k) -> Cand {
-        const int l = i / a.top, b = l / a.slices;
+    // entry j of list l
+    const auto cand = [&](int l, int j, Key k) -> Cand {
+        const int b = a.slices == 1 ? l : l / a.slices;
         const double o = off[b];
         if (o != o) return no_cand();
-        if (ended[b]) return i == b * a.slices * a.top ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
+        if (ended[b]) return j == 0 && l == b * a.slices ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
         if (!k) return no_cand();
         const float z = key_value(k);
         return {weight[b] * (o + (double)z), tie_of(b, z, key_index(k))};
     };
     const bool few = n_heads <= MOST_HEADS;
     if (few) {
-        for (int i = t; i < n_heads; i += JOIN_THREADS) {
-            const int at = i / deep * a.top + i % deep;
-            heads[i] = cand(at, i < JOIN_THREADS ? head : keys[at]).rank;
+        Cand held[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int l = warp + i * WARPS;
+            held[i] = l < lists && lane < a.top ? cand(l, lane, ahead[i]) : no_cand();
+            if (l < lists && lane < deep) heads[l * deep + lane] = held[i].rank;
+            if (l < lists && lane + 32 < deep) heads[l * deep + lane + 32] = cand(l, lane + 32, keys[l * a.top + lane + 32]).rank;
         }
+        for (int l = warp + AHEAD * WARPS; l < lists; l += WARPS)
+            for (int j = lane; j < deep; j += 32) heads[l * deep + j] = cand(l, j, keys[l * a.top + j]).rank;
         __syncthreads();
         for (int i = t; i < n_heads; i += JOIN_THREADS) {
             const double mine = heads[i];
@@ -308,17 +310,20 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         }
         __syncthreads();
         const double limit = bound;
-        const auto offer = [&](int i, Key k) {
-            const Cand c = cand(i, k);
+        const auto offer = [&](const Cand &c) {
             if (c.tie != 0 && c.rank >= limit) {
                 const int at = atomicAdd(&count, 1);
                 if (at < MOST_FOUND) found[at] = c;
             }
         };
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (t + i * JOIN_THREADS < entries) offer(t + i * JOIN_THREADS, ahead[i]);
-        for (int i = t + AHEAD * JOIN_THREADS; i < entries; i += JOIN_THREADS) offer(i, keys[i]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int l = warp + i * WARPS;
+            offer(held[i]);
+            if (l < lists && lane + 32 < a.top) offer(cand(l, lane + 32, keys[l * a.top + lane + 32]));
+        }
+        for (int l = warp + AHEAD * WARPS; l < lists; l += WARPS)
+            for (int j = lane; j < a.top; j += 32) offer(cand(l, j, keys[l * a.top + j]));
         __syncthreads();
     }
     const auto write = [&](int place, const Cand &c) {
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
     for (int place = 0; place < a.top; ++place) {
         Cand top = no_cand();
         for (int i = t; i < entries; i += JOIN_THREADS) {
-            const Cand c = cand(i, keys[i]);
+            const Cand c = cand(i / a.top, i % a.top, keys[i]);
             if (c.tie != 0 && better(last, c) && better(c, top)) top = c;
         }
 #pragma unroll
@@ -365,7 +370,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
 }
 
 int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
-int slices_of(int vocab, int type) { return (vectors_of(vocab, type) + SLICE_THREADS * SLICE_VECS - 1) / (SLICE_THREADS * SLICE_VECS); }
+// Vectors of a thread: what wastes least of the last slice's threads, a slice's bounds and lists counted as two vectors a thread
+int slice_vectors(int vocab, int type) {
+    const int vecs = vectors_of(vocab, type);
+    int best = SLICE_VECS;
+    long long cost = -1;
+    for (int u : {8, 6, 5, 4, 2}) {
+        const long long c = ((vecs + SLICE_THREADS * u - 1) / (SLICE_THREADS * u)) * (long long)(u + 2);
+        if (cost < 0 || c < cost) { cost = c; best = u; }
+    }
+    return best;
+}
+int slices_of(int vocab, int type) { const int n = SLICE_THREADS * slice_vectors(vocab, type); return (vectors_of(vocab, type) + n - 1) / n; }
 
 template <typename T> int select(const T *logits, SelectArgs a, int type, cudaStream_t st) {
     const int vecs = vectors_of(a.vocab, type);
@@ -373,8 +389,18 @@ template <typename T> int select(const T *logits, SelectArgs a, int type, cudaSt
     a.slice = (vecs + a.slices - 1) / a.slices;
     const long long blocks = a.groups * a.beams * a.slices;
     if (blocks > 0x7fffffffll) { set_error("b2_beam_select: %lld rows of %d", a.groups * a.beams, a.vocab); return B2_ERR_BAD_SHAPE; }
-    if (a.mask) beam_rows_kernel<T, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
-    else beam_rows_kernel<T, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    const auto go = [&](auto vectors) {
+        constexpr int U = decltype(vectors)::value;
+        if (a.mask) beam_rows_kernel<T, U, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+        else beam_rows_kernel<T, U, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    };
+    switch (slice_vectors(a.vocab, type)) {
+        case 2: go(std::integral_constant<int, 2>()); break;
+        case 4: go(std::integral_constant<int, 4>()); break;
+        case 5: go(std::integral_constant<int, 5>()); break;
+        case 6: go(std::integral_constant<int, 6>()); break;
+        default: go(std::integral_constant<int, 8>());
+    }
     count_launch();
     B2_CUDA(cudaGetLastError());
     return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(JOIN_THREADS), 0, st, a);
@@ -469,7 +495,8 @@ extern "C" {
 
 size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top) {
     if (!sizes_fit(groups, beams, vocab, top)) return 0;
-    const size_t slices = (size_t)slices_of(vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
+    const int f = slices_of(vocab, B2_F32), h = slices_of(vocab, B2_BF16);
+    const size_t slices = (size_t)(f > h ? f : h) * (size_t)groups * beams;      // the most of any type
     return slices * (sizeof(Part) + (size_t)top * sizeof(Key));
 }
 

@@ -356,131 +356,225 @@ struct BwdArgs {
 };
 struct RowGrad { float base, factor; int what; };      // what: 0 zeros, 1 gradient, 2 NaN
 
-// TEAM threads a row (32: a warp; 256: a block, several of them for a long row), each up to U vectors apart by TEAM
-template <typename T, int TEAM, int U, int SLOTS, bool REST, bool ADD>
-__global__ void __launch_bounds__(256, U <= 4 ? 5 : 3) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
-    constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
-    __shared__ RowGrad shared[TEAMS];
-    const int lane = threadIdx.x & 31, team = threadIdx.x / TEAM, at = threadIdx.x % TEAM;
-    const long long r = TEAM == 256 ? (long long)(blockIdx.x / (unsigned)segs) : (long long)blockIdx.x * TEAMS + team;
-    const int seg = TEAM == 256 ? (int)(blockIdx.x % (unsigned)segs) : 0;
-    if (r >= a.rows) return;                                   // TEAM 256: the block as a whole
-    const T *x = logits + r * a.ld;
-    T *d = dlogits + r * a.ld_out;
-    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
-    const bool out_vec = (((uintptr_t)(d - mis)) & 15) == 0;
-    const int first = seg * TEAM * U + at;
-    // the entries of this block
-    const int lo = max(0, seg * TEAM * U * W - mis), hi = TEAM == 256 ? min(a.vocab, (seg + 1) * TEAM * U * W - mis) : a.vocab;
-    const auto whole = [&](int v) { return v * W >= mis && (v + 1) * W <= mis + a.vocab; };
-    // the list first: everything waits for it
+// A row's vectors: v holds the entries v * W - mis on; whole ones lie inside the row
+template <typename T> struct Place {
+    static constexpr int W = 16 / sizeof(T);
+    const T *x;
+    T *d;
+    int mis, vocab;
+    bool out_vec;
+    __device__ __forceinline__ Place(T *dlogits, const T *logits, const BwdArgs &a, long long r) : x(logits + r * a.ld), d(dlogits + r * a.ld_out), vocab(a.vocab) {
+        mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+        out_vec = (((uintptr_t)(d - mis)) & 15) == 0;
+    }
+    __device__ __forceinline__ bool whole(int v) const { return v * W >= mis && (v + 1) * W <= mis + vocab; }
+    __device__ __forceinline__ void load(uint4 &q, int v) const {
+        if (whole(v)) q = *reinterpret_cast<const uint4 *>(x - mis + (size_t)v * W);
+    }
+};
+// the gradient off the list of vector v, whose logits are q if it is whole
+template <typename T, bool ADD> __device__ __forceinline__ void entry_grads(const Place<T> &p, const uint4 &q, int v, const RowGrad &g, float scale) {
+    constexpr int W = 16 / sizeof(T);
+    const int i0 = v * W - p.mis;
+    if (i0 >= p.vocab) return;
+    const bool inside = p.whole(v);
+    float z[W], o[W], old[W];
+    if (inside) Raw<T>::values(z, q);
+    else
+#pragma unroll
+        for (int j = 0; j < W; ++j) z[j] = i0 + j >= 0 && i0 + j < p.vocab ? to_float(p.x[i0 + j]) : 0.0f;
+    if (ADD) {
+        if (inside && p.out_vec) load_vec<T, W>(old, p.d + i0);
+        else
+#pragma unroll
+            for (int j = 0; j < W; ++j) old[j] = i0 + j >= 0 && i0 + j < p.vocab ? to_float(p.d[i0 + j]) : 0.0f;
+    }
+    if (g.what == 1) {
+        const Pair factor = pair(g.factor, g.factor);
+        less_of(scale, g.base, [&](const auto &less) {
+#pragma unroll
+            for (int j = 0; j < W; j += 2) {
+                const float2 t = halves(mul2(exp_pair<T>(less(z[j], z[j + 1])), factor));
+                o[j] = ADD ? old[j] + t.x : t.x;
+                o[j + 1] = ADD ? old[j + 1] + t.y : t.y;
+            }
+        });
+    } else {
+        const float none = g.what == 2 ? nanf("") : 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[j] = none;
+    }
+    if (inside && p.out_vec) store_vec<T, W>(p.d + i0, o);
+    else
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (i0 + j >= 0 && i0 + j < p.vocab) p.d[i0 + j] = from_float<T>(o[j]);
+}
+
+// The list of a row as it is loaded, and what becomes of it: the row's factors and the gradients of the listed tokens within [lo, hi)
+template <typename T, int SLOTS, bool REST, bool ADD> struct RowList {
     List<SLOTS> list;
-    float lse = 0.0f, rest = 0.0f, weight = 0.0f;
-    if (at < 32) {
+    float own[SLOTS];
+    float lse, rest, weight;
+    __device__ __forceinline__ void load(const BwdArgs &a, long long r) {
         list.load(a.tokens, a.lps, r, a.top);
         lse = a.lse[r];
         rest = REST ? a.lse_rest[r] : 0.0f;
         weight = a.dloss[r] * a.scale;
     }
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (whole(first + u * TEAM)) raw[u] = *reinterpret_cast<const uint4 *>(x - mis + (size_t)(first + u * TEAM) * W);
-    float own[SLOTS];
-    RowGrad g = {0.0f, 0.0f, 0};
-    if (at < 32) {
-        float z[SLOTS], old[SLOTS];
+    __device__ __forceinline__ RowGrad prepare(const BwdArgs &a, const Place<T> &p, int lo, int hi) {
+        float z[SLOTS], old[SLOTS], q[SLOTS], q_rest, minus;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const bool here = list.tok[s] >= lo && list.tok[s] < hi;
-            z[s] = here ? to_float(x[list.tok[s]]) : 0.0f;
-            old[s] = ADD && here ? to_float(d[list.tok[s]]) : 0.0f;
+            z[s] = here ? to_float(p.x[list.tok[s]]) : 0.0f;
+            old[s] = ADD && here ? to_float(p.d[list.tok[s]]) : 0.0f;
         }
-        const bool wrong = list.settle(a.vocab);
-        float q[SLOTS], q_rest, minus;
-        const bool known = teacher<SLOTS, REST>(list, q, q_rest, minus);
-        if (wrong) g.what = 2;
-        else if (known && lse != neg_inf()) g.what = 1;
+        const bool wrong = list.settle(a.vocab), known = teacher<SLOTS, REST>(list, q, q_rest, minus);
+        RowGrad g = {0.0f, 0.0f, wrong ? 2 : known && lse != neg_inf() ? 1 : 0};
         // e^(z - base) * factor off the list; where the rest has no mass all of its logits are -inf
         const bool split = REST && rest != neg_inf();
         g.base = split ? rest : lse;
         g.factor = weight * (split ? expf(rest - lse) - q_rest : 1.0f);
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) own[s] = old[s] + weight * (expf(__fmul_rn(z[s], a.scale) - lse) - q[s]);
-        if (lane == 0) shared[team] = g;
+        return g;
     }
-    if (TEAM == 256) __syncthreads(); else __syncwarp();
-    g = shared[team];
-    if (g.what == 0 && ADD) return;
-    const float none = g.what == 2 ? nanf("") : 0.0f;
-    const Pair factor = pair(g.factor, g.factor);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int v = first + u * TEAM, i0 = v * W - mis;
-        if (i0 >= a.vocab) break;
-        const bool inside = whole(v);
-        float z[W], o[W], old[W];
-        if (inside) Raw<T>::values(z, raw[u]);
-        else
-#pragma unroll
-            for (int j = 0; j < W; ++j) z[j] = i0 + j >= 0 && i0 + j < a.vocab ? to_float(x[i0 + j]) : 0.0f;
-        if (ADD) {
-            if (inside && out_vec) load_vec<T, W>(old, d + i0);
-            else
-#pragma unroll
-                for (int j = 0; j < W; ++j) old[j] = i0 + j >= 0 && i0 + j < a.vocab ? to_float(d[i0 + j]) : 0.0f;
-        }
-        if (g.what == 1) {
-            less_of(a.scale, g.base, [&](const auto &less) {
-#pragma unroll
-                for (int j = 0; j < W; j += 2) {
-                    const float2 t = halves(mul2(exp_pair<T>(less(z[j], z[j + 1])), factor));
-                    o[j] = ADD ? old[j] + t.x : t.x;
-                    o[j + 1] = ADD ? old[j + 1] + t.y : t.y;
-                }
-            });
-        } else {
-#pragma unroll
-            for (int j = 0; j < W; ++j) o[j] = none;
-        }
-        if (inside && out_vec) store_vec<T, W>(d + i0, o);
-        else
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (i0 + j >= 0 && i0 + j < a.vocab) d[i0 + j] = from_float<T>(o[j]);
-    }
-    if (g.what != 1) return;
-    if (TEAM == 256) __syncthreads(); else __syncwarp();
-    if (at < 32)
+    __device__ __forceinline__ void store(T *d, int lo, int hi) const {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
             if (list.tok[s] >= lo && list.tok[s] < hi) d[list.tok[s]] = from_float<T>(own[s]);
+    }
+};
+
+// Narrow rows, up to 32 U vectors: a warp each; the next row's list and logits are on the way while it works on one
+template <typename T, int U, int SLOTS, bool REST, bool ADD>
+__global__ void __launch_bounds__(256, 3) distill_backward_warp_kernel(T *dlogits, const T *logits, const BwdArgs a) {
+    const int lane = threadIdx.x & 31;
+    const long long step = (long long)gridDim.x * 8;
+    long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= a.rows) return;
+    RowList<T, SLOTS, REST, ADD> list, next;
+    uint4 q[U], after[U];
+    const auto ahead = [&](long long row) {
+        if (row >= a.rows) return;
+        next.load(a, row);
+        const Place<T> p(dlogits, logits, a, row);
+#pragma unroll
+        for (int u = 0; u < U; ++u) p.load(after[u], lane + 32 * u);
+    };
+    ahead(r);
+    for (; r < a.rows; r += step) {
+        list = next;
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = after[u];
+        ahead(r + step);
+        const Place<T> p(dlogits, logits, a, r);
+        const RowGrad g = list.prepare(a, p, 0, a.vocab);
+        __syncwarp();
+        if (g.what == 0 && ADD) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], lane + 32 * u, g, a.scale);
+        __syncwarp();
+        if (g.what == 1) list.store(p.d, 0, a.vocab);
+    }
 }
 
-template <typename T, int TEAM, int U, int SLOTS> int launch_backward(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
+// Wide rows in segments of 256 U vectors: eight warps work on a segment while its successor is on the way, a ninth prepares the successor's list and writes the
+// gradients of the predecessor's listed tokens over those that the eight wrote.  One barrier a segment; nobody waits for a list.
+constexpr int STREAM = 256;
+template <typename T, int U, int SLOTS, bool REST, bool ADD>
+__global__ void __launch_bounds__(STREAM + 32, 3) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
+    constexpr int W = 16 / sizeof(T);
+    __shared__ RowGrad shared[2];
+    const int at = threadIdx.x;
+    const bool lists = at >= STREAM;
+    const auto low = [&](const Place<T> &p, int seg) { return max(0, seg * STREAM * U * W - p.mis); };
+    const auto high = [&](const Place<T> &p, int seg) { return min(a.vocab, (seg + 1) * STREAM * U * W - p.mis); };
+    struct Item { long long r; int seg; };
+    const int step_r = (int)(gridDim.x / (unsigned)segs), step_seg = (int)(gridDim.x % (unsigned)segs);
+    const auto step = [&](const Item &i) {
+        Item n = {i.r + step_r, i.seg + step_seg};
+        if (n.seg >= segs) { n.seg -= segs; ++n.r; }
+        return n;
+    };
+    uint4 q[U], after[U];
+    RowList<T, SLOTS, REST, ADD> list, done;
+    bool pending = false, now = false;           // whether done's and list's gradients are to be written
+    const auto ahead = [&](const Item &i) {
+        if (i.r >= a.rows) return;
+        const Place<T> p(dlogits, logits, a, i.r);
+#pragma unroll
+        for (int u = 0; u < U; ++u) p.load(after[u], i.seg * STREAM * U + at + u * STREAM);
+    };
+    const auto prepare = [&](const Item &i, int to) {
+        now = false;
+        if (i.r >= a.rows) return;
+        const Place<T> p(dlogits, logits, a, i.r);
+        list.load(a, i.r);
+        const RowGrad g = list.prepare(a, p, low(p, i.seg), high(p, i.seg));
+        now = g.what == 1;
+        if (at == STREAM) shared[to] = g;
+    };
+    const auto write = [&](const Item &i) {
+        const Place<T> p(dlogits, logits, a, i.r);
+        done.store(p.d, low(p, i.seg), high(p, i.seg));
+    };
+    Item item = {(long long)(blockIdx.x / (unsigned)segs), (int)(blockIdx.x % (unsigned)segs)}, before = item;
+    if (lists) prepare(item, 0); else ahead(item);
+    for (int turn = 0; item.r < a.rows; turn ^= 1) {
+        const Item next = step(item);
+        __syncthreads();
+        if (lists) {
+            if (pending) write(before);
+            done = list;
+            pending = now;
+            prepare(next, turn ^ 1);
+        } else {
+            const RowGrad g = shared[turn];
+#pragma unroll
+            for (int u = 0; u < U; ++u) q[u] = after[u];
+            ahead(next);
+            if (g.what != 0 || !ADD) {
+                const Place<T> p(dlogits, logits, a, item.r);
+#pragma unroll
+                for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], item.seg * STREAM * U + at + u * STREAM, g, a.scale);
+            }
+        }
+        before = item;
+        item = next;
+    }
+    __syncthreads();
+    if (lists && pending) write(before);
+}
+
+template <typename T, int SLOTS, bool REST, bool ADD> int launch_backward(T *dlogits, const T *logits, const BwdArgs &a, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
     const int vecs = (a.vocab + W - 1) / W + 1;               // one more: a row may start inside a vector
-    const int segs = TEAM == 256 ? (vecs + TEAM * U - 1) / (TEAM * U) : 1;
-    const long long blocks = TEAM == 256 ? a.rows * segs : (a.rows + 7) / 8;
-    if (blocks > 0x7fffffffll) { set_error("b2_distill_backward: %lld rows of %d", a.rows, a.vocab); return B2_ERR_BAD_SHAPE; }
-    const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, st>>>(dlogits, logits, a, segs); };
-    if (a.lse_rest) { if (add) go(distill_backward_kernel<T, TEAM, U, SLOTS, true, true>); else go(distill_backward_kernel<T, TEAM, U, SLOTS, true, false>); }
-    else { if (add) go(distill_backward_kernel<T, TEAM, U, SLOTS, false, true>); else go(distill_backward_kernel<T, TEAM, U, SLOTS, false, false>); }
+    if (vecs <= 32 * 4) {
+        const long long teams = (a.rows + 7) / 8, most = 4ll * sm_count();
+        const unsigned blocks = (unsigned)(teams < most ? teams : most);
+        if (vecs <= 32 * 2) distill_backward_warp_kernel<T, 2, SLOTS, REST, ADD><<<blocks, 256, 0, st>>>(dlogits, logits, a);
+        else distill_backward_warp_kernel<T, 4, SLOTS, REST, ADD><<<blocks, 256, 0, st>>>(dlogits, logits, a);
+    } else {
+        const int u = (double)a.rows * vecs < 4096.0 * sm_count() ? 1 : 4, segs = (vecs + STREAM * u - 1) / (STREAM * u);
+        const long long items = a.rows * segs, most = 3ll * sm_count();
+        const unsigned blocks = (unsigned)(items < most ? items : most);
+        if (u == 1) distill_backward_kernel<T, 1, SLOTS, REST, ADD><<<blocks, STREAM + 32, 0, st>>>(dlogits, logits, a, segs);
+        else distill_backward_kernel<T, 4, SLOTS, REST, ADD><<<blocks, STREAM + 32, 0, st>>>(dlogits, logits, a, segs);
+    }
     count_launch();
     B2_CUDA(cudaGetLastError());
     return B2_OK;
 }
-template <typename T, int TEAM, int U> int backward_of(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
-    if (a.top <= 32) return launch_backward<T, TEAM, U, 1>(dlogits, logits, a, add, st);
-    if (a.top <= 64) return launch_backward<T, TEAM, U, 2>(dlogits, logits, a, add, st);
-    return launch_backward<T, TEAM, U, 4>(dlogits, logits, a, add, st);
+template <typename T, int SLOTS> int backward_of(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
+    if (a.lse_rest) return add ? launch_backward<T, SLOTS, true, true>(dlogits, logits, a, st) : launch_backward<T, SLOTS, true, false>(dlogits, logits, a, st);
+    return add ? launch_backward<T, SLOTS, false, true>(dlogits, logits, a, st) : launch_backward<T, SLOTS, false, false>(dlogits, logits, a, st);
 }
 template <typename T> int backward(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
-    constexpr int W = 16 / sizeof(T);
-    const int vecs = (a.vocab + W - 1) / W + 1;
-    if (vecs <= 32 * 4) return backward_of<T, 32, 4>(dlogits, logits, a, add, st);
-    if ((double)a.rows * vecs < 4096.0 * sm_count()) return backward_of<T, 256, 2>(dlogits, logits, a, add, st);
-    return backward_of<T, 256, 4>(dlogits, logits, a, add, st);
+    if (a.top <= 32) return backward_of<T, 1>(dlogits, logits, a, add, st);
+    if (a.top <= 64) return backward_of<T, 2>(dlogits, logits, a, add, st);
+    return backward_of<T, 4>(dlogits, logits, a, add, st);
 }
 
 int check(const char *who, const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *tokens, const float *lps, int top) {

@@ -16,7 +16,7 @@ namespace b2 {
 namespace {
 
 constexpr int MAX_BEAMS = 64, MAX_BEST = 64, MOST_VOCAB = 1 << 26;
-constexpr int SLICE_THREADS = 256, SLICE_VECS = 8;        // threads of a slice, vectors of 16 bytes each holds at most
+constexpr int SLICE_THREADS = 256, SLICE_VECS = 4;        // threads of a slice, vectors of 16 bytes each has in registers
 
 struct Part { float m, s; };         // largest z of a slice, sum of e^(z - m)
 
@@ -54,133 +54,176 @@ template <typename T> __device__ __forceinline__ void rule_out(uint4 &q, const V
     q = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int U, bool MASK>
-__global__ void __launch_bounds__(SLICE_THREADS, U > 6 ? 3 : 4) beam_rows_kernel(const T *logits, const SelectArgs a) {
-    constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), WARPS = THREADS / 32, CAP = 256;
-    __shared__ float tops[WARPS], bounds[WARPS], sums[WARPS];
+// the running sum of a thread
+__device__ __forceinline__ void rise(Part &a, float m) {
+    if (a.m != neg_inf()) {
+        const float r = ex2((a.m - m) * LOG2E);
+        a.s = r == 0.0f ? 0.0f : r * a.s;
+    }
+    a.m = m;
+}
+__device__ __forceinline__ Part join(Part a, Part b) {
+    const float m = max_nan(a.m, b.m);
+    if (m == neg_inf()) return a;
+    if (b.m != neg_inf()) rise(b, m); else b.s = 0.0f;
+    rise(a, m);
+    return {m, a.s + b.s};
+}
+// What the ceil(top / WARPS) best lanes of a warp hold at least: `top` entries reach the least of it over the warps
+template <int WARPS> __device__ __forceinline__ float reached(float best, int top) {
+    unsigned order = ordered(best), least = 0;
+    for (int i = 0; i < top; i += WARPS) {
+        least = __reduce_max_sync(FULL, order);
+        if ((int)(threadIdx.x & 31) == __ffs(__ballot_sync(FULL, order == least)) - 1) order = 0;
+    }
+    return ordered_value(least);
+}
+template <int WARPS> __device__ __forceinline__ float least_of(const float *bounds) {
+    float limit = bounds[threadIdx.x & (WARPS - 1)];
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) limit = fminf(limit, __shfl_xor_sync(FULL, limit, o));
+    return limit;
+}
+
+template <typename T, bool MASK>
+__global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *logits, const SelectArgs a) {
+    constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, CAP = 512;
+    __shared__ float bounds[WARPS];
+    __shared__ Part parts[WARPS];
     __shared__ __align__(16) T hits[CAP][W];            // vectors that hold an entry of interest
     __shared__ int hit_at[CAP];                           // where they are in the row
-    __shared__ Key found[CAP], winner[WARPS];
+    __shared__ Key found[THREADS], winner[WARPS];
     __shared__ int n_hits, count;
     grid_release();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const long long row = blockIdx.x / (unsigned)a.slices;
-    const int part = (int)(blockIdx.x % (unsigned)a.slices);
+    const long long row = a.slices == 1 ? blockIdx.x : blockIdx.x / (unsigned)a.slices;
+    const int part = a.slices == 1 ? 0 : (int)(blockIdx.x % (unsigned)a.slices);
     const T *x = logits + row * a.ld;
     const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
     const unsigned char *mk = MASK ? a.mask + row * a.ld_mask : nullptr;
     const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
     const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
     if (!runs(a, row)) return;
+    if (t == 0) n_hits = count = 0;
+    typedef Vec<unsigned char, W> Flags;
     uint4 q[U];
-    Vec<unsigned char, W> on[MASK ? U : 1];
+    Flags on[MASK ? U : 1];
+    const auto load = [&](int from) {
+        // all of the chunk inside the row, its mask in vectors: what most chunks are
+        if (from * W >= mis && (from + THREADS * U) * W - mis <= a.vocab && from + THREADS * U <= v1 && (!MASK || mask_vec)) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(x - mis) + from + t;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int v = v0 + t + u * THREADS, i0 = v * W - mis;
-        const bool inside = v < v1, whole = i0 >= 0 && i0 + W <= a.vocab;
-        q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
-        if (inside && whole) q[u] = *reinterpret_cast<const uint4 *>(x + i0);
-        if (MASK && inside && whole && mask_vec) on[u] = *reinterpret_cast<const Vec<unsigned char, W> *>(mk + i0);
-    }
-    // the ends of the row, and masks whose bytes lie across the vectors
-    if (v0 * W < mis || (v1 - 1) * W - mis + W > a.vocab || (MASK && !mask_vec)) {
+            for (int u = 0; u < U; ++u) q[u] = src[u * THREADS];
+            if (MASK) {
+                const Flags *m = reinterpret_cast<const Flags *>(mk - mis) + from + t;
+#pragma unroll
+                for (int u = 0; u < U; ++u) on[u] = m[u * THREADS];
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = v0 + t + u * THREADS, i0 = v * W - mis;
-            const bool whole = i0 >= 0 && i0 + W <= a.vocab;
-            if (v < v1 && !whole) {
+            const int v = from + t + u * THREADS, i0 = v * W - mis;
+            const bool inside = v < v1, whole = inside && i0 >= 0 && i0 + W <= a.vocab;
+            q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+            if (whole) q[u] = *reinterpret_cast<const uint4 *>(x + i0);
+            else if (inside) {
                 T e[W];
 #pragma unroll
                 for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < a.vocab ? x[i0 + j] : from_float<T>(neg_inf());
                 memcpy(&q[u], e, 16);
             }
-            if (MASK && v < v1 && !(whole && mask_vec))
+            if (MASK) {
+                if (whole && mask_vec) on[u] = *reinterpret_cast<const Flags *>(mk + i0);
+                else
 #pragma unroll
-                for (int j = 0; j < W; ++j) on[u].v[j] = i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
-        }
-    }
-    if (MASK)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v0 + t + u * THREADS < v1) rule_out<T>(q[u], on[u]);
-    unsigned big[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) big[u] = larger_of<T>(q[u]);
-    unsigned biggest = big[0];
-#pragma unroll
-    for (int u = 1; u < U; ++u) biggest = Raw<T>::larger(biggest, big[u]);
-    const float mine = __fmul_rn(Raw<T>::largest(biggest), a.scale);
-    // The warp's largest, and what its ceil(top / WARPS) first lanes reach: the least of these over the warps is a bound that `top` entries of the slice reach
-    unsigned order = ordered(mine), least = 0;
-    float most = neg_inf();
-    for (int i = 0; i < a.top; i += WARPS) {
-        least = __reduce_max_sync(FULL, order);
-        if (i == 0) most = ordered_value(least);
-        if (lane == __ffs(__ballot_sync(FULL, order == least)) - 1) order = 0;
-    }
-    if (lane == 0) { tops[warp] = most; bounds[warp] = least ? ordered_value(least) : neg_inf(); }
-    if (t == 0) n_hits = count = 0;
-    __syncthreads();
-    most = tops[lane % WARPS];
-    float limit = bounds[lane % WARPS];
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) {
-        most = max_nan(most, __shfl_xor_sync(FULL, most, o));
-        limit = fminf(limit, __shfl_xor_sync(FULL, limit, o));
-    }
-    float s = 0.0f;
-    if (most != neg_inf()) {
-        const Pair l2 = pair(LOG2E, LOG2E);
-        Pair p = 0;
-        less_of(a.scale, most, [&](const auto &less) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float z[W];
-                Raw<T>::values(z, q[u]);
-#pragma unroll
-                for (int j = 0; j < W; j += 2) {
-                    const float2 d = halves(mul2(less(z[j], z[j + 1]), l2));
-                    p = add2(p, pair(ex2(d.x), ex2(d.y)));
-                }
+                    for (int j = 0; j < W; ++j) on[u].v[j] = inside && i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
             }
-        });
-        const float2 h = halves(p);
-        s = h.x + h.y;
+        }
+    };
+    Part sum = {neg_inf(), 0.0f};
+    float best = neg_inf(), limit = neg_inf();             // the thread's largest; what an entry has to reach
+    int renew = 0, chunk = 0;
+    load(v0);
+    for (int from = v0; from < v1; from += THREADS * U, ++chunk) {
+        if (MASK)
+#pragma unroll
+            for (int u = 0; u < U; ++u) rule_out<T>(q[u], on[u]);
+        unsigned big[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) big[u] = larger_of<T>(q[u]);
+        unsigned biggest = big[0];
+#pragma unroll
+        for (int u = 1; u < U; ++u) biggest = Raw<T>::larger(biggest, big[u]);
+        const float mine = __fmul_rn(Raw<T>::largest(biggest), a.scale);
+        best = max_nan(best, mine);
+        if (chunk == renew) {
+            // the bound from what was met so far, after 1, 2, 4, 8, ... chunks
+            const float mine_reached = reached<WARPS>(best, a.top);
+            if (chunk) __syncthreads();
+            if (lane == 0) bounds[warp] = mine_reached;
+            __syncthreads();
+            limit = least_of<WARPS>(bounds);
+            renew = 2 * renew + 1;
+        }
+        if (mine >= limit && mine > neg_inf())
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (__fmul_rn(Raw<T>::largest(big[u]), a.scale) >= limit) {
+                    const int at = atomicAdd(&n_hits, 1);
+                    if (at < CAP) {
+                        *reinterpret_cast<uint4 *>(&hits[at][0]) = q[u];
+                        hit_at[at] = (from + t + u * THREADS) * W - mis;
+                    }
+                }
+        if (!(mine <= sum.m)) rise(sum, mine);
+        if (sum.m != neg_inf()) {
+            const Pair l2 = pair(LOG2E, LOG2E);
+            Pair p = 0;
+            less_of(a.scale, sum.m, [&](const auto &less) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float z[W];
+                    Raw<T>::values(z, q[u]);
+#pragma unroll
+                    for (int j = 0; j < W; j += 2) {
+                        const float2 d = halves(mul2(less(z[j], z[j + 1]), l2));
+                        p = add2(p, pair(ex2(d.x), ex2(d.y)));
+                    }
+                }
+            });
+            const float2 h = halves(p);
+            sum.s += h.x + h.y;
+        }
+        if (from + THREADS * U < v1) load(from + THREADS * U);
     }
-    s = warp_sum(s);
-    if (lane == 0) sums[warp] = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum = join(sum, {__shfl_xor_sync(FULL, sum.m, o), __shfl_xor_sync(FULL, sum.s, o)});
+    const float all_reached = reached<WARPS>(best, a.top);         // the bound of the whole slice
+    if (lane == 0) parts[warp] = sum;
+    __syncthreads();
+    if (lane == 0) bounds[warp] = all_reached;
+    __syncthreads();
+    limit = least_of<WARPS>(bounds);
     Key *const list = a.lists + (row * a.slices + part) * a.top;
-    if (mine >= limit)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float m = __fmul_rn(Raw<T>::largest(big[u]), a.scale);
-            if (m >= limit && m > neg_inf()) {
-                const int at = atomicAdd(&n_hits, 1);
-                if (at < CAP) {
-                    *reinterpret_cast<uint4 *>(&hits[at][0]) = q[u];
-                    hit_at[at] = (v0 + t + u * THREADS) * W - mis;
-                }
-            }
-        }
-    __syncthreads();
-    if (t == 0) {
-        float all = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) all += sums[w];
-        a.parts[row * a.slices + part] = {most, all};
-    }
     const int h = n_hits;
     if (h <= CAP)
         for (int i = t; i < h * W; i += THREADS) {
             const float z = __fmul_rn(to_float(hits[i / W][i % W]), a.scale);
             if (z >= limit && z > neg_inf()) {
                 const int at = atomicAdd(&count, 1);
-                if (at < CAP) found[at] = make_key(z, hit_at[i / W] + i % W);
+                if (at < THREADS) found[at] = make_key(z, hit_at[i / W] + i % W);
             }
         }
+    if (warp == WARPS - 1) {
+        Part all = lane < WARPS ? parts[lane] : Part{neg_inf(), 0.0f};
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) all = join(all, {__shfl_xor_sync(FULL, all.m, o), __shfl_xor_sync(FULL, all.s, o)});
+        if (lane == 0) a.parts[row * a.slices + part] = all;
+    }
     __syncthreads();
     const int n = count;
-    if (h <= CAP && n <= CAP) {
+    if (h <= CAP && n <= THREADS) {
         if (t < n) {
             const Key k = found[t];
             int before = 0;
@@ -234,9 +277,9 @@ constexpr int JOIN_THREADS = 256, AHEAD = 4, MOST_HEADS = 1024, MOST_FOUND = 102
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArgs a) {
     __shared__ double off[MAX_BEAMS], weight[MAX_BEAMS];
     __shared__ bool ended[MAX_BEAMS];
-    __shared__ __align__(16) double heads[MOST_HEADS];
+    __shared__ __align__(16) float heads[MOST_HEADS];
     __shared__ Cand found[MOST_FOUND];
-    __shared__ double bound;
+    __shared__ float bound;
     __shared__ int count;
     __shared__ Cand winner[JOIN_THREADS / 32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -276,7 +319,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         }
         if (lane == 0) { off[b] = o; weight[b] = (double)w; ended[b] = end; }
     }
-    if (t == 0) { count = 0; bound = -INFINITY; }
+    if (t == 0) { count = 0; bound = neg_inf(); }
     __syncthreads();
     // entry j of list l
     const auto cand = [&](int l, int j, Key k) -> Cand {
@@ -295,23 +338,28 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         for (int i = 0; i < AHEAD; ++i) {
             const int l = warp + i * WARPS;
             held[i] = l < lists && lane < a.top ? cand(l, lane, ahead[i]) : no_cand();
-            if (l < lists && lane < deep) heads[l * deep + lane] = held[i].rank;
-            if (l < lists && lane + 32 < deep) heads[l * deep + lane + 32] = cand(l, lane + 32, keys[l * a.top + lane + 32]).rank;
+            if (l < lists && lane < deep) heads[l * deep + lane] = (float)held[i].rank;
+            if (l < lists && lane + 32 < deep) heads[l * deep + lane + 32] = (float)cand(l, lane + 32, keys[l * a.top + lane + 32]).rank;
         }
         for (int l = warp + AHEAD * WARPS; l < lists; l += WARPS)
-            for (int j = lane; j < deep; j += 32) heads[l * deep + j] = cand(l, j, keys[l * a.top + j]).rank;
+            for (int j = lane; j < deep; j += 32) heads[l * deep + j] = (float)cand(l, j, keys[l * a.top + j]).rank;
         __syncthreads();
+        // A rounding to fewer bits keeps the order, so that the bound in 32 bits lets all through that reach the one in 64
         for (int i = t; i < n_heads; i += JOIN_THREADS) {
-            const double mine = heads[i];
-            int before = 0;
-#pragma unroll 8
-            for (int j = 0; j < n_heads; ++j) before += heads[j] > mine || (heads[j] == mine && j < i);
+            const float mine = heads[i];
+            int before = 0, j = 0;
+            for (; j + 4 <= n_heads; j += 4) {
+                const float4 m = *reinterpret_cast<const float4 *>(&heads[j]);
+                before += (m.x > mine || (m.x == mine && j < i)) + (m.y > mine || (m.y == mine && j + 1 < i)) + (m.z > mine || (m.z == mine && j + 2 < i)) +
+                          (m.w > mine || (m.w == mine && j + 3 < i));
+            }
+            for (; j < n_heads; ++j) before += heads[j] > mine || (heads[j] == mine && j < i);
             if (before == a.top - 1) bound = mine;
         }
         __syncthreads();
-        const double limit = bound;
+        const float limit = bound;
         const auto offer = [&](const Cand &c) {
-            if (c.tie != 0 && c.rank >= limit) {
+            if (c.tie != 0 && (float)c.rank >= limit) {
                 const int at = atomicAdd(&count, 1);
                 if (at < MOST_FOUND) found[at] = c;
             }
@@ -370,37 +418,21 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
 }
 
 int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
-// Vectors of a thread: what wastes least of the last slice's threads, a slice's bounds and lists counted as two vectors a thread
-int slice_vectors(int vocab, int type) {
-    const int vecs = vectors_of(vocab, type);
-    int best = SLICE_VECS;
-    long long cost = -1;
-    for (int u : {8, 6, 5, 4, 2}) {
-        const long long c = ((vecs + SLICE_THREADS * u - 1) / (SLICE_THREADS * u)) * (long long)(u + 2);
-        if (cost < 0 || c < cost) { cost = c; best = u; }
-    }
-    return best;
+// Slices of a row: one where the rows fill the device (bounds and lists cost a slice several chunks' time), more where they do not, as long as each has a chunk of 1024
+// vectors
+int slices_of(long long rows, int vocab, int type) {
+    const int chunks = (vectors_of(vocab, type) + SLICE_THREADS * SLICE_VECS - 1) / (SLICE_THREADS * SLICE_VECS);
+    const long long most = rows ? (592 + rows - 1) / rows : 1;          // blocks that run at a time: 4 an SM
+    return (int)(chunks < most ? chunks : most);
 }
-int slices_of(int vocab, int type) { const int n = SLICE_THREADS * slice_vectors(vocab, type); return (vectors_of(vocab, type) + n - 1) / n; }
 
 template <typename T> int select(const T *logits, SelectArgs a, int type, cudaStream_t st) {
     const int vecs = vectors_of(a.vocab, type);
-    a.slices = slices_of(a.vocab, type);
     a.slice = (vecs + a.slices - 1) / a.slices;
     const long long blocks = a.groups * a.beams * a.slices;
     if (blocks > 0x7fffffffll) { set_error("b2_beam_select: %lld rows of %d", a.groups * a.beams, a.vocab); return B2_ERR_BAD_SHAPE; }
-    const auto go = [&](auto vectors) {
-        constexpr int U = decltype(vectors)::value;
-        if (a.mask) beam_rows_kernel<T, U, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
-        else beam_rows_kernel<T, U, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
-    };
-    switch (slice_vectors(a.vocab, type)) {
-        case 2: go(std::integral_constant<int, 2>()); break;
-        case 4: go(std::integral_constant<int, 4>()); break;
-        case 5: go(std::integral_constant<int, 5>()); break;
-        case 6: go(std::integral_constant<int, 6>()); break;
-        default: go(std::integral_constant<int, 8>());
-    }
+    if (a.mask) beam_rows_kernel<T, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
+    else beam_rows_kernel<T, false><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);
     count_launch();
     B2_CUDA(cudaGetLastError());
     return launch_chained(beam_join_kernel, dim3((unsigned)a.groups), dim3(JOIN_THREADS), 0, st, a);
@@ -495,8 +527,7 @@ extern "C" {
 
 size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top) {
     if (!sizes_fit(groups, beams, vocab, top)) return 0;
-    const int f = slices_of(vocab, B2_F32), h = slices_of(vocab, B2_BF16);
-    const size_t slices = (size_t)(f > h ? f : h) * (size_t)groups * beams;      // the most of any type
+    const size_t slices = (size_t)slices_of(groups * beams, vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
     return slices * (sizeof(Part) + (size_t)top * sizeof(Key));
 }
 
@@ -528,8 +559,9 @@ int b2_beam_select(const void *logits, int type, long long groups, int beams, in
     SelectArgs a = {};
     a.mask = mask; a.ld_mask = ld_mask; a.scores = scores; a.finished = finished; a.weights = weights;
     a.groups = groups; a.ld = ld; a.beams = beams; a.vocab = vocab; a.top = top; a.end_token = end_token; a.scale = scale;
+    a.slices = slices_of(groups * beams, vocab, type);
     a.lists = (Key *)workspace;
-    a.parts = (Part *)(a.lists + (size_t)slices_of(vocab, type) * (size_t)groups * beams * top);
+    a.parts = (Part *)(a.lists + (size_t)a.slices * (size_t)groups * beams * top);
     a.best = top_scores; a.from = top_beams; a.tokens = top_tokens;
     return with_type(type, [&](auto *t) { return select((const B2_ELEM(t) *)logits, a, type, (cudaStream_t)stream); });
 }

@@ -21,17 +21,22 @@ namespace {
 constexpr int MAX_LIST = 128;
 constexpr float LEAST_REST = 9.5367431640625e-7f;      // 2^-20
 
-// The places of a row's list that a lane holds: place s * 32 + lane.  tok -1: empty, or listed further ahead
-template <int SLOTS> struct List {
+// The places of a row's list that a lane holds: place s * TEAM + lane, the lanes of a row being TEAM neighbours of a warp.  tok -1: empty, or listed further
+// ahead
+template <int SLOTS, int TEAM> struct List {
+    static_assert(SLOTS == 1 || TEAM == 32, "a short list has a place a lane");
     int tok[SLOTS];
     float lp[SLOTS];
+    static __device__ __forceinline__ unsigned lanes() { return TEAM == 32 ? FULL : ((1u << (TEAM & 31)) - 1u) << (threadIdx.x & 31 & ~(TEAM - 1)); }
+    static __device__ __forceinline__ bool any_of(bool x) { return (__ballot_sync(FULL, x) & lanes()) != 0; }
     __device__ __forceinline__ void load(const int *tokens, const float *lps, long long r, int top) {
-        const int lane = threadIdx.x & 31;
+        const int lane = threadIdx.x & (TEAM - 1);
+        const long long at = r * top;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const int k = s * 32 + lane;
-            tok[s] = k < top ? tokens[r * top + k] : -1;
-            lp[s] = k < top ? lps[r * top + k] : neg_inf();
+            tok[s] = k < top ? tokens[at + k] : -1;
+            lp[s] = k < top ? lps[at + k] : neg_inf();
         }
     }
     // empties the places whose token is negative or stands further ahead; true where a token is not below vocab or a log probability is NaN or +inf
@@ -40,7 +45,7 @@ template <int SLOTS> struct List {
         bool wrong = false, twice[SLOTS];
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            twice[s] = (__ffs(__match_any_sync(FULL, tok[s])) - 1) != lane;
+            twice[s] = (__ffs(__match_any_sync(FULL, tok[s]) & lanes()) - 1) != lane;
 #pragma unroll
             for (int e = 0; e < s; ++e)
 #pragma unroll 8
@@ -52,38 +57,35 @@ template <int SLOTS> struct List {
             if (tok[s] < 0) { tok[s] = -1; lp[s] = neg_inf(); }
             else if (tok[s] >= vocab || !(lp[s] < __int_as_float(0x7f800000))) wrong = true;
         }
-        return __any_sync(FULL, wrong);
+        return any_of(wrong);
     }
     __device__ __forceinline__ bool any() const {
         bool one = false;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) one |= tok[s] >= 0;
-        return __any_sync(FULL, one);
+        return any_of(one);
     }
 };
 // The teacher's probabilities (q of the lane's places, the rest's, what log q is less than lp); false: the row says nothing
-template <int SLOTS, bool REST> __device__ __forceinline__ bool teacher(const List<SLOTS> &list, float (&q)[SLOTS], float &rest, float &minus) {
+template <int SLOTS, int TEAM, bool REST> __device__ __forceinline__ bool teacher(const List<SLOTS, TEAM> &list, float (&q)[SLOTS], float &rest, float &minus) {
     float most = neg_inf(), sum = 0.0f;
     rest = minus = 0.0f;
     if (!REST) {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) most = fmaxf(most, list.lp[s]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, o));
-        if (most == neg_inf()) {
-#pragma unroll
-            for (int s = 0; s < SLOTS; ++s) q[s] = 0.0f;
-            return false;
-        }
+        for (int o = TEAM / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, o));
     }
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) sum += q[s] = expf(REST ? list.lp[s] : list.lp[s] - most);
-    sum = warp_sum(sum);
+    for (int s = 0; s < SLOTS; ++s) sum += q[s] = REST ? expf(list.lp[s]) : most == neg_inf() ? 0.0f : expf(list.lp[s] - most);
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
     if (REST) {
         rest = 1.0f - sum;
         if (rest < LEAST_REST) rest = 0.0f;
         return list.any();
     }
+    if (most == neg_inf()) return false;
     const float inv = 1.0f / sum;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) q[s] *= inv;
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
         cp_commit();
     };
     enter();
-    List<SLOTS> list, next;
+    List<SLOTS, 32> list, next;
     float edge = 0.0f;
     const auto ahead = [&](long long r) {
         if (r >= a.rows) return;
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
         }
         // the row's results
         float q[SLOTS], q_rest, minus;
-        const bool known = teacher<SLOTS, REST>(list, q, q_rest, minus);
+        const bool known = teacher<SLOTS, 32, REST>(list, q, q_rest, minus);
         Sum all = t;
         if (REST) {
             Sum mine = {neg_inf(), 0.0f};
@@ -411,161 +413,121 @@ template <typename T, bool ADD> __device__ __forceinline__ void entry_grads(cons
             if (i0 + j >= 0 && i0 + j < p.vocab) p.d[i0 + j] = from_float<T>(o[j]);
 }
 
-// The list of a row as it is loaded, and what becomes of it: the row's factors and the gradients of the listed tokens within [lo, hi)
-template <typename T, int SLOTS, bool REST, bool ADD> struct RowList {
-    List<SLOTS> list;
-    float own[SLOTS];
-    float lse, rest, weight;
+// The list of a row: the row's factors, and the gradients of the listed tokens within [lo, hi)
+template <typename T, int SLOTS, int TEAM, bool REST, bool ADD> struct RowList {
+    List<SLOTS, TEAM> list;
+    float q[SLOTS], lse, rest, weight;
+    T z[SLOTS], old[SLOTS];
     __device__ __forceinline__ void load(const BwdArgs &a, long long r) {
         list.load(a.tokens, a.lps, r, a.top);
         lse = a.lse[r];
         rest = REST ? a.lse_rest[r] : 0.0f;
         weight = a.dloss[r] * a.scale;
     }
-    __device__ __forceinline__ RowGrad prepare(const BwdArgs &a, const Place<T> &p, int lo, int hi) {
-        float z[SLOTS], old[SLOTS], q[SLOTS], q_rest, minus;
+    // what stands at the listed tokens before anything is written
+    __device__ __forceinline__ void gather(const Place<T> &p, int lo, int hi) {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const bool here = list.tok[s] >= lo && list.tok[s] < hi;
-            z[s] = here ? to_float(p.x[list.tok[s]]) : 0.0f;
-            old[s] = ADD && here ? to_float(p.d[list.tok[s]]) : 0.0f;
+            z[s] = here ? p.x[list.tok[s]] : from_float<T>(0.0f);
+            if (ADD) old[s] = here ? p.d[list.tok[s]] : from_float<T>(0.0f);
         }
-        const bool wrong = list.settle(a.vocab), known = teacher<SLOTS, REST>(list, q, q_rest, minus);
+    }
+    __device__ __forceinline__ RowGrad factors(int vocab) {
+        float q_rest, minus;
+        const bool wrong = list.settle(vocab), known = teacher<SLOTS, TEAM, REST>(list, q, q_rest, minus);
         RowGrad g = {0.0f, 0.0f, wrong ? 2 : known && lse != neg_inf() ? 1 : 0};
         // e^(z - base) * factor off the list; where the rest has no mass all of its logits are -inf
         const bool split = REST && rest != neg_inf();
         g.base = split ? rest : lse;
         g.factor = weight * (split ? expf(rest - lse) - q_rest : 1.0f);
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) own[s] = old[s] + weight * (expf(__fmul_rn(z[s], a.scale) - lse) - q[s]);
         return g;
     }
-    __device__ __forceinline__ void store(T *d, int lo, int hi) const {
+    __device__ __forceinline__ void store(T *d, int lo, int hi, float scale) const {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
-            if (list.tok[s] >= lo && list.tok[s] < hi) d[list.tok[s]] = from_float<T>(own[s]);
+            if (list.tok[s] >= lo && list.tok[s] < hi) {
+                const float o = weight * (expf(__fmul_rn(to_float(z[s]), scale) - lse) - q[s]);
+                d[list.tok[s]] = from_float<T>(ADD ? to_float(old[s]) + o : o);
+            }
     }
 };
 
-// Narrow rows, up to 32 U vectors: a warp each; the next row's list and logits are on the way while it works on one
-template <typename T, int U, int SLOTS, bool REST, bool ADD>
-__global__ void __launch_bounds__(256, 3) distill_backward_warp_kernel(T *dlogits, const T *logits, const BwdArgs a) {
-    const int lane = threadIdx.x & 31;
-    const long long step = (long long)gridDim.x * 8;
-    long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (r >= a.rows) return;
-    RowList<T, SLOTS, REST, ADD> list, next;
-    uint4 q[U], after[U];
-    const auto ahead = [&](long long row) {
-        if (row >= a.rows) return;
-        next.load(a, row);
-        const Place<T> p(dlogits, logits, a, row);
+// Narrow rows, up to TEAM * U vectors: TEAM neighbouring lanes each, as few as the list has places
+template <typename T, int TEAM, int U, int SLOTS, bool REST, bool ADD>
+__global__ void __launch_bounds__(256, 4) distill_backward_rows_kernel(T *dlogits, const T *logits, const BwdArgs a) {
+    const int lane = threadIdx.x & (TEAM - 1);
+    const long long row = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    const bool real = row < a.rows;
+    const long long r = real ? row : a.rows - 1;              // whole warps take part in the lists
+    const Place<T> p(dlogits, logits, a, r);
+    RowList<T, SLOTS, TEAM, REST, ADD> list;
+    list.load(a, r);
+    uint4 q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) p.load(after[u], lane + 32 * u);
-    };
-    ahead(r);
-    for (; r < a.rows; r += step) {
-        list = next;
+    for (int u = 0; u < U; ++u) p.load(q[u], lane + TEAM * u);
+    list.gather(p, 0, a.vocab);
+    const RowGrad g = list.factors(a.vocab);
+    __syncwarp();
+    if (!real || (g.what == 0 && ADD)) return;
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = after[u];
-        ahead(r + step);
-        const Place<T> p(dlogits, logits, a, r);
-        const RowGrad g = list.prepare(a, p, 0, a.vocab);
-        __syncwarp();
-        if (g.what == 0 && ADD) continue;
-#pragma unroll
-        for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], lane + 32 * u, g, a.scale);
-        __syncwarp();
-        if (g.what == 1) list.store(p.d, 0, a.vocab);
-    }
+    for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], lane + TEAM * u, g, a.scale);
+    __syncwarp(List<SLOTS, TEAM>::lanes());
+    if (g.what == 1) list.store(p.d, 0, a.vocab, a.scale);
 }
 
-// Wide rows in segments of 256 U vectors: eight warps work on a segment while its successor is on the way, a ninth prepares the successor's list and writes the
-// gradients of the predecessor's listed tokens over those that the eight wrote.  One barrier a segment; nobody waits for a list.
+// Wide rows in segments of 256 U vectors: eight warps have their logits on the way while a ninth takes the list in hand; it writes the gradients of the listed
+// tokens over those that the eight wrote.
 constexpr int STREAM = 256;
 template <typename T, int U, int SLOTS, bool REST, bool ADD>
 __global__ void __launch_bounds__(STREAM + 32, 3) distill_backward_kernel(T *dlogits, const T *logits, const BwdArgs a, int segs) {
     constexpr int W = 16 / sizeof(T);
-    __shared__ RowGrad shared[2];
-    const int at = threadIdx.x;
-    const bool lists = at >= STREAM;
-    const auto low = [&](const Place<T> &p, int seg) { return max(0, seg * STREAM * U * W - p.mis); };
-    const auto high = [&](const Place<T> &p, int seg) { return min(a.vocab, (seg + 1) * STREAM * U * W - p.mis); };
-    struct Item { long long r; int seg; };
-    const int step_r = (int)(gridDim.x / (unsigned)segs), step_seg = (int)(gridDim.x % (unsigned)segs);
-    const auto step = [&](const Item &i) {
-        Item n = {i.r + step_r, i.seg + step_seg};
-        if (n.seg >= segs) { n.seg -= segs; ++n.r; }
-        return n;
-    };
-    uint4 q[U], after[U];
-    RowList<T, SLOTS, REST, ADD> list, done;
-    bool pending = false, now = false;           // whether done's and list's gradients are to be written
-    const auto ahead = [&](const Item &i) {
-        if (i.r >= a.rows) return;
-        const Place<T> p(dlogits, logits, a, i.r);
-#pragma unroll
-        for (int u = 0; u < U; ++u) p.load(after[u], i.seg * STREAM * U + at + u * STREAM);
-    };
-    const auto prepare = [&](const Item &i, int to) {
-        now = false;
-        if (i.r >= a.rows) return;
-        const Place<T> p(dlogits, logits, a, i.r);
-        list.load(a, i.r);
-        const RowGrad g = list.prepare(a, p, low(p, i.seg), high(p, i.seg));
-        now = g.what == 1;
-        if (at == STREAM) shared[to] = g;
-    };
-    const auto write = [&](const Item &i) {
-        const Place<T> p(dlogits, logits, a, i.r);
-        done.store(p.d, low(p, i.seg), high(p, i.seg));
-    };
-    Item item = {(long long)(blockIdx.x / (unsigned)segs), (int)(blockIdx.x % (unsigned)segs)}, before = item;
-    if (lists) prepare(item, 0); else ahead(item);
-    for (int turn = 0; item.r < a.rows; turn ^= 1) {
-        const Item next = step(item);
+    __shared__ RowGrad shared;
+    const int at = threadIdx.x, seg = (int)(blockIdx.x % (unsigned)segs);
+    const long long r = blockIdx.x / (unsigned)segs;
+    const Place<T> p(dlogits, logits, a, r);
+    if (at >= STREAM) {
+        const int lo = max(0, seg * STREAM * U * W - p.mis), hi = min(a.vocab, (seg + 1) * STREAM * U * W - p.mis);
+        RowList<T, SLOTS, 32, REST, ADD> list;
+        list.load(a, r);
+        list.gather(p, lo, hi);
+        const RowGrad g = list.factors(a.vocab);
+        if (at == STREAM) shared = g;
         __syncthreads();
-        if (lists) {
-            if (pending) write(before);
-            done = list;
-            pending = now;
-            prepare(next, turn ^ 1);
-        } else {
-            const RowGrad g = shared[turn];
-#pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = after[u];
-            ahead(next);
-            if (g.what != 0 || !ADD) {
-                const Place<T> p(dlogits, logits, a, item.r);
-#pragma unroll
-                for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], item.seg * STREAM * U + at + u * STREAM, g, a.scale);
-            }
-        }
-        before = item;
-        item = next;
+        __syncthreads();
+        if (g.what == 1) list.store(p.d, lo, hi, a.scale);
+        return;
     }
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) p.load(q[u], seg * STREAM * U + at + u * STREAM);
     __syncthreads();
-    if (lists && pending) write(before);
+    const RowGrad g = shared;
+    if (g.what != 0 || !ADD)
+#pragma unroll
+        for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], seg * STREAM * U + at + u * STREAM, g, a.scale);
+    __syncthreads();
 }
 
 template <typename T, int SLOTS, bool REST, bool ADD> int launch_backward(T *dlogits, const T *logits, const BwdArgs &a, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
     const int vecs = (a.vocab + W - 1) / W + 1;               // one more: a row may start inside a vector
-    if (vecs <= 32 * 4) {
-        const long long teams = (a.rows + 7) / 8, most = 4ll * sm_count();
-        const unsigned blocks = (unsigned)(teams < most ? teams : most);
-        if (vecs <= 32 * 2) distill_backward_warp_kernel<T, 2, SLOTS, REST, ADD><<<blocks, 256, 0, st>>>(dlogits, logits, a);
-        else distill_backward_warp_kernel<T, 4, SLOTS, REST, ADD><<<blocks, 256, 0, st>>>(dlogits, logits, a);
-    } else {
-        const int u = (double)a.rows * vecs < 4096.0 * sm_count() ? 1 : 4, segs = (vecs + STREAM * u - 1) / (STREAM * u);
-        const long long items = a.rows * segs, most = 3ll * sm_count();
-        const unsigned blocks = (unsigned)(items < most ? items : most);
-        if (u == 1) distill_backward_kernel<T, 1, SLOTS, REST, ADD><<<blocks, STREAM + 32, 0, st>>>(dlogits, logits, a, segs);
-        else distill_backward_kernel<T, 4, SLOTS, REST, ADD><<<blocks, STREAM + 32, 0, st>>>(dlogits, logits, a, segs);
+    const auto go = [&](auto kernel, long long blocks, int threads, auto... more) -> int {
+        if (blocks > 0x7fffffffll) { set_error("b2_distill_backward: %lld rows of %d", a.rows, a.vocab); return B2_ERR_BAD_SHAPE; }
+        kernel<<<(unsigned)blocks, threads, 0, st>>>(dlogits, logits, a, more...);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+        return B2_OK;
+    };
+    if constexpr (SLOTS == 1) {
+        if (a.top <= 8 && vecs <= 8 * 4) return go(distill_backward_rows_kernel<T, 8, 4, 1, REST, ADD>, (a.rows + 31) / 32, 256);
+        if (a.top <= 16 && vecs <= 16 * 6) return go(distill_backward_rows_kernel<T, 16, 6, 1, REST, ADD>, (a.rows + 15) / 16, 256);
     }
-    count_launch();
-    B2_CUDA(cudaGetLastError());
-    return B2_OK;
+    if (vecs <= 32 * 4) return go(distill_backward_rows_kernel<T, 32, 4, SLOTS, REST, ADD>, (a.rows + 7) / 8, 256);
+    const bool few = (double)a.rows * vecs < 4096.0 * sm_count();
+    const int u = few ? 2 : 8, segs = (vecs + STREAM * u - 1) / (STREAM * u);
+    if (few) return go(distill_backward_kernel<T, 2, SLOTS, REST, ADD>, a.rows * segs, STREAM + 32, segs);
+    return go(distill_backward_kernel<T, 8, SLOTS, REST, ADD>, a.rows * segs, STREAM + 32, segs);
 }
 template <typename T, int SLOTS> int backward_of(T *dlogits, const T *logits, const BwdArgs &a, bool add, cudaStream_t st) {
     if (a.lse_rest) return add ? launch_backward<T, SLOTS, true, true>(dlogits, logits, a, st) : launch_backward<T, SLOTS, true, false>(dlogits, logits, a, st);

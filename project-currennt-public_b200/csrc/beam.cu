@@ -17,6 +17,7 @@ namespace {
 
 constexpr int MAX_BEAMS = 64, MAX_BEST = 64, MOST_VOCAB = 1 << 26;
 constexpr int SLICE_THREADS = 256, SLICE_VECS = 4;        // threads of a slice, vectors of 16 bytes each has in registers
+constexpr int CHUNK = SLICE_THREADS * SLICE_VECS;
 
 struct Part { float m, s; };         // largest z of a slice, sum of e^(z - m)
 
@@ -37,21 +38,31 @@ __device__ __forceinline__ bool runs(const SelectArgs &a, long long row) {
 
 // bytes of x as the selector's digits tell; 8 and above: the sign of byte digit - 8, all over
 template <unsigned S> __device__ __forceinline__ unsigned signs(unsigned x) { unsigned y; asm("prmt.b32 %0, %1, 0, %2;" : "=r"(y) : "r"(x), "n"(S)); return y; }
-// -inf in the places of q whose bytes of `on` are 0
-template <typename T> __device__ __forceinline__ void rule_out(uint4 &q, const Vec<unsigned char, 16 / sizeof(T)> &on) {
-    unsigned w[4] = {q.x, q.y, q.z, q.w}, bytes[4 / sizeof(T) + 1];
-    memcpy(bytes, &on, sizeof(on));
+// The mask's bytes of a vector's entries, in words: as an array of bytes they would be taken apart and put together again
+template <typename T> struct Flags { unsigned w[4 / sizeof(T)]; };
+// -inf in the places of q whose bytes are 0
+template <typename T> __device__ __forceinline__ void rule_out(uint4 &q, const Flags<T> &on) {
+    unsigned w[4] = {q.x, q.y, q.z, q.w}, s[2] = {0, 0}, keep[4];      // keep: a sign all over an entry's bytes
 #pragma unroll
-    for (int i = 0; i < 4 / (int)sizeof(T); ++i) bytes[i] |= (bytes[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu;     // the sign of a byte that is not 0
-    unsigned keep[4];                                     // a sign all over an entry's bytes
+    for (int i = 0; i < 4 / (int)sizeof(T); ++i) s[i] = ((on.w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | on.w[i];     // the sign of a byte that is not 0
     if constexpr (sizeof(T) == 4) {
-        keep[0] = signs<0x8888>(bytes[0]); keep[1] = signs<0x9999>(bytes[0]); keep[2] = signs<0xaaaa>(bytes[0]); keep[3] = signs<0xbbbb>(bytes[0]);
+        keep[0] = signs<0x8888>(s[0]); keep[1] = signs<0x9999>(s[0]); keep[2] = signs<0xaaaa>(s[0]); keep[3] = signs<0xbbbb>(s[0]);
     } else {
-        keep[0] = signs<0x9988>(bytes[0]); keep[1] = signs<0xbbaa>(bytes[0]); keep[2] = signs<0x9988>(bytes[1]); keep[3] = signs<0xbbaa>(bytes[1]);
+        keep[0] = signs<0x9988>(s[0]); keep[1] = signs<0xbbaa>(s[0]); keep[2] = signs<0x9988>(s[1]); keep[3] = signs<0xbbaa>(s[1]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = (w[i] & keep[i]) | (Raw<T>::NONE & ~keep[i]);
     q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ Flags<T> load_flags(const unsigned char *m) {
+    Flags<T> f;
+    if constexpr (sizeof(T) == 4) f.w[0] = *reinterpret_cast<const unsigned *>(m);
+    else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(m);
+        f.w[0] = v.x;
+        f.w[1] = v.y;
+    }
+    return f;
 }
 
 // the running sum of a thread
@@ -105,20 +116,17 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
     if (!runs(a, row)) return;
     if (t == 0) n_hits = count = 0;
-    typedef Vec<unsigned char, W> Flags;
     uint4 q[U];
-    Flags on[MASK ? U : 1];
+    Flags<T> on[MASK ? U : 1];
     const auto load = [&](int from) {
         // all of the chunk inside the row, its mask in vectors: what most chunks are
         if (from * W >= mis && (from + THREADS * U) * W - mis <= a.vocab && from + THREADS * U <= v1 && (!MASK || mask_vec)) {
             const uint4 *src = reinterpret_cast<const uint4 *>(x - mis) + from + t;
 #pragma unroll
             for (int u = 0; u < U; ++u) q[u] = src[u * THREADS];
-            if (MASK) {
-                const Flags *m = reinterpret_cast<const Flags *>(mk - mis) + from + t;
+            if (MASK)
 #pragma unroll
-                for (int u = 0; u < U; ++u) on[u] = m[u * THREADS];
-            }
+                for (int u = 0; u < U; ++u) on[u] = load_flags<T>(mk - mis + (from + t + u * THREADS) * W);
             return;
         }
 #pragma unroll
@@ -134,10 +142,14 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
                 memcpy(&q[u], e, 16);
             }
             if (MASK) {
-                if (whole && mask_vec) on[u] = *reinterpret_cast<const Flags *>(mk + i0);
-                else
+                if (whole && mask_vec) on[u] = load_flags<T>(mk + i0);
+                else {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) on[u].v[j] = inside && i0 + j >= 0 && i0 + j < a.vocab ? mk[i0 + j] : 0;
+                    for (int i = 0; i < W / 4; ++i) on[u].w[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (inside && i0 + j >= 0 && i0 + j < a.vocab) on[u].w[j / 4] |= (unsigned)mk[i0 + j] << (8 * (j % 4));
+                }
             }
         }
     };
@@ -273,7 +285,7 @@ __device__ __forceinline__ int token_of(unsigned long long tie) { return MOST_VO
 
 // One block a sequence.  A slice's list is sorted, so the first few entries of every list, 2 K of them together, hold a bound that K continuations reach: the K-th best of
 // them.  All entries that reach it are counted into their places.
-constexpr int JOIN_THREADS = 256, AHEAD = 4, MOST_HEADS = 1024, MOST_FOUND = 1024;
+constexpr int JOIN_THREADS = 256, AHEAD = 2, MOST_HEADS = 1024, MOST_FOUND = 1024;
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArgs a) {
     __shared__ double off[MAX_BEAMS], weight[MAX_BEAMS];
     __shared__ bool ended[MAX_BEAMS];
@@ -418,17 +430,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
 }
 
 int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
-// Slices of a row: one where the rows fill the device (bounds and lists cost a slice several chunks' time), more where they do not, as long as each has a chunk of 1024
-// vectors
+// Slices of a row, of whole chunks of 1024 vectors: one where the rows fill the device (bounds and lists cost a slice several chunks' time), more where they do not
 int slices_of(long long rows, int vocab, int type) {
-    const int chunks = (vectors_of(vocab, type) + SLICE_THREADS * SLICE_VECS - 1) / (SLICE_THREADS * SLICE_VECS);
-    const long long most = rows ? (592 + rows - 1) / rows : 1;          // blocks that run at a time: 4 an SM
-    return (int)(chunks < most ? chunks : most);
+    const int chunks = (vectors_of(vocab, type) + CHUNK - 1) / CHUNK;
+    const long long most = rows && rows < 592 ? 592 / rows : 1;          // blocks that run at a time: 4 an SM
+    const int each = (int)((chunks + most - 1) / most);
+    return (chunks + each - 1) / each;
 }
 
 template <typename T> int select(const T *logits, SelectArgs a, int type, cudaStream_t st) {
-    const int vecs = vectors_of(a.vocab, type);
-    a.slice = (vecs + a.slices - 1) / a.slices;
+    const int chunks = (vectors_of(a.vocab, type) + CHUNK - 1) / CHUNK;
+    a.slice = (chunks + a.slices - 1) / a.slices * CHUNK;
     const long long blocks = a.groups * a.beams * a.slices;
     if (blocks > 0x7fffffffll) { set_error("b2_beam_select: %lld rows of %d", a.groups * a.beams, a.vocab); return B2_ERR_BAD_SHAPE; }
     if (a.mask) beam_rows_kernel<T, true><<<(unsigned)blocks, SLICE_THREADS, 0, st>>>(logits, a);

@@ -484,12 +484,48 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
 
 // Many rows: a pair of blocks (cta_group::2) has a tile of 256 channels, 128 in each block, and 256 rows, of which each block holds 128 in its shared memory.  A
 // slab so costs a block 32 KB of copies and 32 KB of operand reads for 512 cycles of multiplication; by itself, with the same tile, it would be 48 and 48.
-constexpr int PAIR_BN = 256, PAIR_STAGE = A_BYTES + PAIR_BN / 2 * BK, PAIR_STAGES = 6, PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024, PAIR_TMEM = 512;
-template <typename O>
+// The data path of the shared memory is what bounds short contractions: with 8 slabs a tile takes 4096 cycles of multiplication, 2048 of operand reads, as many of
+// copies, 1024 of accumulators read and 2200 of stores.  So up to 9 slabs of weights stay in shared memory over all tiles of their channels (RESIDENT), and only the
+// activations pass through the ring.
+constexpr int PAIR_BN = 256, PAIR_B = PAIR_BN / 2 * BK, PAIR_TMEM = 512, MOST_RESIDENT = 9;
+template <bool RESIDENT> struct PairShape {
+    static constexpr int STAGE = RESIDENT ? PAIR_B : A_BYTES + PAIR_B, STAGES = RESIDENT ? 4 : 6;
+    static constexpr int SMEM = STAGES * STAGE + (RESIDENT ? MOST_RESIDENT * A_BYTES : 0) + 1024;
+};
+// The tiles of a pair.  Neighbouring pairs work on neighbouring channels of the same rows at the same time: where rows of `out` are not aligned, a sector between two
+// tiles is written by both, and should be in the L2 still when the second one comes (8192 x 50001 x 1024: 498 us with a run of tiles for each pair).
+// RESIDENT: all rows of a channel tile, round by round; the channel tiles of the last round are dealt out in runs of rows.  Else: rows first, in turn.
+template <bool RESIDENT> struct PairTiles {
+    unsigned pair, pairs, rows, whole, rest0, count;       // whole: tiles of the full rounds
+    __device__ __forceinline__ PairTiles(const ProductArgs &a) : pair(blockIdx.x >> 1), pairs(gridDim.x >> 1), rows(a.row_tiles) {
+        if (RESIDENT) {
+            const unsigned rounds = a.channel_tiles / pairs;
+            const unsigned long long rest = (unsigned long long)(a.channel_tiles - rounds * pairs) * rows;
+            whole = rounds * rows;
+            rest0 = (unsigned)(rest * pair / pairs);
+            count = whole + (unsigned)(rest * (pair + 1) / pairs) - rest0;
+        } else {
+            whole = rest0 = 0;
+            count = (rows * a.channel_tiles - pair + pairs - 1) / pairs;
+        }
+    }
+    // row and channel tile of the n-th one; whether its weights are others than those of the one before
+    __device__ __forceinline__ bool at(unsigned n, unsigned &r, unsigned &c) const {
+        unsigned t, c0;
+        if (!RESIDENT) { t = pair + n * pairs; c0 = 0; }
+        else if (n < whole) { t = n % rows; c0 = pair + n / rows * pairs; }
+        else { t = rest0 + n - whole; c0 = whole / rows * pairs; }
+        r = t % rows;
+        c = c0 + t / rows;
+        return !RESIDENT || n == 0 || n == whole || r == 0;
+    }
+};
+template <bool RESIDENT, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
     using namespace ptx;
-    constexpr int BN = PAIR_BN, STAGES = PAIR_STAGES;
+    typedef PairShape<RESIDENT> S;
+    constexpr int BN = PAIR_BN, STAGES = S::STAGES, STAGE = S::STAGE;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * STAGES + 5];
     __shared__ __align__(16) float scales[8][BN / 2];
@@ -497,14 +533,14 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __shared__ volatile int fail;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars), held = ring + STAGES * STAGE;      // held: the weights that stay
     // full and acc_empty: the even block's count; empty, acc_full: each block has its own
     const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
     const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
     const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
     const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
     const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4);
-    const unsigned tiles = a.row_tiles * a.channel_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const PairTiles<RESIDENT> tiles(a);
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 16); }
@@ -525,15 +561,18 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             unsigned i = 0;
             bool ok = true;
             if (a.chained) { grid_wait(); fence_async_global(); }
-            for (unsigned tile = pair; tile < tiles && ok; tile += pairs) {
-                const int r0 = (int)(tile % a.row_tiles) * BN + (int)rank * (BN / 2), c0 = (int)(tile / a.row_tiles) * (2 * BM) + (int)rank * BM;
+            for (unsigned n = 0; n < tiles.count && ok; ++n) {
+                unsigned r, c;
+                const bool fresh = tiles.at(n, r, c);
+                const int r0 = (int)r * BN + (int)rank * (BN / 2), c0 = (int)c * (2 * BM) + (int)rank * BM;
                 for (int k = 0; k < a.slabs; ++k, ++i) {
                     const int s = (int)(i % STAGES);
                     if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                    const uint32_t at = ring + (uint32_t)s * PAIR_STAGE, bar = map_to_rank(full(s), 0);
-                    if (rank == 0) mbar_expect_tx(full(s), 2 * PAIR_STAGE);
-                    tma_load_2d_pair(at, &map_w, k * BK, c0, bar);
-                    tma_load_2d_pair(at + A_BYTES, &map_x, k * BK, r0, bar);
+                    // (the weights that were in slab k are read: its last products came before those that freed the slot)
+                    const uint32_t at = ring + (uint32_t)s * STAGE, bar = map_to_rank(full(s), 0);
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * (PAIR_B + (fresh ? A_BYTES : 0)));
+                    if (fresh) tma_load_2d_pair(RESIDENT ? held + (uint32_t)k * A_BYTES : at + PAIR_B, &map_w, k * BK, c0, bar);
+                    tma_load_2d_pair(at, &map_x, k * BK, r0, bar);
                 }
             }
             if (!ok && rank == 0)      // copies under way end before the blocks do
@@ -545,9 +584,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             const uint32_t idesc = idesc_s8(2 * BM, BN);
-            unsigned i = 0, n = 0;
+            unsigned i = 0;
             bool ok = true;
-            for (unsigned tile = pair; tile < tiles && ok; tile += pairs, ++n) {
+            for (unsigned n = 0; n < tiles.count && ok; ++n) {
                 const uint32_t d = tmem + (n & 1u) * BN;
                 if (!mbar_wait_bounded<true>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                 tc_fence_after();
@@ -555,10 +594,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     const int s = (int)(i % STAGES);
                     if (!mbar_wait_bounded<true>(full(s), (i / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                     tc_fence_after();
-                    const uint32_t at = ring + (uint32_t)s * PAIR_STAGE;
+                    const uint32_t x = ring + (uint32_t)s * STAGE, w = RESIDENT ? held + (uint32_t)k * A_BYTES : x + PAIR_B;
 #pragma unroll
-                    for (int kk = 0; kk < BK / 32; ++kk)
-                        mma_s8_pair(d, desc_kmajor_sw128(at + kk * 32, 1024), desc_kmajor_sw128(at + A_BYTES + kk * 32, 1024), idesc, (k | kk) ? 1u : 0u);
+                    for (int kk = 0; kk < BK / 32; ++kk) mma_s8_pair(d, desc_kmajor_sw128(w + kk * 32, 1024), desc_kmajor_sw128(x + kk * 32, 1024), idesc, (k | kk) ? 1u : 0u);
                     mma_commit_pair(empty(s));
                 }
                 if (ok) mma_commit_pair(acc_full((int)(n & 1u)));
@@ -572,12 +610,13 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     } else {
         constexpr int HALF = BN / 2;
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        unsigned n = 0;
         bool ok = true;
         if (a.chained) grid_wait();
-        for (unsigned tile = pair; tile < tiles; tile += pairs, ++n) {
-            const long long r0 = (long long)(tile % a.row_tiles) * BN + half * HALF;
-            const int c = (int)(tile / a.row_tiles) * (2 * BM) + (int)rank * BM + 32 * quarter + lane;
+        for (unsigned n = 0; n < tiles.count; ++n) {
+            unsigned row_tile, channel_tile;
+            tiles.at(n, row_tile, channel_tile);
+            const long long r0 = (long long)row_tile * BN + half * HALF;
+            const int c = (int)channel_tile * (2 * BM) + (int)rank * BM + 32 * quarter + lane;
             const bool real = c < a.channels;
             const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
             load_scales<HALF>(scales[warp - 2], a.x_scales, r0, a.rows);
@@ -597,7 +636,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 }
 
 // pairs of blocks that run side by side, by device
-int pair_count(const void *kernel, int *out) {
+int pair_count(const void *kernel, int bytes, int *out) {
     static std::mutex mu;
     static int known[MAX_DEVICES];      // of all element types: a block has its SM to itself
     const int dev = current_device();
@@ -608,7 +647,7 @@ int pair_count(const void *kernel, int *out) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * (unsigned)(sm_count() / 2 > 0 ? sm_count() / 2 : 1));
         cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = PAIR_SMEM;
+        cfg.dynamicSmemBytes = bytes;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = 2;
@@ -636,15 +675,16 @@ template <int BN, typename O> int launch_product(const CUtensorMap &mw, const CU
     B2_CUDA(cudaGetLastError());
     return B2_OK;
 }
-template <typename O> int launch_pairs(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
-    const auto kernel = int8_pair_kernel<O>;
-    B2_TRY(set_max_dynamic_smem((const void *)kernel, PAIR_SMEM));
+template <bool RESIDENT, typename O> int launch_pairs(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
+    const auto kernel = int8_pair_kernel<RESIDENT, O>;
+    constexpr int BYTES = PairShape<RESIDENT>::SMEM;
+    B2_TRY(set_max_dynamic_smem((const void *)kernel, BYTES));
     int pairs;
-    B2_TRY(pair_count((const void *)kernel, &pairs));
+    B2_TRY(pair_count((const void *)kernel, BYTES, &pairs));
     const long long tiles = (long long)a.row_tiles * a.channel_tiles;
     const unsigned blocks = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-    if (a.chained) return launch_chained(int8_pair_kernel<O>, dim3(blocks), dim3(THREADS), PAIR_SMEM, st, mw, mx, out, a);
-    kernel<<<blocks, THREADS, PAIR_SMEM, st>>>(mw, mx, out, a);
+    if (a.chained) return launch_chained(int8_pair_kernel<RESIDENT, O>, dim3(blocks), dim3(THREADS), BYTES, st, mw, mx, out, a);
+    kernel<<<blocks, THREADS, BYTES, st>>>(mw, mx, out, a);
     count_launch();
     B2_CUDA(cudaGetLastError());
     return B2_OK;
@@ -663,7 +703,7 @@ template <typename O> int product(O *out, const signed char *x, long long ld_x, 
         a.row_tiles = (unsigned)((a.rows + BN - 1) / BN);
         a.channel_tiles = (unsigned)((a.channels + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM));
         if ((double)a.row_tiles * a.channel_tiles > 4e9) { set_error("b2_int8_product: %lld rows of %d channels", a.rows, a.channels); return B2_ERR_BAD_SHAPE; }
-        if constexpr (PAIR) return launch_pairs<O>(mw, mx, out, a, st);
+        if constexpr (PAIR) return a.slabs <= MOST_RESIDENT ? launch_pairs<true, O>(mw, mx, out, a, st) : launch_pairs<false, O>(mw, mx, out, a, st);
         else return launch_product<BN, O>(mw, mx, out, a, st);
     };
     if (a.rows <= 16) return go(std::integral_constant<int, 16>());

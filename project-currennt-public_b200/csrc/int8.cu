@@ -51,13 +51,14 @@ struct RowScale {
         inv = some ? __fdiv_rn(127.0f, most) : 0.0f;
         scale = !finite ? nanf("") : some ? __fdiv_rn(most, 127.0f) : 0.0f;
     }
+    __device__ __forceinline__ unsigned char quantised(float x) const { return finite ? (unsigned char)__float_as_uint(fmaf(x, inv, 12582912.0f)) : 0; }
     template <typename T> __device__ __forceinline__ Vec<unsigned char, 16 / sizeof(T)> quantised(const uint4 &h) const {
         constexpr int W = 16 / sizeof(T);
         T e[W];
         memcpy(e, &h, 16);
         Vec<unsigned char, W> o;
 #pragma unroll
-        for (int j = 0; j < W; ++j) o.v[j] = finite ? (unsigned char)__float_as_uint(fmaf(to_float(e[j]), inv, 12582912.0f)) : 0;
+        for (int j = 0; j < W; ++j) o.v[j] = quantised(to_float(e[j]));
         return o;
     }
 };
@@ -149,13 +150,14 @@ struct ProductArgs {
     const float *x_scales, *w_scales, *bias;
     long long ld_out, rows;
     int channels, slabs;
-    unsigned row_tiles, channel_tiles;
+    unsigned row_tiles, channel_tiles, splits;
     int chained;
 };
 
 // N columns (rows r0 on of out) of a thread's tensor-memory lane (channel c; real: there is one) to out.  xs: their scales in shared memory, 16-byte aligned
-template <int N, typename O>
-__device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, float ws, float bias, bool real, bool ok, O *out, long long ld, long long r0, long long rows, int c) {
+// more(v, j): what is added to the columns j on, of which v holds the sums
+template <int N, typename O, typename F>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, float ws, float bias, bool real, bool ok, O *out, long long ld, long long r0, long long rows, int c, F &&more) {
     constexpr int STEP = N < 32 ? N : 32;
     const long long left = rows - r0;
     O *p = out + r0 * ld + c;
@@ -167,6 +169,7 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, f
         else if constexpr (STEP == 16) ptx::tmem_ld16(taddr + j0, v);
         else ptx::tmem_ld8(taddr + j0, v);
         ptx::tmem_ld_wait();
+        more(v, j0);
         const auto put = [&](bool all) {
 #pragma unroll
             for (int j = 0; j < STEP; j += 4) {
@@ -184,6 +187,10 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, f
         if (j0 + STEP <= left) put(true); else put(false);
     }
 }
+template <int N, typename O>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const float *xs, float ws, float bias, bool real, bool ok, O *out, long long ld, long long r0, long long rows, int c) {
+    store_columns<N>(taddr, xs, ws, bias, real, ok, out, ld, r0, rows, c, [](auto &, int) {});
+}
 // a warp's copy of the scales of N rows from r0 on
 template <int N> __device__ __forceinline__ void load_scales(float *xs, const float *x_scales, long long r0, long long rows) {
     const int lane = threadIdx.x & 31;
@@ -194,95 +201,90 @@ template <int N> __device__ __forceinline__ void load_scales(float *xs, const fl
     __syncwarp();
 }
 
-// Up to 128 rows: a block's tile has BN columns, the weights stream through the ring
-template <int BN> struct Shape {
-    static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
-    static constexpr int STAGES = BN >= 128 ? 6 : 8;
+// Up to 128 rows: a block's tile has BN columns, the weights stream through the ring.  Few channels: the blocks of a cluster (a.splits of them) share the slabs of a tile, and
+// the first one adds up their sums, which the others lay down in its shared memory: whole numbers, so that the split changes nothing.
+template <int BN, int STAGES_> struct Shape {
+    static constexpr int STAGE_BYTES = A_BYTES + BN * BK, STAGES = STAGES_;
     static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // slack: the swizzle wants 1024-byte alignment
     static constexpr int TMEM = 2 * BN;
 };
-template <int BN, typename O>
-__global__ void __launch_bounds__(THREADS, 1)
+// the most blocks that share a tile: the others' sums lie in the first one's ring
+template <int BN> constexpr int most_splits() { return 4 * Shape<BN, 4>::STAGE_BYTES >= 7 * BN * BM * 4 ? 8 : 4 * Shape<BN, 4>::STAGE_BYTES >= 3 * BN * BM * 4 ? 4 : 2; }
+template <int BN, int STAGES, typename O>
+__global__ void __launch_bounds__(THREADS, STAGES == 4 && BN < 128 ? 2 : 1)
 int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
     using namespace ptx;
-    typedef Shape<BN> S;
+    typedef Shape<BN, STAGES> S;
+    constexpr int HALF = BN / 2;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 5];
-    __shared__ __align__(16) float scales[8][BN / 2];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES + 5];
+    __shared__ __align__(16) float scales[8][HALF];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int fail;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
     const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
-    const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(S::STAGES + s); };
-    const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * S::STAGES + b); };
-    const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * S::STAGES + 2 + b); };
-    const uint32_t idle = bar0 + 8u * (uint32_t)(2 * S::STAGES + 4);
-    const unsigned tiles = a.row_tiles * a.channel_tiles;
+    const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
+    const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4);
+    // the tiles t0, t0 + step, ... (split: the one), and of each the slabs s0 on
+    const unsigned tiles = a.row_tiles * a.channel_tiles, rank = a.splits > 1 ? cluster_ctarank() : 0, t0 = blockIdx.x / a.splits, step = gridDim.x / a.splits;
+    const int s0 = (int)(a.slabs * rank / a.splits), slabs = (int)(a.slabs * (rank + 1) / a.splits) - s0;
+    const unsigned mine = (tiles - t0 + step - 1) / step * (unsigned)slabs, first = min(mine, (unsigned)STAGES);      // slabs of this block
+    const auto copy_w = [&](unsigned i) {
+        const int s = (int)(i % STAGES);
+        mbar_expect_tx(full(s), S::STAGE_BYTES);
+        tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES, &map_w, (s0 + (int)(i % (unsigned)slabs)) * BK, (int)((t0 + i / (unsigned)slabs * step) / a.row_tiles) * BM, full(s));
+    };
+    const auto copy_x = [&](unsigned i) {
+        const int s = (int)(i % STAGES);
+        tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES + A_BYTES, &map_x, (s0 + (int)(i % (unsigned)slabs)) * BK, (int)((t0 + i / (unsigned)slabs * step) % a.row_tiles) * BN, full(s));
+    };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 8); }
         mbar_init(idle, 1);
         fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
+        // The first slabs' weights are on the way before the block is set up, and before the activations, which the launch before this one may still be writing
+        for (unsigned i = 0; i < first; ++i) copy_w(i);
     }
     if (warp == 1) tmem_alloc(smem_u32((const void *)&tmem_slot), S::TMEM);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    bool ok = true;
 
     if (warp == 0) {
         if (lane == 0) {
-            unsigned i = 0;
-            bool ok = true;
-            const unsigned mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * (unsigned)a.slabs;     // slabs of this block
-            const auto of = [&](unsigned k, int &r0, int &c0, int &at) {
-                const unsigned tile = blockIdx.x + k / (unsigned)a.slabs * gridDim.x;
-                r0 = (int)(tile % a.row_tiles) * BN;
-                c0 = (int)(tile / a.row_tiles) * BM;
-                at = (int)(k % (unsigned)a.slabs) * BK;
-            };
-            int r0, c0, at;
-            // The first slabs' weights are on the way before the activations, which the launch before this one may still be writing
-            const unsigned first = min(mine, (unsigned)S::STAGES);
-            for (i = 0; i < first; ++i) {
-                of(i, r0, c0, at);
-                mbar_expect_tx(full((int)i), S::STAGE_BYTES);
-                tma_load_2d(ring + i * S::STAGE_BYTES, &map_w, at, c0, full((int)i));
-            }
             if (a.chained) { grid_wait(); fence_async_global(); }
-            for (i = 0; i < first; ++i) {
-                of(i, r0, c0, at);
-                tma_load_2d(ring + i * S::STAGE_BYTES + A_BYTES, &map_x, at, r0, full((int)i));
-            }
+            unsigned i = 0;
+            for (; i < first; ++i) copy_x(i);
             for (; i < mine; ++i) {
-                const int s = (int)(i % S::STAGES);
-                if (!mbar_wait_bounded<false>(empty(s), ((i / S::STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                of(i, r0, c0, at);
-                mbar_expect_tx(full(s), S::STAGE_BYTES);
-                tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES, &map_w, at, c0, full(s));
-                tma_load_2d(ring + (uint32_t)s * S::STAGE_BYTES + A_BYTES, &map_x, at, r0, full(s));
+                if (!mbar_wait_bounded<false>(empty((int)(i % STAGES)), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                copy_w(i);
+                copy_x(i);
             }
             if (!ok)      // copies under way end before the block does
-                for (unsigned j = i > (unsigned)S::STAGES ? i - S::STAGES : 0; j < i; ++j) {
+                for (unsigned j = i > (unsigned)STAGES ? i - STAGES : 0; j < i; ++j) {
                     volatile int never = 0;
-                    mbar_wait_bounded<false>(full((int)(j % S::STAGES)), (j / S::STAGES) & 1u, &never, WAIT_CYCLES);
+                    mbar_wait_bounded<false>(full((int)(j % STAGES)), (j / STAGES) & 1u, &never, WAIT_CYCLES);
                 }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             const uint32_t idesc = idesc_s8(BM, BN);
             unsigned i = 0, n = 0;
-            bool ok = true;
-            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+            for (unsigned tile = t0; tile < tiles && ok; tile += step, ++n) {
                 const uint32_t d = tmem + (n & 1u) * BN;
                 if (!mbar_wait_bounded<false>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                 tc_fence_after();
-                for (int k = 0; k < a.slabs; ++k, ++i) {
-                    const int s = (int)(i % S::STAGES);
-                    if (!mbar_wait_bounded<false>(full(s), (i / S::STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                for (int k = 0; k < slabs; ++k, ++i) {
+                    const int s = (int)(i % STAGES);
+                    if (!mbar_wait_bounded<false>(full(s), (i / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                     tc_fence_after();
                     const uint32_t at = ring + (uint32_t)s * S::STAGE_BYTES;
 #pragma unroll
@@ -298,26 +300,58 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 mbar_wait_bounded<false>(idle, 0, &never, WAIT_CYCLES);
             }
         }
-    } else {
-        // A warp reads the tensor-memory lanes 32 * (warp % 4) on; warps 2 to 5 take the first half of the columns, 6 to 9 the second
-        constexpr int HALF = BN / 2;
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+    }
+    // A warp reads the tensor-memory lanes 32 * (warp % 4) on; warps 2 to 5 take the first half of the columns, 6 to 9 the second
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t sums = tmem + ((uint32_t)(32 * quarter) << 16) + half * HALF;
+    long long r0 = 0;
+    int c = 0;
+    float ws = 0.0f, bias = 0.0f;
+    if (warp >= 2) {
         unsigned n = 0;
-        bool ok = true;
         if (a.chained) grid_wait();
-        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-            const long long r0 = (long long)(tile % a.row_tiles) * BN + half * HALF;
-            const int c = (int)(tile / a.row_tiles) * BM + 32 * quarter + lane;
+        for (unsigned tile = t0; tile < tiles; tile += step, ++n) {
+            r0 = (long long)(tile % a.row_tiles) * BN + half * HALF;
+            c = (int)(tile / a.row_tiles) * BM + 32 * quarter + lane;
             const bool real = c < a.channels;
-            const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
+            ws = real ? a.w_scales[c] : 0.0f;
+            bias = real && a.bias ? a.bias[c] : 0.0f;
             load_scales<HALF>(scales[warp - 2], a.x_scales, r0, a.rows);
             ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
             if (!ok && lane == 0) fail = 1;
             tc_fence_after();
-            store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales[warp - 2], ws, bias, real, ok, out, a.ld_out, r0, a.rows, c);
+            if (a.splits > 1) break;
+            store_columns<HALF>(sums + (n & 1u) * BN, scales[warp - 2], ws, bias, real, ok, out, a.ld_out, r0, a.rows, c);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty((int)(n & 1u)));
+        }
+    }
+    if (a.splits > 1) {
+        // the products of all blocks are complete, and the first one's ring is free
+        __syncwarp();
+        cluster_sync_all();
+        const uint32_t place = ring + (uint32_t)(half * HALF) * (4 * BM) + 4u * (uint32_t)(32 * quarter + lane);
+        if (warp >= 2 && rank) {
+            const uint32_t there = map_to_rank(place + (rank - 1) * (BN * BM * 4), 0);
+#pragma unroll 2
+            for (int j0 = 0; j0 < HALF; j0 += 8) {
+                uint32_t v[8];
+                tmem_ld8(sums + j0, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) st_cluster_u32(there + (uint32_t)(j0 + j) * (4 * BM), v[j]);
+            }
+            if (!ok && lane == 0) st_cluster_u32(map_to_rank(smem_u32((const void *)&fail), 0), 1);
+        }
+        cluster_sync_all();
+        if (warp >= 2 && !rank) {
+            const int *others = reinterpret_cast<const int *>(smem_raw + (place - smem_u32(smem_raw)));
+            store_columns<HALF>(sums, scales[warp - 2], ws, bias, c < a.channels, ok && !fail, out, a.ld_out, r0, a.rows, c, [&](auto &v, int j0) {
+                for (unsigned p = 0; p + 1 < a.splits; ++p)
+#pragma unroll
+                    for (unsigned j = 0; j < sizeof(v) / 4; ++j) v[j] += (uint32_t)others[(p * BN + j0 + j) * BM];
+            });
         }
     }
     tc_fence_before();
@@ -325,29 +359,52 @@ int8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (warp == 1) tmem_dealloc(tmem, S::TMEM);
 }
 
-// Few rows of activations that are no integers yet: every block quantises them for itself, into the layout of the tensor cores' operand, while its
+// Up to 8 short rows of activations that are no integers yet: every block quantises them for itself, into the layout of the tensor cores' operand, while its
 // first slabs of weights are on the way.  One launch, and the activations pass through no memory.
-constexpr int ROWS_STAGES = 8, ROWS_X_BYTES = 80 * 1024;
-template <int BN> constexpr int rows_smem(int slabs) { return ROWS_STAGES * A_BYTES + slabs * BN * BK + 1024; }
-template <int BN, typename T, typename O>
+constexpr int ROWS_BN = 16, ROWS_STAGES = 8;      // columns of a tile, slabs of the ring
+constexpr int rows_smem(int slabs) { return ROWS_STAGES * A_BYTES + slabs * ROWS_BN * BK + 1024; }
+template <typename T, typename O>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long long ld_x, int dim, O *out, const ProductArgs a) {
     using namespace ptx;
-    constexpr int STAGES = ROWS_STAGES, W = 16 / sizeof(T), TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    constexpr int BN = ROWS_BN, STAGES = ROWS_STAGES, W = 16 / sizeof(T), U = sizeof(T) == 4 ? 8 : 4, TMEM = 2 * BN, HALF = BN / 2;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * STAGES + 6];
     __shared__ __align__(16) float scales[BN];
+    __shared__ float most[8];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int fail;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp - 2;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = smem_u32(bars), operand = ring + STAGES * A_BYTES;
     const auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
     const auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
     const auto acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
     const auto acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
     const uint32_t idle = bar0 + 8u * (uint32_t)(2 * STAGES + 4), x_full = bar0 + 8u * (uint32_t)(2 * STAGES + 5);
-    const unsigned tiles = a.channel_tiles;
-    const unsigned mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * (unsigned)a.slabs, first = min(mine, (unsigned)STAGES);      // slabs of this block
+    const unsigned tiles = a.channel_tiles, t0 = blockIdx.x, step = gridDim.x;
+    const int slabs = a.slabs;
+    const unsigned mine = (tiles - t0 + step - 1) / step * (unsigned)slabs, first = min(mine, (unsigned)STAGES);      // slabs of this block
+    const auto copy = [&](unsigned i) {
+        const int s = (int)(i % STAGES);
+        mbar_expect_tx(full(s), A_BYTES);
+        tma_load_2d(ring + (uint32_t)s * A_BYTES, &map_w, (int)(i % (unsigned)slabs) * BK, (int)(t0 + i / (unsigned)slabs * step) * BM, full(s));
+    };
+    // Warp w has row w % together of x, the vectors of part w / together of `parts`: with few rows several warps share one
+    const int together = a.rows > 4 ? 8 : a.rows > 2 ? 4 : (int)a.rows, parts = 8 / together, part = w / together, r = w % together;
+    const bool there = warp >= 2 && r < a.rows;
+    const T *row = x + (there ? r : 0) * ld_x;
+    // in vectors where the row allows it, else entry by entry: a launch runs through its code once, and what it has to fetch of it counts
+    const bool vectors = there && (((uintptr_t)row & 15) == 0) && dim % W == 0;
+    uint4 held[U];
+    float m = 0.0f;
+    if (vectors) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = ((part + u * parts) * 32 + lane) * W;
+            held[u] = i < dim ? *reinterpret_cast<const uint4 *>(row + i) : make_uint4(0, 0, 0, 0);
+        }
+    } else if (there)
+        for (int i = part * 32 + lane; i < dim; i += 32 * parts) m = larger_magnitude(m, fabsf(to_float(row[i])));
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 8); }
@@ -357,28 +414,23 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
         // the first slabs are on the way before the block is set up
-        for (unsigned i = 0; i < first; ++i) {
-            mbar_expect_tx(full((int)i), A_BYTES);
-            tma_load_2d(ring + i * A_BYTES, &map_w, (int)(i % (unsigned)a.slabs) * BK, (int)(blockIdx.x + i / (unsigned)a.slabs * gridDim.x) * BM, full((int)i));
-        }
+        for (unsigned i = 0; i < first; ++i) copy(i);
     }
     if (warp == 1) tmem_alloc(smem_u32((const void *)&tmem_slot), TMEM);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    bool ok = true;
 
     if (warp == 0) {
         if (lane == 0) {
             unsigned i = first;
-            bool ok = true;
             for (; i < mine; ++i) {
-                const int s = (int)(i % STAGES);
-                if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                mbar_expect_tx(full(s), A_BYTES);
-                tma_load_2d(ring + (uint32_t)s * A_BYTES, &map_w, (int)(i % (unsigned)a.slabs) * BK, (int)(blockIdx.x + i / (unsigned)a.slabs * gridDim.x) * BM, full(s));
+                if (!mbar_wait_bounded<false>(empty((int)(i % STAGES)), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                copy(i);
             }
-            if (!ok)
+            if (!ok)      // copies under way end before the block does
                 for (unsigned j = i > (unsigned)STAGES ? i - STAGES : 0; j < i; ++j) {
                     volatile int never = 0;
                     mbar_wait_bounded<false>(full((int)(j % STAGES)), (j / STAGES) & 1u, &never, WAIT_CYCLES);
@@ -388,13 +440,13 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
         if (lane == 0) {
             const uint32_t idesc = idesc_s8(BM, BN);
             unsigned i = 0, n = 0;
-            bool ok = mbar_wait_bounded<false>(x_full, 0, &fail, WAIT_CYCLES);
+            ok = mbar_wait_bounded<false>(x_full, 0, &fail, WAIT_CYCLES);
             if (!ok) fail = 1;
-            for (unsigned tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+            for (unsigned tile = t0; tile < tiles && ok; tile += step, ++n) {
                 const uint32_t d = tmem + (n & 1u) * BN;
                 if (!mbar_wait_bounded<false>(acc_empty((int)(n & 1u)), ((n >> 1) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                 tc_fence_after();
-                for (int k = 0; k < a.slabs; ++k, ++i) {
+                for (int k = 0; k < slabs; ++k, ++i) {
                     const int s = (int)(i % STAGES);
                     if (!mbar_wait_bounded<false>(full(s), (i / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
                     tc_fence_after();
@@ -412,66 +464,50 @@ int8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const T *x, long lon
             }
         }
     } else {
-        // the rows of x: a warp's rows w, w + 8, ...; columns without a row, and positions behind the last one, meet zeros of the weights or are not stored
-        const int w = warp - 2;
+        // Columns without a row, and positions behind the last one, meet zeros of the weights or are not stored
         unsigned char *const to = smem_raw + (operand - smem_u32(smem_raw));
-        for (int r = w; r < BN && r < a.rows; r += 8) {
-            const T *row = x + r * ld_x;
-            const int mis = (int)(((uintptr_t)row & 15) / sizeof(T)), vecs = (mis + dim + W - 1) / W;
-            const auto load = [&](int v) -> uint4 {
-                const int i0 = v * W - mis;
-                if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(row + i0);
-                T e[W];
-#pragma unroll
-                for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? row[i0 + j] : from_float<T>(0.0f);
-                uint4 o;
-                memcpy(&o, e, 16);
-                return o;
-            };
-            constexpr int U = 8;
-            uint4 held[U];
-            float m = 0.0f;
-#pragma unroll
-            for (int u = 0; u < U; ++u) held[u] = lane + 32 * u < vecs ? load(lane + 32 * u) : make_uint4(0, 0, 0, 0);
+        if (vectors)
 #pragma unroll
             for (int u = 0; u < U; ++u) m = larger_magnitude(m, largest_magnitude<T>(held[u]));
-            for (int v = lane + 32 * U; v < vecs; v += 32) m = larger_magnitude(m, largest_magnitude<T>(load(v)));
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const RowScale s(m);
-            if (lane == 0) scales[r] = s.scale;
-            const auto store = [&](int v, const uint4 &h) {
-                const int i0 = v * W - mis;
-                const Vec<unsigned char, W> o = s.template quantised<T>(h);
-                // slab, row of 128 bytes, 16-byte chunk with its index xor the row's
-                const auto place = [&](int k) { return (k / BK) * (BN * BK) + r * BK + ((((k % BK) >> 4) ^ (r & 7)) << 4) + (k & 15); };
-                if (mis == 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + place(i0)) = o;
-                else
+        for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (parts > 1) {
+            if (lane == 0) most[w] = m;
+            bar_named(1, 256);
+            for (int p = 0; p < parts; ++p) m = larger_magnitude(m, most[r + p * together]);
+        }
+        if (there) {
+            const RowScale q(m);
+            if (lane == 0 && part == 0) scales[r] = q.scale;
+            // slab, row of 128 bytes, 16-byte chunk with its index xor the row's
+            const auto place = [&](int k) { return (k / BK) * (BN * BK) + r * BK + ((((k % BK) >> 4) ^ (r & 7)) << 4) + (k & 15); };
+            if (vectors) {
 #pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        if (i0 + j >= 0 && i0 + j < dim) to[place(i0 + j)] = o.v[j];
-            };
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (lane + 32 * u < vecs) store(lane + 32 * u, held[u]);
-            for (int v = lane + 32 * U; v < vecs; v += 32) store(v, load(v));
+                for (int u = 0; u < U; ++u) {
+                    const int i = ((part + u * parts) * 32 + lane) * W;
+                    if (i < dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + place(i)) = q.template quantised<T>(held[u]);
+                }
+            } else
+                for (int i = part * 32 + lane; i < dim; i += 32 * parts) to[place(i)] = q.quantised(to_float(row[i]));
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(x_full);
         bar_named(1, 256);                   // the scales
-        constexpr int HALF = BN / 2;
-        const int quarter = warp & 3, half = w >> 2;
+    }
+    // A warp reads the tensor-memory lanes 32 * (warp % 4) on; warps 2 to 5 have the first half of the columns, 6 to 9 the second
+    const int quarter = warp & 3, half = w >> 2;
+    const uint32_t sums = tmem + ((uint32_t)(32 * quarter) << 16) + half * HALF;
+    if (warp >= 2) {
         unsigned n = 0;
-        bool ok = true;
-        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+        for (unsigned tile = t0; tile < tiles; tile += step, ++n) {
             const int c = (int)tile * BM + 32 * quarter + lane;
             const bool real = c < a.channels;
             const float ws = real ? a.w_scales[c] : 0.0f, bias = real && a.bias ? a.bias[c] : 0.0f;
             ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded<false>(acc_full((int)(n & 1u)), (n >> 1) & 1u, &fail, WAIT_CYCLES));
             if (!ok && lane == 0) fail = 1;
             tc_fence_after();
-            store_columns<HALF>(tmem + ((uint32_t)(32 * quarter) << 16) + (n & 1u) * BN + half * HALF, scales + half * HALF, ws, bias, real, ok, out, a.ld_out, half * HALF, a.rows, c);
+            store_columns<HALF>(sums + (n & 1u) * BN, scales + half * HALF, ws, bias, real, ok, out, a.ld_out, half * HALF, a.rows, c);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty((int)(n & 1u)));
@@ -521,7 +557,7 @@ template <bool RESIDENT> struct PairTiles {
     }
 };
 template <bool RESIDENT, typename O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, O *out, const ProductArgs a) {
     using namespace ptx;
     typedef PairShape<RESIDENT> S;
@@ -663,17 +699,11 @@ int pair_count(const void *kernel, int bytes, int *out) {
     return B2_OK;
 }
 
-template <int BN, typename O> int launch_product(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
-    typedef Shape<BN> S;
-    const auto kernel = int8_product_kernel<BN, O>;
-    B2_TRY(set_max_dynamic_smem((const void *)kernel, S::SMEM));
-    const long long tiles = (long long)a.row_tiles * a.channel_tiles;
-    const unsigned blocks = (unsigned)(tiles < sm_count() ? tiles : sm_count());
-    if (a.chained) return launch_chained(int8_product_kernel<BN, O>, dim3(blocks), dim3(THREADS), S::SMEM, st, mw, mx, out, a);
-    kernel<<<blocks, THREADS, S::SMEM, st>>>(mw, mx, out, a);
-    count_launch();
-    B2_CUDA(cudaGetLastError());
-    return B2_OK;
+template <int BN, int STAGES, typename O> int launch_product(const CUtensorMap &mw, const CUtensorMap &mx, O *out, const ProductArgs &a, unsigned blocks, cudaStream_t st) {
+    const auto kernel = int8_product_kernel<BN, STAGES, O>;
+    constexpr int BYTES = Shape<BN, STAGES>::SMEM;
+    B2_TRY(set_max_dynamic_smem((const void *)kernel, BYTES));
+    return launch_chained(int8_product_kernel<BN, STAGES, O>, Clusters{a.splits, a.chained}, dim3(blocks), dim3(THREADS), BYTES, st, mw, mx, out, a);
 }
 template <bool RESIDENT, typename O> int launch_pairs(const CUtensorMap &mw, const CUtensorMap &mx, O *out, ProductArgs a, cudaStream_t st) {
     const auto kernel = int8_pair_kernel<RESIDENT, O>;
@@ -683,11 +713,7 @@ template <bool RESIDENT, typename O> int launch_pairs(const CUtensorMap &mw, con
     B2_TRY(pair_count((const void *)kernel, BYTES, &pairs));
     const long long tiles = (long long)a.row_tiles * a.channel_tiles;
     const unsigned blocks = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-    if (a.chained) return launch_chained(int8_pair_kernel<RESIDENT, O>, dim3(blocks), dim3(THREADS), BYTES, st, mw, mx, out, a);
-    kernel<<<blocks, THREADS, BYTES, st>>>(mw, mx, out, a);
-    count_launch();
-    B2_CUDA(cudaGetLastError());
-    return B2_OK;
+    return launch_chained(int8_pair_kernel<RESIDENT, O>, Clusters{2, a.chained}, dim3(blocks), dim3(THREADS), BYTES, st, mw, mx, out, a);
 }
 
 size_t pitch_of(int dim) { return ((size_t)dim + 15) & ~(size_t)15; }
@@ -704,7 +730,16 @@ template <typename O> int product(O *out, const signed char *x, long long ld_x, 
         a.channel_tiles = (unsigned)((a.channels + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM));
         if ((double)a.row_tiles * a.channel_tiles > 4e9) { set_error("b2_int8_product: %lld rows of %d channels", a.rows, a.channels); return B2_ERR_BAD_SHAPE; }
         if constexpr (PAIR) return a.slabs <= MOST_RESIDENT ? launch_pairs<true, O>(mw, mx, out, a, st) : launch_pairs<false, O>(mw, mx, out, a, st);
-        else return launch_product<BN, O>(mw, mx, out, a, st);
+        else {
+            // Where the tiles leave blocks idle, clusters share a tile, each block with 2 slabs at least: two blocks an SM then, with half the ring (8 x 4096 x 4096: 17.3 us
+            // without)
+            constexpr int RING = BN >= 128 ? 6 : 8, RESIDENT = BN < 128 ? 2 : 1;
+            const long long tiles = (long long)a.row_tiles * a.channel_tiles;
+            a.splits = 1;
+            while ((int)a.splits < most_splits<BN>() && tiles * a.splits * 2 <= RESIDENT * sm_count() && a.slabs / (int)(a.splits * 2) >= 2) a.splits *= 2;
+            if (a.splits > 1) return launch_product<BN, 4, O>(mw, mx, out, a, (unsigned)tiles * a.splits, st);
+            return launch_product<BN, RING, O>(mw, mx, out, a, (unsigned)(tiles < sm_count() ? tiles : sm_count()), st);
+        }
     };
     if (a.rows <= 16) return go(std::integral_constant<int, 16>());
     if (a.rows <= 32) return go(std::integral_constant<int, 32>());
@@ -712,23 +747,22 @@ template <typename O> int product(O *out, const signed char *x, long long ld_x, 
     if (a.rows <= 128) return go(std::integral_constant<int, 128>());
     return go(std::integral_constant<int, PAIR_BN>());
 }
-// whether the call runs as one launch that quantises in every block
-bool few_rows(long long rows, int dim) { return rows <= 32 && (rows <= 16 ? 16 : 32) * (((long long)dim + BK - 1) / BK * BK) <= ROWS_X_BYTES; }
+// Whether the call runs as one launch that quantises in every block: up to 8 rows that fit into the registers of 8 warps, and more tiles than a split would fill
+bool few_rows(long long rows, int channels, int dim) {
+    const int parts = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;
+    return rows <= 8 && dim <= 1024 * parts && (dim + BK - 1) / BK * (ROWS_BN * BK) <= 80 * 1024 && ((channels + BM - 1ll) / BM * 2 > sm_count() || dim <= 2 * BK);
+}
 template <typename T, typename O> int product_of_few(O *out, const T *x, long long ld_x, const signed char *w, long long ld_w, int dim, ProductArgs a, cudaStream_t st) {
     CUtensorMap mw;
     B2_TRY(make_byte_map(&mw, w, dim, a.channels, ld_w, BM));
     a.row_tiles = 1;
-    a.channel_tiles = (unsigned)((a.channels + BM - 1) / BM);
-    const unsigned blocks = (unsigned)((long long)a.channel_tiles < sm_count() ? (int)a.channel_tiles : sm_count());
-    const auto go = [&](auto kernel, int bytes) -> int {
-        B2_TRY(set_max_dynamic_smem((const void *)kernel, ROWS_STAGES * A_BYTES + ROWS_X_BYTES + 1024));
-        kernel<<<blocks, THREADS, bytes, st>>>(mw, x, ld_x, dim, out, a);
-        count_launch();
-        B2_CUDA(cudaGetLastError());
-        return B2_OK;
-    };
-    if (a.rows <= 16) return go(int8_rows_kernel<16, T, O>, rows_smem<16>(a.slabs));
-    return go(int8_rows_kernel<32, T, O>, rows_smem<32>(a.slabs));
+    a.channel_tiles = (unsigned)(((long long)a.channels + BM - 1) / BM);
+    const auto kernel = int8_rows_kernel<T, O>;
+    B2_TRY(set_max_dynamic_smem((const void *)kernel, rows_smem(80 * 1024 / (ROWS_BN * BK))));
+    kernel<<<(long long)a.channel_tiles < sm_count() ? a.channel_tiles : (unsigned)sm_count(), THREADS, rows_smem(a.slabs), st>>>(mw, x, ld_x, dim, out, a);
+    count_launch();
+    B2_CUDA(cudaGetLastError());
+    return B2_OK;
 }
 
 }  // namespace
@@ -786,7 +820,7 @@ int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, in
         const size_t need = b2_int8_product_workspace(rows, channels, dim);
         if (!workspace || !aligned_to(workspace, 16)) { set_error("b2_int8_product: the workspace is missing or not aligned to 16 bytes"); return B2_ERR_BAD_ARG; }
         if (workspace_bytes < need) { set_error("b2_int8_product: a workspace of %zu bytes, %zu are needed", workspace_bytes, need); return B2_ERR_BAD_SHAPE; }
-        if (few_rows(rows, dim))
+        if (few_rows(rows, channels, dim))
             return with_type(x_type, [&](auto *t) {
                 const B2_ELEM(t) *in = (const B2_ELEM(t) *)x;
                 return with_type(out_type, [&](auto *o) { return product_of_few((B2_ELEM(o) *)out, in, ld_x, w, ld_w, dim, a, st); });

@@ -50,21 +50,36 @@ template <typename F> int with_type(int type, F &&f) {
 // A launch that may start while the kernel before it on the stream drains; the kernel calls grid_wait() before it touches
 // what that one wrote (and before it writes what that one reads).  Behind the wait it reads by plain loads: __ldg and loads through
 // `const ... *__restrict__` are for memory that nobody writes while the kernel runs, and may be moved above it.
+// In clusters of so many blocks; chained 0: it starts when the kernel before it is done.
+struct Clusters { unsigned blocks; int chained; };
 template <typename... KArgs, typename... Args>
-int launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+int launch_chained(void (*kernel)(KArgs...), Clusters how, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute at[2];
+    unsigned n = 0;
+    if (how.chained) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (how.blocks > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = how.blocks;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = n;
     count_launch();
     B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
     return B2_OK;
+}
+template <typename... KArgs, typename... Args>
+int launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+    return launch_chained(kernel, Clusters{1, 1}, grid, block, smem, st, std::forward<Args>(args)...);
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -114,7 +114,8 @@ def test_product_of_integers(tm, rows, channels, dim, o):  # noqa: F811
         assert torch.equal(plain, total.float())                              # exact sums, rounded once
 
 
-@pytest.mark.parametrize("rows,channels,dim", [(1, 3, 1), (4, 50, 259), (8, 3000, 1024), (20, 129, 77), (100, 300, 2000), (300, 500, 640), (2, 70, 9000), (1000, 129, 4100)])
+@pytest.mark.parametrize("rows,channels,dim", [(1, 3, 1), (4, 50, 259), (8, 3000, 1024), (20, 129, 77), (100, 300, 2000), (300, 500, 640), (2, 70, 9000), (1000, 129, 4100),
+                                                (16, 5000, 2048), (9, 700, 1500), (32, 4000, 4096), (25, 1, 5000), (17, 12900, 2500), (16, 20000, 5000), (12, 37900, 600), (1, 1, 16000)])
 @pytest.mark.parametrize("t,o", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f16")])
 def test_product_of_activations(tm, rows, channels, dim, t, o):  # noqa: F811
     torch, b2 = tm

@@ -63,8 +63,8 @@ struct RowScale {
     }
 };
 
-// TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice
-template <typename T, int TEAM, int U, bool KEPT>
+// TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice.  WHOLE: rows of whole vectors that start on their boundaries, the integers' too
+template <typename T, int TEAM, int U, bool KEPT, bool WHOLE>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long long ld_q, float *scales, const T *x0, long long rows, int dim, long long ld_x) {
     constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
     __shared__ float most[8];
@@ -74,11 +74,11 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     if (r >= rows) return;
     const T *x = x0 + r * ld_x;
     unsigned char *to = reinterpret_cast<unsigned char *>(q) + r * ld_q;
-    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T)), vecs = (mis + dim + W - 1) / W;
-    const bool out_vec = (((uintptr_t)(to - mis)) & (W - 1)) == 0;
+    const int mis = WHOLE ? 0 : (int)(((uintptr_t)x & 15) / sizeof(T)), vecs = WHOLE ? dim / W : (mis + dim + W - 1) / W;
+    const bool out_vec = WHOLE || (((uintptr_t)(to - mis)) & (W - 1)) == 0;
     const auto load = [&](int v) -> uint4 {
         const int i0 = v * W - mis;
-        if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(x + i0);
+        if (WHOLE || (i0 >= 0 && i0 + W <= dim)) return *reinterpret_cast<const uint4 *>(x + i0);
         T e[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? x[i0 + j] : from_float<T>(0.0f);
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
 #pragma unroll
         for (int u = 0; u < U; ++u) m = larger_magnitude(m, largest_magnitude<T>(held[u]));
     } else
+#pragma unroll 4
         for (int v = at; v < vecs; v += TEAM) m = larger_magnitude(m, largest_magnitude<T>(load(v)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     const auto store = [&](int v, const uint4 &h) {
         const int i0 = v * W - mis;
         const Vec<unsigned char, W> o = s.template quantised<T>(h);
-        if (out_vec && i0 >= 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
+        if (WHOLE || (out_vec && i0 >= 0 && i0 + W <= dim)) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
         else
 #pragma unroll
             for (int j = 0; j < W; ++j)
@@ -123,9 +124,9 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
         for (int v = at; v < vecs; v += TEAM) store(v, load(v));
 }
 
-template <typename T> int quantize(signed char *q, long long ld_q, float *scales, const T *x, long long rows, int dim, long long ld_x, cudaStream_t st) {
+template <typename T, bool WHOLE> int quantize_rows(signed char *q, long long ld_q, float *scales, const T *x, long long rows, int dim, long long ld_x, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
-    const int vecs = (dim + W - 1) / W + 1;                  // one more: a row may start inside a vector
+    const int vecs = WHOLE ? dim / W : (dim + W - 1) / W + 1;      // one more: a row may start inside a vector
     const auto go = [&](auto kernel, int teams) -> int {
         const long long blocks = (rows + teams - 1) / teams;
         if (blocks > 0x7fffffffll) { set_error("b2_int8_quantize: %lld rows", rows); return B2_ERR_BAD_SHAPE; }
@@ -134,11 +135,17 @@ template <typename T> int quantize(signed char *q, long long ld_q, float *scales
         B2_CUDA(cudaGetLastError());
         return B2_OK;
     };
-    if (vecs <= 32 * 5) return go(int8_quantize_kernel<T, 32, 5, true>, 8);
-    if (vecs <= 32 * 9) return go(int8_quantize_kernel<T, 32, 9, true>, 8);
-    if (vecs <= 256 * 4) return go(int8_quantize_kernel<T, 256, 4, true>, 1);
-    if (vecs <= 256 * 9) return go(int8_quantize_kernel<T, 256, 9, true>, 1);
-    return go(int8_quantize_kernel<T, 256, 1, false>, 1);
+    if (vecs <= 32 * 4) return go(int8_quantize_kernel<T, 32, 4, true, WHOLE>, 8);
+    if (vecs <= 32 * 8) return go(int8_quantize_kernel<T, 32, 8, true, WHOLE>, 8);
+    if (vecs <= 256 * 4) return go(int8_quantize_kernel<T, 256, 4, true, WHOLE>, 1);
+    if (vecs <= 256 * 8) return go(int8_quantize_kernel<T, 256, 8, true, WHOLE>, 1);
+    return go(int8_quantize_kernel<T, 256, 4, false, WHOLE>, 1);
+}
+template <typename T> int quantize(signed char *q, long long ld_q, float *scales, const T *x, long long rows, int dim, long long ld_x, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    if (aligned_to(x, 16) && (rows == 1 || ld_x % W == 0) && dim % W == 0 && aligned_to(q, W) && (rows == 1 || ld_q % W == 0))
+        return quantize_rows<T, true>(q, ld_q, scales, x, rows, dim, ld_x, st);
+    return quantize_rows<T, false>(q, ld_q, scales, x, rows, dim, ld_x, st);
 }
 
 // ---- product --------------------------------------------------------------------------------------------------------------------------

@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, CAP = 512;
     __shared__ float bounds[WARPS];
     __shared__ Part parts[WARPS];
+    __shared__ uint4 ring[2][U][THREADS];
     __shared__ __align__(16) T hits[CAP][W];            // vectors that hold an entry of interest
     __shared__ int hit_at[CAP];                           // where they are in the row
     __shared__ Key found[THREADS], winner[WARPS];
@@ -116,51 +117,55 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
     if (!runs(a, row)) return;
     if (t == 0) n_hits = count = 0;
-    uint4 q[U];
-    Flags<T> on[MASK ? U : 1];
-    const auto load = [&](int from) {
-        // all of the chunk inside the row, its mask in vectors: what most chunks are
-        if (from * W >= mis && (from + THREADS * U) * W - mis <= a.vocab && from + THREADS * U <= v1 && (!MASK || mask_vec)) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(x - mis) + from + t;
-#pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = src[u * THREADS];
-            if (MASK)
-#pragma unroll
-                for (int u = 0; u < U; ++u) on[u] = load_flags<T>(mk - mis + (from + t + u * THREADS) * W);
-            return;
-        }
+    // A thread copies the vectors of its next chunk into shared memory while it works on one, for itself alone; their mask's bytes wait in registers
+    Flags<T> on[MASK ? U : 1], on_next[MASK ? U : 1];
+    const auto whole = [&](int v) { return v < v1 && v * W >= mis && (v + 1) * W - mis <= a.vocab; };
+    const auto ahead = [&](int from, int to) {
+        const unsigned at = (unsigned)__cvta_generic_to_shared(&ring[to][0][t]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = from + t + u * THREADS, i0 = v * W - mis;
-            const bool inside = v < v1, whole = inside && i0 >= 0 && i0 + W <= a.vocab;
-            q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
-            if (whole) q[u] = *reinterpret_cast<const uint4 *>(x + i0);
-            else if (inside) {
-                T e[W];
-#pragma unroll
-                for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < a.vocab ? x[i0 + j] : from_float<T>(neg_inf());
-                memcpy(&q[u], e, 16);
-            }
-            if (MASK) {
-                if (whole && mask_vec) on[u] = load_flags<T>(mk + i0);
-                else {
-#pragma unroll
-                    for (int i = 0; i < W / 4; ++i) on[u].w[i] = 0;
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        if (inside && i0 + j >= 0 && i0 + j < a.vocab) on[u].w[j / 4] |= (unsigned)mk[i0 + j] << (8 * (j % 4));
-                }
-            }
+            const int v = from + t + u * THREADS;
+            if (!whole(v)) continue;
+            cp_async<16>(at + u * (THREADS * 16), x - mis + v * W);
+            if (MASK && mask_vec) on_next[u] = load_flags<T>(mk - mis + v * W);
         }
+        cp_commit();
     };
     Part sum = {neg_inf(), 0.0f};
     float best = neg_inf(), limit = neg_inf();             // the thread's largest; what an entry has to reach
     int renew = 0, chunk = 0;
-    load(v0);
+    ahead(v0, 0);
     for (int from = v0; from < v1; from += THREADS * U, ++chunk) {
         if (MASK)
 #pragma unroll
-            for (int u = 0; u < U; ++u) rule_out<T>(q[u], on[u]);
+            for (int u = 0; u < U; ++u) on[u] = on_next[u];
+        ahead(from + THREADS * U, (chunk + 1) & 1);
+        cp_wait<1>();
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = from + t + u * THREADS;
+            if (whole(v)) {
+                q[u] = ring[chunk & 1][u][t];
+                if (MASK && mask_vec) rule_out<T>(q[u], on[u]);
+            } else q[u] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+        }
+        // the ends of the row, and masks whose bytes lie across the vectors: entry by entry, through this thread's place in the ring
+        if ((MASK && !mask_vec) || from * W < mis || (from + THREADS * U) * W - mis > a.vocab) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int v = from + t + u * THREADS, i0 = v * W - mis;
+                if (v >= v1 || (whole(v) && !(MASK && !mask_vec))) continue;
+                T *const mine = reinterpret_cast<T *>(&ring[chunk & 1][u][t]);
+#pragma unroll 1
+                for (int j = 0; j < W; ++j) {
+                    const int i = i0 + j;
+                    if (i < 0 || i >= a.vocab || (MASK && !mk[i])) mine[j] = from_float<T>(neg_inf());
+                    else if (!whole(v)) mine[j] = x[i];
+                }
+                q[u] = ring[chunk & 1][u][t];
+            }
+        }
         unsigned big[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) big[u] = larger_of<T>(q[u]);
@@ -207,7 +212,6 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
             const float2 h = halves(p);
             sum.s += h.x + h.y;
         }
-        if (from + THREADS * U < v1) load(from + THREADS * U);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum = join(sum, {__shfl_xor_sync(FULL, sum.m, o), __shfl_xor_sync(FULL, sum.s, o)});

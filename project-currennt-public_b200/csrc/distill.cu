@@ -374,25 +374,21 @@ template <typename T> struct Place {
         if (whole(v)) q = *reinterpret_cast<const uint4 *>(x - mis + (size_t)v * W);
     }
 };
-// the gradient off the list of vector v, whose logits are q if it is whole
-template <typename T, bool ADD> __device__ __forceinline__ void entry_grads(const Place<T> &p, const uint4 &q, int v, const RowGrad &g, float scale) {
+// the gradients off the list of the entries of vector v, whose logits are q; nothing if it is not whole
+template <typename T, bool ADD> __device__ __forceinline__ void vector_grads(const Place<T> &p, const uint4 &q, int v, const RowGrad &g, float scale) {
     constexpr int W = 16 / sizeof(T);
-    const int i0 = v * W - p.mis;
-    if (i0 >= p.vocab) return;
-    const bool inside = p.whole(v);
+    if (!p.whole(v)) return;
+    T *const d = p.d + v * W - p.mis;
     float z[W], o[W], old[W];
-    if (inside) Raw<T>::values(z, q);
-    else
-#pragma unroll
-        for (int j = 0; j < W; ++j) z[j] = i0 + j >= 0 && i0 + j < p.vocab ? to_float(p.x[i0 + j]) : 0.0f;
     if (ADD) {
-        if (inside && p.out_vec) load_vec<T, W>(old, p.d + i0);
+        if (p.out_vec) load_vec<T, W>(old, d);
         else
 #pragma unroll
-            for (int j = 0; j < W; ++j) old[j] = i0 + j >= 0 && i0 + j < p.vocab ? to_float(p.d[i0 + j]) : 0.0f;
+            for (int j = 0; j < W; ++j) old[j] = to_float(d[j]);
     }
     if (g.what == 1) {
         const Pair factor = pair(g.factor, g.factor);
+        Raw<T>::values(z, q);
         less_of(scale, g.base, [&](const auto &less) {
 #pragma unroll
             for (int j = 0; j < W; j += 2) {
@@ -406,11 +402,21 @@ template <typename T, bool ADD> __device__ __forceinline__ void entry_grads(cons
 #pragma unroll
         for (int j = 0; j < W; ++j) o[j] = none;
     }
-    if (inside && p.out_vec) store_vec<T, W>(p.d + i0, o);
+    if (p.out_vec) store_vec<T, W>(d, o);
     else
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (i0 + j >= 0 && i0 + j < p.vocab) p.d[i0 + j] = from_float<T>(o[j]);
+        for (int j = 0; j < W; ++j) d[j] = from_float<T>(o[j]);
+}
+// The entries in front of the first whole vector and behind the last one, at most 2 W - 2: entry e of them
+template <typename T> __device__ __forceinline__ int edge_entry(const Place<T> &p, int e) {
+    constexpr int W = 16 / sizeof(T);
+    const int head = min(p.vocab, (W - p.mis) % W), body = (p.vocab - head) / W * W;
+    return e < head ? e : e + body;                    // not below vocab: there is none
+}
+template <typename T, bool ADD> __device__ __forceinline__ void edge_grad(const Place<T> &p, int i, T x, const RowGrad &g, float scale) {
+    if (i >= p.vocab) return;
+    const float o = g.what == 1 ? expf(__fmul_rn(to_float(x), scale) - g.base) * g.factor : g.what == 2 ? nanf("") : 0.0f;
+    p.d[i] = from_float<T>(ADD ? to_float(p.d[i]) + o : o);
 }
 
 // The list of a row: the row's factors, and the gradients of the listed tokens within [lo, hi)
@@ -466,12 +472,18 @@ __global__ void __launch_bounds__(256, 4) distill_backward_rows_kernel(T *dlogit
     uint4 q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) p.load(q[u], lane + TEAM * u);
+    constexpr int EDGES = (2 * 16 / sizeof(T) - 2 + TEAM - 1) / TEAM;
+    T edge[EDGES];
+#pragma unroll
+    for (int e = 0; e < EDGES; ++e) edge[e] = edge_entry(p, lane + TEAM * e) < a.vocab ? p.x[edge_entry(p, lane + TEAM * e)] : from_float<T>(0.0f);
     list.gather(p, 0, a.vocab);
     const RowGrad g = list.factors(a.vocab);
     __syncwarp();
     if (!real || (g.what == 0 && ADD)) return;
 #pragma unroll
-    for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], lane + TEAM * u, g, a.scale);
+    for (int u = 0; u < U; ++u) vector_grads<T, ADD>(p, q[u], lane + TEAM * u, g, a.scale);
+#pragma unroll
+    for (int e = 0; e < EDGES; ++e) edge_grad<T, ADD>(p, edge_entry(p, lane + TEAM * e), edge[e], g, a.scale);
     __syncwarp(List<SLOTS, TEAM>::lanes());
     if (g.what == 1) list.store(p.d, 0, a.vocab, a.scale);
 }
@@ -490,10 +502,13 @@ __global__ void __launch_bounds__(STREAM + 32, 3) distill_backward_kernel(T *dlo
         const int lo = max(0, seg * STREAM * U * W - p.mis), hi = min(a.vocab, (seg + 1) * STREAM * U * W - p.mis);
         RowList<T, SLOTS, 32, REST, ADD> list;
         list.load(a, r);
+        const int i = seg == 0 ? edge_entry(p, at - STREAM) : a.vocab;       // the row's ends are this warp's too
+        const T edge = i < a.vocab ? p.x[i] : from_float<T>(0.0f);
         list.gather(p, lo, hi);
         const RowGrad g = list.factors(a.vocab);
         if (at == STREAM) shared = g;
         __syncthreads();
+        if (g.what != 0 || !ADD) edge_grad<T, ADD>(p, i, edge, g, a.scale);
         __syncthreads();
         if (g.what == 1) list.store(p.d, lo, hi, a.scale);
         return;
@@ -505,7 +520,7 @@ __global__ void __launch_bounds__(STREAM + 32, 3) distill_backward_kernel(T *dlo
     const RowGrad g = shared;
     if (g.what != 0 || !ADD)
 #pragma unroll
-        for (int u = 0; u < U; ++u) entry_grads<T, ADD>(p, q[u], seg * STREAM * U + at + u * STREAM, g, a.scale);
+        for (int u = 0; u < U; ++u) vector_grads<T, ADD>(p, q[u], seg * STREAM * U + at + u * STREAM, g, a.scale);
     __syncthreads();
 }
 

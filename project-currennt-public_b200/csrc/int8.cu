@@ -78,13 +78,16 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     const bool out_vec = WHOLE || (((uintptr_t)(to - mis)) & (W - 1)) == 0;
     const auto load = [&](int v) -> uint4 {
         const int i0 = v * W - mis;
-        if (WHOLE || (i0 >= 0 && i0 + W <= dim)) return *reinterpret_cast<const uint4 *>(x + i0);
-        T e[W];
+        if constexpr (WHOLE) return *reinterpret_cast<const uint4 *>(x + i0);
+        else {
+            if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(x + i0);
+            T e[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? x[i0 + j] : from_float<T>(0.0f);
-        uint4 o;
-        memcpy(&o, e, 16);
-        return o;
+            for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? x[i0 + j] : from_float<T>(0.0f);
+            uint4 o;
+            memcpy(&o, e, 16);
+            return o;
+        }
     };
     uint4 held[KEPT ? U : 1];
     float m = 0.0f;
@@ -93,9 +96,10 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
         for (int u = 0; u < U; ++u) held[u] = at + u * TEAM < vecs ? load(at + u * TEAM) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < U; ++u) m = larger_magnitude(m, largest_magnitude<T>(held[u]));
-    } else
+    } else {
 #pragma unroll 4
         for (int v = at; v < vecs; v += TEAM) m = larger_magnitude(m, largest_magnitude<T>(load(v)));
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = larger_magnitude(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (TEAM == 256) {
@@ -110,11 +114,13 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     const auto store = [&](int v, const uint4 &h) {
         const int i0 = v * W - mis;
         const Vec<unsigned char, W> o = s.template quantised<T>(h);
-        if (WHOLE || (out_vec && i0 >= 0 && i0 + W <= dim)) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
-        else
+        if constexpr (WHOLE) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
+        else if (out_vec && i0 >= 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
+        else {
 #pragma unroll
             for (int j = 0; j < W; ++j)
                 if (i0 + j >= 0 && i0 + j < dim) to[i0 + j] = o.v[j];
+        }
     };
     if (KEPT) {
 #pragma unroll

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
         if (sum.m != neg_inf()) {
             const Pair l2 = pair(LOG2E, LOG2E);
             Pair p = 0;
-            less_of(a.scale, sum.m, [&](const auto &less) {
+            less_of_type<T>(a.scale, sum.m, [&](const auto &less) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     float z[W];

@@ -124,7 +124,7 @@ template <typename T, int U> __device__ __forceinline__ void add_vectors(Sum &a,
     if (a.m == neg_inf()) return;
     const Pair l2 = pair(LOG2E, LOG2E);
     Pair s = 0;
-    less_of(scale, a.m, [&](const auto &less) {
+    less_of_type<T>(scale, a.m, [&](const auto &less) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[W];
@@ -389,7 +389,7 @@ template <typename T, bool ADD> __device__ __forceinline__ void vector_grads(con
     if (g.what == 1) {
         const Pair factor = pair(g.factor, g.factor);
         Raw<T>::values(z, q);
-        less_of(scale, g.base, [&](const auto &less) {
+        less_of_type<T>(scale, g.base, [&](const auto &less) {
 #pragma unroll
             for (int j = 0; j < W; j += 2) {
                 const float2 t = halves(mul2(exp_pair<T>(less(z[j], z[j + 1])), factor));

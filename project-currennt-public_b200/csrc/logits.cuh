@@ -1,6 +1,8 @@
 // What the kernels over rows of logits share: the exponential, differences of scaled logits, 16-byte vectors as they were loaded, and entries
 // ordered by value and index.
 #pragma once
+#include <type_traits>
+
 #include "typed.cuh"
 
 namespace b2 {
@@ -30,6 +32,18 @@ struct Rounded {
     }
     __device__ __forceinline__ Pair operator()(float x, float y) const { return add2(fma2(pair(x, y), s, none), off); }
 };
+// the same by two products of their own
+struct Apart {
+    float s; Pair off;
+    __device__ __forceinline__ Pair operator()(float x, float y) const { return add2(pair(__fmul_rn(x, s), __fmul_rn(y, s)), off); }
+};
+// f(function of two logits of type T), the one that the scale asks for: the product of a logit of b bits and a scale of 24 - b bits needs no rounding
+template <typename T, typename F> __device__ __forceinline__ void less_of_type(float scale, float minus, F &&f) {
+    constexpr unsigned BITS = sizeof(T) == 4 ? 0x7fffffu : std::is_same<T, __half>::value ? 0x7ffu : 0xffu;
+    const Pair off = pair(-minus, -minus);
+    if ((__float_as_uint(scale) & BITS) == 0) f(Exact{pair(scale, scale), off});
+    else f(Apart{scale, off});
+}
 // f(function of two logits), the one that the scale asks for
 template <typename F> __device__ __forceinline__ void less_of(float scale, float minus, F &&f) {
     const Pair s = pair(scale, scale), off = pair(-minus, -minus);

@@ -80,31 +80,27 @@ __device__ __forceinline__ Part join(Part a, Part b) {
     rise(a, m);
     return {m, a.s + b.s};
 }
-// What the ceil(top / WARPS) best lanes of a warp hold at least: `top` entries reach the least of it over the warps
-template <int WARPS> __device__ __forceinline__ float reached(float best, int top) {
-    unsigned order = ordered(best), least = 0;
-    for (int i = 0; i < top; i += WARPS) {
-        least = __reduce_max_sync(FULL, order);
-        if ((int)(threadIdx.x & 31) == __ffs(__ballot_sync(FULL, order == least)) - 1) order = 0;
+// What the `rounds` best lanes of a warp hold at least: rounds * warps entries reach the least of it over the warps
+__device__ __forceinline__ unsigned reached(unsigned best, int rounds) {
+    unsigned least = 0;
+    for (int i = 0; i < rounds; ++i) {
+        least = __reduce_max_sync(FULL, best);
+        if ((int)(threadIdx.x & 31) == __ffs(__ballot_sync(FULL, best == least)) - 1) best = 0;
     }
-    return ordered_value(least);
+    return least;
 }
-template <int WARPS> __device__ __forceinline__ float least_of(const float *bounds) {
-    float limit = bounds[threadIdx.x & (WARPS - 1)];
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) limit = fminf(limit, __shfl_xor_sync(FULL, limit, o));
-    return limit;
-}
+// the least over the first `warps` of 8
+__device__ __forceinline__ unsigned least_of(const unsigned *bounds, int warps) { return __reduce_min_sync(FULL, bounds[min((int)(threadIdx.x & 31), warps - 1)]); }
 
 template <typename T, bool MASK>
 __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *logits, const SelectArgs a) {
     constexpr int THREADS = SLICE_THREADS, W = 16 / sizeof(T), U = SLICE_VECS, WARPS = THREADS / 32, CAP = 512;
-    __shared__ float bounds[WARPS];
+    __shared__ unsigned bounds[WARPS];
     __shared__ Part parts[WARPS];
     __shared__ uint4 ring[2][U][THREADS];
     __shared__ __align__(16) T hits[CAP][W];            // vectors that hold an entry of interest
     __shared__ int hit_at[CAP];                           // where they are in the row
-    __shared__ Key found[THREADS], winner[WARPS];
+    __shared__ Key found[CAP], winner[WARPS];
     __shared__ int n_hits, count;
     grid_release();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -115,7 +111,6 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     const unsigned char *mk = MASK ? a.mask + row * a.ld_mask : nullptr;
     const bool mask_vec = MASK && ((uintptr_t)(mk - mis) & (W - 1)) == 0;
     const int v0 = part * a.slice, v1 = min(v0 + a.slice, (mis + a.vocab + W - 1) / W);
-    if (!runs(a, row)) return;
     if (t == 0) n_hits = count = 0;
     // A thread copies the vectors of its next chunk into shared memory while it works on one, for itself alone; their mask's bytes wait in registers
     Flags<T> on[MASK ? U : 1], on_next[MASK ? U : 1];
@@ -133,8 +128,14 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     };
     Part sum = {neg_inf(), 0.0f};
     float best = neg_inf(), limit = neg_inf();             // the thread's largest; what an entry has to reach
+    // warps full of vectors, and the lanes of each that hold `top` entries together (more than 32: too few entries for a bound)
+    const int warps = min(WARPS, (v1 - v0) / 32), rounds = warps > 0 ? (a.top + warps - 1) / warps : 33;
     int renew = 0, chunk = 0;
     ahead(v0, 0);
+    if (!runs(a, row)) {                                   // asked while the logits are on the way
+        cp_wait<0>();
+        return;
+    }
     for (int from = v0; from < v1; from += THREADS * U, ++chunk) {
         if (MASK)
 #pragma unroll
@@ -176,11 +177,13 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
         best = max_nan(best, mine);
         if (chunk == renew) {
             // the bound from what was met so far, after 1, 2, 4, 8, ... chunks
-            const float mine_reached = reached<WARPS>(best, a.top);
-            if (chunk) __syncthreads();
-            if (lane == 0) bounds[warp] = mine_reached;
-            __syncthreads();
-            limit = least_of<WARPS>(bounds);
+            if (rounds <= 32) {
+                const unsigned mine_reached = reached(ordered(best), rounds);
+                if (chunk) __syncthreads();
+                if (lane == 0) bounds[warp] = mine_reached;
+                __syncthreads();
+                limit = ordered_value(least_of(bounds, warps));
+            }
             renew = 2 * renew + 1;
         }
         if (mine >= limit && mine > neg_inf())
@@ -215,12 +218,14 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum = join(sum, {__shfl_xor_sync(FULL, sum.m, o), __shfl_xor_sync(FULL, sum.s, o)});
-    const float all_reached = reached<WARPS>(best, a.top);         // the bound of the whole slice
+    const unsigned all_reached = chunk > 1 && rounds <= 32 ? reached(ordered(best), rounds) : 0;         // the bound of the whole slice
     if (lane == 0) parts[warp] = sum;
     __syncthreads();
-    if (lane == 0) bounds[warp] = all_reached;
-    __syncthreads();
-    limit = least_of<WARPS>(bounds);
+    if (chunk > 1 && rounds <= 32) {
+        if (lane == 0) bounds[warp] = all_reached;
+        __syncthreads();
+        limit = ordered_value(least_of(bounds, warps));
+    }
     Key *const list = a.lists + (row * a.slices + part) * a.top;
     const int h = n_hits;
     if (h <= CAP)
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
             const float z = __fmul_rn(to_float(hits[i / W][i % W]), a.scale);
             if (z >= limit && z > neg_inf()) {
                 const int at = atomicAdd(&count, 1);
-                if (at < THREADS) found[at] = make_key(z, hit_at[i / W] + i % W);
+                if (at < CAP) found[at] = make_key(z, hit_at[i / W] + i % W);
             }
         }
     if (warp == WARPS - 1) {
@@ -239,14 +244,15 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     }
     __syncthreads();
     const int n = count;
-    if (h <= CAP && n <= THREADS) {
-        if (t < n) {
-            const Key k = found[t];
+    if (h <= CAP && n <= CAP) {
+        for (int i = t; i < n; i += THREADS) {
+            const Key k = found[i];
             int before = 0;
 #pragma unroll 4
             for (int j = 0; j < n; ++j) before += found[j] > k;
             if (before < a.top) list[before] = k;
-        } else if (t < a.top) list[t] = 0;
+        }
+        for (int i = n + t; i < a.top; i += THREADS) list[i] = 0;
         return;
     }
     // many that reach the bound, as in a row of equal logits: the next best in turn
@@ -287,109 +293,146 @@ __device__ __forceinline__ int beam_of(unsigned long long tie) { return MAX_BEAM
 __device__ __forceinline__ float logit_of(unsigned long long tie) { return ordered_value((unsigned)(tie >> 26)); }
 __device__ __forceinline__ int token_of(unsigned long long tie) { return MOST_VOCAB - 1 - (int)(tie & (MOST_VOCAB - 1)); }
 
-// One block a sequence.  A slice's list is sorted, so the first few entries of every list, 2 K of them together, hold a bound that K continuations reach: the K-th best of
-// them.  All entries that reach it are counted into their places.
-constexpr int JOIN_THREADS = 256, AHEAD = 2, MOST_HEADS = 1024, MOST_FOUND = 1024;
+// One block a sequence.  A bound from the threads' best entries first, as above; where beams of different strength let too many pass, the one that the K best reach is found
+// digit by digit, from the counts of the ranks' digits in 32 bits (a rounding to fewer bits keeps the order, so that whatever reaches the bound in 64 bits
+// reaches it in 32).  The entries that reach it are counted into their places.
+constexpr int JOIN_THREADS = 256, DIGIT_BITS = 11, DIGITS = 1 << DIGIT_BITS, MOST_FOUND = 512, MOST_ENTRIES = 64 * MAX_BEST;
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArgs a) {
     __shared__ double off[MAX_BEAMS], weight[MAX_BEAMS];
     __shared__ bool ended[MAX_BEAMS];
-    __shared__ __align__(16) float heads[MOST_HEADS];
+    __shared__ int counts[DIGITS], warp_counts[JOIN_THREADS / 32];
+    __shared__ unsigned ranks[MOST_ENTRIES], bounds[JOIN_THREADS / 32];      // the entries' ranks as ordered integers, 0: none
     __shared__ Cand found[MOST_FOUND];
-    __shared__ float bound;
-    __shared__ int count;
+    __shared__ __align__(16) unsigned orders[MOST_FOUND];                        // the same entries' ranks as ordered integers
+    __shared__ int digit, left, reach, count;
     __shared__ Cand winner[JOIN_THREADS / 32];
+    constexpr int WARPS = JOIN_THREADS / 32, EACH = DIGITS / JOIN_THREADS;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const long long g = blockIdx.x;
     const int lists = a.beams * a.slices, entries = lists * a.top;
     const Key *const keys = a.lists + g * entries;
     grid_wait();
-    // a warp has the lists w, w + 8, ..., a lane their entries l and l + 32
-    constexpr int WARPS = JOIN_THREADS / 32;
-    const int deep = min(a.top, (2 * a.top + lists - 1) / lists), n_heads = lists * deep;
-    Key ahead[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ahead[i] = warp + i * WARPS < lists && lane < a.top ? keys[(warp + i * WARPS) * a.top + lane] : 0;
+    const Key first = t < entries ? keys[t] : 0;             // on the way while the sums are joined
     // score_b - lse_b of the beams; NaN: no continuations
-    for (int b = warp; b < a.beams; b += JOIN_THREADS / 32) {
+    for (int b = warp; b < a.beams; b += WARPS) {
         const long long row = g * a.beams + b;
         const float score = a.scores[row], w = a.weights ? a.weights[row] : 1.0f;
         const bool end = a.finished && a.finished[row];
-        Part p = {neg_inf(), 0.0f};
-        if (lane < a.slices) p = a.parts[row * a.slices + lane];
+        const Part mine = lane < a.slices ? a.parts[row * a.slices + lane] : Part{neg_inf(), 0.0f};      // (what stands there for a beam at its end is not used)
         const bool fit = score > neg_inf() && score < __int_as_float(0x7f800000) && w > 0.0f && w < __int_as_float(0x7f800000);
         double o = nan("");
         if (fit && end) o = (double)score;
         else if (fit) {
-            float m = p.m;
+            float m = mine.m;
             for (int i = lane + 32; i < a.slices; i += 32) m = max_nan(m, a.parts[row * a.slices + i].m);
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, x));
             // a slice's sum has the error of 32 bits already: the factors need no more
-            double s = p.m != neg_inf() ? (double)(p.s * expf(p.m - m)) : 0.0;
+            double s = mine.m != neg_inf() ? (double)(mine.s * expf(mine.m - m)) : 0.0;
             for (int i = lane + 32; i < a.slices; i += 32) {
-                const Part q = a.parts[row * a.slices + i];
-                if (q.m != neg_inf()) s += (double)(q.s * expf(q.m - m));
+                const Part p = a.parts[row * a.slices + i];
+                if (p.m != neg_inf()) s += (double)(p.s * expf(p.m - m));
             }
             s = warp_sum(s);
             o = m == neg_inf() ? nan("") : (double)score - (double)m - log(s);
         }
         if (lane == 0) { off[b] = o; weight[b] = (double)w; ended[b] = end; }
     }
-    if (t == 0) { count = 0; bound = neg_inf(); }
+    if (t == 0) { count = 0; left = a.top; }
     __syncthreads();
-    // entry j of list l
-    const auto cand = [&](int l, int j, Key k) -> Cand {
-        const int b = a.slices == 1 ? l : l / a.slices;
+    // entry i, the i % top th of a list
+    const unsigned per_top = a.top > 1 ? 0xffffffffu / (unsigned)a.top + 1 : 0;
+    const auto cand = [&](int i, Key k) -> Cand {
+        const int l = a.top > 1 ? (int)__umulhi((unsigned)i, per_top) : i, b = a.slices == 1 ? l : l / a.slices;
         const double o = off[b];
         if (o != o) return no_cand();
-        if (ended[b]) return j == 0 && l == b * a.slices ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
+        if (ended[b]) return i == b * a.slices * a.top ? Cand{weight[b] * o, tie_of(b, 0.0f, a.end_token)} : no_cand();
         if (!k) return no_cand();
         const float z = key_value(k);
         return {weight[b] * (o + (double)z), tie_of(b, z, key_index(k))};
     };
-    const bool few = n_heads <= MOST_HEADS;
-    if (few) {
-        Cand held[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int l = warp + i * WARPS;
-            held[i] = l < lists && lane < a.top ? cand(l, lane, ahead[i]) : no_cand();
-            if (l < lists && lane < deep) heads[l * deep + lane] = (float)held[i].rank;
-            if (l < lists && lane + 32 < deep) heads[l * deep + lane + 32] = (float)cand(l, lane + 32, keys[l * a.top + lane + 32]).rank;
-        }
-        for (int l = warp + AHEAD * WARPS; l < lists; l += WARPS)
-            for (int j = lane; j < deep; j += 32) heads[l * deep + j] = (float)cand(l, j, keys[l * a.top + j]).rank;
-        __syncthreads();
-        // A rounding to fewer bits keeps the order, so that the bound in 32 bits lets all through that reach the one in 64
-        for (int i = t; i < n_heads; i += JOIN_THREADS) {
-            const float mine = heads[i];
-            int before = 0, j = 0;
-            for (; j + 4 <= n_heads; j += 4) {
-                const float4 m = *reinterpret_cast<const float4 *>(&heads[j]);
-                before += (m.x > mine || (m.x == mine && j < i)) + (m.y > mine || (m.y == mine && j + 1 < i)) + (m.z > mine || (m.z == mine && j + 2 < i)) +
-                          (m.w > mine || (m.w == mine && j + 3 < i));
-            }
-            for (; j < n_heads; ++j) before += heads[j] > mine || (heads[j] == mine && j < i);
-            if (before == a.top - 1) bound = mine;
-        }
-        __syncthreads();
-        const float limit = bound;
-        const auto offer = [&](const Cand &c) {
-            if (c.tie != 0 && (float)c.rank >= limit) {
-                const int at = atomicAdd(&count, 1);
-                if (at < MOST_FOUND) found[at] = c;
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int l = warp + i * WARPS;
-            offer(held[i]);
-            if (l < lists && lane + 32 < a.top) offer(cand(l, lane + 32, keys[l * a.top + lane + 32]));
-        }
-        for (int l = warp + AHEAD * WARPS; l < lists; l += WARPS)
-            for (int j = lane; j < a.top; j += 32) offer(cand(l, j, keys[l * a.top + j]));
-        __syncthreads();
+    unsigned best = 0;
+#pragma unroll 1
+    for (int i = t; i < entries; i += JOIN_THREADS) {
+        const Cand c = cand(i, i == t ? first : keys[i]);
+        const unsigned k = c.tie ? ordered((float)c.rank) : 0;
+        ranks[i] = k;
+        best = max(best, k);
     }
+    const auto for_all = [&](auto &&f) {
+        for (int i = t; i < entries; i += JOIN_THREADS)
+            if (ranks[i]) f(i, ranks[i]);
+    };
+    const int full = min(entries, JOIN_THREADS) / 32, rounds = full > 0 ? (a.top + full - 1) / full : 33;
+    unsigned guess = 0;
+    if (rounds <= 32) {
+        const unsigned mine = reached(best, rounds);
+        if (lane == 0) bounds[warp] = mine;
+        __syncthreads();
+        guess = least_of(bounds, full);
+    }
+    int passed = 0;
+    for_all([&](int, unsigned k) { passed += k >= guess; });
+    passed = __reduce_add_sync(FULL, passed);
+    if (lane == 0) warp_counts[warp] = passed;
+    __syncthreads();
+    passed = __reduce_add_sync(FULL, lane < WARPS ? warp_counts[lane] : 0);
+    // counting 160 entries into their places takes as long as finding two digits
+    const bool enough = passed <= max(160, 2 * a.top + 32);
+    unsigned bound = enough ? guess : 0;                       // or the digits found so far, and zeros
+#pragma unroll 1
+    for (int shift = enough ? -1 : 32 - DIGIT_BITS; shift >= 0;) {
+        for (int i = t; i < DIGITS; i += JOIN_THREADS) counts[i] = 0;
+        if (t == 0) digit = -1;
+        __syncthreads();
+        const int above = shift + DIGIT_BITS;
+        for_all([&](int, unsigned k) {
+            if (above >= 32 || k >> above == bound >> above) atomicAdd(&counts[(k >> shift) & (DIGITS - 1)], 1);
+        });
+        __syncthreads();
+        // the digits in falling order, EACH a thread: the one with which `left` entries are reached
+        int mine[EACH], sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) sum += mine[i] = counts[DIGITS - 1 - (t * EACH + i)];
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(FULL, before, o);
+            if (lane >= o) before += x;
+        }
+        if (lane == 31) warp_counts[warp] = before;
+        __syncthreads();
+        before -= sum;
+        for (int w = 0; w < warp; ++w) before += warp_counts[w];
+        const int want = left;
+        if (before < want && want <= before + sum) {
+            int at = before;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                if (at < want && want <= at + mine[i]) {
+                    digit = DIGITS - 1 - (t * EACH + i);
+                    reach = a.top - want + at + mine[i];             // all that reach the bound with this digit
+                    left = want - at;
+                }
+                at += mine[i];
+            }
+        }
+        __syncthreads();
+        if (digit < 0) break;                                // fewer than `top` altogether: all of them
+        bound |= (unsigned)digit << shift;
+        if (shift == 0 || reach <= 2 * a.top) break;
+        shift = max(0, shift - DIGIT_BITS);
+    }
+    for_all([&](int i, unsigned k) {
+        if (k >= bound) {
+            const int at = atomicAdd(&count, 1);
+            if (at < MOST_FOUND) {
+                found[at] = cand(i, keys[i]);
+                orders[at] = k;
+            }
+        }
+    });
+    __syncthreads();
     const auto write = [&](int place, const Cand &c) {
         const long long i = g * a.top + place;
         const bool none = c.tie == 0;
@@ -399,25 +442,32 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         a.tokens[i] = none ? -1 : token_of(c.tie);
     };
     const int n = count;
-    if (few && n <= MOST_FOUND) {
+    if (n <= MOST_FOUND) {
+        // in 32 bits, and in 64 where those are equal
+        if (t < -n % 4 + 4 && n + t < MOST_FOUND) orders[n + t] = 0;
+        __syncthreads();
         for (int i = t; i < n; i += JOIN_THREADS) {
-            const Cand c = found[i];
+            const unsigned mine = orders[i];
             int before = 0;
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) before += better(found[j], c);
-            if (before < a.top) write(before, c);
+            for (int j = 0; j < n; j += 4) {
+                const uint4 k = *reinterpret_cast<const uint4 *>(&orders[j]);
+                before += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+                if (k.x == mine || k.y == mine || k.z == mine || k.w == mine)
+                    for (int e = j; e < min(n, j + 4); ++e) before += orders[e] == mine && better(found[e], found[i]);
+            }
+            if (before < a.top) write(before, found[i]);
         }
         for (int i = n + t; i < a.top; i += JOIN_THREADS) write(i, no_cand());
         return;
     }
-    // very many slices, or many equal ranks: the next best in turn
+    // many equal ranks: the next best in turn
     Cand last = {INFINITY, ~0ull};
     for (int place = 0; place < a.top; ++place) {
         Cand top = no_cand();
-        for (int i = t; i < entries; i += JOIN_THREADS) {
-            const Cand c = cand(i / a.top, i % a.top, keys[i]);
-            if (c.tie != 0 && better(last, c) && better(c, top)) top = c;
-        }
+        for_all([&](int i, unsigned) {
+            const Cand c = cand(i, keys[i]);
+            if (better(last, c) && better(c, top)) top = c;
+        });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const Cand other = {__shfl_xor_sync(FULL, top.rank, o), __shfl_xor_sync(FULL, top.tie, o)};
@@ -425,19 +475,21 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         }
         if (lane == 0) winner[warp] = top;
         __syncthreads();
-        for (int w = 0; w < JOIN_THREADS / 32; ++w)
+        for (int w = 0; w < WARPS; ++w)
             if (better(winner[w], top)) top = winner[w];
         if (t == 0) write(place, top);
-        if (top.tie != 0) last = top; else last = no_cand();
+        last = top.tie != 0 ? top : no_cand();
         __syncthreads();
     }
 }
 
 int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return (vocab + w - 1) / w + 1; }   // one more: a row may start inside a vector
 // Slices of a row, of whole chunks of 1024 vectors: one where the rows fill the device (bounds and lists cost a slice several chunks' time), more where they do not
-int slices_of(long long rows, int vocab, int type) {
+// (and 64 lists for a sequence at most, which the second kernel goes through)
+int slices_of(long long rows, int beams, int vocab, int type) {
     const int chunks = (vectors_of(vocab, type) + CHUNK - 1) / CHUNK;
-    const long long most = rows && rows < 592 ? 592 / rows : 1;          // blocks that run at a time: 4 an SM
+    long long most = rows && rows < 592 ? 592 / rows : 1;          // blocks that run at a time: 4 an SM
+    if (most > 64 / beams) most = 64 / beams;
     const int each = (int)((chunks + most - 1) / most);
     return (chunks + each - 1) / each;
 }
@@ -543,7 +595,7 @@ extern "C" {
 
 size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top) {
     if (!sizes_fit(groups, beams, vocab, top)) return 0;
-    const size_t slices = (size_t)slices_of(groups * beams, vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
+    const size_t slices = (size_t)slices_of(groups * beams, beams, vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
     return slices * (sizeof(Part) + (size_t)top * sizeof(Key));
 }
 
@@ -575,7 +627,7 @@ int b2_beam_select(const void *logits, int type, long long groups, int beams, in
     SelectArgs a = {};
     a.mask = mask; a.ld_mask = ld_mask; a.scores = scores; a.finished = finished; a.weights = weights;
     a.groups = groups; a.ld = ld; a.beams = beams; a.vocab = vocab; a.top = top; a.end_token = end_token; a.scale = scale;
-    a.slices = slices_of(groups * beams, vocab, type);
+    a.slices = slices_of(groups * beams, beams, vocab, type);
     a.lists = (Key *)workspace;
     a.parts = (Part *)(a.lists + (size_t)a.slices * (size_t)groups * beams * top);
     a.best = top_scores; a.from = top_beams; a.tokens = top_tokens;

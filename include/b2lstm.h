@@ -263,7 +263,8 @@ int b2_distill_forward(const void *logits, int type, long long rows, int vocab, 
                        const float *top_logprobs, int top, float *loss, float *lse, float *lse_rest, b2_stream stream);
 /* The gradient of sum(dloss * loss) with respect to the logits, in their type; lse and lse_rest as the forward pass left them:
  *   dlogits = dloss * scale * (p - q),  and off the list, with lse_rest:  dloss * scale * (p - q_rest * exp(z - lse_rest))
- * Rows without a listed token get zeros, those with one that is not below vocab NaN.  With accumulate non-zero it is added to dlogits (rows of zeros leave it
+ * (where lse_rest is -inf: dloss * scale * p).  Rows without a listed token and rows with nothing above -inf get zeros, those with a token that is not below vocab or a log
+ * probability that is NaN or +inf NaN.  With accumulate non-zero it is added to dlogits (rows of zeros leave it
  * as it is); else dlogits may take the place of the logits. */
 int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits, int type, long long rows, int vocab, long long ld, float scale,
                         const int *top_tokens, const float *top_logprobs, int top, const float *lse, const float *lse_rest, const float *dloss,
@@ -275,7 +276,7 @@ int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits,
  *   score = scores[b] + z[v] - log sum exp z
  * and they are ranked by weights[b] * score, in 64 bits, equal ones by beam, logit (larger first) and token.  weights (NULL: 1) are a length penalty's factors,
  * above 0.  A beam with finished[b] (NULL: none) non-zero is at its end: it has one continuation, end_token with the score it has; its logits are not
- * looked at.  No continuations: beams whose score is -inf or NaN or whose weight is no positive finite number, rows with NaN or +inf among the allowed logits,
+ * looked at.  No continuations: beams whose score is no finite number or whose weight no positive finite one, rows with NaN or +inf among the allowed logits,
  * tokens that are not allowed or have z = -inf.  top_scores, top_beams (below beams) and top_tokens are [groups][top], best first; -inf, -1 and -1 where
  * there are fewer.  workspace: aligned to 16 bytes; its size is 0 for sizes that the call refuses. */
 size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top);
@@ -303,7 +304,7 @@ int b2_int8_quantize(signed char *q, long long ld_q, float *scales, const void *
  * w is [channels][dim], bias (channels floats) may be NULL.  The sums are exact (dim at most 131071); each is rounded to fp32, then the product, the sum with
  * the bias and the conversion to out_type are.  x_type B2_F32, B2_BF16 or B2_F16: x is quantised in the call as b2_int8_quantize does (x_scales is NULL,
  * workspace aligned to 16 bytes); B2_I8: x and x_scales are given and no workspace is needed.  8-bit integers start at a multiple of 16 bytes, and so does each
- * of their rows (ld_w, and ld_x with B2_I8). */
+ * of their rows (ld_w, and ld_x with B2_I8).  A tile that the tensor cores' kernel gave up waiting for comes out as NaN. */
 enum { B2_I8 = 3 };
 size_t b2_int8_product_workspace(long long rows, int channels, int dim);
 int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, int x_type, long long ld_x, const float *x_scales, const signed char *w,

@@ -109,9 +109,9 @@ __device__ __forceinline__ Sum join(Sum a, Sum b) {
     rise(a, m);
     return {m, a.s + b.s};
 }
-__device__ __forceinline__ Sum warp_join(Sum a) {
+template <int TEAM> __device__ __forceinline__ Sum team_join(Sum a) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = join(a, {__shfl_xor_sync(FULL, a.m, o), __shfl_xor_sync(FULL, a.s, o)});
+    for (int o = TEAM / 2; o > 0; o >>= 1) a = join(a, {__shfl_xor_sync(FULL, a.m, o), __shfl_xor_sync(FULL, a.s, o)});
     return a;
 }
 template <typename T, int U> __device__ __forceinline__ void add_vectors(Sum &a, const uint4 (&q)[U], float scale) {
@@ -147,6 +147,95 @@ struct FwdArgs {
     int vocab, top;
     float scale;
 };
+// A row's results from its list, the listed tokens' z (-inf where a place is empty) and the sum t over the other tokens (without a rest: over all)
+template <int SLOTS, int TEAM, bool REST>
+__device__ __forceinline__ void finish_row(const FwdArgs &a, long long r, const List<SLOTS, TEAM> &list, const float (&z)[SLOTS], const Sum &t, bool wrong) {
+    const float inf = __int_as_float(0x7f800000);
+    float q[SLOTS], q_rest, minus;
+    const bool known = teacher<SLOTS, TEAM, REST>(list, q, q_rest, minus);
+    Sum all = t;
+    if (REST) {
+        Sum mine = {neg_inf(), 0.0f};
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (!(z[s] <= neg_inf())) mine = join(mine, z[s] == inf ? Sum{nanf(""), 1.0f} : Sum{z[s], 1.0f});
+        all = join(t, team_join<TEAM>(mine));
+    }
+    const float log_all = logf(all.s), log_rest = logf(t.s);
+    float part = 0.0f;
+    if (all.m != neg_inf()) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (q[s] > 0.0f) part += q[s] * ((list.lp[s] - minus) - ((z[s] - all.m) - log_all));
+    } else {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (q[s] > 0.0f) part = inf;
+    }
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) part += __shfl_xor_sync(FULL, part, o);
+    if ((threadIdx.x & (TEAM - 1)) == 0 && r < a.rows) {
+        const float lse = all.m == neg_inf() ? neg_inf() : all.m + log_all;
+        if (REST && q_rest > 0.0f) part += t.m == neg_inf() ? inf : q_rest * (logf(q_rest) - (((t.m - all.m) + log_rest) - log_all));
+        a.loss[r] = wrong || (known && lse != lse) ? nanf("") : known ? part : 0.0f;
+        a.lse[r] = lse;
+        if (REST) a.lse_rest[r] = t.m == neg_inf() ? neg_inf() : t.m + log_rest;
+    }
+}
+
+// Narrow rows, up to TEAM * U vectors: TEAM neighbouring lanes each, as few as the list has places.  The row lies in shared memory as it does behind a 16-byte boundary.
+template <typename T, int TEAM, int U, int SLOTS, bool REST>
+__global__ void __launch_bounds__(256) distill_forward_rows_kernel(const T *logits, const FwdArgs a) {
+    constexpr int W = 16 / sizeof(T), EDGES = (2 * W - 2 + TEAM - 1) / TEAM;
+    __shared__ uint4 rows[256 / TEAM][TEAM * U];
+    const int lane = threadIdx.x & (TEAM - 1);
+    const long long row = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;      // whole warps take part in the lists
+    const T *x = logits + r * a.ld;
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+    uint4 *const mine = rows[threadIdx.x / TEAM];
+    T *const flat = reinterpret_cast<T *>(mine);                 // entry i at i + mis
+    List<SLOTS, TEAM> list;
+    list.load(a.tokens, a.lps, r, a.top);
+    const unsigned at = (unsigned)__cvta_generic_to_shared(mine + lane);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = lane + TEAM * u;
+        if (v * W >= mis && (v + 1) * W <= mis + a.vocab) cp_async<16>(at + u * (TEAM * 16), x - mis + v * W);
+        else mine[v] = make_uint4(Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE, Raw<T>::NONE);
+    }
+    cp_commit();
+    const int head = min(a.vocab, (W - mis) % W), body = (a.vocab - head) / W * W;
+    T edge[EDGES];
+#pragma unroll
+    for (int e = 0; e < EDGES; ++e) {
+        const int i = lane + TEAM * e < head ? lane + TEAM * e : lane + TEAM * e + body;
+        edge[e] = i < a.vocab ? x[i] : from_float<T>(0.0f);
+    }
+    const bool wrong = list.settle(a.vocab);
+    __syncwarp();                                                // the vectors at the ends are emptied
+#pragma unroll
+    for (int e = 0; e < EDGES; ++e) {
+        const int i = lane + TEAM * e < head ? lane + TEAM * e : lane + TEAM * e + body;
+        if (i < a.vocab) flat[i + mis] = edge[e];
+    }
+    cp_wait<0>();
+    __syncwarp();
+    float z[SLOTS];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const bool there = list.tok[s] >= 0 && list.tok[s] < a.vocab;
+        z[s] = there ? __fmul_rn(to_float(flat[list.tok[s] + mis]), a.scale) : neg_inf();
+        if (REST && there) flat[list.tok[s] + mis] = from_float<T>(neg_inf());
+    }
+    __syncwarp();
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = mine[lane + TEAM * u];
+    Sum t = {neg_inf(), 0.0f};
+    add_vectors<T, U>(t, q, a.scale);
+    finish_row<SLOTS, TEAM, REST>(a, row, list, z, team_join<TEAM>(t), wrong);
+}
+
 constexpr int PIECE = 128, RING = 3;      // vectors of 16 bytes in a piece (4 a lane), pieces in a warp's ring
 
 // A row's place among the 16-byte boundaries: `head` entries before the first one, nv vectors, the rest behind
@@ -273,7 +362,7 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
             add_vectors<T, PIECE / 32>(t, q, a.scale);
             slot = slot == RING - 1 ? 0 : slot + 1;
         }
-        t = warp_join(t);
+        t = team_join<32>(t);
         if (WARPS > 1) {
             if (lane == 0) sums[warp] = t;
 #pragma unroll
@@ -285,7 +374,7 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
                 }
             __syncthreads();
             if (w == 0) {
-                t = warp_join(lane < WARPS ? sums[lane] : Sum{neg_inf(), 0.0f});
+                t = team_join<32>(lane < WARPS ? sums[lane] : Sum{neg_inf(), 0.0f});
 #pragma unroll
                 for (int s = 0; s < SLOTS; ++s)
                     if (list.tok[s] >= 0 && list.tok[s] < a.vocab) z[s] = picked[s * 32 + lane];
@@ -293,59 +382,46 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
             __syncthreads();
             if (w != 0) continue;
         }
-        // the row's results
-        float q[SLOTS], q_rest, minus;
-        const bool known = teacher<SLOTS, 32, REST>(list, q, q_rest, minus);
-        Sum all = t;
-        if (REST) {
-            Sum mine = {neg_inf(), 0.0f};
-#pragma unroll
-            for (int s = 0; s < SLOTS; ++s)
-                if (!(z[s] <= neg_inf())) mine = join(mine, z[s] == __int_as_float(0x7f800000) ? Sum{nanf(""), 1.0f} : Sum{z[s], 1.0f});
-            all = join(t, warp_join(mine));
-        }
-        const float log_all = logf(all.s), log_rest = logf(t.s);
-        float part = 0.0f;
-        const float inf = __int_as_float(0x7f800000);
-        if (all.m != neg_inf()) {
-#pragma unroll
-            for (int s = 0; s < SLOTS; ++s)
-                if (q[s] > 0.0f) part += q[s] * ((list.lp[s] - minus) - ((z[s] - all.m) - log_all));
-        } else {
-#pragma unroll
-            for (int s = 0; s < SLOTS; ++s)
-                if (q[s] > 0.0f) part = inf;
-        }
-        part = warp_sum(part);
-        if (lane == 0) {
-            const float lse = all.m == neg_inf() ? neg_inf() : all.m + log_all;
-            if (REST && q_rest > 0.0f) part += t.m == neg_inf() ? inf : q_rest * (logf(q_rest) - (((t.m - all.m) + log_rest) - log_all));
-            a.loss[r] = wrong || (known && lse != lse) ? nanf("") : known ? part : 0.0f;
-            a.lse[r] = lse;
-            if (REST) a.lse_rest[r] = t.m == neg_inf() ? neg_inf() : t.m + log_rest;
-        }
+        finish_row<SLOTS, 32, REST>(a, r, list, z, t, wrong);
     }
     cp_wait<0>();
 }
 
-template <typename T, int WARPS, int SLOTS> int launch_forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
-    const long long teams = WARPS > 1 ? a.rows : (a.rows + 7) / 8, most = 3ll * sm_count();      // what runs at a time
-    const unsigned blocks = (unsigned)(teams < most ? teams : most);
-    constexpr int BYTES = 8 * RING * PIECE * 16;
-    const auto go = [&](auto kernel) -> int {
-        B2_TRY(set_max_dynamic_smem((const void *)kernel, BYTES));
-        kernel<<<blocks, 256, BYTES, st>>>(logits, a);
+template <typename T, int SLOTS, bool REST> int launch_forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T), BYTES = 8 * RING * PIECE * 16;
+    const int vecs = (a.vocab + W - 1) / W + 1;                   // one more: a row may start inside a vector
+    const auto rows = [&](auto kernel, long long blocks) -> int {
+        if (blocks > 0x7fffffffll) { set_error("b2_distill_forward: %lld rows", a.rows); return B2_ERR_BAD_SHAPE; }
+        kernel<<<(unsigned)blocks, 256, 0, st>>>(logits, a);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
         return B2_OK;
     };
-    if (a.lse_rest) B2_TRY(go(distill_forward_kernel<T, WARPS, SLOTS, true>)); else B2_TRY(go(distill_forward_kernel<T, WARPS, SLOTS, false>));
-    count_launch();
-    B2_CUDA(cudaGetLastError());
-    return B2_OK;
+    if constexpr (SLOTS == 1) {
+        if (a.top <= 8 && vecs <= 8 * 4) return rows(distill_forward_rows_kernel<T, 8, 4, 1, REST>, (a.rows + 31) / 32);
+        if (a.top <= 16 && vecs <= 16 * 6) return rows(distill_forward_rows_kernel<T, 16, 6, 1, REST>, (a.rows + 15) / 16);
+    }
+    if (vecs <= 32 * 4) return rows(distill_forward_rows_kernel<T, 32, 4, SLOTS, REST>, (a.rows + 7) / 8);
+    // a warp a row where the rows fill the device, a block a row else; 4 blocks an SM for long rows (8192 x 50001: 126 us, with 3 137 us), 3 for shorter ones (40000 x 3000:
+    // 69 us, with 4 75 us)
+    const bool many = a.rows >= 16 * sm_count();
+    const long long teams = many ? (a.rows + 7) / 8 : a.rows, most = (vecs >= 1024 ? 4ll : 3ll) * sm_count();
+    const auto go = [&](auto kernel) -> int {
+        B2_TRY(set_max_dynamic_smem((const void *)kernel, BYTES));
+        kernel<<<(unsigned)(teams < most ? teams : most), 256, BYTES, st>>>(logits, a);
+        count_launch();
+        B2_CUDA(cudaGetLastError());
+        return B2_OK;
+    };
+    return many ? go(distill_forward_kernel<T, 1, SLOTS, REST>) : go(distill_forward_kernel<T, 8, SLOTS, REST>);
 }
-template <typename T, int WARPS> int forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
-    if (a.top <= 32) return launch_forward<T, WARPS, 1>(logits, a, st);
-    if (a.top <= 64) return launch_forward<T, WARPS, 2>(logits, a, st);
-    return launch_forward<T, WARPS, 4>(logits, a, st);
+template <typename T, int SLOTS> int forward_of(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    return a.lse_rest ? launch_forward<T, SLOTS, true>(logits, a, st) : launch_forward<T, SLOTS, false>(logits, a, st);
+}
+template <typename T> int forward(const T *logits, const FwdArgs &a, cudaStream_t st) {
+    if (a.top <= 32) return forward_of<T, 1>(logits, a, st);
+    if (a.top <= 64) return forward_of<T, 2>(logits, a, st);
+    return forward_of<T, 4>(logits, a, st);
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------
@@ -583,11 +659,7 @@ int b2_distill_forward(const void *logits, int type, long long rows, int vocab, 
     if (!loss || !lse) { set_error("b2_distill_forward: null pointer"); return B2_ERR_BAD_ARG; }
     if (!aligned_to(loss, 4) || !aligned_to(lse, 4) || !aligned_to(lse_rest, 4)) { set_error("b2_distill_forward: a vector of numbers is not aligned to 4 bytes"); return B2_ERR_BAD_ARG; }
     const FwdArgs a = {top_tokens, top_logprobs, loss, lse, lse_rest, rows, ld, vocab, top, scale};
-    return with_type(type, [&](auto *t) {
-        typedef B2_ELEM(t) T;
-        const T *x = (const T *)logits;
-        return a.rows >= 16 * sm_count() || a.vocab <= 2048 ? forward<T, 1>(x, a, (cudaStream_t)stream) : forward<T, 8>(x, a, (cudaStream_t)stream);
-    });
+    return with_type(type, [&](auto *t) { return forward((const B2_ELEM(t) *)logits, a, (cudaStream_t)stream); });
 }
 
 int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits, int type, long long rows, int vocab, long long ld, float scale, const int *top_tokens,

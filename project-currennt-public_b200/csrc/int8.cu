@@ -820,11 +820,15 @@ int b2_int8_product(void *out, int out_type, long long ld_out, const void *x, in
         set_error("b2_int8_product: a tensor is not aligned to its elements");
         return B2_ERR_BAD_ARG;
     }
+    // the distance from a only row to the next
+    if (channels == 1) ld_w = (long long)pitch_of(dim);
+    if (rows == 1 && x_type == B2_I8) ld_x = (long long)pitch_of(dim);
     if (!aligned_to(w, 16) || ld_w % 16 || (x_type == B2_I8 && (!aligned_to(x, 16) || ld_x % 16))) {
         set_error("b2_int8_product: rows of 8-bit integers that do not start at multiples of 16 bytes");
         return B2_ERR_BAD_ARG;
     }
     ProductArgs a = {};
+    a.splits = 1;
     a.x_scales = x_scales; a.w_scales = w_scales; a.bias = bias;
     a.ld_out = ld_out; a.rows = rows; a.channels = channels; a.slabs = (dim + BK - 1) / BK;
     const signed char *xq = (const signed char *)x;

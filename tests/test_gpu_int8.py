@@ -138,6 +138,15 @@ def test_product_of_activations(tm, rows, channels, dim, t, o):  # noqa: F811
     assert torch.equal(two, out)
 
 
+def test_a_single_row_needs_no_pitch(tm):  # noqa: F811
+    torch, b2 = tm
+    x = torch.randint(-128, 128, (1, 41), dtype=torch.int8, device="cuda")
+    w = torch.randint(-128, 128, (1, 41), dtype=torch.int8, device="cuda")
+    out, one = torch.empty(1, 1, device="cuda"), torch.ones(1, device="cuda")
+    b2.int8_product(out, x, w, one, x_scales=one)
+    assert out.item() == (x.double() @ w.double().t()).item()
+
+
 def test_products_in_turn_share_a_workspace(tm):  # noqa: F811
     """many products in a row, captured too: a product reads what its own quantisation wrote"""
     torch, b2 = tm

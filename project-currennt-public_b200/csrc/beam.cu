@@ -8,7 +8,7 @@
 // vector whose largest entry reaches it is laid aside; in the end the entries that reach the bound of the whole slice are counted into their places.
 // Second kernel, started while the first one drains: a block joins the sums and the lists of a sequence's beams, the ranks in 64 bits (scores of different
 // beams meet, and 32 bits would make ties of what the beams' logits tell apart).
-// Bound by instructions (10 an entry, 4 of them for its exponential) and by the launches' latency.  Measured on a B200 (device time over the same buffers; in brackets a pass over
+// Bound by instructions (22 an entry with a mask, 14 without, 5 of them for its exponential) and by the launches' latency.  Measured on a B200 (device time over the same buffers; in brackets a pass over
 // buffers that change): 64 x 8 rows of 50001 bf16 with a mask, 16 continuations 33 us (37; the bytes' floor is 8), of that the second kernel 6 us; 4 rows of 32000 fp32 9.6 us (11.8), two launches.
 // Reordering: 64 x 8 beams with 112 MB of states and frames 33 us for the copy there and back (6.8 TB/s).
 #include <math.h>

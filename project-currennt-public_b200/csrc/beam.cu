@@ -8,8 +8,8 @@
 // vector whose largest entry reaches it is laid aside; in the end the entries that reach the bound of the whole slice are counted into their places.
 // Second kernel, started while the first one drains: a block joins the sums and the lists of a sequence's beams, the ranks in 64 bits (scores of different
 // beams meet, and 32 bits would make ties of what the beams' logits tell apart).
-// Bound by instructions (22 an entry with a mask, 14 without, 5 of them for its exponential) and by the launches' latency.  Measured on a B200 (device time over the same buffers; in brackets a pass over
-// buffers that change): 64 x 8 rows of 50001 bf16 with a mask, 16 continuations 33 us (37; the bytes' floor is 8), of that the second kernel 6 us; 4 rows of 32000 fp32 9.6 us (11.8), two launches.
+// Bound by instructions (18 an entry with a mask, 14 without, 5 of them for its exponential) and by the launches' latency.  Measured on a B200 (device time over the same buffers; in brackets a pass over
+// buffers that change): 64 x 8 rows of 50001 bf16 with a mask, 16 continuations 31 us (35; the bytes' floor is 8), of that the second kernel 6 us; 4 rows of 32000 fp32 9.6 us (11.8), two launches.
 // Reordering: 64 x 8 beams with 112 MB of states and frames 33 us for the copy there and back (6.8 TB/s).
 #include <math.h>
 
@@ -103,8 +103,23 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
     // A thread copies the vectors of its next chunk into shared memory while it works on one, for itself alone; their mask's bytes wait in registers
     Flags<T> on[MASK ? U : 1], on_next[MASK ? U : 1];
     const auto whole = [&](int v) { return v < v1 && v * W >= mis && (v + 1) * W - mis <= a.vocab; };
+    // most chunks lie inside their row, and need no tests
+    const auto inside = [&](int from) { return from * W >= mis && (from + CHUNK) * W - mis <= a.vocab && from + CHUNK <= v1 && (!MASK || mask_vec); };
+    const T *const x_here = x - mis + t * W;
+    const unsigned char *const mk_here = MASK ? mk - mis + t * W : nullptr;
+    const unsigned ring_here = (unsigned)__cvta_generic_to_shared(&ring[0][0][t]);
     const auto ahead = [&](int from, int to) {
-        const unsigned at = (unsigned)__cvta_generic_to_shared(&ring[to][0][t]);
+        const unsigned at = ring_here + to * (U * THREADS * 16);
+        if (inside(from)) {
+            const T *src = x_here + from * W;
+#pragma unroll
+            for (int u = 0; u < U; ++u) cp_async<16>(at + u * (THREADS * 16), src + u * (THREADS * W));
+            if (MASK)
+#pragma unroll
+                for (int u = 0; u < U; ++u) on_next[u] = load_flags<T>(mk_here + (from + u * THREADS) * W);
+            cp_commit();
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int v = from + t + u * THREADS;
@@ -131,6 +146,13 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
         ahead(from + THREADS * U, (chunk + 1) & 1);
         cp_wait<1>();
         uint4 q[U];
+        if (inside(from)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                q[u] = ring[chunk & 1][u][t];
+                if (MASK) rule_out<T>(q[u], on[u]);
+            }
+        } else
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int v = from + t + u * THREADS;

@@ -620,7 +620,12 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 for (int k = 0; k < a.slabs; ++k, ++i) {
                     const int s = (int)(i % STAGES);
                     if (!mbar_wait_bounded<false>(empty(s), ((i / STAGES) & 1u) ^ 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
-                    // (the weights that were in slab k are read: its last products came before those that freed the slot)
+                    // The weights that were in slab k have to be read, `slabs` uses of the ring ago.  With as many slabs as slots or more, that use came before the one which freed this
+                    // slot; else it is waited for.
+                    if (RESIDENT && fresh && n > 0 && a.slabs < STAGES) {
+                        const unsigned j = i - (unsigned)a.slabs;
+                        if (!mbar_wait_bounded<false>(empty((int)(j % STAGES)), (j / STAGES) & 1u, &fail, WAIT_CYCLES)) { fail = 1; ok = false; break; }
+                    }
                     const uint32_t at = ring + (uint32_t)s * STAGE, bar = map_to_rank(full(s), 0);
                     if (rank == 0) mbar_expect_tx(full(s), 2 * (PAIR_B + (fresh ? A_BYTES : 0)));
                     if (fresh) tma_load_2d_pair(RESIDENT ? held + (uint32_t)k * A_BYTES : at + PAIR_B, &map_w, k * BK, c0, bar);

@@ -130,7 +130,8 @@ def test_forward(tm, rows, vocab, top, pad, shift, t, rest, scale):  # noqa: F81
     assert torch.equal(again[0], loss) and torch.equal(again[1], lse)
 
 
-@pytest.mark.parametrize("rows,vocab,top,rest", [(2500, 300, 12, True), (2400, 2100, 40, False), (1300, 259, 70, True), (2370, 4500, 9, True)])
+@pytest.mark.parametrize("rows,vocab,top,rest", [(2500, 300, 12, True), (2400, 2100, 40, False), (1300, 259, 70, True), (2370, 4500, 9, True), (2400, 9001, 20, True), (5000, 31, 6, True),
+                                                 (2400, 1100, 128, False)])
 def test_forward_of_many_rows(tm, rows, vocab, top, rest):  # noqa: F811
     """more rows than run at a time, rows that start anywhere"""
     torch, b2 = tm

@@ -85,7 +85,8 @@ def test_quantize_special_rows(tm, dim):  # noqa: F811
 
 # around the borders of a slab (128 positions), a tile (128 channels; 16 to 256 rows) and the ways in which a product is split
 PRODUCTS = [(1, 1, 1), (1, 5, 16), (3, 130, 40), (8, 1000, 1024), (16, 127, 129), (17, 128, 128), (32, 300, 257), (33, 260, 511), (64, 129, 100), (65, 4000, 130), (128, 200, 1000), (129, 513, 384),
-            (257, 385, 650), (300, 1030, 1), (1, 20000, 300), (520, 700, 2050), (2000, 33, 64), (700, 5000, 259), (5, 64, 8192), (40, 40, 100000), (600, 600, 131071)]
+            (257, 385, 650), (300, 1030, 1), (1, 20000, 300), (520, 700, 2050), (2000, 33, 64), (700, 5000, 259), (5, 64, 8192), (40, 40, 100000), (600, 600, 131071),
+            (300, 40000, 130), (1500, 8000, 1300), (513, 19000, 1152)]
 
 
 @pytest.mark.parametrize("rows,channels,dim", PRODUCTS)
@@ -176,6 +177,47 @@ def test_products_in_turn_share_a_workspace(tm):  # noqa: F811
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dim", [60, 100, 200, 300, 400, 500, 640, 800, 1000, 1152, 1200])
+def test_products_of_short_contractions_over_many_channels(tm, dim):  # noqa: F811
+    """a pair of blocks has several tiles of channels, whose weights follow each other in the same place: one slab to ten of them"""
+    torch, b2 = tm
+    rows, channels = 300, 60001
+    x, w = _int8(torch, rows, dim, 1), _int8(torch, channels, dim, 2)
+    out = torch.empty(rows, channels, device="cuda")
+    b2.int8_product(out, x, w, torch.ones(channels, device="cuda"), x_scales=torch.ones(rows, device="cuda"))
+    assert torch.equal(out, (x.double() @ w.double().t()).float())
+
+
+@pytest.mark.parametrize("rows,channels,dim", [(8, 5000, 700), (20, 1000, 4000), (700, 3000, 900), (400, 2000, 2000)])
+def test_products_at_once(tm, rows, channels, dim):  # noqa: F811
+    """on two streams, each with its own workspace, and in a graph with one for both in turn"""
+    torch, b2 = tm
+    xs = [_rand(torch, (rows, dim), "bf16", s, 1.0) for s in (1, 2)]
+    w, ws = _int8(torch, channels, dim, 2), torch.rand(channels, device="cuda")
+    work = [torch.empty(b2.int8_product_workspace(rows, channels, dim), dtype=torch.uint8, device="cuda") for _ in xs]
+    outs = [torch.empty(rows, channels, device="cuda") for _ in xs]
+    want = []
+    for x, o, k in zip(xs, outs, work):
+        b2.int8_product(o, x, w, ws, workspace=k)
+        torch.cuda.synchronize()
+        want.append(o.clone())
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(20):
+        for x, o, k, st in zip(xs, outs, work, streams):
+            b2.int8_product(o, x, w, ws, workspace=k, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        for x, o in zip(xs, outs):
+            b2.int8_product(o, x, w, ws, workspace=work[0], stream=streams[0].cuda_stream)
+    for o in outs:
+        o.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 def test_offsets_beyond_32_bits(tm):  # noqa: F811

@@ -13,6 +13,8 @@
 // Reordering: 64 x 8 beams with 112 MB of states and frames 33 us for the copy there and back (6.8 TB/s).
 #include <math.h>
 
+#include <type_traits>
+
 #include "logits.cuh"
 
 namespace b2 {
@@ -558,10 +560,54 @@ template <int N, int HELD> __device__ __forceinline__ void move(const b2_state &
         }
     }
 }
-// bytes of a column: what the addresses and the rows allow, and 4 where more than MOST_HELD beams have to be in registers at once
-__host__ __device__ __forceinline__ int column_width(const b2_state &s, int beams) {
-    const unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & (s.data == s.out && beams > MOST_HELD ? 3 : 15);
-    return at & 1 ? 1 : at & 2 ? 2 : at & 4 ? 4 : at & 8 ? 8 : s.data == s.out && beams > MOST_HELD ? 4 : 16;
+// Narrow rows (tokens so far, say): the beams of a sequence and outer index are up to ITEMS pieces of each of `team` lanes, next to each other in memory.  A lane has its own of
+// BATCH outer indices in registers before any is written.
+constexpr int SMALL = 4;
+template <int ITEMS> struct Batch { static constexpr int N = ITEMS == 1 ? 8 : 2; };
+template <int N, int ITEMS>
+__device__ __forceinline__ void move_small(const b2_state &s, const int *parent, int beams, int columns, int team, long long chunk, long long groups, unsigned group) {
+    typedef typename Bytes<N>::T V;
+    constexpr int BATCH = Batch<ITEMS>::N;
+    const int lane = (int)threadIdx.x & (team - 1), pieces = beams * columns, step = MOVE_THREADS / team;
+    const long long row = beams * s.row_bytes, first = chunk * (step * BATCH) + threadIdx.x / team;
+    long long from[ITEMS];                 // where a piece comes from, -1: zeros
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int k = lane + i * team, b = min(k, pieces - 1) / columns, p = parent[b];
+        from[i] = p < 0 ? -1 : p * s.row_bytes + (long long)(k - b * columns) * N;
+    }
+    V v[BATCH][ITEMS];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) {
+        const long long o = first + e * step;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (o < s.outer && lane + i * team < pieces)
+                v[e][i] = from[i] < 0 ? zero_of<V>() : *reinterpret_cast<const V *>((const char *)s.data + (o * groups + group) * row + from[i]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) {
+        const long long o = first + e * step;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (o < s.outer && lane + i * team < pieces) *reinterpret_cast<V *>((char *)s.out + (o * groups + group) * row + (long long)(lane + i * team) * N) = v[e][i];
+    }
+}
+// How a tensor is moved.  width: bytes of a column or piece, what the addresses and the rows allow, and 4 where more than MOST_HELD beams have to be in registers at once.
+// team: lanes of a sequence and outer index with narrow rows, else 0; batch: outer indices of each
+struct Way { int width, team, batch; };
+__host__ __device__ __forceinline__ Way way_of(const b2_state &s, int beams) {
+    const unsigned long long at = ((uintptr_t)s.data | (uintptr_t)s.out | (uintptr_t)s.row_bytes) & 15;
+    int width = at == 0 ? 16 : at & 1 ? 1 : at & 2 ? 2 : at & 4 ? 4 : 8;
+    const long long pieces = s.row_bytes / width * beams;
+    if (pieces <= 32 * SMALL) {
+        int team = 1;
+        while (team < 32 && team < pieces) team *= 2;
+        return {width, team, pieces <= team ? Batch<1>::N : Batch<SMALL>::N};
+    }
+    if (s.data == s.out && beams > MOST_HELD && width > 4) width = 4;
+    return {width, 0, 0};
 }
 // a block's threads have columns of one sequence, those of all outer indices one after the other
 template <int HELD> __global__ void __launch_bounds__(MOVE_THREADS) beam_reorder_kernel(const __grid_constant__ StateArgs a) {
@@ -569,11 +615,28 @@ template <int HELD> __global__ void __launch_bounds__(MOVE_THREADS) beam_reorder
     int i = 0;
     while (i + 1 < a.n && blockIdx.x >= a.first[i + 1]) ++i;
     const b2_state &s = a.s[i];
-    const int width = column_width(s, a.beams);
+    const Way way = way_of(s, a.beams);
+    const int width = way.width;
     const unsigned groups = (unsigned)a.groups, k = blockIdx.x - a.first[i], group = k % groups;     // blocks of a tensor: [chunk][group]
     if ((int)threadIdx.x < a.beams) {
         const int p = a.parents[(long long)group * a.beams + threadIdx.x];
         parent[threadIdx.x] = p >= 0 && p < a.beams ? p : -1;
+    }
+    if (way.team) {
+        const int columns = (int)(s.row_bytes / width);
+        __syncthreads();
+        const auto go = [&](auto bytes) {
+            constexpr int N = decltype(bytes)::value;
+            if (columns * a.beams <= way.team) move_small<N, 1>(s, parent, a.beams, columns, way.team, k / groups, a.groups, group);
+            else move_small<N, SMALL>(s, parent, a.beams, columns, way.team, k / groups, a.groups, group);
+        };
+        switch (width) {
+            case 16: return go(std::integral_constant<int, 16>());
+            case 8: return go(std::integral_constant<int, 8>());
+            case 4: return go(std::integral_constant<int, 4>());
+            case 2: return go(std::integral_constant<int, 2>());
+            default: return go(std::integral_constant<int, 1>());
+        }
     }
     const long long columns = s.row_bytes / width, at = (long long)(k / groups) * MOVE_THREADS + threadIdx.x;
     long long o, column;
@@ -670,8 +733,9 @@ int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long
                 b2_state s = states[i];
                 if (!s.outer || !s.row_bytes) continue;
                 if (!s.out) s.out = s.data;
-                if ((s.out == s.data && beams > MOST_HELD) != (pass == 1)) continue;
-                const double more = (double)groups * ceil((double)s.outer * (double)(s.row_bytes / column_width(s, beams)) / MOVE_THREADS);
+                const Way way = way_of(s, beams);
+                if ((!way.team && s.out == s.data && beams > MOST_HELD) != (pass == 1)) continue;
+                const double more = (double)groups * ceil((way.team ? (double)s.outer * way.team / way.batch : (double)s.outer * (double)(s.row_bytes / way.width)) / MOVE_THREADS);
                 if (more > 2147483647.0) { set_error("b2_beam_reorder: tensor %d is too large", i); return B2_ERR_BAD_SHAPE; }
                 if (blocks + (unsigned long long)more > 2147483647ull) break;
                 a.s[a.n] = s;

@@ -13,6 +13,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "typed.cuh"
@@ -66,10 +67,13 @@ struct RowScale {
     }
 };
 
-// TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice.  WHOLE: rows of whole vectors that start on their boundaries, the integers' too
+// TEAM threads a row; up to U vectors of each in registers (KEPT), or the row is read twice.  WHOLE: rows of whole vectors that start on their boundaries, the integers' too.
+// Else a vector's integers lie across the boundaries of what they are stored to: a lane takes the first bytes of a store from the lane before it, shifted by what
+// the row's two starts differ (60000 x 401 bf16: single bytes 41 us).
 template <typename T, int TEAM, int U, bool KEPT, bool WHOLE>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long long ld_q, float *scales, const T *x0, long long rows, int dim, long long ld_x) {
     constexpr int W = 16 / sizeof(T), TEAMS = 256 / TEAM;
+    typedef std::conditional_t<W == 8, unsigned long long, unsigned> Word;         // W integers
     __shared__ float most[8];
     const int team = threadIdx.x / TEAM, at = threadIdx.x % TEAM, lane = threadIdx.x & 31;
     const long long r = (long long)blockIdx.x * TEAMS + team;
@@ -77,19 +81,26 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     if (r >= rows) return;
     const T *x = x0 + r * ld_x;
     unsigned char *to = reinterpret_cast<unsigned char *>(q) + r * ld_q;
-    const int mis = WHOLE ? 0 : (int)(((uintptr_t)x & 15) / sizeof(T)), vecs = WHOLE ? dim / W : (mis + dim + W - 1) / W;
-    const bool out_vec = WHOLE || (((uintptr_t)(to - mis)) & (W - 1)) == 0;
+    // vectors hold the entries v * W - mis on; one more than there are takes the last bytes
+    const int mis = WHOLE ? 0 : (int)(((uintptr_t)x & 15) / sizeof(T)), vecs = WHOLE ? dim / W : (mis + dim + W - 1) / W + 1;
+    const int shift = WHOLE ? 0 : (mis - (int)((uintptr_t)to & (W - 1))) & (W - 1);      // bytes of the vector before that go to where the one behind it begins
     const auto load = [&](int v) -> uint4 {
         const int i0 = v * W - mis;
         if constexpr (WHOLE) return *reinterpret_cast<const uint4 *>(x + i0);
         else {
             if (i0 >= 0 && i0 + W <= dim) return *reinterpret_cast<const uint4 *>(x + i0);
-            T e[W];
+            // the row's ends; entry by entry, in a loop: a launch fetches the code of every vector anew
+            unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll 1
+            for (int i = max(0, i0); i < min(dim, i0 + W); ++i) {
+                unsigned bits = 0;
+                memcpy(&bits, x + i, sizeof(T));
+                const int j = i - i0, at_word = j * (int)sizeof(T) / 4, by = j * (int)sizeof(T) % 4 * 8;
 #pragma unroll
-            for (int j = 0; j < W; ++j) e[j] = i0 + j >= 0 && i0 + j < dim ? x[i0 + j] : from_float<T>(0.0f);
-            uint4 o;
-            memcpy(&o, e, 16);
-            return o;
+                for (int k = 0; k < 4; ++k)
+                    if (k == at_word) w[k] |= bits << by;
+            }
+            return make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
     uint4 held[KEPT ? U : 1];
@@ -114,28 +125,54 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(signed char *q, long
     }
     const RowScale s(m);
     if (at == 0) scales[r] = s.scale;
-    const auto store = [&](int v, const uint4 &h) {
-        const int i0 = v * W - mis;
+    const auto word = [&](const uint4 &h) {
         const Vec<unsigned char, W> o = s.template quantised<T>(h);
-        if constexpr (WHOLE) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
-        else if (out_vec && i0 >= 0 && i0 + W <= dim) *reinterpret_cast<Vec<unsigned char, W> *>(to + i0) = o;
+        Word w;
+        memcpy(&w, &o, W);
+        return w;
+    };
+    // w: the integers of vector v, last: those of the vector before the warp's first one; whole warps come here, and a vector behind the last one stores nothing
+    const auto store = [&](int v, Word w, Word last) {
+        int i0 = v * W - mis;
+        if constexpr (!WHOLE) {
+            Word before = __shfl_up_sync(0xffffffffu, w, 1);
+            if (lane == 0) before = last;
+            if (shift) {
+                w = (before >> (8 * shift)) | (w << (8 * (W - shift)));
+                i0 += shift - W;
+            }
+        }
+        if (v >= vecs) return;
+        if (WHOLE || (i0 >= 0 && i0 + W <= dim)) *reinterpret_cast<Word *>(to + i0) = w;
         else {
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (i0 + j >= 0 && i0 + j < dim) to[i0 + j] = o.v[j];
+#pragma unroll 1
+            for (int j = max(0, -i0); j < min(W, dim - i0); ++j) to[i0 + j] = (unsigned char)(w >> (8 * j));
         }
     };
-    if (KEPT) {
+    if (KEPT && TEAM == 32) {
+        Word last = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (at + u * TEAM < vecs) store(at + u * TEAM, held[u]);
-    } else
-        for (int v = at; v < vecs; v += TEAM) store(v, load(v));
+        for (int u = 0; u < U; ++u) {
+            if (WHOLE ? at + u * TEAM >= vecs : u * TEAM >= vecs) break;
+            const Word w = word(held[u]);
+            store(at + u * TEAM, w, last);
+            if constexpr (!WHOLE) last = __shfl_sync(0xffffffffu, w, 31);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; KEPT && u < U; ++u) {
+            const int v = at + u * TEAM;
+            if (WHOLE ? v >= vecs : (v & ~31) >= vecs) break;
+            store(v, word(held[u]), !WHOLE && lane == 0 && v > 0 && v <= vecs ? word(load(v - 1)) : 0);
+        }
+        for (int v = at; !KEPT && (WHOLE ? v < vecs : (v & ~31) < vecs); v += TEAM)
+            store(v, word(v < vecs ? load(v) : make_uint4(0, 0, 0, 0)), !WHOLE && lane == 0 && v > 0 && v <= vecs ? word(load(v - 1)) : 0);
+    }
 }
 
 template <typename T, bool WHOLE> int quantize_rows(signed char *q, long long ld_q, float *scales, const T *x, long long rows, int dim, long long ld_x, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
-    const int vecs = WHOLE ? dim / W : (dim + W - 1) / W + 1;      // one more: a row may start inside a vector
+    const int vecs = WHOLE ? dim / W : (dim + W - 1) / W + 2;      // a row may start inside a vector, and its last bytes come with one more
     const auto go = [&](auto kernel, int teams) -> int {
         const long long blocks = (rows + teams - 1) / teams;
         if (blocks > 0x7fffffffll) { set_error("b2_int8_quantize: %lld rows", rows); return B2_ERR_BAD_SHAPE; }

@@ -666,7 +666,8 @@ extern "C" {
 
 size_t b2_beam_select_workspace(long long groups, int beams, int vocab, int top) {
     if (!sizes_fit(groups, beams, vocab, top)) return 0;
-    const size_t slices = (size_t)slices_of(groups * beams, beams, vocab, B2_F32) * (size_t)groups * beams;      // the most of any type
+    const int wide = slices_of(groups * beams, beams, vocab, B2_F32), narrow = slices_of(groups * beams, beams, vocab, B2_BF16);
+    const size_t slices = (size_t)(wide > narrow ? wide : narrow) * (size_t)groups * beams;      // the most of any type
     return slices * (sizeof(Part) + (size_t)top * sizeof(Key));
 }
 

@@ -563,7 +563,8 @@ __global__ void __launch_bounds__(STREAM + 32, 3) distill_backward_kernel(T *dlo
         const int lo = max(0, seg * STREAM * U * W - p.mis), hi = min(a.vocab, (seg + 1) * STREAM * U * W - p.mis);
         RowList<T, SLOTS, 32, REST, ADD> list;
         list.load(a, r);
-        const int i = seg == 0 ? edge_entry(p, at - STREAM) : a.vocab;       // the row's ends are this warp's too
+        // the entries outside the vectors are this warp's too, where they lie in its segment: no other block reads or writes what is listed there
+        const int end = edge_entry(p, at - STREAM), i = end >= lo && end < hi ? end : a.vocab;
         const T edge = i < a.vocab ? p.x[i] : from_float<T>(0.0f);
         list.gather(p, lo, hi);
         const RowGrad g = list.factors(a.vocab);

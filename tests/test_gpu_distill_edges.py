@@ -1,0 +1,45 @@
+"""GPU tests of the divergence from a teacher's most likely tokens (b2_distill_*) where rows, lists and numbers end: listed tokens among a row's last entries, NaN in the
+middle of long rows, logits that a scale takes to -inf.  Oracles and error bounds are those of test_gpu_distill.py."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_distill import _backward, _forward, _list
+from test_gpu_token_operators import TINY, U, _close, _host, _rand, tm, u  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# segments of 512 vectors in small calls and of 2048 in large ones: more blocks than run at a time, and rows that start and end anywhere
+@pytest.mark.parametrize("rows,vocab,pad,shift,t", [(3000, 20011, 0, 0, "bf16"), (1500, 50001, 47, 0, "bf16"), (1500, 9002, 0, 3, "f32"), (700, 20011, 2, 5, "f16"), (40, 20011, 0, 1, "bf16"),
+                                                    (3, 4099, 0, 0, "f32")])
+@pytest.mark.parametrize("rest", [True, False])
+def test_gradient_of_listed_tokens_at_the_ends_of_wide_rows(tm, rows, vocab, pad, shift, t, rest):  # noqa: F811
+    """The first and the last three tokens are in every list.  In place and added to zeros gives the bits that a buffer of its own gets, and that is right; so is what is
+    added to other numbers."""
+    torch, b2 = tm
+    x = _rand(torch, (rows, vocab), t, 3, 2.0, pad, shift)
+    tok, lp = _list(torch, rows, vocab, 12, 5, "plain")
+    ends = np.array([vocab - 1, vocab - 2, vocab - 3, 0, 1, 2], np.int32)
+    tok[:, 6:], lp[:, 6:] = ends, np.float32(-3.0) - 0.5 * np.arange(6, dtype=np.float32)
+    tokens, lps = torch.from_numpy(tok).cuda(), torch.from_numpy(lp).cuda()
+    loss, lse, other = (torch.empty(rows, device="cuda") for _ in range(3))
+    kw = dict(lse_rest=other) if rest else {}
+    b2.distill_forward(x, tokens, lps, loss, lse, **kw)
+    g = torch.rand(rows, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) + 0.5
+    d = torch.full_like(x, math.nan)
+    b2.distill_backward(d, x, tokens, lps, lse, g, **kw)
+    old = _rand(torch, (rows, vocab), t, 4, 0.01, pad, shift)
+    added = [torch.zeros_like(x), old.clone()]
+    for a in added:
+        b2.distill_backward(a, x, tokens, lps, lse, g, accumulate=True, **kw)
+    pick = sorted(set(range(0, rows, max(1, rows // 40))) | {rows - 1})
+    z = x[pick].double().cpu().numpy()
+    b2.distill_backward(x, x, tokens, lps, lse, g, **kw)                     # in place
+    assert torch.equal(x, d) and torch.equal(added[0], d)
+    got, sums, before = _host(d[pick]), _host(added[1][pick]), _host(old[pick])
+    for i, r in enumerate(pick):
+        want, tol = _backward(z[i], tok[r], lp[r], float(lse[r]), float(other[r]), float(g[r]), rest, vocab)
+        _close(got[i], want, tol + (U[t] + 2 * u) * np.abs(want) + TINY[t])
+        _close(sums[i], before[i] + want, tol + (U[t] + 4 * u) * np.abs(before[i] + want) + 2 * u * np.abs(want) + TINY[t])

@@ -393,8 +393,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
 #pragma unroll 1
     for (int shift = enough ? -1 : 32 - DIGIT_BITS; shift >= 0;) {
         for (int i = t; i < DIGITS; i += JOIN_THREADS) counts[i] = 0;
-        if (t == 0) digit = -1;
         __syncthreads();
+        if (t == 0) digit = -1;                              // all have taken the one before
+        const int want = left;                               // before the barriers behind which it is written
         const int above = shift + DIGIT_BITS;
         for_all([&](int, unsigned k) {
             if (above >= 32 || k >> above == bound >> above) atomicAdd(&counts[(k >> shift) & (DIGITS - 1)], 1);
@@ -414,7 +415,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         __syncthreads();
         before -= sum;
         for (int w = 0; w < warp; ++w) before += warp_counts[w];
-        const int want = left;
         if (before < want && want <= before + sum) {
             int at = before;
 #pragma unroll

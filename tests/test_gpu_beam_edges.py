@@ -1,0 +1,48 @@
+"""GPU tests of the selection of beam search (b2_beam_select) where many continuations are close to each other: the ways of its second kernel to find the best ones.  The
+oracle and the bounds of a score's error are those of test_gpu_beam.py."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_beam import _run, _same, _select
+from test_gpu_token_operators import _host, tm, u  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _near(got, z, scores, groups, top):
+    """Beams whose log sums differ may swap places where their scores are closer than these are exact.  Every candidate's score is off by e at most (as _same says), so the k-th best is,
+    and so is each one's own; no place is left empty, and none is there twice."""
+    rows, vocab = z.shape
+    beams = rows // groups
+    best, beam, token = _host(got[0]), got[1].cpu().numpy(), got[2].cpu().numpy()
+    m = z.max(1)
+    all_of = (np.asarray(scores, np.float64) - m - np.log(np.exp(z - m[:, None]).sum(1)))[:, None] + z
+    for g in range(groups):
+        mine = all_of[g * beams:(g + 1) * beams]
+        n = min(top, mine.size)
+        want = np.sort(mine.reshape(-1))[::-1][:n]
+        e = (vocab / 64 + 64) * u + 2.0 ** -20 + 2 * u * np.abs(want)
+        assert (beam[g, :n] >= 0).all() and (beam[g, n:] == -1).all() and (best[g, n:] == -math.inf).all(), "sequence %d: %d of %d" % (g, (beam[g] >= 0).sum(), n)
+        assert (np.abs(best[g, :n] - want) <= e).all()
+        assert (np.abs(best[g, :n] - mine[beam[g, :n], token[g, :n]]) <= e).all()
+        assert (np.diff(best[g, :n]) <= 0).all() and len(set(zip(beam[g, :n], token[g, :n]))) == n
+
+
+def _beams(torch, groups, beams, vocab, spread, at, seed):
+    """logits and scores that differ by `spread`, the scores around `at`"""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(groups * beams, vocab, generator=g) * spread).cuda()
+    return x, (at + torch.randn(groups * beams, generator=g) * spread).cuda()
+
+
+@pytest.mark.parametrize("groups,beams,vocab,top", [(150, 64, 259, 64), (40, 16, 2000, 32), (60, 8, 5000, 64)])
+def test_beams_of_different_strength_again_and_again(tm, groups, beams, vocab, top):  # noqa: F811
+    """continuations that are found by their ranks' first two digits: the same ones in every pass"""
+    torch, b2 = tm
+    x, scores = _beams(torch, groups, beams, vocab, 2.0, -20.0, 1)
+    first = _run(torch, b2, x, scores, groups, top)
+    _near(first, x.double().cpu().numpy(), scores.cpu().numpy(), groups, top)
+    for _ in range(100):
+        assert all(torch.equal(a, b) for a, b in zip(first, _run(torch, b2, x, scores, groups, top)))

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(SLICE_THREADS, 4) beam_rows_kernel(const T *lo
         cp_wait<0>();
         return;
     }
+    if (rounds > 32) __syncthreads();                      // n_hits is set; else the first bound's barrier comes before the first hit
     for (int from = v0; from < v1; from += THREADS * U, ++chunk) {
         if (MASK)
 #pragma unroll

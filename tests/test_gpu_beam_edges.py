@@ -46,3 +46,22 @@ def test_beams_of_different_strength_again_and_again(tm, groups, beams, vocab, t
     _near(first, x.double().cpu().numpy(), scores.cpu().numpy(), groups, top)
     for _ in range(100):
         assert all(torch.equal(a, b) for a, b in zip(first, _run(torch, b2, x, scores, groups, top)))
+
+
+@pytest.mark.parametrize("vocab,t", [(200, "float32"), (131, "float32"), (249, "float32"), (300, "bfloat16"), (500, "float16")])
+@pytest.mark.parametrize("top", [33, 64])
+@pytest.mark.parametrize("masked", [False, True])
+def test_two_warps_of_a_row_and_many_continuations(tm, vocab, t, top, masked):  # noqa: F811
+    """rows of 33 to 63 vectors, which have no bound for more than 32 continuations: every entry is of interest from the start"""
+    torch, b2 = tm
+    rows = 1200
+    x = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(vocab)) * 3).to(getattr(torch, t)).cuda()
+    scores = torch.zeros(rows, device="cuda")
+    mask = torch.ones(vocab, dtype=torch.uint8, device="cuda")
+    if masked:
+        mask[::7] = 0
+    z = x.double().cpu().numpy()
+    z[:, (mask == 0).cpu().numpy()] = -math.inf
+    want = _select(z, scores.cpu().numpy(), None, None, 0, rows, top)
+    for _ in range(5):
+        _same(_run(torch, b2, x, scores, rows, top, mask=mask if masked else None), want, 0, vocab)

@@ -65,3 +65,29 @@ def test_two_warps_of_a_row_and_many_continuations(tm, vocab, t, top, masked):  
     want = _select(z, scores.cpu().numpy(), None, None, 0, rows, top)
     for _ in range(5):
         _same(_run(torch, b2, x, scores, rows, top, mask=mask if masked else None), want, 0, vocab)
+
+
+@pytest.mark.parametrize("groups,beams,vocab,top", [(4, 64, 259, 64), (2, 16, 50001, 32), (6, 32, 1000, 32), (5, 8, 5000, 64), (7, 64, 300, 16)])
+@pytest.mark.parametrize("spread", [1e-3, 0.01, 0.1])
+@pytest.mark.parametrize("at", [-20.0, -100.0, -1000.0])
+def test_continuations_next_to_each_other(tm, groups, beams, vocab, top, spread, at):  # noqa: F811
+    """ranks that have the bits of their first two digits in common: no place stays empty"""
+    torch, b2 = tm
+    x, scores = _beams(torch, groups, beams, vocab, spread, at, 5)
+    _near(_run(torch, b2, x, scores, groups, top), x.double().cpu().numpy(), scores.cpu().numpy(), groups, top)
+
+
+@pytest.mark.parametrize("beams,vocab,top", [(64, 260, 64), (16, 50000, 32), (32, 1000, 48)])
+@pytest.mark.parametrize("spread,at", [(1e-3, -20.0), (0.01, -100.0), (0.1, -1000.0)])
+def test_the_order_of_continuations_next_to_each_other(tm, beams, vocab, top, spread, at):  # noqa: F811
+    """beams with the same logits have the same log sum, whatever its error: their continuations' order is exact"""
+    torch, b2 = tm
+    groups = 3
+    x = torch.cat([_beams(torch, 1, 1, vocab, spread, at, s)[0].repeat(beams, 1) for s in range(groups)])
+    scores = _beams(torch, groups, beams, 1, spread, at, 9)[1]
+    z, sc = x.double().cpu().numpy(), scores.cpu().numpy()
+    for g in range(groups):                                   # no two of them are closer than the roundings in 64 bits
+        ranks = np.sort((sc[g * beams:(g + 1) * beams, None].astype(np.float64) + z[g * beams]).reshape(-1))[::-1][:top + 1]
+        assert (-np.diff(ranks) > 1e-11).all()
+    got, want = _run(torch, b2, x, scores, groups, top), _select(z, sc, None, None, 0, groups, top)
+    _same(got, want, 0, vocab)

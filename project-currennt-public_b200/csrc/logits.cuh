@@ -59,13 +59,13 @@ template <typename T> __device__ __forceinline__ Pair exp_pair(Pair x) {
 }
 
 // ---- running sums of exponentials --------------------------------------------------------------------------------------------------
-struct Sum { float m, s; };      // largest z met, sum of e^(z - m)
+struct Sum { float m, s; };      // largest z met (-inf: none, and s is 0), sum of e^(z - m).  NaN in m stays, whatever is met behind it
 __device__ __forceinline__ void rise(Sum &a, float m) {
     if (a.m != neg_inf()) {
         const float r = ex2((a.m - m) * LOG2E);
         a.s = r == 0.0f ? 0.0f : r * a.s;
     }
-    a.m = m;
+    a.m = max_nan(a.m, m);
 }
 __device__ __forceinline__ Sum join(Sum a, Sum b) {
     const float m = max_nan(a.m, b.m);

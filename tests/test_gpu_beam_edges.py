@@ -91,3 +91,34 @@ def test_the_order_of_continuations_next_to_each_other(tm, beams, vocab, top, sp
         assert (-np.diff(ranks) > 1e-11).all()
     got, want = _run(torch, b2, x, scores, groups, top), _select(z, sc, None, None, 0, groups, top)
     _same(got, want, 0, vocab)
+
+
+@pytest.mark.parametrize("t", ["bfloat16", "float32"])
+@pytest.mark.parametrize("behind", ["nothing", "masked", "more", "much more"])
+@pytest.mark.parametrize("beams", [64, 5])
+def test_nan_anywhere_in_a_row(tm, t, behind, beams):  # noqa: F811
+    """a beam with a NaN among its allowed logits has no continuations, whatever comes behind it; the others have theirs"""
+    torch, b2 = tm
+    chunk = 1024 * (4 if t == "float32" else 8)
+    vocab = 2 * chunk + chunk // 3
+    x = (torch.randn(beams, vocab, generator=torch.Generator().manual_seed(4)) * 2.5).to(getattr(torch, t)).cuda()
+    at = np.linspace(3, vocab - 1, beams).astype(int)
+    allowed = np.ones((beams, vocab), np.uint8)
+    for b in range(0, beams, 2):
+        p = at[b]
+        if behind == "nothing":
+            x[b, p + 1:] = -math.inf
+        elif behind == "masked":
+            allowed[b, p + 1:] = 0
+        elif behind == "much more":
+            x[b, p + 1:] += 100.0
+            x[b, p + 1 + (vocab - p) // 2:] += 100.0
+        x[b, p] = math.nan
+    scores = -torch.rand(beams, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    mask = torch.from_numpy(allowed).cuda() if behind == "masked" else None
+    got = _run(torch, b2, x, scores, 1, 24, mask=mask)
+    z = x.double().cpu().numpy()
+    z[allowed == 0] = -math.inf
+    want = _select(z, scores.cpu().numpy(), None, None, 0, 1, 24)
+    assert (want[1] % 2 == 1).all()
+    _same(got, want, 0, vocab)

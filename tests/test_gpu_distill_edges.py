@@ -43,3 +43,44 @@ def test_gradient_of_listed_tokens_at_the_ends_of_wide_rows(tm, rows, vocab, pad
         want, tol = _backward(z[i], tok[r], lp[r], float(lse[r]), float(other[r]), float(g[r]), rest, vocab)
         _close(got[i], want, tol + (U[t] + 2 * u) * np.abs(want) + TINY[t])
         _close(sums[i], before[i] + want, tol + (U[t] + 4 * u) * np.abs(before[i] + want) + 2 * u * np.abs(want) + TINY[t])
+
+
+@pytest.mark.parametrize("vocab,t", [(3 * 1024 + 40, "bf16"), (9 * 1024 + 200, "bf16"), (10 * 1024, "f16"), (2 * 512 + 9, "f32"), (9 * 512 + 100, "f32"), (25001, "bf16"), (259, "f32")])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("behind", ["nothing", "more", "much more"])
+def test_nan_anywhere_in_a_row(tm, vocab, t, many, behind):  # noqa: F811
+    """A NaN makes its row's sums NaN whatever comes behind it: logits that can not be, the end of the row, logits of which the one before is nothing.  The other rows are
+    as right as ever."""
+    torch, b2 = tm
+    at = np.unique(np.concatenate([np.arange(5, vocab, 197), vocab - 1 - np.arange(0, vocab // 2, 331)]))
+    rows = 2 * len(at)                                          # every second one without a NaN
+    x = _rand(torch, (rows, vocab), t, 3, 2.0)
+    for i, p in enumerate(at):
+        for r in (2 * i, 2 * i + 1):
+            if behind == "nothing":
+                x[r, p + 1:] = -math.inf
+            elif behind == "much more":
+                x[r, p + 1:] += 100.0
+                x[r, p + 1 + (vocab - p) // 2:] += 100.0
+        x[2 * i, p] = math.nan
+    tok, lp = _list(torch, rows, vocab, 8, 5, "plain")
+    if behind == "nothing":
+        tok[:, :] = -1
+        tok[:, 0] = 0
+        lp[:, 0] = -0.5
+    tok[tok[:, 0] < 0, 0] = 1
+    lp[lp[:, 0] == -np.inf, 0] = -1.0
+    times = 2368 // rows + 1 if many else 1                     # a warp a row, or a block
+    xs = x.repeat(times, 1)
+    tokens, lps = torch.from_numpy(np.tile(tok, (times, 1))).cuda(), torch.from_numpy(np.tile(lp, (times, 1))).cuda()
+    z = x.double().cpu().numpy()
+    for rest in (True, False):
+        loss, lse, other = (torch.full((rows * times,), 7.0, device="cuda") for _ in range(3))
+        b2.distill_forward(xs, tokens, lps, loss, lse, lse_rest=other if rest else None)
+        got = [_host(v).reshape(times, rows) for v in (loss, lse)]
+        assert np.isnan(got[0][:, ::2]).all() and np.isnan(got[1][:, ::2]).all()
+        for r in range(1, rows, 2):
+            w = _forward(z[r], tok[r], lp[r], rest)
+            for c in range(times):
+                _close(got[0][c, r], w[0], w[3])
+                _close(got[1][c, r], w[1], w[4])

@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(256) distill_forward_kernel(const T *logits, c
             __syncwarp();
             z_edge = edges[warp][lane];
             __syncwarp();
-            if (!(z_edge <= neg_inf())) t = {__fmul_rn(z_edge, a.scale), 1.0f};
+            z_edge = __fmul_rn(z_edge, a.scale);               // what the scale takes to -inf adds nothing
+            if (!(z_edge <= neg_inf())) t = {z_edge, 1.0f};
             // +inf as e^(inf - inf)
             if (t.m == __int_as_float(0x7f800000)) t.m = t.s = nanf("");
         }

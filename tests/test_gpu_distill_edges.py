@@ -84,3 +84,30 @@ def test_nan_anywhere_in_a_row(tm, vocab, t, many, behind):  # noqa: F811
             for c in range(times):
                 _close(got[0][c, r], w[0], w[3])
                 _close(got[1][c, r], w[1], w[4])
+
+
+@pytest.mark.parametrize("rows,vocab,shift", [(5, 1031, 3), (2400, 1031, 1), (7, 9005, 0), (2400, 2101, 5)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("rest", [True, False])
+def test_the_lowest_value_at_the_ends_of_a_row_and_a_scale_above_1(tm, rows, vocab, shift, t, rest):  # noqa: F811
+    """logits that the scale takes to -inf add nothing, wherever they stand: in front of the first whole vector and behind the last one too"""
+    torch, b2 = tm
+    x = _rand(torch, (rows, vocab), t, 3, 2.0, 2, shift)
+    x[:, :9] = torch.finfo(x.dtype).min
+    x[:, -9:] = torch.finfo(x.dtype).min
+    x[1, 20:] = torch.finfo(x.dtype).min
+    x[2] = torch.finfo(x.dtype).min                            # nothing that can be
+    tok, lp = _list(torch, rows, vocab, 6, 5, "plain")
+    tok[(tok < 9) | (tok >= vocab - 9)] = -1
+    tok[1:3] = -1
+    tok[1:3, 0], lp[1:3, 0] = 12, -0.25
+    loss, lse, other = (torch.full((rows,), 7.0, device="cuda") for _ in range(3))
+    b2.distill_forward(x, torch.from_numpy(tok).cuda(), torch.from_numpy(lp).cuda(), loss, lse, lse_rest=other if rest else None, scale=2.0)
+    z = (x.float() * 2.0).double().cpu().numpy()
+    assert (z[:, -9:] == -math.inf).all()
+    for r in sorted({0, 1, 2, 3, 4, rows - 1} | set(range(5, rows, 61))):
+        w = _forward(z[r], tok[r], lp[r], rest)
+        _close(_host(loss[r]), w[0], w[3])
+        _close(_host(lse[r]), w[1], w[4])
+        if rest:
+            _close(_host(other[r]), w[2], w[5])

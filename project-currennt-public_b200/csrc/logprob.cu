@@ -44,7 +44,7 @@ __device__ __forceinline__ void rescale(Sums &a, float m) {
     const float d = a.m - m, r = ex2(d * LOG2E);
     a.e = r == 0.0f ? 0.0f : r * fmaf(a.s, d, a.e);
     a.s = r == 0.0f ? 0.0f : r * a.s;
-    a.m = m;
+    a.m = max_nan(a.m, m);                                  // NaN stays, whatever is met behind it
 }
 __device__ __forceinline__ Sums merge(Sums a, Sums b) {
     const float m = max_nan(a.m, b.m);

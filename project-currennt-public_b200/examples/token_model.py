@@ -78,7 +78,7 @@ class TokenModel:
         return self.logits[:self.n]
 
     def quantize(self):
-        """the output matrix in 8-bit integers, for last_logits"""
+        """the output matrix in 8-bit integers, for last_logits; from then on an update quantises it anew"""
         pitch = (self.D + 15) // 16 * 16
         self.out8 = torch.empty(self.V, pitch, dtype=torch.int8, device="cuda")[:, :self.D], torch.empty(self.V, device="cuda")
         b2lstm.int8_quantize(*self.out8, self.w["out"])
@@ -167,6 +167,8 @@ class TokenModel:
         b2lstm.gradient_clip(self.grads, max_norm, self.norm, workspace=self.work)
         for k, w in self.w.items():
             w.add_(self.g[k], alpha=-lr)
+        if self.out8:
+            b2lstm.int8_quantize(*self.out8, self.w["out"])
 
     def write(self, tokens, beams, steps, end=None, length_power=0.0, allowed=None):
         """Beam search from tokens [T, P / beams] (no padding): the `steps` tokens of every beam [steps, P], best first within a sequence, and their log probabilities

@@ -392,14 +392,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
     const bool enough = passed <= max(160, 2 * a.top + 32);
     unsigned bound = enough ? guess : 0;                       // or the digits found so far, and zeros
 #pragma unroll 1
-    for (int above = 32, shift = enough ? -1 : 32 - DIGIT_BITS; shift >= 0;) {      // the digit's bits are those from shift on and below `above`; the last one has fewer
+    for (int shift = enough ? -1 : 32 - DIGIT_BITS; shift >= 0;) {
         for (int i = t; i < DIGITS; i += JOIN_THREADS) counts[i] = 0;
         __syncthreads();
         if (t == 0) digit = -1;                              // all have taken the one before
         const int want = left;                               // before the barriers behind which it is written
-        const unsigned bits = (1u << (above - shift)) - 1;
+        const int above = shift ? shift + DIGIT_BITS : 32 % DIGIT_BITS;      // the last digit has the bits that are left
         for_all([&](int, unsigned k) {
-            if (above == 32 || k >> above == bound >> above) atomicAdd(&counts[(k >> shift) & bits], 1);
+            if (above >= 32 || k >> above == bound >> above) atomicAdd(&counts[(k >> shift) & ((1u << (above - shift)) - 1)], 1);
         });
         __syncthreads();
         // the digits in falling order, EACH a thread: the one with which `left` entries are reached
@@ -432,7 +432,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const SelectArg
         if (digit < 0) break;                                // fewer than `top` altogether: all of them
         bound |= (unsigned)digit << shift;
         if (shift == 0 || reach <= 2 * a.top) break;
-        above = shift;
         shift = max(0, shift - DIGIT_BITS);
     }
     for_all([&](int i, unsigned k) {

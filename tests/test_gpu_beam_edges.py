@@ -122,3 +122,19 @@ def test_nan_anywhere_in_a_row(tm, t, behind, beams):  # noqa: F811
     want = _select(z, scores.cpu().numpy(), None, None, 0, 1, 24)
     assert (want[1] % 2 == 1).all()
     _same(got, want, 0, vocab)
+
+
+@pytest.mark.parametrize("lo,hi", [(0, 16384), (0, 20000), (0, 40000), (8192, 50001), (16384, 16385), (10000, 49990)])
+@pytest.mark.parametrize("t", ["bfloat16", "float32"])
+def test_a_range_of_tokens_ruled_out(tm, lo, hi, t):  # noqa: F811
+    """rows of one slice whose mask leaves nothing in whole chunks, first, last or between"""
+    torch, b2 = tm
+    beams, vocab, top = 40, 50001, 24
+    x = (torch.randn(beams, vocab, generator=torch.Generator().manual_seed(6)) * 2.5).to(getattr(torch, t)).cuda()
+    scores = -torch.rand(beams, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    mask = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    mask[lo:hi] = False
+    got = _run(torch, b2, x, scores, 1, top, mask=mask)
+    z = x.double().cpu().numpy()
+    z[:, lo:hi] = -math.inf
+    _same(got, _select(z, scores.cpu().numpy(), None, None, 0, 1, top), 0, vocab)

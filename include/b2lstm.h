@@ -252,7 +252,7 @@ int b2_gradient_clip(const b2_tensor *tensors, const b2_tensor *out, int n, floa
  *   lse_rest NULL: the listed tokens are all there is, q = exp(top_logprobs) over their sum (top_logprobs may then be logits):
  *       loss = sum q (log q - log p)
  *   else:         q = exp(top_logprobs); the rest of the vocabulary is one more outcome, with q_rest = 1 - sum q (0 where that is below 2^-20: log
- *       probabilities in fp32 say no more) and p_rest = exp(lse_rest - lse), lse_rest = log sum exp z over the tokens that are not listed:
+ *       probabilities in fp32 say no more; the sum is one in fp32 as well, off by up to 2^-22 or so) and p_rest = exp(lse_rest - lse), lse_rest = log sum exp z over the tokens that are not listed:
  *       loss = sum q (log q - log p) + q_rest (log q_rest - log p_rest)
  * A temperature T is scale = 1 / T here and in the teacher's b2_logprob_forward.  A place of the list with a negative token is empty, and so is one whose
  * token stands further ahead in its row; a row with nothing but empty places (and, with lse_rest NULL, one whose listed tokens all have the log probability
@@ -274,8 +274,9 @@ int b2_distill_backward(void *dlogits, long long ld_dlogits, const void *logits,
  * logits, vocab (at most 2^26) columns, belongs to beam b of sequence g; scores [groups * beams] are the beams' log probabilities so far.  With z = scale * x
  * where the token is allowed (mask as for b2_logprob_forward) and -inf elsewhere, the continuation of beam b by token v has the
  *   score = scores[b] + z[v] - log sum exp z
- * and they are ranked by weights[b] * score, in 64 bits, equal ones by beam, logit (larger first) and token.  weights (NULL: 1) are a length penalty's factors,
- * above 0.  A beam with finished[b] (NULL: none) non-zero is at its end: it has one continuation, end_token with the score it has; its logits are not
+ * and they are ranked by weights[b] * score, equal ones by beam, logit (larger first) and token.  The ranks are 64-bit numbers, but a beam's log sum is the log of
+ * a sum of exponentials in fp32, good to about 2^-22: continuations of one beam are in their exact order, those of different beams that are closer to each other
+ * than that may be in either.  weights (NULL: 1) are a length penalty's factors, above 0.  A beam with finished[b] (NULL: none) non-zero is at its end: it has one continuation, end_token with the score it has; its logits are not
  * looked at.  No continuations: beams whose score is no finite number or whose weight no positive finite one, rows with NaN or +inf among the allowed logits,
  * tokens that are not allowed or have z = -inf.  top_scores, top_beams (below beams) and top_tokens are [groups][top], best first; -inf, -1 and -1 where
  * there are fewer.  workspace: aligned to 16 bytes; its size is 0 for sizes that the call refuses. */
@@ -301,8 +302,8 @@ int b2_beam_reorder(const b2_state *states, int n, const int *parents, long long
 int b2_int8_quantize(signed char *q, long long ld_q, float *scales, const void *x, int type, long long rows, int dim, long long ld_x, b2_stream stream);
 /* Products in 8-bit integers with a scale for each row and each channel, as for the output matrix of a model that is answered with:
  *   out[r][c] = x_scales[r] * w_scales[c] * sum_k x[r][k] * w[c][k] + bias[c]
- * w is [channels][dim], bias (channels floats) may be NULL.  The sums are exact (dim at most 131071); each is rounded to fp32, then the product, the sum with
- * the bias and the conversion to out_type are.  x_type B2_F32, B2_BF16 or B2_F16: x is quantised in the call as b2_int8_quantize does (x_scales is NULL,
+ * w is [channels][dim], bias (channels floats) may be NULL.  The sums are exact (dim at most 131071).  Rounded to fp32 are: each sum, the product of the two scales,
+ * and, once, what these two and the bias give by a fused multiply-add; then comes the conversion to out_type.  x_type B2_F32, B2_BF16 or B2_F16: x is quantised in the call as b2_int8_quantize does (x_scales is NULL,
  * workspace aligned to 16 bytes); B2_I8: x and x_scales are given and no workspace is needed.  8-bit integers start at a multiple of 16 bytes, and so does each
  * of their rows (ld_w, and ld_x with B2_I8).  A tile that the tensor cores' kernel gave up waiting for comes out as NaN. */
 enum { B2_I8 = 3 };

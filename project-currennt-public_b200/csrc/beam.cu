@@ -8,8 +8,11 @@
 // vector whose largest entry reaches it is laid aside; in the end the entries that reach the bound of the whole slice are counted into their places.
 // Second kernel, started while the first one drains: a block joins the sums and the lists of a sequence's beams, the ranks in 64 bits (scores of different
 // beams meet, and 32 bits would make ties of what the beams' logits tell apart).
+// The sums and their logarithms are fp32 ones, as everywhere here: good to 2^-22 or so, which is what decides between beams that are closer than that.
 // Bound by instructions (18 an entry with a mask, 14 without, 5 of them for its exponential) and by the launches' latency.  Measured on a B200 (device time over the same buffers; in brackets a pass over
-// buffers that change): 64 x 8 rows of 50001 bf16 with a mask, 16 continuations 31 us (35; the bytes' floor is 8), of that the second kernel 6 us; 4 rows of 32000 fp32 9.6 us (11.8), two launches.
+// buffers that change): 64 x 8 rows of 50001 bf16 with a mask, 16 continuations 32 us (35; the bytes' floor is 8), of that the second kernel 6 us; 4 rows of 32000 fp32 9.6 us (11.8), two launches.
+// Slow are rows of one slice whose mask rules out their first tokens up to behind chunk 1 or 3: the bound stays at -inf until the next of the chunks after which it is taken again, so too many vectors are
+// laid aside, and the slice is gone through once for each continuation (the same 64 x 8 rows without their first 20000 tokens 324 us).
 // Reordering: 64 x 8 beams with 112 MB of states and frames 33 us for the copy there and back (6.8 TB/s).
 #include <math.h>
 
@@ -499,7 +502,8 @@ int vectors_of(int vocab, int type) { const int w = 16 / type_size(type); return
 // (and 64 lists for a sequence at most, which the second kernel goes through)
 int slices_of(long long rows, int beams, int vocab, int type) {
     const int chunks = (vectors_of(vocab, type) + CHUNK - 1) / CHUNK;
-    long long most = rows && rows < 592 ? 592 / rows : 1;          // blocks that run at a time: 4 an SM
+    // blocks that run at a time: 4 on each of 148 SMs.  A number, so that the workspace has the same size wherever it is asked for
+    long long most = rows && rows < 592 ? 592 / rows : 1;
     if (most > 64 / beams) most = 64 / beams;
     const int each = (int)((chunks + most - 1) / most);
     return (chunks + each - 1) / each;

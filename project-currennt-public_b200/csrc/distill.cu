@@ -11,7 +11,7 @@
 // rest needs no test at any entry, and nothing is read twice.  Narrow rows lie there whole, and as few lanes as the list has places have a row: with a warp a row the
 // list's arithmetic is most of the work (65536 rows of 100 fp32: 8.9 us, a warp a row 47.7 us).
 // Backward: one read, one write; a ninth warp prepares a block's list while the logits of the eight are on the way; the gradient of unlisted tokens is written
-// everywhere, and then that of the listed ones over it.  Only one exponential an entry: the rest's probabilities given that it is the rest, times the row's
+// everywhere, and then that of the listed ones over it, by the block whose segment holds them: no entry is read or written by two blocks, so that a gradient may take its logits' place.  Only one exponential an entry: the rest's probabilities given that it is the rest, times the row's
 // factor p_r - q_r.
 // Bound, for long rows of 16-bit logits, by memory, the exponentials and 7 issue slots an entry close behind.  Measured on a B200 (device time over the same buffers; in brackets a
 // pass over buffers that change): 8192 rows of 50001 bf16, 32 listed, with a rest 126 us (147; 821 MB: 6.5 TB/s); backward 8192 rows of 32003 bf16, 64 listed 162 us (175;
@@ -86,6 +86,7 @@ template <int SLOTS, int TEAM, bool REST> __device__ __forceinline__ bool teache
 #pragma unroll
     for (int o = TEAM / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
     if (REST) {
+        // in fp32, as the listed probabilities are: a rest of 2e-6 comes out 1.4 % off in the mean, 6 % at most; with 64 bits it would be 0.3 %, of log probabilities that are rounded themselves
         rest = 1.0f - sum;
         if (rest < LEAST_REST) rest = 0.0f;
         return list.any();
@@ -388,7 +389,8 @@ template <typename T, int SLOTS, bool REST> int launch_forward(const T *logits, 
         if (a.top <= 16 && vecs <= 16 * 6) return rows(distill_forward_rows_kernel<T, 16, 6, 1, REST>, (a.rows + 15) / 16);
     }
     if (vecs <= 32 * 4) return rows(distill_forward_rows_kernel<T, 32, 4, SLOTS, REST>, (a.rows + 7) / 8);
-    // a warp a row where the rows fill the device, a block a row else; 4 blocks an SM for long rows (8192 x 50001: 126 us, with 3 137 us), 3 for shorter ones (40000 x 3000:
+    // A warp a row where the rows fill the device, a block a row else (bf16, 32 listed, a warp / a block: 1200 x 50000 41 / 29 us, 2000 x 50000 42 / 42, 4000 x 50000 80 / 82; rows of a few pieces would want
+    // the warp earlier, 1200 x 3000 6.7 / 11.9 us); 4 blocks an SM for long rows (8192 x 50001: 126 us, with 3 137 us), 3 for shorter ones (40000 x 3000:
     // 69 us, with 4 75 us)
     const bool many = a.rows >= 16 * sm_count();
     const long long teams = many ? (a.rows + 7) / 8 : a.rows, most = (vecs >= 1024 ? 4ll : 3ll) * sm_count();
@@ -604,6 +606,7 @@ template <typename T, int SLOTS, bool REST, bool ADD> int launch_backward(T *dlo
         if (a.top <= 16 && vecs <= 16 * 6) return go(distill_backward_rows_kernel<T, 16, 6, 1, REST, ADD>, (a.rows + 15) / 16, 256);
     }
     if (vecs <= 32 * 4) return go(distill_backward_rows_kernel<T, 32, 4, SLOTS, REST, ADD>, (a.rows + 7) / 8, 256);
+    // Vectors of a thread: 2 where the rows do not fill the device (rows of 32000 bf16, 2 / 8: 30 rows 2.4 / 3.3 us, 120 3.4 / 3.7, 150 4.7 / 4.6, 600 11.4 / 10.8)
     const bool few = (double)a.rows * vecs < 4096.0 * sm_count();
     const int u = few ? 2 : 8, segs = (vecs + STREAM * u - 1) / (STREAM * u);
     if (few) return go(distill_backward_kernel<T, 2, SLOTS, REST, ADD>, a.rows * segs, STREAM + 32, segs);
